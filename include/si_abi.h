@@ -355,6 +355,81 @@ int si_attention_group(const si_shape_t *s, const float *q, int nheads, int grou
 size_t si_attention_group_workspace(const si_shape_t *s, int nheads, int context);
 
 /* ------------------------------------------------------------------ */
+/* A K/V cache held in 4 bits, and page copies                         */
+/* ------------------------------------------------------------------ */
+
+/* No counterpart in the reference, whose cache is fp16 (qwen_one_layer.c:
+ * 262-266).  Blocks of 32 values of a K or V row share a scale:
+ *   m = the value of largest magnitude (the negative one of a pair; a NaN
+ *       counts as 0), h = -m / 128 limited to +-508, rounded to 7 significant
+ *       bits (ties to even) and to fp16;
+ *   x is held as n = floor(x / (16 h) + 8.5), decided exactly, limited to
+ *   0..15 (8 where h is 0), and stands for 16 h (n - 8)
+ * (Q4_0's rule with a 7-bit scale).  A held value is an fp16 value, so rows
+ * read back (si_kv4_read) are exactly what attention uses.  Values beyond
+ * 65024 are limited to it.
+ *
+ * Caches are paged: K and V pools of npages pages, each of page_size positions
+ * (a power of two in 16..65536) of every KV head, si_kv4_page_bytes(s,
+ * page_size) bytes a page (9/32 of an fp16 page; the layout is the library's),
+ * pools 16-byte aligned.  pages (device int [sequences][max_pages]) lists each
+ * sequence's pages; ids outside [0, npages) are clamped.  A cache that is not
+ * paged is one whose lists are consecutive.  Of the shape only qheads, kvheads
+ * and hdim are read.
+ *
+ * Rows are addressed in one of two ways:
+ *   pos_step 1: ntok positions pos0, pos0 + 1, ... of the first sequence;
+ *   pos_step 0: token t is one position of sequence t, ctx_dev[t] - 1 (device
+ *               ints) or, with ctx_dev NULL, pos0.  A position below 0 or past
+ *               the pages (max_pos, the RoPE tables) from ctx_dev is skipped:
+ *               nothing of that row is read or written.
+ * A page that two sequences share is copied (si_kv_copy_pages) before either
+ * appends to it; two rows written to the same page by one pos_step 0 call are
+ * an error that is not detected (one of them may be lost). */
+size_t si_kv4_page_bytes(const si_shape_t *s, int page_size);
+
+/* si_rope_kv_append (RoPE as qwen_one_layer.c:172-183) into a 4-bit cache: q
+ * of each row to q_out [ntok][qheads*hdim], K rotated and quantized, V
+ * quantized. */
+int si_rope_kv4_append(const si_shape_t *s, const float *qkv, int ldqkv, int ntok, int pos0,
+                       int pos_step, int max_pos, const int *ctx_dev, const float *rope_cos,
+                       const float *rope_sin, float *q_out, uint8_t *k_pool, uint8_t *v_pool,
+                       int npages, int page_size, const int *pages, int max_pages, void *stream);
+
+/* Rows of an fp16 cache, k and v [ntok][kvheads*hdim] (16-byte aligned), into
+ * the pages, e.g. after si_layer_prefill ran over an fp16 cache. */
+int si_kv4_write(const si_shape_t *s, const uint16_t *k, const uint16_t *v, int ntok, int pos0,
+                 int pos_step, const int *ctx_dev, uint8_t *k_pool, uint8_t *v_pool, int npages,
+                 int page_size, const int *pages, int max_pages, void *stream);
+/* Rows of the pages as fp16 (exact), e.g. the prefix that si_layer_prefill's
+ * next piece attends to. */
+int si_kv4_read(const si_shape_t *s, const uint8_t *k_pool, const uint8_t *v_pool, int npages,
+                int page_size, const int *pages, int max_pages, int ntok, int pos0, int pos_step,
+                const int *ctx_dev, uint16_t *k, uint16_t *v, void *stream);
+
+/* si_attention (attention_flash, attention_kernels.h:80-164) over a 4-bit
+ * cache.  ctx_step 0: query i over sequence i, its context ctx_dev[i] (clamped
+ * to max_ctx; <= 0 gives zeros) or ctx0.  ctx_step 1: nq queries of the first
+ * sequence with contexts ctx0, ctx0 + 1, ... (a causal prompt whose rows are in
+ * place).  At most 65535 queries.  Outputs as si_attention's; workspace:
+ * si_attention_kv4_workspace bytes, 256-byte aligned. */
+int si_attention_kv4(const si_shape_t *s, const float *q, int nq, const uint8_t *k_pool,
+                     const uint8_t *v_pool, int npages, int page_size, const int *pages,
+                     int max_pages, const int *ctx_dev, int ctx0, int ctx_step, int max_ctx,
+                     float *attn, int8_t *qs, uint16_t *d, int16_t *bsum, void *workspace,
+                     size_t workspace_bytes, void *stream);
+size_t si_attention_kv4_workspace(const si_shape_t *s, int nq, int ctx_step, int max_ctx);
+
+/* Copies page src[i] to page dst[i] in each of npools pools of npages pages of
+ * page_bytes bytes (any paged cache's, fp16 or 4-bit): a fork's copies before
+ * its next token, or a compaction's moves.  pools, src and dst are HOST
+ * arrays, read before the call returns (under stream capture too: the graph
+ * holds its own copy).  All moves run at once, so a page may be read many
+ * times, but written once, and not both; pools may not overlap. */
+int si_kv_copy_pages(void *const *pools, int npools, size_t page_bytes, int npages,
+                     const int *src, const int *dst, int n, void *stream);
+
+/* ------------------------------------------------------------------ */
 /* Layer level (run_layer / run_layer_fused / pf_run_batch)            */
 /* ------------------------------------------------------------------ */
 

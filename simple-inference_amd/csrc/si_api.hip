@@ -12,6 +12,7 @@
 
 #include <cxxabi.h>
 
+#include <algorithm>
 #include <map>
 #include <memory>
 #include <mutex>
@@ -1615,6 +1616,210 @@ int si_layer_prefill(si_layer_t *L, const float *x, int ntok, int prefix, uint16
     SI_REQUIRE(prefix >= 0 && prefix + ntok <= L->max_pos, "prefix+ntok exceeds %d", L->max_pos);
     return run_rows(L, x, ntok, kc, vc, 0, prefix, nullptr, prefix + 1, 1, prefix + ntok, out,
                     flags, S(stream));
+}
+
+}  // extern "C"
+
+// ---------------------------------------------------------------------------
+// The cache held in 4 bits, and page copies (si_kv4.hip)
+// ---------------------------------------------------------------------------
+
+// The heads of a shape, as the 4-bit calls use it (hidden and ffn unread).
+static int check_heads(const char *what, const si_shape_t *s) {
+    SI_REQUIRE(s, "%s: shape is NULL", what);
+    SI_REQUIRE(s->qheads > 0 && attn_supported(s->qheads, s->kvheads, s->hdim),
+               "%s: unsupported heads %d/%d x hdim %d (need qheads %% kvheads == 0, ratio <= 16, "
+               "hdim 32, 64, 96 or 128)", what, s->qheads, s->kvheads, s->hdim);
+    SI_REQUIRE((long long)s->qheads * s->hdim <= (1 << 20), "%s: %d heads", what, s->qheads);
+    return SI_OK;
+}
+
+static bool kv4_page_ok(int page_size) {
+    return page_size >= 16 && page_size <= (1 << 16) && (page_size & (page_size - 1)) == 0;
+}
+
+static int kv4_cache(const char *what, const si_shape_t *s, const uint8_t *k, const uint8_t *v,
+                     int npages, int page_size, const int *pages, int max_pages, Kv4Cache *c) {
+    SI_REQUIRE(k && v && pages, "%s: NULL pointer", what);
+    SI_REQUIRE((((uintptr_t)k | (uintptr_t)v) & 15) == 0, "%s: the pools must be 16-byte aligned",
+               what);
+    SI_REQUIRE(kv4_page_ok(page_size), "%s: page_size %d must be a power of two in 16..65536",
+               what, page_size);
+    SI_REQUIRE(npages >= 1 && max_pages >= 1, "%s: npages and max_pages must be >= 1", what);
+    SI_REQUIRE((long long)max_pages * page_size <= INT32_MAX, "%s: %d pages of %d a sequence",
+               what, max_pages, page_size);
+    c->k = const_cast<uint8_t *>(k);
+    c->v = const_cast<uint8_t *>(v);
+    c->pages = pages;
+    c->npages = npages;
+    c->max_pages = max_pages;
+    c->kvheads = s->kvheads;
+    c->shift = 0;
+    while ((1 << c->shift) < page_size) ++c->shift;
+    return SI_OK;
+}
+
+// Rows of a call: pos_step 1, ntok positions from pos0 of sequence 0; pos_step 0,
+// a position of each of ntok sequences.
+static int kv4_rows(const char *what, int ntok, int pos0, int pos_step, const int *ctx_dev,
+                    long long limit) {
+    SI_REQUIRE(ntok >= 0 && pos0 >= 0, "%s: bad ntok %d / pos0 %d", what, ntok, pos0);
+    SI_REQUIRE(pos_step == 0 || pos_step == 1, "%s: pos_step %d is neither 0 nor 1", what,
+               pos_step);
+    SI_REQUIRE(!ctx_dev || pos_step == 0, "%s: ctx_dev goes with pos_step 0 (a token a sequence)",
+               what);
+    SI_REQUIRE(ctx_dev || ntok == 0 || pos0 + (long long)(ntok - 1) * pos_step < limit,
+               "%s: positions exceed %lld", what, limit);
+    return SI_OK;
+}
+
+extern "C" {
+
+size_t si_kv4_page_bytes(const si_shape_t *s, int page_size) {
+    if (!s || !attn_supported(s->qheads, s->kvheads, s->hdim) || !kv4_page_ok(page_size)) return 0;
+    return (size_t)s->kvheads * page_size * s->hdim / 16 * 9;
+}
+
+int si_rope_kv4_append(const si_shape_t *s, const float *qkv, int ldqkv, int ntok, int pos0,
+                       int pos_step, int max_pos, const int *ctx_dev, const float *rc,
+                       const float *rs, float *q_out, uint8_t *k_pool, uint8_t *v_pool,
+                       int npages, int page_size, const int *pages, int max_pages,
+                       void *stream) {
+    const char *what = "rope_kv4_append";
+    TRY(check_heads(what, s));
+    Kv4Cache c;
+    TRY(kv4_cache(what, s, k_pool, v_pool, npages, page_size, pages, max_pages, &c));
+    SI_REQUIRE(max_pos >= 1, "%s: max_pos must be >= 1", what);
+    TRY(kv4_rows(what, ntok, pos0, pos_step, ctx_dev,
+                 std::min((long long)max_pos, (long long)max_pages * page_size)));
+    SI_REQUIRE(ldqkv >= (s->qheads + 2 * s->kvheads) * s->hdim, "%s: ldqkv too small", what);
+    SI_REQUIRE(ntok == 0 || (qkv && rc && rs && q_out), "%s: NULL pointer", what);
+    if (ntok == 0) return SI_OK;
+    launch_rope_kv4(qkv, ldqkv, ntok, s->qheads, s->hdim, pos0, pos_step, max_pos, ctx_dev, rc, rs,
+                    q_out, c, S(stream));
+    return check_launch("si_rope_kv4_append");
+}
+
+int si_kv4_write(const si_shape_t *s, const uint16_t *k, const uint16_t *v, int ntok, int pos0,
+                 int pos_step, const int *ctx_dev, uint8_t *k_pool, uint8_t *v_pool, int npages,
+                 int page_size, const int *pages, int max_pages, void *stream) {
+    const char *what = "kv4_write";
+    TRY(check_heads(what, s));
+    Kv4Cache c;
+    TRY(kv4_cache(what, s, k_pool, v_pool, npages, page_size, pages, max_pages, &c));
+    TRY(kv4_rows(what, ntok, pos0, pos_step, ctx_dev, (long long)max_pages * page_size));
+    SI_REQUIRE(ntok == 0 || (k && v), "%s: NULL pointer", what);
+    SI_REQUIRE((((uintptr_t)k | (uintptr_t)v) & 15) == 0, "%s: k and v must be 16-byte aligned",
+               what);
+    if (ntok == 0) return SI_OK;
+    launch_kv4_write(k, v, ntok, s->hdim, pos0, pos_step, ctx_dev, c, S(stream));
+    return check_launch("si_kv4_write");
+}
+
+int si_kv4_read(const si_shape_t *s, const uint8_t *k_pool, const uint8_t *v_pool, int npages,
+                int page_size, const int *pages, int max_pages, int ntok, int pos0, int pos_step,
+                const int *ctx_dev, uint16_t *k, uint16_t *v, void *stream) {
+    const char *what = "kv4_read";
+    TRY(check_heads(what, s));
+    Kv4Cache c;
+    TRY(kv4_cache(what, s, k_pool, v_pool, npages, page_size, pages, max_pages, &c));
+    TRY(kv4_rows(what, ntok, pos0, pos_step, ctx_dev, (long long)max_pages * page_size));
+    SI_REQUIRE(ntok == 0 || (k && v), "%s: NULL pointer", what);
+    SI_REQUIRE((((uintptr_t)k | (uintptr_t)v) & 15) == 0, "%s: k and v must be 16-byte aligned",
+               what);
+    if (ntok == 0) return SI_OK;
+    launch_kv4_read(c, ntok, s->hdim, pos0, pos_step, ctx_dev, k, v, S(stream));
+    return check_launch("si_kv4_read");
+}
+
+size_t si_attention_kv4_workspace(const si_shape_t *s, int nq, int ctx_step, int max_ctx) {
+    if (!s || !attn_supported(s->qheads, s->kvheads, s->hdim) || nq <= 0 || max_ctx <= 0 ||
+        ctx_step < 0 || ctx_step > 1)
+        return 0;
+    return attn_kv4_workspace(s->qheads, s->kvheads, s->hdim, nq, ctx_step, max_ctx);
+}
+
+int si_attention_kv4(const si_shape_t *s, const float *q, int nq, const uint8_t *k_pool,
+                     const uint8_t *v_pool, int npages, int page_size, const int *pages,
+                     int max_pages, const int *ctx_dev, int ctx0, int ctx_step, int max_ctx,
+                     float *attn, int8_t *qs, uint16_t *d, int16_t *bsum, void *ws,
+                     size_t ws_bytes, void *stream) {
+    const char *what = "attention_kv4";
+    TRY(check_heads(what, s));
+    Kv4Cache c;
+    TRY(kv4_cache(what, s, k_pool, v_pool, npages, page_size, pages, max_pages, &c));
+    SI_REQUIRE(nq >= 0 && nq <= 65535 && max_ctx >= 1, "%s: bad nq %d / max_ctx %d", what, nq,
+               max_ctx);
+    SI_REQUIRE((long long)max_pages * page_size >= max_ctx, "%s: pages do not cover max_ctx %d",
+               what, max_ctx);
+    SI_REQUIRE(ctx_step == 0 || ctx_step == 1, "%s: ctx_step %d is neither 0 nor 1", what,
+               ctx_step);
+    SI_REQUIRE(!ctx_dev || ctx_step == 0, "%s: ctx_dev goes with ctx_step 0 (a query a sequence)",
+               what);
+    if (!ctx_dev) {
+        SI_REQUIRE(ctx0 >= 1, "%s: contexts must be >= 1", what);
+        SI_REQUIRE(nq == 0 || ctx0 + (long long)(nq - 1) * ctx_step <= max_ctx,
+                   "%s: context exceeds max_ctx", what);
+    }
+    SI_REQUIRE(nq == 0 || (q && attn), "%s: NULL pointer", what);
+    SI_REQUIRE(!qs || d, "%s: qs without d", what);
+    const size_t need =
+        nq ? attn_kv4_workspace(s->qheads, s->kvheads, s->hdim, nq, ctx_step, max_ctx) : 0;
+    SI_REQUIRE(need == 0 || (ws && ws_bytes >= need && ((uintptr_t)ws & 255) == 0),
+               "%s: needs %zu bytes of 256-byte aligned workspace", what, need);
+    if (nq == 0) return SI_OK;
+    launch_attention_kv4(q, nq, s->qheads, s->hdim, c, ctx_dev, ctx0, ctx_step, max_ctx, attn, qs,
+                         d, bsum, ws, ws_bytes, S(stream));
+    return check_launch("si_attention_kv4");
+}
+
+int si_kv_copy_pages(void *const *pools, int npools, size_t page_bytes, int npages,
+                     const int *src, const int *dst, int n, void *stream) {
+    const char *what = "kv_copy_pages";
+    SI_REQUIRE(npools >= 0 && n >= 0 && npages >= 1 && page_bytes >= 1, "%s: bad sizes", what);
+    SI_REQUIRE(page_bytes <= ((size_t)1 << 40) / (size_t)npages, "%s: %d pages of %zu bytes", what,
+               npages, page_bytes);
+    SI_REQUIRE((npools == 0 || pools) && (n == 0 || (src && dst)), "%s: NULL pointer", what);
+    bool wide = page_bytes % 16 == 0;
+    try {
+        std::vector<uintptr_t> at(npools);
+        for (int p = 0; p < npools; ++p) {
+            SI_REQUIRE(pools[p], "%s: pool %d is NULL", what, p);
+            at[p] = (uintptr_t)pools[p];
+            wide = wide && at[p] % 16 == 0;
+        }
+        std::sort(at.begin(), at.end());
+        for (int p = 1; p < npools; ++p)
+            SI_REQUIRE(at[p] - at[p - 1] >= page_bytes * (size_t)npages, "%s: two pools overlap",
+                       what);
+        for (int i = 0; i < n; ++i)
+            SI_REQUIRE(src[i] >= 0 && src[i] < npages && dst[i] >= 0 && dst[i] < npages,
+                       "%s: move %d, page %d to %d, outside 0..%d", what, i, src[i], dst[i],
+                       npages - 1);
+        // the moves run at once: no page is written twice, or written and read
+        std::vector<int> to(dst, dst + n);
+        std::sort(to.begin(), to.end());
+        for (int i = 1; i < n; ++i)
+            SI_REQUIRE(to[i] != to[i - 1], "%s: page %d is written twice", what, to[i]);
+        for (int i = 0; i < n; ++i)
+            SI_REQUIRE(!std::binary_search(to.begin(), to.end(), src[i]),
+                       "%s: page %d is read and written", what, src[i]);
+    } catch (const std::exception &) {
+        return fail(SI_ERR_NOMEM, "%s: no host memory for %d moves", what, n);
+    }
+    if (n == 0 || npools == 0) return SI_OK;
+    KvMoves mv;
+    for (int p0 = 0; p0 < npools; p0 += KvMoves::POOLS) {
+        const int np = std::min(npools - p0, KvMoves::POOLS);
+        for (int p = 0; p < np; ++p) mv.pool[p] = (uint8_t *)pools[p0 + p];
+        for (int i0 = 0; i0 < n; i0 += KvMoves::MOVES) {
+            const int nm = std::min(n - i0, KvMoves::MOVES);
+            std::copy(src + i0, src + i0 + nm, mv.src);
+            std::copy(dst + i0, dst + i0 + nm, mv.dst);
+            launch_kv_copy(mv, np, nm, page_bytes, wide, S(stream));
+        }
+    }
+    return check_launch("si_kv_copy_pages");
 }
 
 }  // extern "C"

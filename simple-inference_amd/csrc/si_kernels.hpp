@@ -326,3 +326,39 @@ void launch_f16_convert(const void *src, void *dst, size_t n, bool to_half, hipS
 void launch_stream_read(const void *buf, size_t bytes, uint32_t *sink, int workgroups,
                         int depth, hipStream_t st);
 }  // namespace si
+namespace si {
+// A K/V cache held in 4 bits (si_kv4.hip): pools of npages pages of 1 << shift
+// positions, sequence i's page list at pages + i * max_pages (device data, ids
+// clamped to [0, npages)).
+struct Kv4Cache {
+    uint8_t *k, *v;
+    const int *pages;
+    int npages, shift, max_pages, kvheads;
+    // the page of a sequence's position
+    __device__ __forceinline__ int page_of(int seq, int pos) const;
+};
+// RoPE of q|k|v rows, q to q_out, K and V quantized into the pages: tokens at
+// pos0 + t of sequence 0 (pos_step 1), or token t of sequence t at ctx_dev[t] - 1
+// (or pos0).  Positions outside the page lists or max_pos are skipped.
+void launch_rope_kv4(const float *qkv, int ldqkv, int ntok, int qheads, int hdim, int pos0,
+                     int pos_step, int max_pos, const int *ctx_dev, const float *rc,
+                     const float *rs, float *q_out, const Kv4Cache &c, hipStream_t st);
+// fp16 rows [ntok][kvheads * hdim] into the pages, and back
+void launch_kv4_write(const uint16_t *k, const uint16_t *v, int ntok, int hdim, int pos0,
+                      int pos_step, const int *ctx_dev, const Kv4Cache &c, hipStream_t st);
+void launch_kv4_read(const Kv4Cache &c, int ntok, int hdim, int pos0, int pos_step,
+                     const int *ctx_dev, uint16_t *k, uint16_t *v, hipStream_t st);
+size_t attn_kv4_workspace(int qheads, int kvheads, int hdim, int nq, int ctx_step, int max_ctx);
+void launch_attention_kv4(const float *q, int nq, int qheads, int hdim, const Kv4Cache &c,
+                          const int *ctx_dev, int ctx0, int ctx_step, int max_ctx, float *attn,
+                          int8_t *qs, uint16_t *d, int16_t *bsum, void *workspace, size_t ws_bytes,
+                          hipStream_t st);
+// One launch's page copies, in the kernel's arguments.
+struct KvMoves {
+    static constexpr int POOLS = 64, MOVES = 384;
+    uint8_t *pool[POOLS];
+    int src[MOVES], dst[MOVES];
+};
+void launch_kv_copy(const KvMoves &mv, int npools, int nmoves, size_t page_bytes, bool wide,
+                    hipStream_t st);
+}  // namespace si

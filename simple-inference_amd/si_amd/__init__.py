@@ -123,6 +123,17 @@ _SIGS = {
     "si_layer_decode_paged": (_I, [_P, _P, _I, _P, _P, _I, _I, _P, _I, _P, _I, _I, _P, _I, _P]),
     "si_attention_paged": (_I, [ctypes.POINTER(Shape), _P, _I, _P, _P, _I, _I, _P, _I, _P, _I,
                                 _P, _P, _P, _P, _P, _Z, _P]),
+    "si_kv4_page_bytes": (_Z, [ctypes.POINTER(Shape), _I]),
+    "si_rope_kv4_append": (_I, [ctypes.POINTER(Shape), _P, _I, _I, _I, _I, _I, _P, _P, _P, _P, _P,
+                                _P, _I, _I, _P, _I, _P]),
+    "si_kv4_write": (_I, [ctypes.POINTER(Shape), _P, _P, _I, _I, _I, _P, _P, _P, _I, _I, _P, _I,
+                          _P]),
+    "si_kv4_read": (_I, [ctypes.POINTER(Shape), _P, _P, _I, _I, _P, _I, _I, _I, _I, _P, _P, _P,
+                         _P]),
+    "si_attention_kv4": (_I, [ctypes.POINTER(Shape), _P, _I, _P, _P, _I, _I, _P, _I, _P, _I, _I,
+                              _I, _P, _P, _P, _P, _P, _Z, _P]),
+    "si_attention_kv4_workspace": (_Z, [ctypes.POINTER(Shape), _I, _I, _I]),
+    "si_kv_copy_pages": (_I, [_P, _I, _Z, _I, _P, _P, _I, _P]),
     "si_layer_buffer": (_P, [_P, _I]),
     "si_layer_set_timing": (_I, [_P, _I]),
     "si_layer_phase_ms": (_I, [_P, _P]),
