@@ -1769,7 +1769,7 @@ int si_attention_kv4(const si_shape_t *s, const float *q, int nq, const uint8_t 
                "%s: needs %zu bytes of 256-byte aligned workspace", what, need);
     if (nq == 0) return SI_OK;
     launch_attention_kv4(q, nq, s->qheads, s->hdim, c, ctx_dev, ctx0, ctx_step, max_ctx, attn, qs,
-                         d, bsum, ws, ws_bytes, S(stream));
+                         d, bsum, ws, S(stream));
     return check_launch("si_attention_kv4");
 }
 

@@ -272,82 +272,375 @@ __global__ void __launch_bounds__(2 * D) k_kv4_read(Kv4Cache c, int ntok, int po
 }
 
 // ---------------------------------------------------------------------------
-// attention: a workgroup per (query, KV head), 256 positions at a time with the
-// running maximum and sum of the softmax
+// attention over the pages: a workgroup per (context chunk, KV head, query), its
+// four wavefronts take every fourth group of 32 positions.  Per group
+//     S^T[pos][head] = K[pos][:] . q[head][:]        (v_mfma_f32_16x16x32_f16)
+//     O^T[dim][head] += V^T[dim][pos] . P[pos][head]
+// with the group's two score tiles' rows placed so that lane (col, g) gets the
+// scores of positions 8 g .. 8 g + 7 in registers, which is the k-slice its lane
+// supplies of P: nothing moves between lanes.
+//
+// K: a masked nibble is the fp16 subnormal n 2^-24 (or 16 n 2^-24 in the odd
+// places, where q carries 1/16), which the matrix cores take exactly: 5 operations
+// unpack 8 values.  -8 sum q is the product's C operand, the block's scale
+// multiplies the 16x16 result (4 operations a block and lane against 8 values').
+// V: (64 + n) h - 72 h in one fused operation a pair, exact in fp16 (above).
+//
+// q and the weights go in as fp16 hi + lo pairs.  q's are integers of a common
+// unit, 12 bits each of the head's largest value: every sum of 32 products (20
+// bits) is then exact in the matrix core, whose own rounding of a sum with an
+// offset of 8 sum q would show (24 bits of the head's largest q in all; as
+// fp16 roundings of q the result was off by up to 2.7e-5).  The weights' pair
+// has 22 bits.  With at most 8 heads a KV head both halves share one product:
+// columns 0-7 carry hi, 8-15 lo, and their results are added across (WIDE: 9 to
+// 16 heads, two products).
+//
+// The running maximum is moved only when a score passes it by 2^8 (weights up to
+// 256 fit the fp16 pair as well as weights up to 1), a wavefront-uniform branch.
 // ---------------------------------------------------------------------------
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+typedef float f4 __attribute__((ext_vector_type(4)));
+typedef float f2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+
+constexpr int A4_GROUP = 32;             // positions of a wavefront's step
+constexpr int A4_STEP = 4 * A4_GROUP;    // of a workgroup's
+
+__device__ __forceinline__ float ror8_add(float v) { return v + dpp_f<DPP_ROR8>(v); }
+
+// N dwords at p, aligned to what N allows
+template <int N>
+__device__ __forceinline__ void load_dwords(const uint8_t *p, uint32_t (&w)[N]) {
+    if constexpr (N == 1) {
+        w[0] = *(const uint32_t *)p;
+    } else if constexpr (N == 2) {
+        const uint2 t = *(const uint2 *)p;
+        w[0] = t.x, w[1] = t.y;
+    } else if constexpr (N == 3) {
+        const uint3 t = *(const uint3 *)p;
+        w[0] = t.x, w[1] = t.y, w[2] = t.z;
+    } else {
+        const uint4 t = *(const uint4 *)p;
+        w[0] = t.x, w[1] = t.y, w[2] = t.z, w[3] = t.w;
+    }
+}
+
+// What a wavefront reads of a group: lane (col, g)'s K nibbles of both tiles, V
+// nibbles, and the scales of positions 8 g .. 8 g + 7.
 template <int D>
-__global__ void __launch_bounds__(256) k_attn_kv4(const float *__restrict__ q, int qheads,
-                                                  Kv4Cache c, const int *__restrict__ ctx_dev,
-                                                  int ctx0, int ctx_step, int max_ctx,
-                                                  float scale2, float *__restrict__ attn) {
-    constexpr int NB = D / 32;
-    __shared__ float ql[16 * D], p[16][256], red[4];
-    const int g = blockIdx.x, qi = blockIdx.y, tid = threadIdx.x, per = qheads / c.kvheads;
-    const int seq = ctx_step ? 0 : qi, page_size = 1 << c.shift;
+struct Kv4Group {
+    static constexpr int KS = D / 32, DT = D / 16;
+    uint32_t k[2][KS], v[DT];
+    uint4 kh[KS], vh[KS];
+    // kp, vp: of the KV head's part of the page that holds the lane's K row's and
+    // V positions' units; ku, vu: those units' places in it
+    __device__ __forceinline__ void load(const uint8_t *kk, int ku, const uint8_t *ks,
+                                         const uint8_t *vv, int vu, int nib, int lane) {
+        const int r = lane & 15, g = lane >> 4;
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+            load_dwords<KS>(kk + ku * 4 * D + t * 2 * D + g * (D / 2) + (r & 3) * (D / 8), k[t]);
+        constexpr int FULL = D / 64;
+#pragma unroll
+        for (int f = 0; f < FULL; ++f) {
+            uint32_t w[4];
+            load_dwords<4>(vv + vu * 4 * D + f * 256 + r * 16, w);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[4 * f + e] = w[e];
+        }
+        if constexpr (DT % 4) {
+            uint32_t w[2];
+            load_dwords<2>(vv + vu * 4 * D + FULL * 256 + r * 8, w);
+            v[DT - 2] = w[0], v[DT - 1] = w[1];
+        }
+#pragma unroll
+        for (int b = 0; b < KS; ++b) {
+            kh[b] = *(const uint4 *)(ks + nib + (vu * KS + b) * 16);
+            vh[b] = *(const uint4 *)(vv + nib + (vu * KS + b) * 16);
+        }
+    }
+};
+
+__device__ __forceinline__ h2 as_h2(uint32_t u) { return __builtin_bit_cast(h2, u); }
+__device__ __forceinline__ uint32_t as_u(h2 h) { return __builtin_bit_cast(uint32_t, h); }
+
+template <int D, bool WIDE, bool PAGE16>
+__global__ void __launch_bounds__(256, 2) k_attn_kv4(
+    const float *__restrict__ q, int qheads, Kv4Cache c, const int *__restrict__ ctx_dev, int ctx0,
+    int ctx_step, int max_ctx, int chunk, float scale2, float *__restrict__ ws_m,
+    float *__restrict__ ws_l, float *__restrict__ ws_o, float *__restrict__ attn,
+    int8_t *__restrict__ qs, uint16_t *__restrict__ qd8, int16_t *__restrict__ bsum) {
+    constexpr int KS = D / 32, DT = D / 16, COLS = WIDE ? 16 : 8;
+    __shared__ __attribute__((aligned(16))) float mo[4][COLS][D];
+    __shared__ float mm[4][COLS], ml[4][COLS], sc[COLS][4], linv[COLS];
+    const int sp = blockIdx.x, g0 = blockIdx.y, qi = blockIdx.z, ns = gridDim.x;
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int col = lane & 15, g = lane >> 4;
+    const int per = qheads / c.kvheads, seq = ctx_step ? 0 : qi;
     const int ctx = min(ctx_dev ? ctx_dev[qi] : ctx0 + qi * ctx_step, max_ctx);
+    if (ns > 1 && ctx_dev) {
+        // shares of the longest context there is
+        int most = 0;
+        for (int i = lane; i < (int)gridDim.z; i += 64) most = max(most, ctx_dev[i]);
+        most = min(__builtin_amdgcn_readfirstlane(wave_max_i(most)), max_ctx);
+        chunk = max(((most + ns - 1) / ns + A4_STEP - 1) / A4_STEP, 1) * A4_STEP;
+    }
+    const int p0 = sp * chunk, p1 = min(ctx, p0 + chunk);
+    if (ns > 1 && p0 >= p1) {  // an empty state
+        for (int h = tid; h < per; h += 256) {
+            const size_t pi = ((size_t)qi * qheads + g0 * per + h) * ns + sp;
+            ws_m[pi] = -INFINITY;
+            ws_l[pi] = 0.0f;
+        }
+        return;
+    }
+    // groups of this wavefront: s0 = p0 + 32 wave, + 128, ...
+    const int page_size = 1 << c.shift, nib = page_size * (D / 2);
     const size_t hb = (size_t)kv4_head_bytes(D, page_size);
-    const float *qrow = q + ((size_t)qi * qheads + g * per) * D;
-    for (int i = tid; i < per * D; i += 256) ql[i] = qrow[i];
+    const int *pages = c.pages + (size_t)seq * c.max_pages;
+    auto head_at = [&](int pos) {  // of the page holding pos (uniform)
+        const int pg = pages[min(pos >> c.shift, c.max_pages - 1)];
+        return ((size_t)min(max(pg, 0), c.npages - 1) * c.kvheads + g0) * hb;
+    };
+    auto load = [&](Kv4Group<D> &t, int s0) {
+        if constexpr (PAGE16) {
+            // two pages a group: units 0, 1 and 2, 3
+            const size_t a = head_at(s0), b = head_at(s0 + 16);
+            const size_t ka = (lane & 8) ? b : a, va = (lane & 32) ? b : a;
+            t.load(c.k + ka, (lane >> 2) & 1, c.k + va, c.v + va, g & 1, nib, lane);
+        } else {
+            const size_t a = head_at(s0);
+            const int u = (s0 & (page_size - 1)) >> 3;
+            t.load(c.k + a, u + ((lane >> 2) & 3), c.k + a, c.v + a, u + g, nib, lane);
+        }
+    };
+    int s0 = p0 + A4_GROUP * wave;
+    Kv4Group<D> ta, tb;
+    if (s0 < p1) load(ta, s0);
+
+    // q of the lane's column as the B operand, dims 32 b + 8 g + (0, 4, 1, 5, 2, 6,
+    // 3, 7), the odd ones over 16: integers hi and lo, q = (hi + lo 2^-12) 2^(ex - 10)
+    h8 qa[KS], qb[WIDE ? KS : 1];
+    f4 c8[KS], c8l[WIDE ? KS : 1];
+    float fac;
+    const float lo_col = !WIDE && col >= 8 ? 1.0f : 0.0f;
+    {
+        const int hc = WIDE ? col : col & 7;
+        const bool live = hc < per;
+        const float *row = q + ((size_t)qi * qheads + g0 * per + (live ? hc : 0)) * D + 8 * g;
+        float x[KS][8], big = 0.0f;
+#pragma unroll
+        for (int b = 0; b < KS; ++b)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                x[b][e] = live ? row[32 * b + e] : 0.0f;
+                big = fmaxf(big, fabsf(x[b][e]));
+            }
+        big = fmaxf(big, swap16_f(big));
+        big = fmaxf(big, swap32_f(big));
+        const int ex = big == 0.0f ? 0 : (int)(f2u(big) >> 23) - 127;
+        // the scores' units: 2^24 of the subnormals, 16 of the scale, q's
+        fac = __builtin_amdgcn_ldexpf(scale2, 28 + ex - 10 - (!WIDE && col >= 8 ? 12 : 0));
+        const u4 eight = {0x80088008u, 0x80808080u, 0x80088008u, 0x80808080u};  // -8 in them
+#pragma unroll
+        for (int b = 0; b < KS; ++b) {
+            h8 hi, lo;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const int dim = (e >> 1) + (e & 1) * 4;
+                const float y = __builtin_amdgcn_ldexpf(x[b][dim], 10 - ex), yh = rintf(y);
+                const float odd = (dim & 1) ? 0.0625f : 1.0f;
+                hi[e] = (_Float16)(yh * odd);
+                lo[e] = (_Float16)(rintf((y - yh) * 4096.0f) * odd);
+            }
+            c8[b] = (f4){0.0f, 0.0f, 0.0f, 0.0f};
+            if constexpr (WIDE) {
+                qa[b] = hi;
+                qb[b] = lo;
+                c8l[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, eight), lo,
+                                                                c8[b], 0, 0, 0);
+            } else {
+                const u4 uh = __builtin_bit_cast(u4, hi), ul = __builtin_bit_cast(u4, lo);
+                u4 us;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) us[e] = col >= 8 ? ul[e] : uh[e];
+                qa[b] = __builtin_bit_cast(h8, us);
+            }
+            c8[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, eight), qa[b],
+                                                           c8[b], 0, 0, 0);
+        }
+    }
+
+    float m = -INFINITY, lsum = 0.0f;  // of the column; lsum over the lane's positions
+    f4 o[DT];
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) o[dt] = (f4){0.0f, 0.0f, 0.0f, 0.0f};
+
+    auto step = [&](Kv4Group<D> &t, int s) {
+        float p[2][4];
+#pragma unroll
+        for (int tl = 0; tl < 2; ++tl) {
+            f4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int b = 0; b < KS; ++b) {
+                const uint32_t w = t.k[tl][b], w8 = w >> 8;
+                const u4 a = {w & 0x000f000fu, w & 0x00f000f0u, w8 & 0x000f000fu, w8 & 0x00f000f0u};
+                const h8 ka = __builtin_bit_cast(h8, a);
+                f4 d = c8[b];
+                d = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, qa[b], d, 0, 0, 0);
+                if constexpr (WIDE) {
+                    const f4 dl = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, qb[b], c8l[b], 0, 0, 0);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) d[i] = fmaf(dl[i], 0x1p-12f, d[i]);
+                }
+                const uint32_t hw[4] = {t.kh[b].x, t.kh[b].y, t.kh[b].z, t.kh[b].w};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) acc[i] = fmaf((float)as_h2(hw[i])[tl], d[i], acc[i]);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) p[tl][i] = WIDE ? acc[i] * fac : ror8_add(acc[i] * fac);
+        }
+        if (s + A4_GROUP > p1) {  // wavefront-uniform: positions past the end
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const bool l0 = s + 8 * g + i < p1, l1 = s + 8 * g + 4 + i < p1;
+                p[0][i] = l0 ? p[0][i] : -INFINITY;
+                p[1][i] = l1 ? p[1][i] : -INFINITY;
+                // their V scales may be anything: 0 (weight 0 * NaN would stay)
+                const uint32_t mask = (l0 ? 0xffffu : 0u) | (l1 ? 0xffff0000u : 0u);
+#pragma unroll
+                for (int b = 0; b < KS; ++b) (&t.vh[b].x)[i] &= mask;
+            }
+        }
+        float mx = fmaxf(fmaxf(fmaxf(p[0][0], p[0][1]), fmaxf(p[0][2], p[0][3])),
+                         fmaxf(fmaxf(p[1][0], p[1][1]), fmaxf(p[1][2], p[1][3])));
+        if (__ballot(mx > m + 8.0f)) {
+            mx = fmaxf(mx, swap16_f(mx));
+            mx = fmaxf(mx, swap32_f(mx));
+            const float mn = fmaxf(m, mx);
+            const float al = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
+            m = mn;
+            lsum *= al;
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) o[dt] *= al;
+        }
+        u4 pa, pb;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float x = __builtin_amdgcn_exp2f(p[0][i] - m), y = __builtin_amdgcn_exp2f(p[1][i] - m);
+            lsum += x + y;
+            const h2 hi = {(_Float16)x, (_Float16)y};
+            if constexpr (WIDE) {
+                const h2 lo = {(_Float16)(x - (float)hi[0]), (_Float16)(y - (float)hi[1])};
+                pa[i] = as_u(hi);
+                pb[i] = as_u(lo);
+            } else {
+                const float xr = fmaf(-(float)hi[0], lo_col, x), yr = fmaf(-(float)hi[1], lo_col, y);
+                pa[i] = as_u((h2){(_Float16)xr, (_Float16)yr});
+            }
+        }
+#pragma unroll
+        for (int b = 0; b < KS; ++b) {
+            const uint32_t hw[4] = {t.vh[b].x, t.vh[b].y, t.vh[b].z, t.vh[b].w};
+            h2 off[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) off[i] = as_h2(hw[i]) * (h2){(_Float16)-72.0f, (_Float16)-72.0f};
+#pragma unroll
+            for (int dt = 2 * b; dt < 2 * b + 2; ++dt) {
+                const uint32_t w = t.v[dt];
+                const uint32_t n[4] = {w << 4, w, w >> 4, w >> 8};
+                u4 va;
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    va[i] = as_u(__builtin_elementwise_fma(as_h2((n[i] & 0x00f000f0u) | 0x54005400u),
+                                                           as_h2(hw[i]), off[i]));
+                const h8 vv = __builtin_bit_cast(h8, va);
+                if constexpr (WIDE)
+                    o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vv, __builtin_bit_cast(h8, pb),
+                                                                   o[dt], 0, 0, 0);
+                o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vv, __builtin_bit_cast(h8, pa), o[dt],
+                                                               0, 0, 0);
+            }
+        }
+    };
+    while (s0 < p1) {
+        const int s1 = s0 + A4_STEP, s2 = s1 + A4_STEP;
+        if (s1 < p1) load(tb, s1);
+        step(ta, s0);
+        if (s1 >= p1) break;
+        if (s2 < p1) load(ta, s2);
+        step(tb, s1);
+        s0 = s2;
+    }
+    // the wavefronts' states meet in LDS
+    lsum += swap16_f(lsum);
+    lsum += swap32_f(lsum);
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) {
+        f4 v = o[dt];
+        if constexpr (!WIDE)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = ror8_add(v[i]);
+        if (col < per) *(f4 *)&mo[wave][col][16 * dt + 4 * g] = v * 16.0f;
+    }
+    if (g == 0 && col < per) {
+        mm[wave][col] = m;
+        ml[wave][col] = lsum;
+    }
     __syncthreads();
-    float m[16], l[16], o[16];  // o: dim tid of each head (tid < D)
-    for (int h = 0; h < 16; ++h) m[h] = -INFINITY, l[h] = o[h] = 0.0f;
-    for (int s0 = 0; s0 < ctx; s0 += 256) {
-        const int pos = s0 + tid;
-        float s[16];
-        for (int h = 0; h < 16; ++h) s[h] = 0.0f;
-        if (pos < ctx) {
-            const int i = pos & (page_size - 1);
-            const uint8_t *kp = c.k + ((size_t)c.page_of(seq, pos) * c.kvheads + g) * hb;
-            for (int b = 0; b < NB; ++b) {
-                const float d = h2f_fast(*(const uint16_t *)(kp + kv4_scale(D, page_size, i, b))) * 16.0f;
-                for (int gg = 0; gg < 4; ++gg) {
-                    const uint32_t w = *(const uint32_t *)(kp + kv4_k_dword(D, i, 4 * b + gg));
-                    for (int e = 0; e < 8; ++e) {
-                        const float x = (float)((int)(w >> (4 * e) & 15) - 8) * d;
-                        for (int h = 0; h < 16; ++h)
-                            if (h < per) s[h] = fmaf(x, ql[h * D + 32 * b + 8 * gg + e], s[h]);
-                    }
+    if (tid < per) {
+        const float M = fmaxf(fmaxf(mm[0][tid], mm[1][tid]), fmaxf(mm[2][tid], mm[3][tid]));
+        float l = 0.0f;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const float f = M == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mm[w][tid] - M);
+            sc[tid][w] = f;
+            l = fmaf(ml[w][tid], f, l);
+        }
+        if (ns > 1) {
+            const size_t pi = ((size_t)qi * qheads + g0 * per + tid) * ns + sp;
+            ws_m[pi] = M;
+            ws_l[pi] = l;
+        } else {
+            linv[tid] = M == -INFINITY ? 0.0f : 1.0f / l;
+        }
+    }
+    __syncthreads();
+    for (int e0 = 0; e0 < per * D / 4; e0 += 256) {  // 8 lanes hold a Q8_0 block
+        const int e4 = e0 + tid;
+        if (e4 >= per * D / 4) break;
+        const int h = e4 / (D / 4), dd = e4 % (D / 4) * 4;
+        f4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const f4 v = *(const f4 *)&mo[w][h][dd];
+            const float f = sc[h][w];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[i] = fmaf(v[i], f, acc[i]);
+        }
+        const int head = g0 * per + h;
+        if (ns > 1) {
+            *(f4 *)(ws_o + (((size_t)qi * qheads + head) * ns + sp) * D + dd) = acc;
+        } else {
+            const float r = linv[h], y[4] = {acc[0] * r, acc[1] * r, acc[2] * r, acc[3] * r};
+            const size_t off = ((size_t)qi * qheads + head) * D + dd;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) attn[off + i] = y[i];
+            if (qs) {
+                uint16_t dbits;
+                int sum;
+                const uint32_t w = quant_block_oct(y, dbits, sum);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) qs[off + i] = (int8_t)(w >> (8 * i));
+                if ((e4 & 7) == 0) {
+                    qd8[off / SI_QK] = dbits;
+                    if (bsum) bsum[off / SI_QK] = (int16_t)sum;
                 }
             }
         }
-        for (int h = 0; h < 16; ++h) {
-            if (h >= per) break;
-            const float t = pos < ctx ? s[h] * scale2 : -INFINITY;
-            float mx = wave_max(t);
-            __syncthreads();
-            if ((tid & 63) == 0) red[tid >> 6] = mx;
-            __syncthreads();
-            mx = fmaxf(fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])), m[h]);
-            const float ref = mx == -INFINITY ? 0.0f : mx;
-            const float al = __builtin_amdgcn_exp2f(m[h] - ref), pp = __builtin_amdgcn_exp2f(t - ref);
-            p[h][tid] = pp;
-            const float sum = wave_sum(pp);
-            __syncthreads();
-            if ((tid & 63) == 0) red[tid >> 6] = sum;
-            __syncthreads();
-            l[h] = l[h] * al + (red[0] + red[1] + red[2] + red[3]);
-            o[h] *= al;
-            m[h] = mx;
-        }
-        __syncthreads();
-        if (tid < D) {
-            const int n = min(ctx - s0, 256);
-            for (int j = 0; j < n; ++j) {
-                const int ps = s0 + j, i = ps & (page_size - 1);
-                const uint8_t *vp = c.v + ((size_t)c.page_of(seq, ps) * c.kvheads + g) * hb;
-                const uint32_t w = *(const uint32_t *)(vp + kv4_v_dword(D, i >> 3, tid));
-                const float d = h2f_fast(*(const uint16_t *)(vp + kv4_scale(D, page_size, i, tid >> 5))) * 16.0f;
-                const float x = (float)((int)(w >> (4 * (i & 7)) & 15) - 8) * d;
-                for (int h = 0; h < 16; ++h)
-                    if (h < per) o[h] = fmaf(p[h][j], x, o[h]);
-            }
-        }
-        __syncthreads();
     }
-    if (tid < D)
-        for (int h = 0; h < 16; ++h)
-            if (h < per)
-                attn[((size_t)qi * qheads + g * per + h) * D + tid] = ctx > 0 ? o[h] / l[h] : 0.0f;
 }
 
 // ---------------------------------------------------------------------------
@@ -413,19 +706,43 @@ void launch_kv4_read(const Kv4Cache &c, int ntok, int hdim, int pos0, int pos_st
 #undef CALL
 }
 
-size_t attn_kv4_workspace(int, int, int, int, int, int) { return 0; }
+// Chunks of the context: about 1024 workgroups, each of whole steps
+static int attn_kv4_chunks(int kvheads, int nq, int max_ctx) {
+    const int most = (max_ctx + A4_STEP - 1) / A4_STEP;
+    const int want = (int)((1024 + (long long)kvheads * nq - 1) / ((long long)kvheads * nq));
+    return max(1, min(min(most, want), 256));
+}
+
+// Whether a prompt's pages are read into fp16 rows for the prefill kernel
+static bool kv4_by_rows(int nq, int ctx_step) { return ctx_step == 1 && nq > 4; }
+
+size_t attn_kv4_workspace(int qheads, int kvheads, int hdim, int nq, int ctx_step, int max_ctx) {
+    if (kv4_by_rows(nq, ctx_step)) return (size_t)max_ctx * kvheads * hdim * 2 * sizeof(uint16_t);
+    const int ns = attn_kv4_chunks(kvheads, nq, max_ctx);
+    return ns == 1 ? 0 : (size_t)nq * qheads * ns * (hdim + 2) * sizeof(float);
+}
 
 void launch_attention_kv4(const float *q, int nq, int qheads, int hdim, const Kv4Cache &c,
                           const int *ctx_dev, int ctx0, int ctx_step, int max_ctx, float *attn,
-                          int8_t *qs, uint16_t *d, int16_t *bsum, void *, size_t,
-                          hipStream_t st) {
+                          int8_t *qs, uint16_t *d, int16_t *bsum, void *ws, hipStream_t st) {
     if (nq <= 0) return;
-#define CALL(DIM)                                                                              \
-    SI_LAUNCH((k_attn_kv4<DIM>), dim3(c.kvheads, nq), dim3(256), 0, st, q, qheads, c, ctx_dev, \
-              ctx0, ctx_step, max_ctx, softmax_scale2(hdim), attn)
+    if (kv4_by_rows(nq, ctx_step)) {
+        uint16_t *k = (uint16_t *)ws, *v = k + (size_t)max_ctx * c.kvheads * hdim;
+        launch_kv4_read(c, ctx0 - 1 + nq, hdim, 0, 1, nullptr, k, v, st);
+        launch_attn_prefill(q, nq, qheads, c.kvheads, hdim, ctx0 - 1, k, v, attn, qs, d, bsum, st);
+        return;
+    }
+    const int ns = attn_kv4_chunks(c.kvheads, nq, max_ctx);
+    const int chunk = ((max_ctx + ns - 1) / ns + A4_STEP - 1) / A4_STEP * A4_STEP;
+    const AttnParts pt(ws, (size_t)nq * qheads * ns, hdim);
+    const dim3 grid(ns, c.kvheads, nq);
+    const bool wide = qheads / c.kvheads > 8, page16 = c.shift == 4;
+#define CALL2(DIM, W, P)                                                                            SI_LAUNCH((k_attn_kv4<DIM, W, P>), grid, dim3(256), 0, st, q, qheads, c, ctx_dev, ctx0,                   ctx_step, max_ctx, chunk, softmax_scale2(hdim), pt.m, pt.l, pt.o, attn, qs, d, bsum)
+#define CALL(DIM)                                              if (wide && page16) CALL2(DIM, true, true);                else if (wide) CALL2(DIM, true, false);                    else if (page16) CALL2(DIM, false, true);                  else CALL2(DIM, false, false)
     KV4_DIM(hdim, CALL)
 #undef CALL
-    if (qs) launch_quantize_q8_rows(attn, nq, qheads * hdim, qs, d, bsum, st);
+#undef CALL2
+    if (ns > 1) launch_attn_combine(nq, qheads, hdim, ns, ws, attn, qs, d, bsum, st);
 }
 
 void launch_kv_copy(const KvMoves &mv, int npools, int nmoves, size_t page_bytes, bool wide,
