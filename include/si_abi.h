@@ -373,8 +373,8 @@ size_t si_attention_group_workspace(const si_shape_t *s, int nheads, int context
  * (a power of two in 16..65536) of every KV head, si_kv4_page_bytes(s,
  * page_size) bytes a page (9/32 of an fp16 page; the layout is the library's),
  * pools 16-byte aligned.  pages (device int [sequences][max_pages]) lists each
- * sequence's pages; ids outside [0, npages) are clamped.  A cache that is not
- * paged is one whose lists are consecutive.  Of the shape only qheads, kvheads
+ * sequence's pages, at most 2^30 positions; ids outside [0, npages) are
+ * clamped.  A cache that is not paged is one whose lists are consecutive.  Of the shape only qheads, kvheads
  * and hdim are read.
  *
  * Rows are addressed in one of two ways:

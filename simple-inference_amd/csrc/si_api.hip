@@ -1646,8 +1646,8 @@ static int kv4_cache(const char *what, const si_shape_t *s, const uint8_t *k, co
     SI_REQUIRE(kv4_page_ok(page_size), "%s: page_size %d must be a power of two in 16..65536",
                what, page_size);
     SI_REQUIRE(npages >= 1 && max_pages >= 1, "%s: npages and max_pages must be >= 1", what);
-    SI_REQUIRE((long long)max_pages * page_size <= INT32_MAX, "%s: %d pages of %d a sequence",
-               what, max_pages, page_size);
+    SI_REQUIRE((long long)max_pages * page_size <= (1 << 30),
+               "%s: %d pages of %d a sequence exceed 2^30 positions", what, max_pages, page_size);
     c->k = const_cast<uint8_t *>(k);
     c->v = const_cast<uint8_t *>(v);
     c->pages = pages;

@@ -111,12 +111,14 @@ struct Kv4Unit {
             lo = max(-t0, 0);
             hi = min(min(ntok - t0, limit - base), 8);
         } else {
-            const int pos = ctx_dev ? ctx_dev[x] - 1 : pos0;
+            const int ctx = ctx_dev ? ctx_dev[x] : pos0 + 1;
+            const bool live = ctx >= 1 && ctx <= limit;  // device contexts: not host-checked
+            const int pos = live ? ctx - 1 : 0;
             seq = x;
             base = pos & ~7;
             lo = pos & 7;
             t0 = x - lo;
-            hi = pos >= 0 && pos < limit ? lo + 1 : lo;  // device contexts: not host-checked
+            hi = live ? lo + 1 : lo;
         }
     }
 };
@@ -327,17 +329,21 @@ __device__ __forceinline__ void load_dwords(const uint8_t *p, uint32_t (&w)[N]) 
 }
 
 // What a wavefront reads of a group: lane (col, g)'s K nibbles of both tiles, V
-// nibbles, and the scales of positions 8 g .. 8 g + 7.
+// nibbles, and dword col of the D / 8 dwords that hold the scales of positions
+// 8 g .. 8 g + 7: all 16 lanes of a row need them all, and take them with a DPP
+// broadcast in the row where they are used.
 template <int D>
 struct Kv4Group {
     static constexpr int KS = D / 32, DT = D / 16;
-    uint32_t k[2][KS], v[DT];
-    uint4 kh[KS], vh[KS];
-    // kp, vp: of the KV head's part of the page that holds the lane's K row's and
-    // V positions' units; ku, vu: those units' places in it
+    uint32_t k[2][KS], v[DT], kh, vh;
+    // kk, ks, vv: the KV head's part of the page with the K row's, the K scales'
+    // and the V positions' unit; ku, vu: the units' places in it
     __device__ __forceinline__ void load(const uint8_t *kk, int ku, const uint8_t *ks,
                                          const uint8_t *vv, int vu, int nib, int lane) {
         const int r = lane & 15, g = lane >> 4;
+        const int so = nib + vu * KS * 16 + min(r, 4 * KS - 1) * 4;
+        kh = *(const uint32_t *)(ks + so);
+        vh = *(const uint32_t *)(vv + so);
 #pragma unroll
         for (int t = 0; t < 2; ++t)
             load_dwords<KS>(kk + ku * 4 * D + t * 2 * D + g * (D / 2) + (r & 3) * (D / 8), k[t]);
@@ -354,13 +360,23 @@ struct Kv4Group {
             load_dwords<2>(vv + vu * 4 * D + FULL * 256 + r * 8, w);
             v[DT - 2] = w[0], v[DT - 1] = w[1];
         }
-#pragma unroll
-        for (int b = 0; b < KS; ++b) {
-            kh[b] = *(const uint4 *)(ks + nib + (vu * KS + b) * 16);
-            vh[b] = *(const uint4 *)(vv + nib + (vu * KS + b) * 16);
-        }
     }
 };
+
+// lane N of each row of 16 lanes (row_newbcast)
+template <int N>
+__device__ __forceinline__ uint32_t row_bcast(uint32_t v) {
+    return (uint32_t)dpp_i<0x150 + N>((int)v);
+}
+
+// the row's dwords 4 b + i as h[b][i]
+template <int KS>
+__device__ __forceinline__ void spread(uint32_t v, u4 (&h)[KS]) {
+    h[0] = (u4){row_bcast<0>(v), row_bcast<1>(v), row_bcast<2>(v), row_bcast<3>(v)};
+    if constexpr (KS > 1) h[1] = (u4){row_bcast<4>(v), row_bcast<5>(v), row_bcast<6>(v), row_bcast<7>(v)};
+    if constexpr (KS > 2) h[2] = (u4){row_bcast<8>(v), row_bcast<9>(v), row_bcast<10>(v), row_bcast<11>(v)};
+    if constexpr (KS > 3) h[3] = (u4){row_bcast<12>(v), row_bcast<13>(v), row_bcast<14>(v), row_bcast<15>(v)};
+}
 
 __device__ __forceinline__ h2 as_h2(uint32_t u) { return __builtin_bit_cast(h2, u); }
 __device__ __forceinline__ uint32_t as_u(h2 h) { return __builtin_bit_cast(uint32_t, h); }
@@ -400,25 +416,34 @@ __global__ void __launch_bounds__(256, 2) k_attn_kv4(
     const int page_size = 1 << c.shift, nib = page_size * (D / 2);
     const size_t hb = (size_t)kv4_head_bytes(D, page_size);
     const int *pages = c.pages + (size_t)seq * c.max_pages;
-    auto head_at = [&](int pos) {  // of the page holding pos (uniform)
-        const int pg = pages[min(pos >> c.shift, c.max_pages - 1)];
+    // The page ids are read a step before the loads that need them.
+    struct Ids { int a, b; };
+    auto ids_of = [&](int s0) {  // (uniform)
+        Ids i;
+        i.a = pages[min(s0 >> c.shift, c.max_pages - 1)];
+        i.b = PAGE16 ? pages[min((s0 >> c.shift) + 1, c.max_pages - 1)] : 0;
+        return i;
+    };
+    auto head_at = [&](int pg) {
         return ((size_t)min(max(pg, 0), c.npages - 1) * c.kvheads + g0) * hb;
     };
-    auto load = [&](Kv4Group<D> &t, int s0) {
+    auto load = [&](Kv4Group<D> &t, int s0, Ids id) {
+        const size_t a = head_at(id.a);
         if constexpr (PAGE16) {
             // two pages a group: units 0, 1 and 2, 3
-            const size_t a = head_at(s0), b = head_at(s0 + 16);
+            const size_t b = head_at(id.b);
             const size_t ka = (lane & 8) ? b : a, va = (lane & 32) ? b : a;
             t.load(c.k + ka, (lane >> 2) & 1, c.k + va, c.v + va, g & 1, nib, lane);
         } else {
-            const size_t a = head_at(s0);
             const int u = (s0 & (page_size - 1)) >> 3;
             t.load(c.k + a, u + ((lane >> 2) & 3), c.k + a, c.v + a, u + g, nib, lane);
         }
     };
     int s0 = p0 + A4_GROUP * wave;
     Kv4Group<D> ta, tb;
-    if (s0 < p1) load(ta, s0);
+    Ids id = ids_of(s0);
+    if (s0 < p1) load(ta, s0, id);
+    id = ids_of(s0 + A4_STEP);
 
     // q of the lane's column as the B operand, dims 32 b + 8 g + (0, 4, 1, 5, 2, 6,
     // 3, 7), the odd ones over 16: integers hi and lo, q = (hi + lo 2^-12) 2^(ex - 10)
@@ -480,6 +505,8 @@ __global__ void __launch_bounds__(256, 2) k_attn_kv4(
 
     auto step = [&](Kv4Group<D> &t, int s) {
         float p[2][4];
+        u4 hk[KS];
+        spread<KS>(t.kh, hk);
 #pragma unroll
         for (int tl = 0; tl < 2; ++tl) {
             f4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -495,9 +522,8 @@ __global__ void __launch_bounds__(256, 2) k_attn_kv4(
 #pragma unroll
                     for (int i = 0; i < 4; ++i) d[i] = fmaf(dl[i], 0x1p-12f, d[i]);
                 }
-                const uint32_t hw[4] = {t.kh[b].x, t.kh[b].y, t.kh[b].z, t.kh[b].w};
 #pragma unroll
-                for (int i = 0; i < 4; ++i) acc[i] = fmaf((float)as_h2(hw[i])[tl], d[i], acc[i]);
+                for (int i = 0; i < 4; ++i) acc[i] = fmaf((float)as_h2(hk[b][i])[tl], d[i], acc[i]);
             }
 #pragma unroll
             for (int i = 0; i < 4; ++i) p[tl][i] = WIDE ? acc[i] * fac : ror8_add(acc[i] * fac);
@@ -508,11 +534,11 @@ __global__ void __launch_bounds__(256, 2) k_attn_kv4(
                 const bool l0 = s + 8 * g + i < p1, l1 = s + 8 * g + 4 + i < p1;
                 p[0][i] = l0 ? p[0][i] : -INFINITY;
                 p[1][i] = l1 ? p[1][i] : -INFINITY;
-                // their V scales may be anything: 0 (weight 0 * NaN would stay)
-                const uint32_t mask = (l0 ? 0xffffu : 0u) | (l1 ? 0xffff0000u : 0u);
-#pragma unroll
-                for (int b = 0; b < KS; ++b) (&t.vh[b].x)[i] &= mask;
             }
+            // their V scales may be anything: 0 (weight 0 * NaN would stay); dword col
+            // holds positions 8 g + col % 4 and 4 further
+            const int at = s + 8 * g + (col & 3);
+            t.vh &= (at < p1 ? 0xffffu : 0u) | (at + 4 < p1 ? 0xffff0000u : 0u);
         }
         float mx = fmaxf(fmaxf(fmaxf(p[0][0], p[0][1]), fmaxf(p[0][2], p[0][3])),
                          fmaxf(fmaxf(p[1][0], p[1][1]), fmaxf(p[1][2], p[1][3])));
@@ -541,9 +567,11 @@ __global__ void __launch_bounds__(256, 2) k_attn_kv4(
                 pa[i] = as_u((h2){(_Float16)xr, (_Float16)yr});
             }
         }
+        u4 hv[KS];
+        spread<KS>(t.vh, hv);
 #pragma unroll
         for (int b = 0; b < KS; ++b) {
-            const uint32_t hw[4] = {t.vh[b].x, t.vh[b].y, t.vh[b].z, t.vh[b].w};
+            const u4 hw = hv[b];
             h2 off[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) off[i] = as_h2(hw[i]) * (h2){(_Float16)-72.0f, (_Float16)-72.0f};
@@ -567,10 +595,12 @@ __global__ void __launch_bounds__(256, 2) k_attn_kv4(
     };
     while (s0 < p1) {
         const int s1 = s0 + A4_STEP, s2 = s1 + A4_STEP;
-        if (s1 < p1) load(tb, s1);
+        if (s1 < p1) load(tb, s1, id);
+        id = ids_of(s2);
         step(ta, s0);
         if (s1 >= p1) break;
-        if (s2 < p1) load(ta, s2);
+        if (s2 < p1) load(ta, s2, id);
+        id = ids_of(s2 + A4_STEP);
         step(tb, s1);
         s0 = s2;
     }
