@@ -351,7 +351,8 @@ void launch_kv4_read(const Kv4Cache &c, int ntok, int hdim, int pos0, int pos_st
 size_t attn_kv4_workspace(int qheads, int kvheads, int hdim, int nq, int ctx_step, int max_ctx);
 void launch_attention_kv4(const float *q, int nq, int qheads, int hdim, const Kv4Cache &c,
                           const int *ctx_dev, int ctx0, int ctx_step, int max_ctx, float *attn,
-                          int8_t *qs, uint16_t *d, int16_t *bsum, void *workspace, hipStream_t st);
+                          int8_t *qs, uint16_t *d, int16_t *bsum, void *workspace, hipStream_t st,
+                          int8_t *tq = nullptr, uint16_t *td = nullptr);
 // One launch's page copies, in the kernel's arguments.
 struct KvMoves {
     static constexpr int POOLS = 64, MOVES = 384;

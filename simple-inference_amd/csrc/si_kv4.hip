@@ -311,111 +311,217 @@ constexpr int A4_STEP = 4 * A4_GROUP;    // of a workgroup's
 
 __device__ __forceinline__ float ror8_add(float v) { return v + dpp_f<DPP_ROR8>(v); }
 
-// N dwords at p, aligned to what N allows
-template <int N>
-__device__ __forceinline__ void load_dwords(const uint8_t *p, uint32_t (&w)[N]) {
-    if constexpr (N == 1) {
-        w[0] = *(const uint32_t *)p;
-    } else if constexpr (N == 2) {
-        const uint2 t = *(const uint2 *)p;
-        w[0] = t.x, w[1] = t.y;
-    } else if constexpr (N == 3) {
-        const uint3 t = *(const uint3 *)p;
-        w[0] = t.x, w[1] = t.y, w[2] = t.z;
-    } else {
-        const uint4 t = *(const uint4 *)p;
-        w[0] = t.x, w[1] = t.y, w[2] = t.z, w[3] = t.w;
-    }
-}
-
-// What a wavefront reads of a group: lane (col, g)'s K nibbles of both tiles, V
-// nibbles, and dword col of the D / 8 dwords that hold the scales of positions
-// 8 g .. 8 g + 7: all 16 lanes of a row need them all, and take them with a DPP
-// broadcast in the row where they are used.
-template <int D>
-struct Kv4Group {
-    static constexpr int KS = D / 32, DT = D / 16;
-    uint32_t k[2][KS], v[DT], kh, vh;
-    // kk, ks, vv: the KV head's part of the page with the K row's, the K scales'
-    // and the V positions' unit; ku, vu: the units' places in it
-    __device__ __forceinline__ void load(const uint8_t *kk, int ku, const uint8_t *ks,
-                                         const uint8_t *vv, int vu, int nib, int lane) {
-        const int r = lane & 15, g = lane >> 4;
-        const int so = nib + vu * KS * 16 + min(r, 4 * KS - 1) * 4;
-        kh = *(const uint32_t *)(ks + so);
-        vh = *(const uint32_t *)(vv + so);
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-            load_dwords<KS>(kk + ku * 4 * D + t * 2 * D + g * (D / 2) + (r & 3) * (D / 8), k[t]);
-        constexpr int FULL = D / 64;
-#pragma unroll
-        for (int f = 0; f < FULL; ++f) {
-            uint32_t w[4];
-            load_dwords<4>(vv + vu * 4 * D + f * 256 + r * 16, w);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[4 * f + e] = w[e];
+// Where a wavefront reads: one page's part of a KV head, as a buffer descriptor
+// (the group's place in it is the load's scalar offset, so a step computes no
+// addresses in vector registers, and nothing past the page is touched), or, for
+// pages of half a group, the lane's own address.
+struct Kv4InPage {
+    __amdgpu_buffer_rsrc_t r;
+    int at;
+    template <int N>
+    __device__ __forceinline__ void load(int off, uint32_t *w) const {
+        if constexpr (N == 1) {
+            w[0] = __builtin_amdgcn_raw_buffer_load_b32(r, off, at, 0);
+        } else if constexpr (N == 2) {
+            const auto t = __builtin_amdgcn_raw_buffer_load_b64(r, off, at, 0);
+            w[0] = t[0], w[1] = t[1];
+        } else if constexpr (N == 3) {
+            const auto t = __builtin_amdgcn_raw_buffer_load_b96(r, off, at, 0);
+            w[0] = t[0], w[1] = t[1], w[2] = t[2];
+        } else {
+            const auto t = __builtin_amdgcn_raw_buffer_load_b128(r, off, at, 0);
+            w[0] = t[0], w[1] = t[1], w[2] = t[2], w[3] = t[3];
         }
-        if constexpr (DT % 4) {
-            uint32_t w[2];
-            load_dwords<2>(vv + vu * 4 * D + FULL * 256 + r * 8, w);
-            v[DT - 2] = w[0], v[DT - 1] = w[1];
+    }
+};
+struct Kv4InHalf {
+    const uint8_t *p;
+    template <int N>
+    __device__ __forceinline__ void load(int off, uint32_t *w) const {
+        if constexpr (N == 1) {
+            w[0] = *(const uint32_t *)(p + off);
+        } else if constexpr (N == 2) {
+            const uint2 t = *(const uint2 *)(p + off);
+            w[0] = t.x, w[1] = t.y;
+        } else if constexpr (N == 3) {
+            const uint3 t = *(const uint3 *)(p + off);
+            w[0] = t.x, w[1] = t.y, w[2] = t.z;
+        } else {
+            const uint4 t = *(const uint4 *)(p + off);
+            w[0] = t.x, w[1] = t.y, w[2] = t.z, w[3] = t.w;
         }
     }
 };
 
-// lane N of each row of 16 lanes (row_newbcast)
-template <int N>
-__device__ __forceinline__ uint32_t row_bcast(uint32_t v) {
-    return (uint32_t)dpp_i<0x150 + N>((int)v);
-}
-
-// the row's dwords 4 b + i as h[b][i]
-template <int KS>
-__device__ __forceinline__ void spread(uint32_t v, u4 (&h)[KS]) {
-    h[0] = (u4){row_bcast<0>(v), row_bcast<1>(v), row_bcast<2>(v), row_bcast<3>(v)};
-    if constexpr (KS > 1) h[1] = (u4){row_bcast<4>(v), row_bcast<5>(v), row_bcast<6>(v), row_bcast<7>(v)};
-    if constexpr (KS > 2) h[2] = (u4){row_bcast<8>(v), row_bcast<9>(v), row_bcast<10>(v), row_bcast<11>(v)};
-    if constexpr (KS > 3) h[3] = (u4){row_bcast<12>(v), row_bcast<13>(v), row_bcast<14>(v), row_bcast<15>(v)};
-}
+// What a wavefront reads of a group: lane (col, g)'s K nibbles of both tiles, V
+// nibbles, and dword col of the D / 8 dwords that hold the scales of positions
+// 8 g .. 8 g + 7: all 16 lanes of a row need them all, and read them from the
+// wavefront's own room in LDS (as DPP broadcasts they were 48 of a step's 275
+// vector operations, what bounds the kernel; loaded by every lane, 32 registers
+// and 8 of the 14 loads).
+template <int D>
+struct Kv4Group {
+    static constexpr int KS = D / 32, DT = D / 16;
+    uint32_t k[2][KS], v[DT], kh, vh;
+    // ku, vu: the places of the K row's and the V positions' unit
+    template <class P>
+    __device__ __forceinline__ void load(const P &kk, const P &ks, const P &vv, const P &vs,
+                                         int ku, int vu, int lane) {
+        const int r = lane & 15, g = lane >> 4;
+        const int so = vu * KS * 16 + min(r, 4 * KS - 1) * 4;
+        ks.template load<1>(so, &kh);
+        vs.template load<1>(so, &vh);
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+            kk.template load<KS>(ku * 4 * D + t * 2 * D + g * (D / 2) + (r & 3) * (D / 8), k[t]);
+        constexpr int FULL = D / 64;
+#pragma unroll
+        for (int f = 0; f < FULL; ++f)
+            vv.template load<4>(vu * 4 * D + f * 256 + r * 16, v + 4 * f);
+        if constexpr (DT % 4) vv.template load<2>(vu * 4 * D + FULL * 256 + r * 8, v + 4 * FULL);
+    }
+};
 
 __device__ __forceinline__ h2 as_h2(uint32_t u) { return __builtin_bit_cast(h2, u); }
 __device__ __forceinline__ uint32_t as_u(h2 h) { return __builtin_bit_cast(uint32_t, h); }
+__device__ __forceinline__ h8 to_h8(const float (&x)[8]) {
+    h8 y;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) y[e] = (_Float16)x[e];
+    return y;
+}
+
+// An oct's 32 outputs, 4 a lane (lane l8 at off), and their Q8_0; row qi of qd
+// values in the operand-tiled copy.
+__device__ __forceinline__ void kv4_store(const float (&y)[4], size_t off, int l8, float *attn,
+                                          int8_t *qs, uint16_t *d, int16_t *bsum, int8_t *tq,
+                                          uint16_t *td, int qd, int qi) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) attn[off + i] = y[i];
+    if (!qs) return;
+    uint16_t dbits;
+    int sum;
+    const uint32_t w = quant_block_oct(y, dbits, sum);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) qs[off + i] = (int8_t)(w >> (8 * i));
+    const size_t pb = (size_t)(qi >> 5) * (qd / SI_QK) + off % qd / SI_QK;
+    if (tq) *(uint32_t *)(tq + q8_tiled_byte(pb, qi & 31, 4 * l8)) = w;
+    if (l8 == 0) {
+        d[off / SI_QK] = dbits;
+        if (bsum) bsum[off / SI_QK] = (int16_t)sum;
+        if (tq) td[pb * 32 + (qi & 31)] = dbits;
+    }
+}
+
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ float uniform(float v) { return u2f((uint32_t)uniform((int)f2u(v))); }
+// inclusive sum over the wavefront's lanes before this one and its own
+__device__ __forceinline__ int wave_scan(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);  // row_shr:1, 2, 4, 8
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row_bcast:15, 31
+    return v + __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);
+}
+
+// Which chunk of which query a workgroup takes.
+struct A4Item {
+    int qi, sp, ctx, chunk, parts;  // parts: chunks of the query; ctx 0: nothing to do
+};
+// Contexts on the device: item w of the list of all queries' chunks, in order.
+// The chunk makes about `slots` of them in all, what the GPU holds at once, by
+// sum of ctx_i / chunk + half a chunk a query for the last ones (never over slots /
+// kvheads + nq, the launch), and the longest context's chunks equal; at most ns a
+// query.  (A grid of query x chunk instead, each workgroup past its context
+// leaving at once, kept the slots busy with those: 48 x 200-4096 24.8 us
+// against 21.3.)
+__device__ __forceinline__ A4Item a4_item(int w, const int *ctx_dev, int nq, int kvheads, int ns,
+                                          int max_ctx, int slots) {
+    const int lane = threadIdx.x & 63;
+    int most = 0, live = 0;
+    float total = 0.0f;
+    const int first = lane < nq ? max(min(ctx_dev[lane], max_ctx), 0) : 0;
+    for (int i = lane; i < nq; i += 64) {
+        const int n = i < 64 ? first : max(min(ctx_dev[i], max_ctx), 0);
+        most = max(most, n);
+        total += (float)n;
+        live += n > 0;
+    }
+    most = max(uniform(wave_max_i(most)), 1);
+    total = uniform(wave_sum(total));
+    const float n = uniform(wave_sum((float)live));
+    const float share = total / fmaxf((float)slots / (float)kvheads - 0.5f * n, 1.0f);
+    const int k = min((int)((float)most / fmaxf(share, (float)A4_STEP)), ns);
+    auto steps_of = [&](int k) { return ((most + k - 1) / k + A4_STEP - 1) / A4_STEP; };
+    auto parts_of = [](int ctx, int steps) {
+        return ((ctx + A4_STEP - 1) / A4_STEP + steps - 1) / steps;
+    };
+    int steps = steps_of(max(k, 1));
+    if (k < ns) {  // one chunk more where that still fits (equal contexts)
+        const int more = steps_of(k + 1);
+        int count = 0;
+        for (int i = lane; i < nq; i += 64)
+            count += parts_of(i < 64 ? first : max(min(ctx_dev[i], max_ctx), 0), more);
+        if (uniform(wave_sum((float)count)) * (float)kvheads <= (float)slots) steps = more;
+    }
+    A4Item it = {0, 0, 0, steps * A4_STEP, 0};
+    for (int i0 = 0; i0 < nq; i0 += 64) {
+        const int i = i0 + lane;
+        const int c = i >= nq ? 0 : i0 == 0 ? first : max(min(ctx_dev[i], max_ctx), 0);
+        const int parts = parts_of(c, steps);
+        const int upto = wave_scan(parts);
+        const unsigned long long past = __ballot(upto > w);
+        if (past) {
+            const int l = uniform((int)__builtin_ctzll(past));
+            it.qi = i0 + l;
+            it.ctx = __builtin_amdgcn_readlane(c, l);
+            it.parts = __builtin_amdgcn_readlane(parts, l);
+            it.sp = w - (__builtin_amdgcn_readlane(upto, l) - it.parts);
+            break;
+        }
+        w -= __builtin_amdgcn_readlane(upto, 63);
+    }
+    return it;
+}
 
 template <int D, bool WIDE, bool PAGE16>
-__global__ void __launch_bounds__(256, 2) k_attn_kv4(
+__global__ void __launch_bounds__(256, WIDE ? 2 : 3) k_attn_kv4(
     const float *__restrict__ q, int qheads, Kv4Cache c, const int *__restrict__ ctx_dev, int ctx0,
-    int ctx_step, int max_ctx, int chunk, float scale2, float *__restrict__ ws_m,
+    int ctx_step, int nq, int max_ctx, int ns, int chunk, int slots, float scale2,
+    int *__restrict__ parts, float *__restrict__ ws_m,
     float *__restrict__ ws_l, float *__restrict__ ws_o, float *__restrict__ attn,
-    int8_t *__restrict__ qs, uint16_t *__restrict__ qd8, int16_t *__restrict__ bsum) {
+    int8_t *__restrict__ qs, uint16_t *__restrict__ qd8, int16_t *__restrict__ bsum,
+    int8_t *__restrict__ tq, uint16_t *__restrict__ td) {
     constexpr int KS = D / 32, DT = D / 16, COLS = WIDE ? 16 : 8;
     __shared__ __attribute__((aligned(16))) float mo[4][COLS][D];
+    __shared__ __attribute__((aligned(16))) u4 qop[(WIDE ? 2 : 1) * KS * 64];  // hi (, lo)
+    __shared__ __attribute__((aligned(16))) f4 qc[(WIDE ? 2 : 1) * KS * 64];
+    __shared__ __attribute__((aligned(16))) uint32_t scales[4][3][64];  // K's, V's, V's * -72
     __shared__ float mm[4][COLS], ml[4][COLS], sc[COLS][4], linv[COLS];
-    const int sp = blockIdx.x, g0 = blockIdx.y, qi = blockIdx.z, ns = gridDim.x;
+    const int g0 = blockIdx.x, per = qheads / c.kvheads;
     const int tid = threadIdx.x, lane = tid & 63;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wave = uniform(tid >> 6);
     const int col = lane & 15, g = lane >> 4;
-    const int per = qheads / c.kvheads, seq = ctx_step ? 0 : qi;
-    const int ctx = min(ctx_dev ? ctx_dev[qi] : ctx0 + qi * ctx_step, max_ctx);
-    if (ns > 1 && ctx_dev) {
-        // shares of the longest context there is
-        int most = 0;
-        for (int i = lane; i < (int)gridDim.z; i += 64) most = max(most, ctx_dev[i]);
-        most = min(__builtin_amdgcn_readfirstlane(wave_max_i(most)), max_ctx);
-        chunk = max(((most + ns - 1) / ns + A4_STEP - 1) / A4_STEP, 1) * A4_STEP;
+    A4Item it;
+    if (parts) {
+        it = a4_item(blockIdx.y, ctx_dev, nq, c.kvheads, ns, max_ctx, slots);
+        if (it.ctx == 0) return;  // past the list
+        if (g0 == 0 && it.sp == 0 && tid == 0) parts[it.qi] = it.parts;
+    } else {
+        it.qi = blockIdx.y;
+        it.sp = blockIdx.z;
+        it.ctx = min(ctx_dev ? ctx_dev[it.qi] : ctx0 + it.qi * ctx_step, max_ctx);
+        it.chunk = chunk;
     }
-    const int p0 = sp * chunk, p1 = min(ctx, p0 + chunk);
-    if (ns > 1 && p0 >= p1) {  // an empty state
-        for (int h = tid; h < per; h += 256) {
-            const size_t pi = ((size_t)qi * qheads + g0 * per + h) * ns + sp;
-            ws_m[pi] = -INFINITY;
-            ws_l[pi] = 0.0f;
-        }
-        return;
-    }
+    const int qi = uniform(it.qi), sp = uniform(it.sp), seq = ctx_step ? 0 : qi;
+    const int p0 = uniform(sp * it.chunk), p1 = uniform(min(it.ctx, p0 + it.chunk));
     // groups of this wavefront: s0 = p0 + 32 wave, + 128, ...
     const int page_size = 1 << c.shift, nib = page_size * (D / 2);
     const size_t hb = (size_t)kv4_head_bytes(D, page_size);
-    const int *pages = c.pages + (size_t)seq * c.max_pages;
+    // (constant memory: scalar loads, which the vector loads' order does not wait for)
+    typedef const __attribute__((address_space(4))) int *const_ints;
+    const const_ints pages = (const_ints)(uintptr_t)(c.pages + (size_t)seq * c.max_pages);
     // The page ids are read a step before the loads that need them.
     struct Ids { int a, b; };
     auto ids_of = [&](int s0) {  // (uniform)
@@ -433,148 +539,192 @@ __global__ void __launch_bounds__(256, 2) k_attn_kv4(
             // two pages a group: units 0, 1 and 2, 3
             const size_t b = head_at(id.b);
             const size_t ka = (lane & 8) ? b : a, va = (lane & 32) ? b : a;
-            t.load(c.k + ka, (lane >> 2) & 1, c.k + va, c.v + va, g & 1, nib, lane);
+            t.load(Kv4InHalf{c.k + ka}, Kv4InHalf{c.k + va + nib}, Kv4InHalf{c.v + va},
+                   Kv4InHalf{c.v + va + nib}, (lane >> 2) & 1, g & 1, lane);
         } else {
-            const int u = (s0 & (page_size - 1)) >> 3;
-            t.load(c.k + a, u + ((lane >> 2) & 3), c.k + a, c.v + a, u + g, nib, lane);
+            const int u = (s0 & (page_size - 1)) >> 3, sc = nib + u * KS * 16;
+            const auto rk = buf_rsrc(c.k + a, (uint32_t)hb), rv = buf_rsrc(c.v + a, (uint32_t)hb);
+            t.load(Kv4InPage{rk, u * 4 * D}, Kv4InPage{rk, sc}, Kv4InPage{rv, u * 4 * D},
+                   Kv4InPage{rv, sc}, (lane >> 2) & 3, g, lane);
         }
     };
     int s0 = p0 + A4_GROUP * wave;
     Kv4Group<D> ta, tb;
-    Ids id = ids_of(s0);
-    if (s0 < p1) load(ta, s0, id);
-    id = ids_of(s0 + A4_STEP);
+    {
+        const Ids ia = ids_of(s0), ib = ids_of(s0 + A4_STEP);
+        if (s0 < p1) load(ta, s0, ia);
+        if (s0 + A4_STEP < p1) load(tb, s0 + A4_STEP, ib);
+    }
+    Ids id = ids_of(s0 + 2 * A4_STEP);
 
     // q of the lane's column as the B operand, dims 32 b + 8 g + (0, 4, 1, 5, 2, 6,
     // 3, 7), the odd ones over 16: integers hi and lo, q = (hi + lo 2^-12) 2^(ex - 10)
-    h8 qa[KS], qb[WIDE ? KS : 1];
-    f4 c8[KS], c8l[WIDE ? KS : 1];
+    // (lo 2^-12 is the operand: a 12-bit integer over 2^16 is an fp16 value).
+    // Wavefront b makes block b for all of them (each making all took 370
+    // operations of a wavefront's 250 a step); the operands and -8 sum q stay in LDS
+    // and are read again in each step (kept in registers they are 32 of them, the
+    // difference between three wavefronts a SIMD and two).
     float fac;
-    const float lo_col = !WIDE && col >= 8 ? 1.0f : 0.0f;
+    const bool lo_half = !WIDE && col >= 8;
+    const float lo_col = lo_half ? 1.0f : 0.0f;
     {
+        float *qmax = &mo[0][0][0];  // [KS][64]
         const int hc = WIDE ? col : col & 7;
-        const bool live = hc < per;
-        const float *row = q + ((size_t)qi * qheads + g0 * per + (live ? hc : 0)) * D + 8 * g;
-        float x[KS][8], big = 0.0f;
+        float x[8];
+        if (wave < KS) {
+            const float *row = q + ((size_t)qi * qheads + g0 * per + min(hc, per - 1)) * D +
+                               32 * wave + 8 * g;
+            float big = 0.0f;
 #pragma unroll
-        for (int b = 0; b < KS; ++b)
+            for (int e = 0; e < 8; ++e) x[e] = row[e];
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                x[b][e] = live ? row[32 * b + e] : 0.0f;
-                big = fmaxf(big, fabsf(x[b][e]));
+                x[e] = hc < per ? x[e] : 0.0f;
+                big = fmaxf(big, fabsf(x[e]));
             }
+            qmax[wave * 64 + lane] = big;
+        }
+        __syncthreads();
+        float big = 0.0f;
+#pragma unroll
+        for (int b = 0; b < KS; ++b) big = fmaxf(big, qmax[b * 64 + lane]);
         big = fmaxf(big, swap16_f(big));
         big = fmaxf(big, swap32_f(big));
         const int ex = big == 0.0f ? 0 : (int)(f2u(big) >> 23) - 127;
         // the scores' units: 2^24 of the subnormals, 16 of the scale, q's
-        fac = __builtin_amdgcn_ldexpf(scale2, 28 + ex - 10 - (!WIDE && col >= 8 ? 12 : 0));
-        const u4 eight = {0x80088008u, 0x80808080u, 0x80088008u, 0x80808080u};  // -8 in them
-#pragma unroll
-        for (int b = 0; b < KS; ++b) {
-            h8 hi, lo;
+        fac = __builtin_amdgcn_ldexpf(scale2, 28 + ex - 10);
+        if (wave < KS) {
+            float hi[8], lo[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 const int dim = (e >> 1) + (e & 1) * 4;
-                const float y = __builtin_amdgcn_ldexpf(x[b][dim], 10 - ex), yh = rintf(y);
+                const float y = __builtin_amdgcn_ldexpf(x[dim], 10 - ex);
                 const float odd = (dim & 1) ? 0.0625f : 1.0f;
-                hi[e] = (_Float16)(yh * odd);
-                lo[e] = (_Float16)(rintf((y - yh) * 4096.0f) * odd);
+                hi[e] = rintf(y) * odd;
+                lo[e] = rintf((y - rintf(y)) * 4096.0f) * (odd * 0x1p-12f);
+                if (!WIDE) hi[e] = lo_half ? lo[e] : hi[e];
             }
-            c8[b] = (f4){0.0f, 0.0f, 0.0f, 0.0f};
-            if constexpr (WIDE) {
-                qa[b] = hi;
-                qb[b] = lo;
-                c8l[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, eight), lo,
-                                                                c8[b], 0, 0, 0);
-            } else {
-                const u4 uh = __builtin_bit_cast(u4, hi), ul = __builtin_bit_cast(u4, lo);
-                u4 us;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) us[e] = col >= 8 ? ul[e] : uh[e];
-                qa[b] = __builtin_bit_cast(h8, us);
-            }
-            c8[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, eight), qa[b],
-                                                           c8[b], 0, 0, 0);
+            qop[wave * 64 + lane] = __builtin_bit_cast(u4, to_h8(hi));
+            if constexpr (WIDE) qop[(KS + wave) * 64 + lane] = __builtin_bit_cast(u4, to_h8(lo));
         }
+        const u4 eight = {0x80088008u, 0x80808080u, 0x80088008u, 0x80808080u};  // -8 in K's units
+        if (wave < KS) {
+#pragma unroll
+            for (int w = 0; w < (WIDE ? 2 : 1); ++w) {
+                const h8 x8 = __builtin_bit_cast(h8, qop[(w * KS + wave) * 64 + lane]);
+                qc[(w * KS + wave) * 64 + lane] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                    __builtin_bit_cast(h8, eight), x8, (f4){0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
+            }
+        }
+        __syncthreads();
     }
-
-    float m = -INFINITY, lsum = 0.0f;  // of the column; lsum over the lane's positions
-    f4 o[DT];
+    // The running maximum m and its limit lim in the scores' raw units; in powers
+    // of two m is mf = m fac.  The sums of the weights are one more product's rows
+    // (ones . P), like the outputs in hi and lo columns.
+    const float over = 8.0f * __builtin_amdgcn_rcpf(fac);
+    float m = -INFINITY, mf = -INFINITY, lim = -INFINITY;
+    f4 o[DT], ol = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) o[dt] = (f4){0.0f, 0.0f, 0.0f, 0.0f};
+    // constants held in registers, so that (n & mask) | magic is one operation
+    uint32_t mask = 0x00f000f0u, magic = 0x54005400u;
+    asm("" : "+s"(mask));
+    asm("" : "+v"(magic));
 
     auto step = [&](Kv4Group<D> &t, int s) {
         float p[2][4];
-        u4 hk[KS];
-        spread<KS>(t.kh, hk);
-#pragma unroll
-        for (int tl = 0; tl < 2; ++tl) {
-            f4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-            for (int b = 0; b < KS; ++b) {
-                const uint32_t w = t.k[tl][b], w8 = w >> 8;
-                const u4 a = {w & 0x000f000fu, w & 0x00f000f0u, w8 & 0x000f000fu, w8 & 0x00f000f0u};
-                const h8 ka = __builtin_bit_cast(h8, a);
-                f4 d = c8[b];
-                d = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, qa[b], d, 0, 0, 0);
-                if constexpr (WIDE) {
-                    const f4 dl = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, qb[b], c8l[b], 0, 0, 0);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) d[i] = fmaf(dl[i], 0x1p-12f, d[i]);
-                }
-#pragma unroll
-                for (int i = 0; i < 4; ++i) acc[i] = fmaf((float)as_h2(hk[b][i])[tl], d[i], acc[i]);
-            }
-#pragma unroll
-            for (int i = 0; i < 4; ++i) p[tl][i] = WIDE ? acc[i] * fac : ror8_add(acc[i] * fac);
-        }
-        if (s + A4_GROUP > p1) {  // wavefront-uniform: positions past the end
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const bool l0 = s + 8 * g + i < p1, l1 = s + 8 * g + 4 + i < p1;
-                p[0][i] = l0 ? p[0][i] : -INFINITY;
-                p[1][i] = l1 ? p[1][i] : -INFINITY;
-            }
+        f4 d[2][KS];
+        // lane (col, g)'s dword to [g][col]; a wavefront's LDS operations keep their
+        // order, the compiler is to keep it too (and to read q here, not before the
+        // loop)
+        uint32_t (*const sl)[64] = scales[wave];
+        const bool tail = s + A4_GROUP > p1;  // wavefront-uniform: positions past the end
+        if (tail) {
             // their V scales may be anything: 0 (weight 0 * NaN would stay); dword col
             // holds positions 8 g + col % 4 and 4 further
             const int at = s + 8 * g + (col & 3);
             t.vh &= (at < p1 ? 0xffffu : 0u) | (at + 4 < p1 ? 0xffff0000u : 0u);
         }
+        asm volatile("" ::: "memory");
+        sl[0][lane] = t.kh;
+        sl[1][lane] = t.vh;
+        sl[2][lane] = as_u(as_h2(t.vh) * (h2){(_Float16)-72.0f, (_Float16)-72.0f});
+        asm volatile("" ::: "memory");
+#pragma unroll
+        for (int b = 0; b < KS; ++b) {
+            const h8 qa = __builtin_bit_cast(h8, qop[b * 64 + lane]);
+            const f4 c8 = qc[b * 64 + lane];
+#pragma unroll
+            for (int tl = 0; tl < 2; ++tl) {
+                const uint32_t w = t.k[tl][b], w8 = w >> 8;
+                const u4 a = {w & 0x000f000fu, w & 0x00f000f0u, w8 & 0x000f000fu, w8 & 0x00f000f0u};
+                const h8 ka = __builtin_bit_cast(h8, a);
+                d[tl][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, qa, c8, 0, 0, 0);
+                if constexpr (WIDE)
+                    d[tl][b] += __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                        ka, __builtin_bit_cast(h8, qop[(KS + b) * 64 + lane]),
+                        qc[(KS + b) * 64 + lane], 0, 0, 0);
+            }
+        }
+        f4 acc[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
+#pragma unroll
+        for (int b = 0; b < KS; ++b) {
+            const u4 hk = *(const u4 *)&sl[0][16 * g + 4 * b];
+#pragma unroll
+            for (int tl = 0; tl < 2; ++tl)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    acc[tl][i] = fmaf((float)as_h2(hk[i])[tl], d[tl][b][i], acc[tl][i]);
+        }
+#pragma unroll
+        for (int tl = 0; tl < 2; ++tl)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) p[tl][i] = WIDE ? acc[tl][i] : ror8_add(acc[tl][i]);
+        if (tail) {
+            int end = p1;
+            asm volatile("" : "+s"(end));  // (a branch, not selects in every step)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                p[0][i] = s + 8 * g + i < end ? p[0][i] : -INFINITY;
+                p[1][i] = s + 8 * g + 4 + i < end ? p[1][i] : -INFINITY;
+            }
+        }
         float mx = fmaxf(fmaxf(fmaxf(p[0][0], p[0][1]), fmaxf(p[0][2], p[0][3])),
                          fmaxf(fmaxf(p[1][0], p[1][1]), fmaxf(p[1][2], p[1][3])));
-        if (__ballot(mx > m + 8.0f)) {
+        if (__ballot(mx > lim)) {
             mx = fmaxf(mx, swap16_f(mx));
             mx = fmaxf(mx, swap32_f(mx));
             const float mn = fmaxf(m, mx);
-            const float al = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
+            const float al = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - mn) * fac);
             m = mn;
-            lsum *= al;
+            mf = mn * fac;
+            lim = mn + over;
+            ol *= al;
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt) o[dt] *= al;
         }
         u4 pa, pb;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const float x = __builtin_amdgcn_exp2f(p[0][i] - m), y = __builtin_amdgcn_exp2f(p[1][i] - m);
-            lsum += x + y;
-            const h2 hi = {(_Float16)x, (_Float16)y};
+            const f2 x = {__builtin_amdgcn_exp2f(fmaf(p[0][i], fac, -mf)),
+                          __builtin_amdgcn_exp2f(fmaf(p[1][i], fac, -mf))};
+            const h2 hi = __builtin_convertvector(x, h2);
             if constexpr (WIDE) {
-                const h2 lo = {(_Float16)(x - (float)hi[0]), (_Float16)(y - (float)hi[1])};
                 pa[i] = as_u(hi);
-                pb[i] = as_u(lo);
+                pb[i] = as_u((h2){(_Float16)(x[0] - (float)hi[0]), (_Float16)(x[1] - (float)hi[1])});
             } else {
-                const float xr = fmaf(-(float)hi[0], lo_col, x), yr = fmaf(-(float)hi[1], lo_col, y);
-                pa[i] = as_u((h2){(_Float16)xr, (_Float16)yr});
+                pa[i] = as_u((h2){(_Float16)fmaf(-(float)hi[0], lo_col, x[0]),
+                                  (_Float16)fmaf(-(float)hi[1], lo_col, x[1])});
             }
         }
-        u4 hv[KS];
-        spread<KS>(t.vh, hv);
+        const h8 ph = __builtin_bit_cast(h8, pa), pl = __builtin_bit_cast(h8, pb);
+        const u4 one = {0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u};
+        if constexpr (WIDE)
+            ol = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, one), pl, ol, 0, 0, 0);
+        ol = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, one), ph, ol, 0, 0, 0);
 #pragma unroll
         for (int b = 0; b < KS; ++b) {
-            const u4 hw = hv[b];
-            h2 off[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) off[i] = as_h2(hw[i]) * (h2){(_Float16)-72.0f, (_Float16)-72.0f};
+            const u4 hv = *(const u4 *)&sl[1][16 * g + 4 * b], off = *(const u4 *)&sl[2][16 * g + 4 * b];
 #pragma unroll
             for (int dt = 2 * b; dt < 2 * b + 2; ++dt) {
                 const uint32_t w = t.v[dt];
@@ -582,31 +732,28 @@ __global__ void __launch_bounds__(256, 2) k_attn_kv4(
                 u4 va;
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    va[i] = as_u(__builtin_elementwise_fma(as_h2((n[i] & 0x00f000f0u) | 0x54005400u),
-                                                           as_h2(hw[i]), off[i]));
+                    va[i] = as_u(__builtin_elementwise_fma(as_h2((n[i] & mask) | magic),
+                                                           as_h2(hv[i]), as_h2(off[i])));
                 const h8 vv = __builtin_bit_cast(h8, va);
                 if constexpr (WIDE)
-                    o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vv, __builtin_bit_cast(h8, pb),
-                                                                   o[dt], 0, 0, 0);
-                o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vv, __builtin_bit_cast(h8, pa), o[dt],
-                                                               0, 0, 0);
+                    o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vv, pl, o[dt], 0, 0, 0);
+                o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vv, ph, o[dt], 0, 0, 0);
             }
         }
     };
     while (s0 < p1) {
-        const int s1 = s0 + A4_STEP, s2 = s1 + A4_STEP;
-        if (s1 < p1) load(tb, s1, id);
-        id = ids_of(s2);
         step(ta, s0);
-        if (s1 >= p1) break;
-        if (s2 < p1) load(ta, s2, id);
-        id = ids_of(s2 + A4_STEP);
-        step(tb, s1);
-        s0 = s2;
+        s0 += A4_STEP;
+        if (s0 >= p1) break;
+        if (s0 + A4_STEP < p1) load(ta, s0 + A4_STEP, id);
+        id = ids_of(s0 + 2 * A4_STEP);
+        step(tb, s0);
+        s0 += A4_STEP;
+        if (s0 + A4_STEP < p1) load(tb, s0 + A4_STEP, id);
+        id = ids_of(s0 + 2 * A4_STEP);
     }
     // the wavefronts' states meet in LDS
-    lsum += swap16_f(lsum);
-    lsum += swap32_f(lsum);
+    const float lsum = WIDE ? ol[0] : ror8_add(ol[0]);
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) {
         f4 v = o[dt];
@@ -616,7 +763,7 @@ __global__ void __launch_bounds__(256, 2) k_attn_kv4(
         if (col < per) *(f4 *)&mo[wave][col][16 * dt + 4 * g] = v * 16.0f;
     }
     if (g == 0 && col < per) {
-        mm[wave][col] = m;
+        mm[wave][col] = mf;
         ml[wave][col] = lsum;
     }
     __syncthreads();
@@ -655,22 +802,94 @@ __global__ void __launch_bounds__(256, 2) k_attn_kv4(
             *(f4 *)(ws_o + (((size_t)qi * qheads + head) * ns + sp) * D + dd) = acc;
         } else {
             const float r = linv[h], y[4] = {acc[0] * r, acc[1] * r, acc[2] * r, acc[3] * r};
-            const size_t off = ((size_t)qi * qheads + head) * D + dd;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) attn[off + i] = y[i];
-            if (qs) {
-                uint16_t dbits;
-                int sum;
-                const uint32_t w = quant_block_oct(y, dbits, sum);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) qs[off + i] = (int8_t)(w >> (8 * i));
-                if ((e4 & 7) == 0) {
-                    qd8[off / SI_QK] = dbits;
-                    if (bsum) bsum[off / SI_QK] = (int16_t)sum;
-                }
-            }
+            kv4_store(y, ((size_t)qi * qheads + head) * D + dd, e4 & 7, attn, qs, qd8, bsum, tq, td,
+                      qheads * D, qi);
         }
     }
+}
+
+// ---------------------------------------------------------------------------
+// The chunks' states of a (query, head) to its output: a workgroup per 32 dims
+// (one Q8_0 block), 8 lanes a state, G states at once, at most 8 G in all, so
+// that every load is in flight at once.  tq/td (optional): the Q8_0 also
+// operand-tiled (q8_tiled_byte).
+// ---------------------------------------------------------------------------
+template <int G>
+__global__ void __launch_bounds__(8 * G) k_kv4_merge(
+    int qheads, int hdim, int ns, const int *__restrict__ ctx_dev, const int *__restrict__ parts,
+    const float *__restrict__ ws_m, const float *__restrict__ ws_l,
+    const float *__restrict__ ws_o, float *__restrict__ attn, int8_t *__restrict__ qs,
+    uint16_t *__restrict__ d, int16_t *__restrict__ bsum, int8_t *__restrict__ tq,
+    uint16_t *__restrict__ td) {
+    constexpr int W = G / 8;  // wavefronts
+    __shared__ float red_m[W], red_l[W];
+    __shared__ f4 red_o[W][8];
+    const int nb = hdim / 32, h = blockIdx.x / nb, blk = blockIdx.x % nb, qi = blockIdx.y;
+    const int tid = threadIdx.x, l8 = tid & 7, grp = tid >> 3, wave = tid >> 6;
+    const size_t base = ((size_t)qi * qheads + h) * ns;
+    const int each = (ns + G - 1) / G;
+    const int have = !parts ? ns : ctx_dev[qi] > 0 ? parts[qi] : 0;  // states that were written
+    f4 o[8];
+    float m[8], l[8], mx = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+        m[k] = -INFINITY;
+        if (k < each && grp + k * G < ns) {
+            const size_t i = base + grp + k * G;
+            m[k] = ws_m[i];
+            l[k] = ws_l[i];
+            o[k] = *(const f4 *)(ws_o + i * hdim + 32 * blk + 4 * l8);
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+        m[k] = grp + k * G < have ? m[k] : -INFINITY;
+        mx = fmaxf(mx, m[k]);
+    }
+    mx = fmaxf(mx, dpp_f<DPP_ROR8>(mx));
+    mx = fmaxf(mx, swap16_f(mx));
+    mx = fmaxf(mx, swap32_f(mx));
+    if constexpr (W > 1) {
+        if ((tid & 63) == 0) red_m[wave] = mx;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < W; ++w) mx = fmaxf(mx, red_m[w]);
+    }
+    f4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+    float sum = 0.0f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+        if (m[k] == -INFINITY) continue;  // none, or an empty chunk (its output unwritten)
+        const float w = __builtin_amdgcn_exp2f(m[k] - mx);
+        sum = fmaf(l[k], w, sum);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[i] = fmaf(o[k][i], w, acc[i]);
+    }
+    auto across = [](float v) {
+        v = ror8_add(v);
+        v += swap16_f(v);
+        return v + swap32_f(v);
+    };
+    sum = across(sum);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[i] = across(acc[i]);
+    if constexpr (W > 1) {
+        if ((tid & 63) < 8) red_o[wave][l8] = acc;
+        if ((tid & 63) == 0) red_l[wave] = sum;
+        __syncthreads();
+        acc = red_o[0][l8];
+        sum = red_l[0];
+#pragma unroll
+        for (int w = 1; w < W; ++w) {
+            acc += red_o[w][l8];
+            sum += red_l[w];
+        }
+    }
+    if (tid >= 8) return;
+    const float r = mx == -INFINITY ? 0.0f : 1.0f / sum;  // no context: zeros
+    const float y[4] = {acc[0] * r, acc[1] * r, acc[2] * r, acc[3] * r};
+    const size_t off = ((size_t)qi * qheads + h) * hdim + 32 * blk + 4 * l8;
+    kv4_store(y, off, l8, attn, qs, d, bsum, tq, td, qheads * hdim, qi);
 }
 
 // ---------------------------------------------------------------------------
@@ -690,8 +909,8 @@ __global__ void __launch_bounds__(256) k_kv_copy(KvMoves mv, size_t page_bytes) 
 // ---------------------------------------------------------------------------
 // launchers
 // ---------------------------------------------------------------------------
-#define KV4_DIM(hdim, CALL)      \
-    switch (hdim) {              \
+#define KV4_DIM(hdim, CALL)       \
+    switch (hdim) {               \
         case 32: CALL(32); break; \
         case 64: CALL(64); break; \
         case 96: CALL(96); break; \
@@ -736,11 +955,15 @@ void launch_kv4_read(const Kv4Cache &c, int ntok, int hdim, int pos0, int pos_st
 #undef CALL
 }
 
-// Chunks of the context: about 1024 workgroups, each of whole steps
-static int attn_kv4_chunks(int kvheads, int nq, int max_ctx) {
-    const int most = (max_ctx + A4_STEP - 1) / A4_STEP;
-    const int want = (int)((1024 + (long long)kvheads * nq - 1) / ((long long)kvheads * nq));
-    return max(1, min(min(most, want), 256));
+// Workgroups the GPU holds at once (by the kernel's registers)
+static int a4_slots(int hdim) { return hdim > 64 ? 768 : 1024; }
+// Most chunks of a context: of equal contexts as many as fill those; of contexts
+// on the device up to twice that, which the kernel uses as they are ragged.
+static int attn_kv4_chunks(int hdim, int kvheads, int nq, int max_ctx, bool ragged) {
+    const long long most = (max_ctx + A4_STEP - 1) / A4_STEP, base = (long long)kvheads * nq;
+    if (base >= a4_slots(hdim)) return 1;
+    const long long want = (a4_slots(hdim) + base - 1) / base * (ragged ? 2 : 1);
+    return (int)max(1ll, min(min(most, want), 256ll));
 }
 
 // Whether a prompt's pages are read into fp16 rows for the prefill kernel
@@ -748,13 +971,15 @@ static bool kv4_by_rows(int nq, int ctx_step) { return ctx_step == 1 && nq > 4; 
 
 size_t attn_kv4_workspace(int qheads, int kvheads, int hdim, int nq, int ctx_step, int max_ctx) {
     if (kv4_by_rows(nq, ctx_step)) return (size_t)max_ctx * kvheads * hdim * 2 * sizeof(uint16_t);
-    const int ns = attn_kv4_chunks(kvheads, nq, max_ctx);
-    return ns == 1 ? 0 : (size_t)nq * qheads * ns * (hdim + 2) * sizeof(float);
+    const int ns = attn_kv4_chunks(hdim, kvheads, nq, max_ctx, ctx_step == 0);
+    if (ns == 1) return 0;
+    return (size_t)nq * qheads * ns * (hdim + 2) * sizeof(float) + (size_t)nq * sizeof(int);
 }
 
 void launch_attention_kv4(const float *q, int nq, int qheads, int hdim, const Kv4Cache &c,
                           const int *ctx_dev, int ctx0, int ctx_step, int max_ctx, float *attn,
-                          int8_t *qs, uint16_t *d, int16_t *bsum, void *ws, hipStream_t st) {
+                          int8_t *qs, uint16_t *d, int16_t *bsum, void *ws, hipStream_t st,
+                          int8_t *tq, uint16_t *td) {
     if (nq <= 0) return;
     if (kv4_by_rows(nq, ctx_step)) {
         uint16_t *k = (uint16_t *)ws, *v = k + (size_t)max_ctx * c.kvheads * hdim;
@@ -762,17 +987,34 @@ void launch_attention_kv4(const float *q, int nq, int qheads, int hdim, const Kv
         launch_attn_prefill(q, nq, qheads, c.kvheads, hdim, ctx0 - 1, k, v, attn, qs, d, bsum, st);
         return;
     }
-    const int ns = attn_kv4_chunks(c.kvheads, nq, max_ctx);
+    const int ns = attn_kv4_chunks(hdim, c.kvheads, nq, max_ctx, ctx_dev != nullptr);
     const int chunk = ((max_ctx + ns - 1) / ns + A4_STEP - 1) / A4_STEP * A4_STEP;
+    const int slots = a4_slots(hdim);
     const AttnParts pt(ws, (size_t)nq * qheads * ns, hdim);
-    const dim3 grid(ns, c.kvheads, nq);
+    // contexts on the device: a list of chunks, its length made on the GPU
+    int *parts = ns > 1 && ctx_dev ? (int *)(pt.l + (size_t)nq * qheads * ns) : nullptr;
+    const dim3 grid(c.kvheads, parts ? slots / c.kvheads + nq : nq, parts ? 1 : ns);
     const bool wide = qheads / c.kvheads > 8, page16 = c.shift == 4;
-#define CALL2(DIM, W, P)                                                                            SI_LAUNCH((k_attn_kv4<DIM, W, P>), grid, dim3(256), 0, st, q, qheads, c, ctx_dev, ctx0,                   ctx_step, max_ctx, chunk, softmax_scale2(hdim), pt.m, pt.l, pt.o, attn, qs, d, bsum)
-#define CALL(DIM)                                              if (wide && page16) CALL2(DIM, true, true);                else if (wide) CALL2(DIM, true, false);                    else if (page16) CALL2(DIM, false, true);                  else CALL2(DIM, false, false)
+#define CALL2(DIM, W, P)                                                                        \
+    SI_LAUNCH((k_attn_kv4<DIM, W, P>), grid, dim3(256), 0, st, q, qheads, c, ctx_dev, ctx0,     \
+              ctx_step, nq, max_ctx, ns, chunk, slots, softmax_scale2(hdim), parts, pt.m, pt.l, \
+              pt.o, attn, qs, d, bsum, tq, td)
+#define CALL(DIM)                               \
+    if (wide && page16) CALL2(DIM, true, true); \
+    else if (wide) CALL2(DIM, true, false);     \
+    else if (page16) CALL2(DIM, false, true);   \
+    else CALL2(DIM, false, false)
     KV4_DIM(hdim, CALL)
 #undef CALL
 #undef CALL2
-    if (ns > 1) launch_attn_combine(nq, qheads, hdim, ns, ws, attn, qs, d, bsum, st);
+    if (ns == 1) return;
+    const dim3 blocks(qheads * (hdim / 32), nq);
+#define CALL(G)                                                                                  \
+    SI_LAUNCH(k_kv4_merge<G>, blocks, dim3(8 * G), 0, st, qheads, hdim, ns, ctx_dev, parts, pt.m, \
+              pt.l, pt.o, attn, qs, d, bsum, tq, td)
+    if (ns <= 64) CALL(8);
+    else CALL(32);
+#undef CALL
 }
 
 void launch_kv_copy(const KvMoves &mv, int npools, int nmoves, size_t page_bytes, bool wide,
