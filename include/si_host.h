@@ -223,6 +223,27 @@ int si_kv_seq_add(si_kv_pages_t *p);
  * sequence's max_pages cannot hold them */
 int si_kv_seq_grow(si_kv_pages_t *p, int seq, int len);
 void si_kv_seq_free(si_kv_pages_t *p, int seq);
+/* a new sequence with another's positions, sharing its pages: its id, or -1
+ * when every slot is taken.  Shared pages are only read: the sequence that
+ * grows into one first gets a page of its own, whose copy is pending
+ * (si_kv_copies), which si_kv_seq_grow counts as a page taken. */
+int si_kv_seq_fork(si_kv_pages_t *p, int seq);
+/* forgets the positions from len on (0..its length); whole pages return */
+void si_kv_seq_truncate(si_kv_pages_t *p, int seq, int len);
+/* Pending page copies, host arrays valid until the next call on p: their
+ * number.  They are for si_kv_copy_pages, in every pool, before the next
+ * kernel that reads or appends to these sequences; then si_kv_copies_done.
+ * Until then the pages they read are held.  A copy whose target is freed
+ * meanwhile is dropped. */
+int si_kv_copies(const si_kv_pages_t *p, const int **src, const int **dst);
+void si_kv_copies_done(si_kv_pages_t *p);
+/* Moves the held pages to the lowest ids (their copies pending, none may be
+ * before) and returns their number: the pool's tail from there on is free once
+ * the copies are done.  The page tables change. */
+int si_kv_compact(si_kv_pages_t *p);
+/* The pool now has npages pages: 0, or -1 (unchanged) when a page past them is
+ * held.  The tail of a smaller pool is the caller's again. */
+int si_kv_pages_resize(si_kv_pages_t *p, int npages);
 int si_kv_seq_len(const si_kv_pages_t *p, int seq);
 int si_kv_pages_free(const si_kv_pages_t *p);
 /* host [max_seqs][max_pages] page ids by sequence id (unused entries 0) */
@@ -234,6 +255,12 @@ const int *si_kv_page_table(const si_kv_pages_t *p);
 typedef struct si_stack si_stack_t;
 si_stack_t *si_stack_create(const si_shape_t *s, const si_layer_host_t *layers, int nlayers,
                             int max_seqs, int max_ctx, int npages, int page_size);
+/* The same with the pools' format: SI_KV_F16, or SI_KV_Q4, a 4-bit cache
+ * (si_kv4_page_bytes(s, page_size) bytes a page, page_size 16..65536; the pool
+ * pointers below are then uint8_t's). */
+enum { SI_KV_F16 = 0, SI_KV_Q4 = 1 };
+si_stack_t *si_stack_create_kv(const si_shape_t *s, const si_layer_host_t *layers, int nlayers,
+                               int max_seqs, int max_ctx, int npages, int page_size, int format);
 void si_stack_destroy(si_stack_t *st);
 si_kv_pages_t *si_stack_pages(si_stack_t *st);
 uint16_t *si_stack_k_pool(si_stack_t *st, int layer);
@@ -251,6 +278,12 @@ int si_stack_nseq(const si_stack_t *st);
  * sequences, and si_stack_decode dies until a later prepare succeeds),
  * else 0. */
 int si_stack_prepare(si_stack_t *st, const int *seqs, int nseq);
+/* si_kv_seq_fork of the stack's pages: the next si_stack_prepare with one of
+ * them copies the page they would both append to, in every pool. */
+int si_stack_fork(si_stack_t *st, int seq);
+/* si_kv_compact with its copies in every pool (waits for them, and for the
+ * stream of the last decode); a si_stack_prepare has to follow. */
+int si_stack_compact(si_stack_t *st);
 /* x [nseq][hidden] (device) through every layer -> out [nseq][hidden]: the
  * residual stream of a decode step; kernel launches only (capturable). */
 void si_stack_decode(si_stack_t *st, const float *x, float *out, int flags, void *stream);

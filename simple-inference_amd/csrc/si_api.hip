@@ -884,6 +884,7 @@ static int make_workspace(const si_shape_t *s, int max_tokens, int max_pos,
         size_t b = si_attention_workspace(s, nq, max_pos);
         const size_t bd = dec_attn_workspace_bytes(s->qheads, s->hdim, s->kvheads, nq, max_pos);
         if (bd > b) b = bd;
+        b = std::max(b, attn_kv4_workspace(s->qheads, s->kvheads, s->hdim, nq, 0, max_pos));
         if (b > W->attn_ws_bytes) W->attn_ws_bytes = b;
     }
     uint8_t *ws = nullptr;
@@ -1338,7 +1339,7 @@ static int run_decode_ffn(si_layer *L, float *out, bool exact, bool cap, hipStre
 static int run_rows(si_layer *L, const float *x, int rows, uint16_t *kc, uint16_t *vc,
                     size_t kv_seq_stride, int pos0, const int *ctx_dev, int ctx0, int ctx_step,
                     int max_ctx, float *out, int flags, hipStream_t st,
-                    KvPages pg = KvPages()) {
+                    KvPages pg = KvPages(), const Kv4Cache *kv4 = nullptr) {
     const int pos_step = ctx_step;  // positions advance with the contexts
     const si_shape_t &s = L->s;
     const int H = s.hidden, QD = s.qheads * s.hdim, NQKV = QD + 2 * s.kvheads * s.hdim;
@@ -1390,7 +1391,18 @@ static int run_rows(si_layer *L, const float *x, int rows, uint16_t *kc, uint16_
     else
         project(L, L->wqkv, rows, L->xq, L->bqkv, nullptr, L->qkv, flags, st);
     bool tl_att = false;  // the attention's Q8 written operand-tiled too
-    if (ctx_step == 0) {
+    if (kv4) {
+        // batched decode over a 4-bit cache: RoPE + quantized K/V append, then
+        // attention over the pages -> Q8
+        mark(L, SI_PHASE_ROPE_KV, st);
+        launch_rope_kv4(L->qkv, NQKV, rows, s.qheads, s.hdim, pos0, 0, max_ctx, ctx_dev,
+                        L->rope_cos, L->rope_sin, L->q, *kv4, st);
+        mark(L, SI_PHASE_ATTENTION_Q8, st);
+        tl_att = tl_x;
+        launch_attention_kv4(L->q, rows, s.qheads, s.hdim, *kv4, ctx_dev, ctx0, 0, max_ctx,
+                             L->attn, L->attq.qs, L->attq.d, L->attq.s, L->attn_ws, st,
+                             tl_x ? L->attq.tq : nullptr, tl_x ? L->attq.td : nullptr);
+    } else if (ctx_step == 0) {
         // batched decode: RoPE + K/V append inside the attention kernel,
         // contiguous caches or a paged pool (pg)
         mark(L, SI_PHASE_ATTENTION_Q8, st);
@@ -1771,6 +1783,30 @@ int si_attention_kv4(const si_shape_t *s, const float *q, int nq, const uint8_t 
     launch_attention_kv4(q, nq, s->qheads, s->hdim, c, ctx_dev, ctx0, ctx_step, max_ctx, attn, qs,
                          d, bsum, ws, S(stream));
     return check_launch("si_attention_kv4");
+}
+
+int si_layer_decode_kv4(si_layer_t *L, const float *x, int nseq, uint8_t *k_pool, uint8_t *v_pool,
+                        int npages, int page_size, const int *pages, int max_pages,
+                        const int *ctx_dev, int context, int max_ctx, float *out, int flags,
+                        void *stream) {
+    const char *what = "layer_decode_kv4";
+    SI_REQUIRE(L && x && out, "%s: NULL pointer", what);
+    SI_REQUIRE((flags & ~(SI_LAYER_ATTN_ONLY | SI_LAYER_EXACT | SI_LAYER_CAPTURE)) == 0,
+               "%s: unsupported flags %d (standard attention is single-token decode only)", what,
+               flags);
+    SI_REQUIRE(nseq >= 1 && nseq <= L->max_tokens, "%s: nseq %d outside 1..%d", what, nseq,
+               L->max_tokens);
+    SI_REQUIRE(nseq <= 65535, "%s: nseq %d exceeds 65535", what, nseq);
+    SI_REQUIRE(max_ctx >= 1 && max_ctx <= L->max_pos, "%s: max_ctx %d outside 1..%d", what,
+               max_ctx, L->max_pos);
+    SI_REQUIRE(ctx_dev || (context >= 1 && context <= max_ctx), "%s: context %d outside 1..%d",
+               what, context, max_ctx);
+    Kv4Cache c;
+    TRY(kv4_cache(what, &L->s, k_pool, v_pool, npages, page_size, pages, max_pages, &c));
+    SI_REQUIRE((long long)max_pages * page_size >= max_ctx, "%s: pages do not cover max_ctx %d",
+               what, max_ctx);
+    return run_rows(L, x, nseq, nullptr, nullptr, 0, context - 1, ctx_dev, context, 0, max_ctx,
+                    out, flags, S(stream), KvPages(), &c);
 }
 
 int si_kv_copy_pages(void *const *pools, int npools, size_t page_bytes, int npages,

@@ -24,6 +24,7 @@ Q8_DTYPE = np.dtype([("d", "<u2"), ("qs", "i1", (QK,))])  # defines.h:27-28
 SI_OK, SI_ERR_ARG, SI_ERR_HIP, SI_ERR_STATE, SI_ERR_NOMEM = range(5)
 SI_LAYER_FULL, SI_LAYER_ATTN_ONLY, SI_LAYER_EXACT, SI_LAYER_ATTN_STANDARD = 0, 1, 2, 4
 SI_LAYER_CAPTURE = 8
+SI_KV_F16, SI_KV_Q4 = 0, 1
 SI_GEMM_EXACT = 1
 SI_GEMM_F16 = 2
 SI_GEMM_TILED_A = 4
@@ -133,6 +134,7 @@ _SIGS = {
     "si_attention_kv4": (_I, [ctypes.POINTER(Shape), _P, _I, _P, _P, _I, _I, _P, _I, _P, _I, _I,
                               _I, _P, _P, _P, _P, _P, _Z, _P]),
     "si_attention_kv4_workspace": (_Z, [ctypes.POINTER(Shape), _I, _I, _I]),
+    "si_layer_decode_kv4": (_I, [_P, _P, _I, _P, _P, _I, _I, _P, _I, _P, _I, _I, _P, _I, _P]),
     "si_kv_copy_pages": (_I, [_P, _I, _Z, _I, _P, _P, _I, _P]),
     "si_layer_buffer": (_P, [_P, _I]),
     "si_layer_set_timing": (_I, [_P, _I]),
@@ -179,10 +181,20 @@ def host_lib():
                 ("si_kv_seq_add", _I, [_P]),
                 ("si_kv_seq_grow", _I, [_P, _I, _I]),
                 ("si_kv_seq_free", None, [_P, _I]),
+                ("si_kv_seq_fork", _I, [_P, _I]),
+                ("si_kv_seq_truncate", None, [_P, _I, _I]),
+                ("si_kv_copies", _I, [_P, ctypes.POINTER(ctypes.POINTER(_I)),
+                                      ctypes.POINTER(ctypes.POINTER(_I))]),
+                ("si_kv_copies_done", None, [_P]),
+                ("si_kv_compact", _I, [_P]),
+                ("si_kv_pages_resize", _I, [_P, _I]),
                 ("si_kv_seq_len", _I, [_P, _I]),
                 ("si_kv_pages_free", _I, [_P]),
                 ("si_kv_page_table", ctypes.POINTER(_I), [_P]),
                 ("si_stack_create", _P, [ctypes.POINTER(Shape), _P, _I, _I, _I, _I, _I]),
+                ("si_stack_create_kv", _P, [ctypes.POINTER(Shape), _P, _I, _I, _I, _I, _I, _I]),
+                ("si_stack_fork", _I, [_P, _I]),
+                ("si_stack_compact", _I, [_P]),
                 ("si_stack_destroy", None, [_P]),
                 ("si_stack_pages", _P, [_P]),
                 ("si_stack_k_pool", _P, [_P, _I]),
@@ -236,8 +248,14 @@ def ptr(t):
 
 def stream_handle(stream=None):
     import torch
-    s = stream if stream is not None else torch.cuda.current_stream()
-    return ctypes.c_void_p(s.cuda_stream)
+    if stream is None:
+        # the current device's current stream, without the stream object that
+        # torch.cuda.current_stream() makes (3.0 us a call)
+        raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+        if raw is not None:
+            return ctypes.c_void_p(raw(torch.cuda.current_device()))
+        stream = torch.cuda.current_stream()
+    return ctypes.c_void_p(stream.cuda_stream)
 
 
 def quantize_q4_0(w):
@@ -339,6 +357,12 @@ class Layer:
     def decode_paged(self, x, nseq, k_pool, v_pool, npages, page_size, pages, max_pages,
                      ctx_dev, max_ctx, out, flags=SI_LAYER_FULL, stream=None, capture=True):
         call("si_layer_decode_paged", self.h, ptr(x), nseq, ptr(k_pool), ptr(v_pool), npages,
+             page_size, ptr(pages), max_pages, ptr(ctx_dev), max_ctx, max_ctx, ptr(out),
+             flags | (SI_LAYER_CAPTURE if capture else 0), stream_handle(stream))
+
+    def decode_kv4(self, x, nseq, k_pool, v_pool, npages, page_size, pages, max_pages, ctx_dev,
+                   max_ctx, out, flags=SI_LAYER_FULL, stream=None, capture=True):
+        call("si_layer_decode_kv4", self.h, ptr(x), nseq, ptr(k_pool), ptr(v_pool), npages,
              page_size, ptr(pages), max_pages, ptr(ctx_dev), max_ctx, max_ctx, ptr(out),
              flags | (SI_LAYER_CAPTURE if capture else 0), stream_handle(stream))
 
