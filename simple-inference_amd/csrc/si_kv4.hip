@@ -129,17 +129,32 @@ static int kv4_units(int ntok, int pos0, int pos_step) {
 
 // ---------------------------------------------------------------------------
 // append: block of 2 D threads per (unit, KV head), then blocks that rotate q.
-// K: thread (position, octet of dims), a block's four octets in a quad of lanes.
-// V: thread per dim with the unit's 8 positions, a block in 32 lanes; a dword
-// whose 8 positions are not all written keeps its other nibbles.
+// A thread per position and octet of dims, D for K and D for V, a block's four
+// octets in a quad of lanes.  V's nibbles pass through LDS to a thread per dim,
+// whose dword holds the unit's 8 positions (one that is not written whole keeps
+// its other nibbles).  (V by a thread per dim with all 8 positions took 8
+// reductions over 32 lanes one after another: 5000 fp16 rows of 2 heads of 128
+// 7.0 us, 5.2 so.)
 // HALF_IN: the rows are fp16 cache rows (kin, vin), copied in without RoPE.
 // ---------------------------------------------------------------------------
+// 8 floats, 16 bytes a load where the call's buffers allow it
+__device__ __forceinline__ void load8(const float *p, bool wide, float (&v)[8]) {
+    if (wide) {
+        const float4 a = *(const float4 *)p, b = *(const float4 *)(p + 4);
+        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
+        v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = p[e];
+    }
+}
+
 template <int D, bool HALF_IN>
 __global__ void __launch_bounds__(2 * D) k_kv4_append(
     const float *__restrict__ qkv, int ldqkv, const uint16_t *__restrict__ kin,
     const uint16_t *__restrict__ vin, int qheads, int ntok, int pos0, int pos_step, int limit,
     const int *__restrict__ ctx_dev, const float *__restrict__ rc, const float *__restrict__ rs,
-    float *__restrict__ q_out, Kv4Cache c) {
+    float *__restrict__ q_out, bool wide, Kv4Cache c) {
     constexpr int HALF = D / 2;
     const Kv4Unit un((int)blockIdx.x, ntok, pos0, pos_step, ctx_dev, limit);
     if (un.lo >= un.hi) return;
@@ -165,75 +180,74 @@ __global__ void __launch_bounds__(2 * D) k_kv4_append(
     const size_t at = ((size_t)c.page_of(un.seq, un.base) * kvh + g) *
                       (size_t)kv4_head_bytes(D, page_size);
     const int in_page = un.base & (page_size - 1);
-    if (tid < D) {
-        uint8_t *kp = c.k + at;
-        const int j = tid / (D / 8), o = tid % (D / 8), pos = un.base + j, i = in_page + j;
-        const bool live = j >= un.lo && j < un.hi;
-        float x[8];
-        uint32_t key = 0;
+    __shared__ __attribute__((aligned(8))) uint8_t vn[D][8];  // V's nibbles [dim][position]
+    const bool is_k = tid < D;
+    const int t = is_k ? tid : tid - D, j = t / (D / 8), o = t % (D / 8);
+    const int pos = un.base + j, i = in_page + j;
+    const bool live = j >= un.lo && j < un.hi;
+    float x[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+    if (live) {
+        if constexpr (HALF_IN) {
+            const uint4 w = *(const uint4 *)((is_k ? kin : vin) + (size_t)(un.t0 + j) * kvd +
+                                             g * D + 8 * o);
+            const uint32_t v[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            float v = 0.0f;
-            if (live) {
-                const int dim = 8 * o + e;
-                if constexpr (HALF_IN) {
-                    v = h2f_fast(kin[(size_t)(un.t0 + j) * kvd + g * D + dim]);
-                } else {
-                    const float *row = qkv + (size_t)(un.t0 + j) * ldqkv + qd + g * D;
-                    const int ii = dim < HALF ? dim : dim - HALF;
-                    const float cs = rc[(size_t)pos * HALF + ii], sn = rs[(size_t)pos * HALF + ii];
-                    const float a = row[ii], b = row[ii + HALF];
-                    v = dim < HALF ? __fsub_rn(__fmul_rn(a, cs), __fmul_rn(b, sn))
-                                   : __fadd_rn(__fmul_rn(b, cs), __fmul_rn(a, sn));
-                }
+            for (int e = 0; e < 8; ++e) x[e] = h2f_fast((uint16_t)(v[e / 2] >> (16 * (e & 1))));
+        } else {
+            const float *row = qkv + (size_t)(un.t0 + j) * ldqkv + qd + g * D;
+            if (is_k) {
+                const int i0 = 8 * o < HALF ? 8 * o : 8 * o - HALF;  // (8 divides HALF)
+                float a[8], b[8], cs[8], sn[8];
+                load8(row + i0, wide, a);
+                load8(row + i0 + HALF, wide, b);
+                load8(rc + (size_t)pos * HALF + i0, wide, cs);
+                load8(rs + (size_t)pos * HALF + i0, wide, sn);
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    x[e] = 8 * o < HALF ? __fsub_rn(__fmul_rn(a[e], cs[e]), __fmul_rn(b[e], sn[e]))
+                                        : __fadd_rn(__fmul_rn(b[e], cs[e]), __fmul_rn(a[e], sn[e]));
+            } else {
+                load8(row + kvd + 8 * o, wide, x);
             }
-            x[e] = v == v ? v : 0.0f;
-            key = max(key, kv4_key(x[e]));
         }
-        key = max(key, (uint32_t)dpp_i<DPP_XOR1>((int)key));
-        key = max(key, (uint32_t)dpp_i<DPP_XOR2>((int)key));
-        const uint16_t h = kv4_scale_of(key);
-        const Kv4Scale sc(h);
-        uint32_t w = 0;
+    }
+    uint32_t key = 0;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) w |= sc.nibble(x[e]) << (4 * e);
-        if (live) {
-            *(uint32_t *)(kp + kv4_k_dword(D, i, o)) = w;
-            if ((o & 3) == 0) *(uint16_t *)(kp + kv4_scale(D, page_size, i, o >> 2)) = h;
-        }
-    } else {
-        uint8_t *vp = c.v + at;
-        const int e = tid - D;
-        uint32_t w = 0, mask = 0;
+    for (int e = 0; e < 8; ++e) {
+        x[e] = x[e] == x[e] ? x[e] : 0.0f;
+        key = max(key, kv4_key(x[e]));
+    }
+    key = max(key, (uint32_t)dpp_i<DPP_XOR1>((int)key));
+    key = max(key, (uint32_t)dpp_i<DPP_XOR2>((int)key));
+    const uint16_t h = kv4_scale_of(key);
+    const Kv4Scale sc(h);
+    uint8_t *page = (is_k ? c.k : c.v) + at;
+    uint32_t w = 0;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const bool live = j >= un.lo && j < un.hi;
-            float v = 0.0f;
-            if (live) {
-                if constexpr (HALF_IN) v = h2f_fast(vin[(size_t)(un.t0 + j) * kvd + g * D + e]);
-                else v = qkv[(size_t)(un.t0 + j) * ldqkv + qd + kvd + g * D + e];
-            }
-            v = v == v ? v : 0.0f;
-            uint32_t key = kv4_key(v);
-            key = max(key, (uint32_t)dpp_i<DPP_XOR1>((int)key));
-            key = max(key, (uint32_t)dpp_i<DPP_XOR2>((int)key));
-            key = max(key, (uint32_t)dpp_i<DPP_ROR4>((int)key));
-            key = max(key, (uint32_t)dpp_i<DPP_ROR8>((int)key));
-            key = max(key, (uint32_t)swap16_i((int)key));
-            const uint16_t h = kv4_scale_of(key);
-            w |= Kv4Scale(h).nibble(v) << (4 * j);
-            mask |= live ? 15u << (4 * j) : 0u;
-            if (live && (e & 31) == 0)
-                *(uint16_t *)(vp + kv4_scale(D, page_size, in_page + j, e >> 5)) = h;
-        }
-        uint32_t *dst = (uint32_t *)(vp + kv4_v_dword(D, in_page >> 3, e));
-        *dst = mask == 0xffffffffu ? w : (*dst & ~mask) | (w & mask);
+    for (int e = 0; e < 8; ++e) {
+        const uint32_t n = sc.nibble(x[e]);
+        w |= n << (4 * e);
+        if (!is_k) vn[8 * o + e][j] = (uint8_t)n;
+    }
+    if (live) {
+        if (is_k) *(uint32_t *)(page + kv4_k_dword(D, i, o)) = w;
+        if ((o & 3) == 0) *(uint16_t *)(page + kv4_scale(D, page_size, i, o >> 2)) = h;
+    }
+    __syncthreads();
+    if (!is_k) {  // a thread per dim: bytes n0 .. n7 to one dword
+        const uint2 n = *(const uint2 *)vn[t];
+        const uint32_t lo = n.x | n.x >> 4, hi = n.y | n.y >> 4;  // n0 + n1 * 16 in byte 0, ..
+        const uint32_t v = __builtin_amdgcn_perm(hi, lo, 0x06040200u);
+        const uint32_t some = un.hi - un.lo == 8
+                                  ? 0xffffffffu
+                                  : ((1u << (4 * (un.hi - un.lo))) - 1) << (4 * un.lo);
+        uint32_t *dst = (uint32_t *)(page + kv4_v_dword(D, in_page >> 3, t));
+        *dst = some == 0xffffffffu ? v : (*dst & ~some) | (v & some);
     }
 }
 
 // ---------------------------------------------------------------------------
-// rows back as fp16, exactly: the same units, a thread per (position, octet) of
-// K and per dim of V
+// rows back as fp16, exactly: the same units and threads
 // ---------------------------------------------------------------------------
 template <int D>
 __global__ void __launch_bounds__(2 * D) k_kv4_read(Kv4Cache c, int ntok, int pos0, int pos_step,
@@ -247,30 +261,31 @@ __global__ void __launch_bounds__(2 * D) k_kv4_read(Kv4Cache c, int ntok, int po
     const size_t at = ((size_t)c.page_of(un.seq, un.base) * kvh + g) *
                       (size_t)kv4_head_bytes(D, page_size);
     const int in_page = un.base & (page_size - 1);
-    if (tid < D) {
-        const uint8_t *kp = c.k + at;
-        const int j = tid / (D / 8), o = tid % (D / 8), i = in_page + j;
-        if (j < un.lo || j >= un.hi) return;
-        const uint32_t w = *(const uint32_t *)(kp + kv4_k_dword(D, i, o));
-        const float d = h2f_fast(*(const uint16_t *)(kp + kv4_scale(D, page_size, i, o >> 2))) * 16.0f;
-        uint16_t y[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-            y[e] = __builtin_bit_cast(uint16_t, (_Float16)((float)((int)(w >> (4 * e) & 15) - 8) * d));
-        *(uint4 *)(kout + (size_t)(un.t0 + j) * kvd + g * D + 8 * o) = *(const uint4 *)y;
+    // V's dwords pass through LDS to a thread per position and octet, like K's
+    __shared__ __attribute__((aligned(16))) uint32_t vw[D];
+    const bool is_k = tid < D;
+    const int t = is_k ? tid : tid - D, j = t / (D / 8), o = t % (D / 8), i = in_page + j;
+    const uint8_t *page = (is_k ? c.k : c.v) + at;
+    if (!is_k) vw[t] = *(const uint32_t *)(page + kv4_v_dword(D, in_page >> 3, t));
+    __syncthreads();
+    if (j < un.lo || j >= un.hi) return;
+    const float d = h2f_fast(*(const uint16_t *)(page + kv4_scale(D, page_size, i, o >> 2))) * 16.0f;
+    uint32_t w = 0;
+    if (is_k) {
+        w = *(const uint32_t *)(page + kv4_k_dword(D, i, o));
     } else {
-        const uint8_t *vp = c.v + at;
-        const int e = tid - D;
-        const uint32_t w = *(const uint32_t *)(vp + kv4_v_dword(D, in_page >> 3, e));
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            if (j < un.lo || j >= un.hi) continue;
-            const float d =
-                h2f_fast(*(const uint16_t *)(vp + kv4_scale(D, page_size, in_page + j, e >> 5))) * 16.0f;
-            vout[(size_t)(un.t0 + j) * kvd + g * D + e] =
-                __builtin_bit_cast(uint16_t, (_Float16)((float)((int)(w >> (4 * j) & 15) - 8) * d));
-        }
+        for (int e = 0; e < 8; ++e) w |= (vw[8 * o + e] >> (4 * j) & 15u) << (4 * e);
     }
+    uint32_t y[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const _Float16 a = (_Float16)((float)((int)(w >> (8 * e) & 15) - 8) * d);
+        const _Float16 b = (_Float16)((float)((int)(w >> (8 * e + 4) & 15) - 8) * d);
+        y[e] = __builtin_bit_cast(uint16_t, a) | (uint32_t)__builtin_bit_cast(uint16_t, b) << 16;
+    }
+    *(uint4 *)((is_k ? kout : vout) + (size_t)(un.t0 + j) * kvd + g * D + 8 * o) =
+        make_uint4(y[0], y[1], y[2], y[3]);
 }
 
 // ---------------------------------------------------------------------------
@@ -923,10 +938,11 @@ void launch_rope_kv4(const float *qkv, int ldqkv, int ntok, int qheads, int hdim
     if (ntok <= 0) return;
     const int limit = (int)min((long long)max_pos, (long long)c.max_pages << c.shift);
     const int qy = (qheads * hdim / 2 + 2 * hdim - 1) / (2 * hdim);
+    const bool wide = ldqkv % 4 == 0 && (((uintptr_t)qkv | (uintptr_t)rc | (uintptr_t)rs) & 15) == 0;
     const dim3 grid(kv4_units(ntok, pos0, pos_step), c.kvheads + qy);
 #define CALL(DIM)                                                                               \
     SI_LAUNCH((k_kv4_append<DIM, false>), grid, dim3(2 * DIM), 0, st, qkv, ldqkv, nullptr,      \
-              nullptr, qheads, ntok, pos0, pos_step, limit, ctx_dev, rc, rs, q_out, c)
+              nullptr, qheads, ntok, pos0, pos_step, limit, ctx_dev, rc, rs, q_out, wide, c)
     KV4_DIM(hdim, CALL)
 #undef CALL
 }
@@ -938,7 +954,7 @@ void launch_kv4_write(const uint16_t *k, const uint16_t *v, int ntok, int hdim, 
     const dim3 grid(kv4_units(ntok, pos0, pos_step), c.kvheads);
 #define CALL(DIM)                                                                            \
     SI_LAUNCH((k_kv4_append<DIM, true>), grid, dim3(2 * DIM), 0, st, nullptr, 0, k, v, 0, ntok, \
-              pos0, pos_step, limit, ctx_dev, nullptr, nullptr, nullptr, c)
+              pos0, pos_step, limit, ctx_dev, nullptr, nullptr, nullptr, false, c)
     KV4_DIM(hdim, CALL)
 #undef CALL
 }
