@@ -504,7 +504,7 @@ template <int D, bool WIDE, bool PAGE16>
 __global__ void __launch_bounds__(256, WIDE ? 2 : 3) k_attn_kv4(
     const float *__restrict__ q, int qheads, Kv4Cache c, const int *__restrict__ ctx_dev, int ctx0,
     int ctx_step, int nq, int max_ctx, int ns, int chunk, int slots, float scale2,
-    int *__restrict__ parts, float *__restrict__ ws_m,
+    int *__restrict__ parts, float *__restrict__ ws_u, float *__restrict__ ws_m,
     float *__restrict__ ws_l, float *__restrict__ ws_o, float *__restrict__ attn,
     int8_t *__restrict__ qs, uint16_t *__restrict__ qd8, int16_t *__restrict__ bsum,
     int8_t *__restrict__ tq, uint16_t *__restrict__ td) {
@@ -513,7 +513,7 @@ __global__ void __launch_bounds__(256, WIDE ? 2 : 3) k_attn_kv4(
     __shared__ __attribute__((aligned(16))) u4 qop[(WIDE ? 2 : 1) * KS * 64];  // hi (, lo)
     __shared__ __attribute__((aligned(16))) f4 qc[(WIDE ? 2 : 1) * KS * 64];
     __shared__ __attribute__((aligned(16))) uint32_t scales[4][3][64];  // K's, V's, V's * -72
-    __shared__ float mm[4][COLS], ml[4][COLS], sc[COLS][4], linv[COLS];
+    __shared__ float mm[4][COLS], ml[4][COLS], sc[COLS][4], linv[COLS], units[COLS];
     const int g0 = blockIdx.x, per = qheads / c.kvheads;
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = uniform(tid >> 6);
@@ -633,11 +633,12 @@ __global__ void __launch_bounds__(256, WIDE ? 2 : 3) k_attn_kv4(
         }
         __syncthreads();
     }
-    // The running maximum m and its limit lim in the scores' raw units; in powers
-    // of two m is mf = m fac.  The sums of the weights are one more product's rows
-    // (ones . P), like the outputs in hi and lo columns.
+    // The running maximum m and its limit lim stay in the scores' raw units (fac
+    // makes them powers of two): weights are 2^((s - m) fac), whose error goes with
+    // the difference, not with the scores.  The sums of the weights are one more
+    // product's rows (ones . P), like the outputs in hi and lo columns.
     const float over = 8.0f * __builtin_amdgcn_rcpf(fac);
-    float m = -INFINITY, mf = -INFINITY, lim = -INFINITY;
+    float m = -INFINITY, lim = -INFINITY;
     f4 o[DT], ol = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) o[dt] = (f4){0.0f, 0.0f, 0.0f, 0.0f};
@@ -712,7 +713,6 @@ __global__ void __launch_bounds__(256, WIDE ? 2 : 3) k_attn_kv4(
             const float mn = fmaxf(m, mx);
             const float al = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - mn) * fac);
             m = mn;
-            mf = mn * fac;
             lim = mn + over;
             ol *= al;
 #pragma unroll
@@ -721,8 +721,8 @@ __global__ void __launch_bounds__(256, WIDE ? 2 : 3) k_attn_kv4(
         u4 pa, pb;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const f2 x = {__builtin_amdgcn_exp2f(fmaf(p[0][i], fac, -mf)),
-                          __builtin_amdgcn_exp2f(fmaf(p[1][i], fac, -mf))};
+            const f2 x = {__builtin_amdgcn_exp2f((p[0][i] - m) * fac),
+                          __builtin_amdgcn_exp2f((p[1][i] - m) * fac)};
             const h2 hi = __builtin_convertvector(x, h2);
             if constexpr (WIDE) {
                 pa[i] = as_u(hi);
@@ -769,6 +769,7 @@ __global__ void __launch_bounds__(256, WIDE ? 2 : 3) k_attn_kv4(
     }
     // the wavefronts' states meet in LDS
     const float lsum = WIDE ? ol[0] : ror8_add(ol[0]);
+    if (lsum != lsum) m = 0.0f;  // no score of a NaN query passes a limit: not an empty state
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) {
         f4 v = o[dt];
@@ -778,8 +779,9 @@ __global__ void __launch_bounds__(256, WIDE ? 2 : 3) k_attn_kv4(
         if (col < per) *(f4 *)&mo[wave][col][16 * dt + 4 * g] = v * 16.0f;
     }
     if (g == 0 && col < per) {
-        mm[wave][col] = mf;
+        mm[wave][col] = m;
         ml[wave][col] = lsum;
+        if (wave == 0) units[col] = fac;
     }
     __syncthreads();
     if (tid < per) {
@@ -787,7 +789,9 @@ __global__ void __launch_bounds__(256, WIDE ? 2 : 3) k_attn_kv4(
         float l = 0.0f;
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
-            const float f = M == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mm[w][tid] - M);
+            const float f = mm[w][tid] == -INFINITY  // no position (M may be none too)
+                                ? 0.0f
+                                : __builtin_amdgcn_exp2f((mm[w][tid] - M) * units[tid]);
             sc[tid][w] = f;
             l = fmaf(ml[w][tid], f, l);
         }
@@ -795,6 +799,7 @@ __global__ void __launch_bounds__(256, WIDE ? 2 : 3) k_attn_kv4(
             const size_t pi = ((size_t)qi * qheads + g0 * per + tid) * ns + sp;
             ws_m[pi] = M;
             ws_l[pi] = l;
+            if (sp == 0) ws_u[(size_t)qi * qheads + g0 * per + tid] = units[tid];
         } else {
             linv[tid] = M == -INFINITY ? 0.0f : 1.0f / l;
         }
@@ -832,8 +837,8 @@ __global__ void __launch_bounds__(256, WIDE ? 2 : 3) k_attn_kv4(
 template <int G>
 __global__ void __launch_bounds__(8 * G) k_kv4_merge(
     int qheads, int hdim, int ns, const int *__restrict__ ctx_dev, const int *__restrict__ parts,
-    const float *__restrict__ ws_m, const float *__restrict__ ws_l,
-    const float *__restrict__ ws_o, float *__restrict__ attn, int8_t *__restrict__ qs,
+    const float *__restrict__ ws_u, const float *__restrict__ ws_m,
+    const float *__restrict__ ws_l, const float *__restrict__ ws_o, float *__restrict__ attn, int8_t *__restrict__ qs,
     uint16_t *__restrict__ d, int16_t *__restrict__ bsum, int8_t *__restrict__ tq,
     uint16_t *__restrict__ td) {
     constexpr int W = G / 8;  // wavefronts
@@ -844,6 +849,7 @@ __global__ void __launch_bounds__(8 * G) k_kv4_merge(
     const size_t base = ((size_t)qi * qheads + h) * ns;
     const int each = (ns + G - 1) / G;
     const int have = !parts ? ns : ctx_dev[qi] > 0 ? parts[qi] : 0;  // states that were written
+    const float unit = ws_u[(size_t)qi * qheads + h];
     f4 o[8];
     float m[8], l[8], mx = -INFINITY;
 #pragma unroll
@@ -875,7 +881,7 @@ __global__ void __launch_bounds__(8 * G) k_kv4_merge(
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
         if (m[k] == -INFINITY) continue;  // none, or an empty chunk (its output unwritten)
-        const float w = __builtin_amdgcn_exp2f(m[k] - mx);
+        const float w = __builtin_amdgcn_exp2f((m[k] - mx) * unit);
         sum = fmaf(l[k], w, sum);
 #pragma unroll
         for (int i = 0; i < 4; ++i) acc[i] = fmaf(o[k][i], w, acc[i]);
@@ -982,14 +988,25 @@ static int attn_kv4_chunks(int hdim, int kvheads, int nq, int max_ctx, bool ragg
     return (int)max(1ll, min(min(most, want), 256ll));
 }
 
-// Whether a prompt's pages are read into fp16 rows for the prefill kernel
-static bool kv4_by_rows(int nq, int ctx_step) { return ctx_step == 1 && nq > 4; }
+// Whether a prompt's pages are read into fp16 rows for the prefill kernel, which
+// walks the context once for 32 rows of queries and heads, in one workgroup: it
+// pays where those fill the GPU.  Both ways (us a call, over the pages | by rows;
+// after 1500 and after 24000 positions): 28/4 heads of 128, 16 queries 14 | 27,
+// 36 | 268; 128 queries 30 | 29, 232 | 268; 192 30 | 31, 325 | 268; 333 53 | 36,
+// 580 | 298.  14/2 of 64, 256 queries 22 | 21, 148 | 192; 24/8 of 96, 64 queries
+// 23 | 26, 191 | 246, 128 31 | 26, 352 | 245; 8/8 of 32, 64 17 | 17, 108 | 170, 128
+// 19 | 17, 204 | 170.
+static bool kv4_by_rows(int kvheads, int nq, int ctx_step) {
+    return ctx_step == 1 && (long long)nq * kvheads > 512;
+}
 
 size_t attn_kv4_workspace(int qheads, int kvheads, int hdim, int nq, int ctx_step, int max_ctx) {
-    if (kv4_by_rows(nq, ctx_step)) return (size_t)max_ctx * kvheads * hdim * 2 * sizeof(uint16_t);
+    if (kv4_by_rows(kvheads, nq, ctx_step))
+        return (size_t)max_ctx * kvheads * hdim * 2 * sizeof(uint16_t);
     const int ns = attn_kv4_chunks(hdim, kvheads, nq, max_ctx, ctx_step == 0);
     if (ns == 1) return 0;
-    return (size_t)nq * qheads * ns * (hdim + 2) * sizeof(float) + (size_t)nq * sizeof(int);
+    return (size_t)nq * qheads * (ns * (size_t)(hdim + 2) + 1) * sizeof(float) +
+           (size_t)nq * sizeof(int);
 }
 
 void launch_attention_kv4(const float *q, int nq, int qheads, int hdim, const Kv4Cache &c,
@@ -997,7 +1014,7 @@ void launch_attention_kv4(const float *q, int nq, int qheads, int hdim, const Kv
                           int8_t *qs, uint16_t *d, int16_t *bsum, void *ws, hipStream_t st,
                           int8_t *tq, uint16_t *td) {
     if (nq <= 0) return;
-    if (kv4_by_rows(nq, ctx_step)) {
+    if (kv4_by_rows(c.kvheads, nq, ctx_step)) {
         uint16_t *k = (uint16_t *)ws, *v = k + (size_t)max_ctx * c.kvheads * hdim;
         launch_kv4_read(c, ctx0 - 1 + nq, hdim, 0, 1, nullptr, k, v, st);
         launch_attn_prefill(q, nq, qheads, c.kvheads, hdim, ctx0 - 1, k, v, attn, qs, d, bsum, st);
@@ -1008,13 +1025,14 @@ void launch_attention_kv4(const float *q, int nq, int qheads, int hdim, const Kv
     const int slots = a4_slots(hdim);
     const AttnParts pt(ws, (size_t)nq * qheads * ns, hdim);
     // contexts on the device: a list of chunks, its length made on the GPU
-    int *parts = ns > 1 && ctx_dev ? (int *)(pt.l + (size_t)nq * qheads * ns) : nullptr;
+    float *unit = pt.l + (size_t)nq * qheads * ns;
+    int *parts = ns > 1 && ctx_dev ? (int *)(unit + (size_t)nq * qheads) : nullptr;
     const dim3 grid(c.kvheads, parts ? slots / c.kvheads + nq : nq, parts ? 1 : ns);
     const bool wide = qheads / c.kvheads > 8, page16 = c.shift == 4;
 #define CALL2(DIM, W, P)                                                                        \
     SI_LAUNCH((k_attn_kv4<DIM, W, P>), grid, dim3(256), 0, st, q, qheads, c, ctx_dev, ctx0,     \
-              ctx_step, nq, max_ctx, ns, chunk, slots, softmax_scale2(hdim), parts, pt.m, pt.l, \
-              pt.o, attn, qs, d, bsum, tq, td)
+              ctx_step, nq, max_ctx, ns, chunk, slots, softmax_scale2(hdim), parts, unit, pt.m,  \
+              pt.l, pt.o, attn, qs, d, bsum, tq, td)
 #define CALL(DIM)                               \
     if (wide && page16) CALL2(DIM, true, true); \
     else if (wide) CALL2(DIM, true, false);     \
@@ -1026,8 +1044,8 @@ void launch_attention_kv4(const float *q, int nq, int qheads, int hdim, const Kv
     if (ns == 1) return;
     const dim3 blocks(qheads * (hdim / 32), nq);
 #define CALL(G)                                                                                  \
-    SI_LAUNCH(k_kv4_merge<G>, blocks, dim3(8 * G), 0, st, qheads, hdim, ns, ctx_dev, parts, pt.m, \
-              pt.l, pt.o, attn, qs, d, bsum, tq, td)
+    SI_LAUNCH(k_kv4_merge<G>, blocks, dim3(8 * G), 0, st, qheads, hdim, ns, ctx_dev, parts, unit, \
+              pt.m, pt.l, pt.o, attn, qs, d, bsum, tq, td)
     if (ns <= 64) CALL(8);
     else CALL(32);
 #undef CALL

@@ -433,3 +433,53 @@ def test_copy_pages_captured():
         g.replay()
         torch.cuda.synchronize()
         assert torch.equal(pools, want)
+
+
+@pytest.mark.parametrize("name", ["g7_d128", "g16_d64"])
+def test_bad_heads_stay_alone(name):
+    """NaN, infinities and sizes far apart in one query head leave the other heads' bits."""
+    rng = np.random.default_rng(6)
+    c = Cache(rng, name, 3, 700, 64)
+    q = rng.standard_normal((3, c.q, c.D)).astype(np.float32)
+    a = _attention(c, dev(q), 3, None, 700, 0, 700)
+    for bad in (np.nan, np.inf, 1e30, 1e-30):
+        q2 = q.copy()
+        q2[1, 3] *= np.float32(bad)
+        b = _attention(c, dev(q2), 3, None, 700, 0, 700, q8=False)
+        keep = np.ones((3, c.q), bool)
+        keep[1, 3] = False
+        assert np.array_equal(a[keep], b[keep]), bad
+        if np.isnan(bad):
+            assert np.isnan(b[1, 3]).all()
+        if bad in (1e30, 1e-30):  # one weight takes all; all weights are equal
+            k, v = (c.rows(p, 1, np.arange(700), i) for p, i in ((c.k0, True), (c.v0, False)))
+            want = ref.attend(q2[1], k, v)[3]
+            assert np.abs(b[1, 3] - want).max() <= 2e-5 * np.abs(want).max()
+
+
+def test_large_scores_keep_their_differences():
+    """Scores of 2^14 and weights that differ in all their bits: the weights' error goes with the
+    differences of the scores (as a difference of rounded scores it would be 2^14 2^-24 = 1e-3)."""
+    rng = np.random.default_rng(12)
+    for name in ("g7_d128", "g16_d64"):
+        c = Cache(rng, name, 2, 600, 64)
+        x = np.zeros((c.npages * 64, c.kv, c.D), np.float32)
+        x[:, :, 0] = 8.0  # the block's scale, 1: values are whole numbers
+        x[:, :, 1:32] = rng.integers(0, 2, (len(x), c.kv, 31))
+        c.k0 = ref.pack(-x, c.kv, c.D, 64, True)
+        c.k = dev(c.k0)
+        q = np.zeros((2, c.q, c.D), np.float32)
+        q[:, :, 0] = -2.0 ** 14  # times -8 over sqrt(D): the same large score for every position
+        q[:, :, 1:32] = rng.integers(-8, 9, (2, c.q, 31))
+        got = _attention(c, dev(q), 2, None, 600, 0, 600)
+        _close(got, _want(c, q, range(2), [600] * 2), name)
+
+
+@pytest.mark.parametrize("name,n", [("g7_d128", 128), ("g7_d128", 129), ("g1_d32", 64),
+                                    ("g1_d32", 65), ("g16_d128", 512), ("g16_d128", 513)])
+def test_prompts_at_the_border_of_the_two_ways(name, n):
+    rng = np.random.default_rng(n)
+    c = Cache(rng, name, 1, 40 + n, 32)
+    q = rng.standard_normal((n, c.q, c.D)).astype(np.float32)
+    got = _attention(c, dev(q), n, None, 41, 1, 40 + n)
+    _close(got, _want(c, q, [0] * n, np.arange(41, n + 41)), name)
