@@ -321,8 +321,9 @@ typedef float f4 __attribute__((ext_vector_type(4)));
 typedef float f2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 
-constexpr int A4_GROUP = 32;             // positions of a wavefront's step
-constexpr int A4_STEP = 4 * A4_GROUP;    // of a workgroup's
+constexpr int A4_GROUP = 32;  // positions of a wavefront's step
+// Wavefronts of a workgroup that has a CU to itself (3 or 4 a SIMD by its registers)
+constexpr int a4_big(int hdim) { return hdim > 64 ? 12 : 16; }
 
 __device__ __forceinline__ float ror8_add(float v) { return v + dpp_f<DPP_ROR8>(v); }
 
@@ -451,6 +452,7 @@ struct A4Item {
 // query.  (A grid of query x chunk instead, each workgroup past its context
 // leaving at once, kept the slots busy with those: 48 x 200-4096 24.8 us
 // against 21.3.)
+template <int step>
 __device__ __forceinline__ A4Item a4_item(int w, const int *ctx_dev, int nq, int kvheads, int ns,
                                           int max_ctx, int slots) {
     const int lane = threadIdx.x & 63;
@@ -467,10 +469,10 @@ __device__ __forceinline__ A4Item a4_item(int w, const int *ctx_dev, int nq, int
     total = uniform(wave_sum(total));
     const float n = uniform(wave_sum((float)live));
     const float share = total / fmaxf((float)slots / (float)kvheads - 0.5f * n, 1.0f);
-    const int k = min((int)((float)most / fmaxf(share, (float)A4_STEP)), ns);
-    auto steps_of = [&](int k) { return ((most + k - 1) / k + A4_STEP - 1) / A4_STEP; };
+    const int k = min((int)((float)most / fmaxf(share, (float)step)), ns);
+    auto steps_of = [&](int k) { return ((most + k - 1) / k + step - 1) / step; };
     auto parts_of = [](int ctx, int steps) {
-        return ((ctx + A4_STEP - 1) / A4_STEP + steps - 1) / steps;
+        return ((ctx + step - 1) / step + steps - 1) / steps;
     };
     int steps = steps_of(max(k, 1));
     if (k < ns) {  // one chunk more where that still fits (equal contexts)
@@ -480,7 +482,7 @@ __device__ __forceinline__ A4Item a4_item(int w, const int *ctx_dev, int nq, int
             count += parts_of(i < 64 ? first : max(min(ctx_dev[i], max_ctx), 0), more);
         if (uniform(wave_sum((float)count)) * (float)kvheads <= (float)slots) steps = more;
     }
-    A4Item it = {0, 0, 0, steps * A4_STEP, 0};
+    A4Item it = {0, 0, 0, steps * step, 0};
     for (int i0 = 0; i0 < nq; i0 += 64) {
         const int i = i0 + lane;
         const int c = i >= nq ? 0 : i0 == 0 ? first : max(min(ctx_dev[i], max_ctx), 0);
@@ -500,27 +502,27 @@ __device__ __forceinline__ A4Item a4_item(int w, const int *ctx_dev, int nq, int
     return it;
 }
 
-template <int D, bool WIDE, bool PAGE16>
-__global__ void __launch_bounds__(256, WIDE ? 2 : 3) k_attn_kv4(
+template <int D, bool WIDE, bool PAGE16, int NW>
+__global__ void __launch_bounds__(64 * NW, NW > 4 ? NW / 4 : WIDE ? 2 : 3) k_attn_kv4(
     const float *__restrict__ q, int qheads, Kv4Cache c, const int *__restrict__ ctx_dev, int ctx0,
     int ctx_step, int nq, int max_ctx, int ns, int chunk, int slots, float scale2,
     int *__restrict__ parts, float *__restrict__ ws_u, float *__restrict__ ws_m,
     float *__restrict__ ws_l, float *__restrict__ ws_o, float *__restrict__ attn,
     int8_t *__restrict__ qs, uint16_t *__restrict__ qd8, int16_t *__restrict__ bsum,
     int8_t *__restrict__ tq, uint16_t *__restrict__ td) {
-    constexpr int KS = D / 32, DT = D / 16, COLS = WIDE ? 16 : 8;
+    constexpr int KS = D / 32, DT = D / 16, COLS = WIDE ? 16 : 8, STEP = NW * A4_GROUP;
     __shared__ __attribute__((aligned(16))) float mo[4][COLS][D];
     __shared__ __attribute__((aligned(16))) u4 qop[(WIDE ? 2 : 1) * KS * 64];  // hi (, lo)
     __shared__ __attribute__((aligned(16))) f4 qc[(WIDE ? 2 : 1) * KS * 64];
-    __shared__ __attribute__((aligned(16))) uint32_t scales[4][3][64];  // K's, V's, V's * -72
-    __shared__ float mm[4][COLS], ml[4][COLS], sc[COLS][4], linv[COLS], units[COLS];
+    __shared__ __attribute__((aligned(16))) uint32_t scales[NW][3][64];  // K's, V's, V's * -72
+    __shared__ float mm[NW][COLS], ml[NW][COLS], sc[COLS][NW], linv[COLS], units[COLS];
     const int g0 = blockIdx.x, per = qheads / c.kvheads;
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = uniform(tid >> 6);
     const int col = lane & 15, g = lane >> 4;
     A4Item it;
     if (parts) {
-        it = a4_item(blockIdx.y, ctx_dev, nq, c.kvheads, ns, max_ctx, slots);
+        it = a4_item<STEP>(blockIdx.y, ctx_dev, nq, c.kvheads, ns, max_ctx, slots);
         if (it.ctx == 0) return;  // past the list
         if (g0 == 0 && it.sp == 0 && tid == 0) parts[it.qi] = it.parts;
     } else {
@@ -528,6 +530,7 @@ __global__ void __launch_bounds__(256, WIDE ? 2 : 3) k_attn_kv4(
         it.sp = blockIdx.z;
         it.ctx = min(ctx_dev ? ctx_dev[it.qi] : ctx0 + it.qi * ctx_step, max_ctx);
         it.chunk = chunk;
+        it.parts = ns;
     }
     const int qi = uniform(it.qi), sp = uniform(it.sp), seq = ctx_step ? 0 : qi;
     const int p0 = uniform(sp * it.chunk), p1 = uniform(min(it.ctx, p0 + it.chunk));
@@ -566,11 +569,11 @@ __global__ void __launch_bounds__(256, WIDE ? 2 : 3) k_attn_kv4(
     int s0 = p0 + A4_GROUP * wave;
     Kv4Group<D> ta, tb;
     {
-        const Ids ia = ids_of(s0), ib = ids_of(s0 + A4_STEP);
+        const Ids ia = ids_of(s0), ib = ids_of(s0 + STEP);
         if (s0 < p1) load(ta, s0, ia);
-        if (s0 + A4_STEP < p1) load(tb, s0 + A4_STEP, ib);
+        if (s0 + STEP < p1) load(tb, s0 + STEP, ib);
     }
-    Ids id = ids_of(s0 + 2 * A4_STEP);
+    Ids id = ids_of(s0 + 2 * STEP);
 
     // q of the lane's column as the B operand, dims 32 b + 8 g + (0, 4, 1, 5, 2, 6,
     // 3, 7), the odd ones over 16: integers hi and lo, q = (hi + lo 2^-12) 2^(ex - 10)
@@ -758,72 +761,88 @@ __global__ void __launch_bounds__(256, WIDE ? 2 : 3) k_attn_kv4(
     };
     while (s0 < p1) {
         step(ta, s0);
-        s0 += A4_STEP;
+        s0 += STEP;
         if (s0 >= p1) break;
-        if (s0 + A4_STEP < p1) load(ta, s0 + A4_STEP, id);
-        id = ids_of(s0 + 2 * A4_STEP);
+        if (s0 + STEP < p1) load(ta, s0 + STEP, id);
+        id = ids_of(s0 + 2 * STEP);
         step(tb, s0);
-        s0 += A4_STEP;
-        if (s0 + A4_STEP < p1) load(tb, s0 + A4_STEP, id);
-        id = ids_of(s0 + 2 * A4_STEP);
+        s0 += STEP;
+        if (s0 + STEP < p1) load(tb, s0 + STEP, id);
+        id = ids_of(s0 + 2 * STEP);
     }
-    // the wavefronts' states meet in LDS
+    // The wavefronts' states meet in LDS: maxima and sums, then the outputs, four
+    // wavefronts at a time, added by a thread per four dims in wavefront order.
     const float lsum = WIDE ? ol[0] : ror8_add(ol[0]);
     if (lsum != lsum) m = 0.0f;  // no score of a NaN query passes a limit: not an empty state
-#pragma unroll
-    for (int dt = 0; dt < DT; ++dt) {
-        f4 v = o[dt];
-        if constexpr (!WIDE)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] = ror8_add(v[i]);
-        if (col < per) *(f4 *)&mo[wave][col][16 * dt + 4 * g] = v * 16.0f;
-    }
     if (g == 0 && col < per) {
         mm[wave][col] = m;
         ml[wave][col] = lsum;
         if (wave == 0) units[col] = fac;
     }
+    const bool whole = it.parts == 1;  // the query's only chunk
     __syncthreads();
     if (tid < per) {
-        const float M = fmaxf(fmaxf(mm[0][tid], mm[1][tid]), fmaxf(mm[2][tid], mm[3][tid]));
-        float l = 0.0f;
+        float M = mm[0][tid], l = 0.0f;
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
+        for (int w = 1; w < NW; ++w) M = fmaxf(M, mm[w][tid]);
+#pragma unroll
+        for (int w = 0; w < NW; ++w) {
             const float f = mm[w][tid] == -INFINITY  // no position (M may be none too)
                                 ? 0.0f
                                 : __builtin_amdgcn_exp2f((mm[w][tid] - M) * units[tid]);
             sc[tid][w] = f;
             l = fmaf(ml[w][tid], f, l);
         }
-        if (ns > 1) {
+        if (whole) {
+            linv[tid] = M == -INFINITY ? 0.0f : 1.0f / l;
+        } else {
             const size_t pi = ((size_t)qi * qheads + g0 * per + tid) * ns + sp;
             ws_m[pi] = M;
             ws_l[pi] = l;
             if (sp == 0) ws_u[(size_t)qi * qheads + g0 * per + tid] = units[tid];
-        } else {
-            linv[tid] = M == -INFINITY ? 0.0f : 1.0f / l;
         }
     }
-    __syncthreads();
-    for (int e0 = 0; e0 < per * D / 4; e0 += 256) {  // 8 lanes hold a Q8_0 block
-        const int e4 = e0 + tid;
-        if (e4 >= per * D / 4) break;
-        const int h = e4 / (D / 4), dd = e4 % (D / 4) * 4;
-        f4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+    constexpr int SLOTS = (COLS * D / 4 + 64 * NW - 1) / (64 * NW);  // of a thread
+    f4 acc[SLOTS];
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-            const f4 v = *(const f4 *)&mo[w][h][dd];
-            const float f = sc[h][w];
+    for (int i = 0; i < SLOTS; ++i) acc[i] = (f4){0.0f, 0.0f, 0.0f, 0.0f};
+    for (int w0 = 0; w0 < NW; w0 += 4) {
+        if (wave >= w0 && wave < w0 + 4) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) acc[i] = fmaf(v[i], f, acc[i]);
+            for (int dt = 0; dt < DT; ++dt) {
+                f4 v = o[dt];
+                if constexpr (!WIDE)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) v[i] = ror8_add(v[i]);
+                if (col < per) *(f4 *)&mo[wave - w0][col][16 * dt + 4 * g] = v * 16.0f;
+            }
         }
-        const int head = g0 * per + h;
-        if (ns > 1) {
-            *(f4 *)(ws_o + (((size_t)qi * qheads + head) * ns + sp) * D + dd) = acc;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < SLOTS; ++i) {
+            const int e4 = i * 64 * NW + tid, h = e4 / (D / 4), dd = e4 % (D / 4) * 4;
+            if (h >= per) break;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                const f4 v = *(const f4 *)&mo[w][h][dd];
+                const float f = sc[h][w0 + w];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(v[j], f, acc[i][j]);
+            }
+        }
+        if (w0 + 4 < NW) __syncthreads();
+    }
+#pragma unroll
+    for (int i = 0; i < SLOTS; ++i) {  // 8 lanes hold a Q8_0 block
+        const int e4 = i * 64 * NW + tid, h = e4 / (D / 4), dd = e4 % (D / 4) * 4;
+        if (h >= per) break;
+        const size_t row = (size_t)qi * qheads + g0 * per + h;
+        if (whole) {
+            const float r = linv[h];
+            const float y[4] = {acc[i][0] * r, acc[i][1] * r, acc[i][2] * r, acc[i][3] * r};
+            kv4_store(y, row * D + dd, e4 & 7, attn, qs, qd8, bsum, tq, td, qheads * D, qi);
         } else {
-            const float r = linv[h], y[4] = {acc[0] * r, acc[1] * r, acc[2] * r, acc[3] * r};
-            kv4_store(y, ((size_t)qi * qheads + head) * D + dd, e4 & 7, attn, qs, qd8, bsum, tq, td,
-                      qheads * D, qi);
+            *(f4 *)(ws_o + (row * ns + sp) * D + dd) = acc[i];
         }
     }
 }
@@ -849,6 +868,7 @@ __global__ void __launch_bounds__(8 * G) k_kv4_merge(
     const size_t base = ((size_t)qi * qheads + h) * ns;
     const int each = (ns + G - 1) / G;
     const int have = !parts ? ns : ctx_dev[qi] > 0 ? parts[qi] : 0;  // states that were written
+    if (parts && have == 1) return;  // its workgroup wrote the output
     const float unit = ws_u[(size_t)qi * qheads + h];
     f4 o[8];
     float m[8], l[8], mx = -INFINITY;
@@ -977,15 +997,34 @@ void launch_kv4_read(const Kv4Cache &c, int ntok, int hdim, int pos0, int pos_st
 #undef CALL
 }
 
-// Workgroups the GPU holds at once (by the kernel's registers)
-static int a4_slots(int hdim) { return hdim > 64 ? 768 : 1024; }
-// Most chunks of a context: of equal contexts as many as fill those; of contexts
-// on the device up to twice that, which the kernel uses as they are ragged.
-static int attn_kv4_chunks(int hdim, int kvheads, int nq, int max_ctx, bool ragged) {
-    const long long most = (max_ctx + A4_STEP - 1) / A4_STEP, base = (long long)kvheads * nq;
-    if (base >= a4_slots(hdim)) return 1;
-    const long long want = (a4_slots(hdim) + base - 1) / base * (ragged ? 2 : 1);
-    return (int)max(1ll, min(min(most, want), 256ll));
+// How a call runs: wavefronts a workgroup, the most chunks of a context, and the
+// workgroups that the GPU holds at once.  By base, the (query, KV head) pairs, and
+// the steps of 128 positions of the longest context (device contexts: of max_ctx);
+// us a call, split | whole | whole in big workgroups, contexts equal (, 1/16 to all
+// of the longest):
+//   - whole in four wavefronts up to 5 + base / 32 steps: the merge and its launch
+//     cost about 4 us, and a wavefront alone on its SIMD steps twice as fast as one
+//     of three.  28/4 heads of 128: 1 query of 512 9 | 8, of 1024 9 | 11; 32 of 1024 15
+//     | 14; 48 of 1024 18 | 14, of 2048 22 | 22; 128 of 2048 41 | 36, of 4096 70 | 69.
+//     14/2 of 64: 64 of 1024 13 | 10, of 2048 15 | 16.
+//   - whole in a workgroup as large as a CU holds where those about fill the GPU,
+//     and up to 32 steps, past which a ragged batch waits for its longest: 28/4 heads of
+//     128, 64 queries of 2048 25 | 23 | 21, of 4096 41 | 46 | 37 (29 | 39 | 29); 48 of 4096
+//     33 | 42 | 31 (25 | 37 | 28).  14/2 of 64, 128 of 4096 26 | 28 | 21 (21 | 27 | 20), of
+//     16384 73 | 112 | 69 (46 | 105 | 58).
+//   - else split into chunks: as many as fill the GPU, twice that for contexts on the
+//     device, which the kernel uses as they are ragged.
+struct A4Plan {
+    int nw, ns, slots;
+};
+static A4Plan a4_plan(int hdim, int kvheads, int nq, int max_ctx, bool ragged) {
+    const long long base = (long long)kvheads * nq;
+    const long long steps = (max_ctx + 4 * A4_GROUP - 1) / (4 * A4_GROUP);
+    const int slots = hdim > 64 ? 768 : 1024;
+    if (base >= slots || steps <= 5 + base / 32) return {4, 1, slots};
+    if (base > 192 && base <= 256 && steps <= 32) return {a4_big(hdim), 1, slots};
+    const long long want = (slots + base - 1) / base * (ragged ? 2 : 1);
+    return {4, (int)min(min(steps, want), 256ll), slots};
 }
 
 // Whether a prompt's pages are read into fp16 rows for the prefill kernel, which
@@ -1003,7 +1042,8 @@ static bool kv4_by_rows(int kvheads, int nq, int ctx_step) {
 size_t attn_kv4_workspace(int qheads, int kvheads, int hdim, int nq, int ctx_step, int max_ctx) {
     if (kv4_by_rows(kvheads, nq, ctx_step))
         return (size_t)max_ctx * kvheads * hdim * 2 * sizeof(uint16_t);
-    const int ns = attn_kv4_chunks(hdim, kvheads, nq, max_ctx, ctx_step == 0);
+    const int ns = max(a4_plan(hdim, kvheads, nq, max_ctx, false).ns,
+                       ctx_step ? 1 : a4_plan(hdim, kvheads, nq, max_ctx, true).ns);
     if (ns == 1) return 0;
     return (size_t)nq * qheads * (ns * (size_t)(hdim + 2) + 1) * sizeof(float) +
            (size_t)nq * sizeof(int);
@@ -1020,27 +1060,32 @@ void launch_attention_kv4(const float *q, int nq, int qheads, int hdim, const Kv
         launch_attn_prefill(q, nq, qheads, c.kvheads, hdim, ctx0 - 1, k, v, attn, qs, d, bsum, st);
         return;
     }
-    const int ns = attn_kv4_chunks(hdim, c.kvheads, nq, max_ctx, ctx_dev != nullptr);
-    const int chunk = ((max_ctx + ns - 1) / ns + A4_STEP - 1) / A4_STEP * A4_STEP;
-    const int slots = a4_slots(hdim);
+    const A4Plan plan = a4_plan(hdim, c.kvheads, nq, max_ctx, ctx_dev != nullptr);
+    const int ns = plan.ns, slots = plan.slots, step = plan.nw * A4_GROUP;
+    const int chunk = ((max_ctx + ns - 1) / ns + step - 1) / step * step;
     const AttnParts pt(ws, (size_t)nq * qheads * ns, hdim);
     // contexts on the device: a list of chunks, its length made on the GPU
     float *unit = pt.l + (size_t)nq * qheads * ns;
     int *parts = ns > 1 && ctx_dev ? (int *)(unit + (size_t)nq * qheads) : nullptr;
-    const dim3 grid(c.kvheads, parts ? slots / c.kvheads + nq : nq, parts ? 1 : ns);
+    const long long items = parts ? min((long long)slots / c.kvheads + nq, (long long)nq * ns) : nq;
+    const dim3 grid(c.kvheads, (unsigned)items, parts ? 1 : ns);
     const bool wide = qheads / c.kvheads > 8, page16 = c.shift == 4;
-#define CALL2(DIM, W, P)                                                                        \
-    SI_LAUNCH((k_attn_kv4<DIM, W, P>), grid, dim3(256), 0, st, q, qheads, c, ctx_dev, ctx0,     \
-              ctx_step, nq, max_ctx, ns, chunk, slots, softmax_scale2(hdim), parts, unit, pt.m,  \
-              pt.l, pt.o, attn, qs, d, bsum, tq, td)
-#define CALL(DIM)                               \
-    if (wide && page16) CALL2(DIM, true, true); \
-    else if (wide) CALL2(DIM, true, false);     \
-    else if (page16) CALL2(DIM, false, true);   \
-    else CALL2(DIM, false, false)
+#define CALL3(DIM, W, P, NW)                                                                     \
+    SI_LAUNCH((k_attn_kv4<DIM, W, P, NW>), grid, dim3(64 * NW), 0, st, q, qheads, c, ctx_dev,    \
+              ctx0, ctx_step, nq, max_ctx, ns, chunk, slots, softmax_scale2(hdim), parts, unit, \
+              pt.m, pt.l, pt.o, attn, qs, d, bsum, tq, td)
+#define CALL2(DIM, W, P)                            \
+    if (plan.nw == 4) CALL3(DIM, W, P, 4);          \
+    else CALL3(DIM, W, P, a4_big(DIM))
+#define CALL(DIM)                                   \
+    if (wide && page16) { CALL2(DIM, true, true); } \
+    else if (wide) { CALL2(DIM, true, false); }     \
+    else if (page16) { CALL2(DIM, false, true); }   \
+    else { CALL2(DIM, false, false); }
     KV4_DIM(hdim, CALL)
 #undef CALL
 #undef CALL2
+#undef CALL3
     if (ns == 1) return;
     const dim3 blocks(qheads * (hdim / 32), nq);
 #define CALL(G)                                                                                  \

@@ -483,3 +483,29 @@ def test_prompts_at_the_border_of_the_two_ways(name, n):
     q = rng.standard_normal((n, c.q, c.D)).astype(np.float32)
     got = _attention(c, dev(q), n, None, 41, 1, 40 + n)
     _close(got, _want(c, q, [0] * n, np.arange(41, n + 41)), name)
+
+
+@pytest.mark.parametrize("name,nq,longest", [
+    ("g7_d128", 1, 640), ("g7_d128", 1, 641), ("g7_d128", 49, 1500), ("g7_d128", 64, 2047),
+    ("g7_d128", 65, 1700), ("g7_d64", 97, 2000), ("g16_d64", 128, 1900), ("g16_d64", 300, 300),
+    ("g3_d96", 30, 1801), ("g3_d96", 96, 33), ("g1_d32", 32, 2000), ("g1_d32", 25, 4096),
+    ("g16_d128", 193, 1500), ("g16_d128", 70, 3000), ("g9_d32", 200, 1700)])
+def test_every_plan(name, nq, longest):
+    """Calls on both sides of the rules that choose workgroups and chunks, with contexts from
+    none to the longest: a few rows against 64 bits, all of them against calls of one query
+    (another plan: fp32 sums in another order)."""
+    rng = np.random.default_rng(nq)
+    c = Cache(rng, name, nq, longest, 64)
+    ctx = rng.integers(0, longest + 1, nq).astype(np.int32)
+    ctx[rng.integers(0, nq)] = longest
+    q = rng.standard_normal((nq, c.q, c.D)).astype(np.float32)
+    got = _attention(c, dev(q), nq, dev(ctx), 0, 0, longest)
+    some = sorted({0, nq - 1, int(ctx.argmax()), int(ctx.argmin())})
+    _close(got[some], _want(c, q[some], some, ctx[some]), name)
+    equal = _attention(c, dev(q), nq, None, longest, 0, longest)  # contexts from the host
+    _close(equal[some], _want(c, q[some], some, [longest] * len(some)), name)
+    pages = c.dpages
+    for i in range(0, nq, 7):
+        c.dpages = pages[i:i + 1]
+        one = _attention(c, dev(q[i:i + 1]), 1, dev(ctx[i:i + 1]), 0, 0, longest)
+        _close(got[i:i + 1], one.astype(np.float64), (name, i))
