@@ -502,14 +502,20 @@ __device__ __forceinline__ A4Item a4_item(int w, const int *ctx_dev, int nq, int
     return it;
 }
 
-template <int D, bool WIDE, bool PAGE16, int NW>
-__global__ void __launch_bounds__(64 * NW, NW > 4 ? NW / 4 : WIDE ? 2 : 3) k_attn_kv4(
+// What a workgroup's columns are: one query's heads, up to 8 in hi and lo columns, or
+// up to 16 in two products; or 16 rows (query, head) of a prompt, whose contexts
+// end query by query.
+enum A4Mode { A4_NARROW, A4_WIDE, A4_ROWS };
+
+template <int D, int MODE, bool PAGE16, int NW>
+__global__ void __launch_bounds__(64 * NW, NW > 4 ? NW / 4 : MODE ? 2 : 3) k_attn_kv4(
     const float *__restrict__ q, int qheads, Kv4Cache c, const int *__restrict__ ctx_dev, int ctx0,
     int ctx_step, int nq, int max_ctx, int ns, int chunk, int slots, float scale2,
     int *__restrict__ parts, float *__restrict__ ws_u, float *__restrict__ ws_m,
     float *__restrict__ ws_l, float *__restrict__ ws_o, float *__restrict__ attn,
     int8_t *__restrict__ qs, uint16_t *__restrict__ qd8, int16_t *__restrict__ bsum,
     int8_t *__restrict__ tq, uint16_t *__restrict__ td) {
+    constexpr bool WIDE = MODE != A4_NARROW, ROWS = MODE == A4_ROWS;
     constexpr int KS = D / 32, DT = D / 16, COLS = WIDE ? 16 : 8, STEP = NW * A4_GROUP;
     __shared__ __attribute__((aligned(16))) float mo[4][COLS][D];
     __shared__ __attribute__((aligned(16))) u4 qop[(WIDE ? 2 : 1) * KS * 64];  // hi (, lo)
@@ -520,13 +526,17 @@ __global__ void __launch_bounds__(64 * NW, NW > 4 ? NW / 4 : WIDE ? 2 : 3) k_att
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = uniform(tid >> 6);
     const int col = lane & 15, g = lane >> 4;
+    // rows of this workgroup, the first of all its KV head's; their heads in q and
+    // the outputs
+    const int row0 = ROWS ? 16 * (int)blockIdx.y : 0;
+    const int rows = ROWS ? min(16, nq * per - row0) : per;
     A4Item it;
-    if (parts) {
+    if (!ROWS && parts) {
         it = a4_item<STEP>(blockIdx.y, ctx_dev, nq, c.kvheads, ns, max_ctx, slots);
         if (it.ctx == 0) return;  // past the list
         if (g0 == 0 && it.sp == 0 && tid == 0) parts[it.qi] = it.parts;
     } else {
-        it.qi = blockIdx.y;
+        it.qi = ROWS ? (row0 + rows - 1) / per : blockIdx.y;  // (the last one)
         it.sp = blockIdx.z;
         it.ctx = min(ctx_dev ? ctx_dev[it.qi] : ctx0 + it.qi * ctx_step, max_ctx);
         it.chunk = chunk;
@@ -534,6 +544,17 @@ __global__ void __launch_bounds__(64 * NW, NW > 4 ? NW / 4 : WIDE ? 2 : 3) k_att
     }
     const int qi = uniform(it.qi), sp = uniform(it.sp), seq = ctx_step ? 0 : qi;
     const int p0 = uniform(sp * it.chunk), p1 = uniform(min(it.ctx, p0 + it.chunk));
+    auto head_of = [&](int r) {
+        if constexpr (ROWS) {
+            const int qr = (row0 + r) / per;
+            return (size_t)qr * qheads + g0 * per + (row0 + r - qr * per);
+        } else {
+            return (size_t)qi * qheads + g0 * per + r;
+        }
+    };
+    // positions that the lane's column sees end at `end`, every column's at `all` or past it
+    const int end = ROWS ? min(ctx0 + (row0 + min(col, rows - 1)) / per, p1) : p1;
+    const int all = ROWS ? uniform(min(ctx0 + row0 / per, p1)) : p1;
     // groups of this wavefront: s0 = p0 + 32 wave, + 128, ...
     const int page_size = 1 << c.shift, nib = page_size * (D / 2);
     const size_t hb = (size_t)kv4_head_bytes(D, page_size);
@@ -590,14 +611,13 @@ __global__ void __launch_bounds__(64 * NW, NW > 4 ? NW / 4 : WIDE ? 2 : 3) k_att
         const int hc = WIDE ? col : col & 7;
         float x[8];
         if (wave < KS) {
-            const float *row = q + ((size_t)qi * qheads + g0 * per + min(hc, per - 1)) * D +
-                               32 * wave + 8 * g;
+            const float *row = q + head_of(min(hc, rows - 1)) * D + 32 * wave + 8 * g;
             float big = 0.0f;
 #pragma unroll
             for (int e = 0; e < 8; ++e) x[e] = row[e];
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                x[e] = hc < per ? x[e] : 0.0f;
+                x[e] = hc < rows ? x[e] : 0.0f;
                 big = fmaxf(big, fabsf(x[e]));
             }
             qmax[wave * 64 + lane] = big;
@@ -641,7 +661,8 @@ __global__ void __launch_bounds__(64 * NW, NW > 4 ? NW / 4 : WIDE ? 2 : 3) k_att
     // the difference, not with the scores.  The sums of the weights are one more
     // product's rows (ones . P), like the outputs in hi and lo columns.
     const float over = 8.0f * __builtin_amdgcn_rcpf(fac);
-    float m = -INFINITY, lim = -INFINITY;
+    // ref: m, or 0 while a column has seen no position.
+    float m = -INFINITY, ref = 0.0f, lim = -INFINITY;
     f4 o[DT], ol = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) o[dt] = (f4){0.0f, 0.0f, 0.0f, 0.0f};
@@ -657,8 +678,8 @@ __global__ void __launch_bounds__(64 * NW, NW > 4 ? NW / 4 : WIDE ? 2 : 3) k_att
         // order, the compiler is to keep it too (and to read q here, not before the
         // loop)
         uint32_t (*const sl)[64] = scales[wave];
-        const bool tail = s + A4_GROUP > p1;  // wavefront-uniform: positions past the end
-        if (tail) {
+        const bool tail = s + A4_GROUP > all;  // wavefront-uniform: positions past an end
+        if (s + A4_GROUP > p1) {
             // their V scales may be anything: 0 (weight 0 * NaN would stay); dword col
             // holds positions 8 g + col % 4 and 4 further
             const int at = s + 8 * g + (col & 3);
@@ -700,12 +721,12 @@ __global__ void __launch_bounds__(64 * NW, NW > 4 ? NW / 4 : WIDE ? 2 : 3) k_att
 #pragma unroll
             for (int i = 0; i < 4; ++i) p[tl][i] = WIDE ? acc[tl][i] : ror8_add(acc[tl][i]);
         if (tail) {
-            int end = p1;
-            asm volatile("" : "+s"(end));  // (a branch, not selects in every step)
+            int left = end - s - 8 * g;
+            asm volatile("" : "+v"(left));  // (a branch, not selects in every step)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                p[0][i] = s + 8 * g + i < end ? p[0][i] : -INFINITY;
-                p[1][i] = s + 8 * g + 4 + i < end ? p[1][i] : -INFINITY;
+                p[0][i] = i < left ? p[0][i] : -INFINITY;
+                p[1][i] = 4 + i < left ? p[1][i] : -INFINITY;
             }
         }
         float mx = fmaxf(fmaxf(fmaxf(p[0][0], p[0][1]), fmaxf(p[0][2], p[0][3])),
@@ -716,6 +737,7 @@ __global__ void __launch_bounds__(64 * NW, NW > 4 ? NW / 4 : WIDE ? 2 : 3) k_att
             const float mn = fmaxf(m, mx);
             const float al = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - mn) * fac);
             m = mn;
+            ref = mn == -INFINITY ? 0.0f : mn;
             lim = mn + over;
             ol *= al;
 #pragma unroll
@@ -724,8 +746,8 @@ __global__ void __launch_bounds__(64 * NW, NW > 4 ? NW / 4 : WIDE ? 2 : 3) k_att
         u4 pa, pb;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const f2 x = {__builtin_amdgcn_exp2f((p[0][i] - m) * fac),
-                          __builtin_amdgcn_exp2f((p[1][i] - m) * fac)};
+            const f2 x = {__builtin_amdgcn_exp2f((p[0][i] - ref) * fac),
+                          __builtin_amdgcn_exp2f((p[1][i] - ref) * fac)};
             const h2 hi = __builtin_convertvector(x, h2);
             if constexpr (WIDE) {
                 pa[i] = as_u(hi);
@@ -774,14 +796,14 @@ __global__ void __launch_bounds__(64 * NW, NW > 4 ? NW / 4 : WIDE ? 2 : 3) k_att
     // wavefronts at a time, added by a thread per four dims in wavefront order.
     const float lsum = WIDE ? ol[0] : ror8_add(ol[0]);
     if (lsum != lsum) m = 0.0f;  // no score of a NaN query passes a limit: not an empty state
-    if (g == 0 && col < per) {
+    if (g == 0 && col < rows) {
         mm[wave][col] = m;
         ml[wave][col] = lsum;
         if (wave == 0) units[col] = fac;
     }
     const bool whole = it.parts == 1;  // the query's only chunk
     __syncthreads();
-    if (tid < per) {
+    if (tid < rows) {
         float M = mm[0][tid], l = 0.0f;
 #pragma unroll
         for (int w = 1; w < NW; ++w) M = fmaxf(M, mm[w][tid]);
@@ -796,10 +818,10 @@ __global__ void __launch_bounds__(64 * NW, NW > 4 ? NW / 4 : WIDE ? 2 : 3) k_att
         if (whole) {
             linv[tid] = M == -INFINITY ? 0.0f : 1.0f / l;
         } else {
-            const size_t pi = ((size_t)qi * qheads + g0 * per + tid) * ns + sp;
+            const size_t head = head_of(tid), pi = head * ns + sp;
             ws_m[pi] = M;
             ws_l[pi] = l;
-            if (sp == 0) ws_u[(size_t)qi * qheads + g0 * per + tid] = units[tid];
+            if (sp == 0) ws_u[head] = units[tid];
         }
     }
     constexpr int SLOTS = (COLS * D / 4 + 64 * NW - 1) / (64 * NW);  // of a thread
@@ -814,14 +836,14 @@ __global__ void __launch_bounds__(64 * NW, NW > 4 ? NW / 4 : WIDE ? 2 : 3) k_att
                 if constexpr (!WIDE)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) v[i] = ror8_add(v[i]);
-                if (col < per) *(f4 *)&mo[wave - w0][col][16 * dt + 4 * g] = v * 16.0f;
+                if (col < rows) *(f4 *)&mo[wave - w0][col][16 * dt + 4 * g] = v * 16.0f;
             }
         }
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < SLOTS; ++i) {
             const int e4 = i * 64 * NW + tid, h = e4 / (D / 4), dd = e4 % (D / 4) * 4;
-            if (h >= per) break;
+            if (h >= rows) break;
 #pragma unroll
             for (int w = 0; w < 4; ++w) {
                 const f4 v = *(const f4 *)&mo[w][h][dd];
@@ -835,8 +857,8 @@ __global__ void __launch_bounds__(64 * NW, NW > 4 ? NW / 4 : WIDE ? 2 : 3) k_att
 #pragma unroll
     for (int i = 0; i < SLOTS; ++i) {  // 8 lanes hold a Q8_0 block
         const int e4 = i * 64 * NW + tid, h = e4 / (D / 4), dd = e4 % (D / 4) * 4;
-        if (h >= per) break;
-        const size_t row = (size_t)qi * qheads + g0 * per + h;
+        if (h >= rows) break;
+        const size_t row = head_of(h);
         if (whole) {
             const float r = linv[h];
             const float y[4] = {acc[i][0] * r, acc[i][1] * r, acc[i][2] * r, acc[i][3] * r};
@@ -998,7 +1020,8 @@ void launch_kv4_read(const Kv4Cache &c, int ntok, int hdim, int pos0, int pos_st
 }
 
 // How a call runs: wavefronts a workgroup, the most chunks of a context, and the
-// workgroups that the GPU holds at once.  By base, the (query, KV head) pairs, and
+// workgroups that the GPU holds at once.  By base, the (query, KV head) pairs or
+// blocks of 16 rows, and
 // the steps of 128 positions of the longest context (device contexts: of max_ctx);
 // us a call, split | whole | whole in big workgroups, contexts equal (, 1/16 to all
 // of the longest):
@@ -1017,8 +1040,7 @@ void launch_kv4_read(const Kv4Cache &c, int ntok, int hdim, int pos0, int pos_st
 struct A4Plan {
     int nw, ns, slots;
 };
-static A4Plan a4_plan(int hdim, int kvheads, int nq, int max_ctx, bool ragged) {
-    const long long base = (long long)kvheads * nq;
+static A4Plan a4_plan(int hdim, long long base, int max_ctx, bool ragged) {
     const long long steps = (max_ctx + 4 * A4_GROUP - 1) / (4 * A4_GROUP);
     const int slots = hdim > 64 ? 768 : 1024;
     if (base >= slots || steps <= 5 + base / 32) return {4, 1, slots};
@@ -1028,22 +1050,28 @@ static A4Plan a4_plan(int hdim, int kvheads, int nq, int max_ctx, bool ragged) {
 }
 
 // Whether a prompt's pages are read into fp16 rows for the prefill kernel, which
-// walks the context once for 32 rows of queries and heads, in one workgroup: it
-// pays where those fill the GPU.  Both ways (us a call, over the pages | by rows;
-// after 1500 and after 24000 positions): 28/4 heads of 128, 16 queries 14 | 27,
-// 36 | 268; 128 queries 30 | 29, 232 | 268; 192 30 | 31, 325 | 268; 333 53 | 36,
-// 580 | 298.  14/2 of 64, 256 queries 22 | 21, 148 | 192; 24/8 of 96, 64 queries
-// 23 | 26, 191 | 246, 128 31 | 26, 352 | 245; 8/8 of 32, 64 17 | 17, 108 | 170, 128
-// 19 | 17, 204 | 170.
-static bool kv4_by_rows(int kvheads, int nq, int ctx_step) {
-    return ctx_step == 1 && (long long)nq * kvheads > 512;
+// unpacks nothing and takes 32 rows a tile, but walks a tile's context in one
+// workgroup: it pays once its tiles fill the GPU.  Both ways (us a call, over the
+// pages | by rows, after 300 and after 6000 positions): 28/4 heads of 128, 16 queries
+// 8 | 13, 18 | 81; 256 14 | 17, 89 | 87; 333 18 | 19, 106 | 97; 512 25 | 23, 144 | 118.
+// 14/2 of 64, 512 queries 11 | 14, 56 | 58; 768 16 | 16, 77 | 64.  24/8 of 96, 333 12 | 16,
+// 72 | 80; 512 18 | 20, 93 | 93.  8/8 of 32, 1024 12 | 15, 44 | 56; 2000 22 | 23, 79 | 66.
+static bool kv4_by_rows(int qheads, int nq, int ctx_step) {
+    return ctx_step == 1 && (long long)nq * qheads > 9000;
+}
+
+// Workgroups of a call that splits no context
+static long long a4_base(int qheads, int kvheads, int nq, int ctx_step) {
+    const long long rows = (long long)nq * (qheads / kvheads);
+    return kvheads * (ctx_step && nq > 1 ? (rows + 15) / 16 : (long long)nq);
 }
 
 size_t attn_kv4_workspace(int qheads, int kvheads, int hdim, int nq, int ctx_step, int max_ctx) {
-    if (kv4_by_rows(kvheads, nq, ctx_step))
+    if (kv4_by_rows(qheads, nq, ctx_step))
         return (size_t)max_ctx * kvheads * hdim * 2 * sizeof(uint16_t);
-    const int ns = max(a4_plan(hdim, kvheads, nq, max_ctx, false).ns,
-                       ctx_step ? 1 : a4_plan(hdim, kvheads, nq, max_ctx, true).ns);
+    const long long base = a4_base(qheads, kvheads, nq, ctx_step);
+    const int ns = max(a4_plan(hdim, base, max_ctx, false).ns,
+                       ctx_step ? 1 : a4_plan(hdim, base, max_ctx, true).ns);
     if (ns == 1) return 0;
     return (size_t)nq * qheads * (ns * (size_t)(hdim + 2) + 1) * sizeof(float) +
            (size_t)nq * sizeof(int);
@@ -1054,34 +1082,37 @@ void launch_attention_kv4(const float *q, int nq, int qheads, int hdim, const Kv
                           int8_t *qs, uint16_t *d, int16_t *bsum, void *ws, hipStream_t st,
                           int8_t *tq, uint16_t *td) {
     if (nq <= 0) return;
-    if (kv4_by_rows(c.kvheads, nq, ctx_step)) {
+    if (kv4_by_rows(qheads, nq, ctx_step)) {
         uint16_t *k = (uint16_t *)ws, *v = k + (size_t)max_ctx * c.kvheads * hdim;
         launch_kv4_read(c, ctx0 - 1 + nq, hdim, 0, 1, nullptr, k, v, st);
         launch_attn_prefill(q, nq, qheads, c.kvheads, hdim, ctx0 - 1, k, v, attn, qs, d, bsum, st);
         return;
     }
-    const A4Plan plan = a4_plan(hdim, c.kvheads, nq, max_ctx, ctx_dev != nullptr);
+    const long long base = a4_base(qheads, c.kvheads, nq, ctx_step);
+    const A4Plan plan = a4_plan(hdim, base, max_ctx, ctx_dev != nullptr);
     const int ns = plan.ns, slots = plan.slots, step = plan.nw * A4_GROUP;
     const int chunk = ((max_ctx + ns - 1) / ns + step - 1) / step * step;
     const AttnParts pt(ws, (size_t)nq * qheads * ns, hdim);
     // contexts on the device: a list of chunks, its length made on the GPU
     float *unit = pt.l + (size_t)nq * qheads * ns;
     int *parts = ns > 1 && ctx_dev ? (int *)(unit + (size_t)nq * qheads) : nullptr;
-    const long long items = parts ? min((long long)slots / c.kvheads + nq, (long long)nq * ns) : nq;
+    const long long items =
+        parts ? min((long long)slots / c.kvheads + nq, (long long)nq * ns) : base / c.kvheads;
     const dim3 grid(c.kvheads, (unsigned)items, parts ? 1 : ns);
-    const bool wide = qheads / c.kvheads > 8, page16 = c.shift == 4;
-#define CALL3(DIM, W, P, NW)                                                                     \
-    SI_LAUNCH((k_attn_kv4<DIM, W, P, NW>), grid, dim3(64 * NW), 0, st, q, qheads, c, ctx_dev,    \
+    const bool rows = ctx_step && nq > 1, wide = qheads / c.kvheads > 8, page16 = c.shift == 4;
+#define CALL3(DIM, M, P, NW)                                                                    \
+    SI_LAUNCH((k_attn_kv4<DIM, M, P, NW>), grid, dim3(64 * NW), 0, st, q, qheads, c, ctx_dev,    \
               ctx0, ctx_step, nq, max_ctx, ns, chunk, slots, softmax_scale2(hdim), parts, unit, \
               pt.m, pt.l, pt.o, attn, qs, d, bsum, tq, td)
-#define CALL2(DIM, W, P)                            \
-    if (plan.nw == 4) CALL3(DIM, W, P, 4);          \
-    else CALL3(DIM, W, P, a4_big(DIM))
-#define CALL(DIM)                                   \
-    if (wide && page16) { CALL2(DIM, true, true); } \
-    else if (wide) { CALL2(DIM, true, false); }     \
-    else if (page16) { CALL2(DIM, false, true); }   \
-    else { CALL2(DIM, false, false); }
+#define CALL2(DIM, M)                                                  \
+    if (plan.nw == 4 && page16) CALL3(DIM, M, true, 4);                \
+    else if (plan.nw == 4) CALL3(DIM, M, false, 4);                    \
+    else if (page16) CALL3(DIM, M, true, a4_big(DIM));                 \
+    else CALL3(DIM, M, false, a4_big(DIM))
+#define CALL(DIM)                           \
+    if (rows) { CALL2(DIM, A4_ROWS); }      \
+    else if (wide) { CALL2(DIM, A4_WIDE); } \
+    else { CALL2(DIM, A4_NARROW); }
     KV4_DIM(hdim, CALL)
 #undef CALL
 #undef CALL2

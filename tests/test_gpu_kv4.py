@@ -475,14 +475,22 @@ def test_large_scores_keep_their_differences():
         _close(got, _want(c, q, range(2), [600] * 2), name)
 
 
-@pytest.mark.parametrize("name,n", [("g7_d128", 128), ("g7_d128", 129), ("g1_d32", 64),
-                                    ("g1_d32", 65), ("g16_d128", 512), ("g16_d128", 513)])
-def test_prompts_at_the_border_of_the_two_ways(name, n):
+@pytest.mark.parametrize("name,n,first", [
+    ("g7_d128", 321, 40), ("g7_d128", 322, 40), ("g1_d32", 1125, 0), ("g1_d32", 1126, 0),
+    ("g16_d128", 562, 3), ("g16_d128", 563, 3), ("g9_d32", 50, 2500), ("g7_d64", 7, 4000),
+    ("g3_d96", 17, 1203), ("g16_d64", 90, 1000), ("g8_d96", 33, 15)])
+def test_prompts_both_ways(name, n, first):
+    """Over the pages in blocks of 16 rows (split or not) and, past 9000 rows, by fp16 rows: the
+    first, the last and some queries between against 64 bits, and all against each query alone."""
     rng = np.random.default_rng(n)
-    c = Cache(rng, name, 1, 40 + n, 32)
+    c = Cache(rng, name, 1, first + n, 32)
     q = rng.standard_normal((n, c.q, c.D)).astype(np.float32)
-    got = _attention(c, dev(q), n, None, 41, 1, 40 + n)
-    _close(got, _want(c, q, [0] * n, np.arange(41, n + 41)), name)
+    got = _attention(c, dev(q), n, None, first + 1, 1, first + n)
+    some = sorted({0, 1, n // 3, n // 2, n - 2, n - 1})
+    _close(got[some], _want(c, q[some], [0] * len(some), first + 1 + np.array(some)), name)
+    for i in range(0, n, 41):
+        one = _attention(c, dev(q[i:i + 1]), 1, None, first + 1 + i, 0, first + n)
+        _close(got[i:i + 1], one.astype(np.float64), (name, i))
 
 
 @pytest.mark.parametrize("name,nq,longest", [
