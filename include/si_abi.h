@@ -374,10 +374,10 @@ size_t si_attention_group_workspace(const si_shape_t *s, int nheads, int context
  * page_size) bytes a page (9/32 of an fp16 page; the layout is the library's),
  * pools 16-byte aligned.  pages (device int [sequences][max_pages]) lists each
  * sequence's pages, at most 2^30 positions; ids outside [0, npages) are
- * clamped.  A cache that is not paged is one whose lists are consecutive.  Of the shape only qheads, kvheads
- * and hdim are read.
+ * clamped.  A cache that is not paged is one whose lists are consecutive.  Of
+ * the shape only qheads, kvheads and hdim are read.
  *
- * Rows are addressed in one of two ways:
+ * Rows are addressed in one of two ways (fewer than 2^24 a call):
  *   pos_step 1: ntok positions pos0, pos0 + 1, ... of the first sequence;
  *   pos_step 0: token t is one position of sequence t, ctx_dev[t] - 1 (device
  *               ints) or, with ctx_dev NULL, pos0.  A position below 0 or past
@@ -385,7 +385,8 @@ size_t si_attention_group_workspace(const si_shape_t *s, int nheads, int context
  *               nothing of that row is read or written.
  * A page that two sequences share is copied (si_kv_copy_pages) before either
  * appends to it; two rows written to the same page by one pos_step 0 call are
- * an error that is not detected (one of them may be lost). */
+ * an error that is not detected (one of them may be lost).  No buffer of a call
+ * may overlap another one of it. */
 size_t si_kv4_page_bytes(const si_shape_t *s, int page_size);
 
 /* si_rope_kv_append (RoPE as qwen_one_layer.c:172-183) into a 4-bit cache: q

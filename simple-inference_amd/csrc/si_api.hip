@@ -1682,6 +1682,7 @@ static int kv4_rows(const char *what, int ntok, int pos0, int pos_step, const in
                what);
     SI_REQUIRE(ctx_dev || ntok == 0 || pos0 + (long long)(ntok - 1) * pos_step < limit,
                "%s: positions exceed %lld", what, limit);
+    SI_REQUIRE(ntok < 1 << 24, "%s: ntok %d, at most 2^24 - 1 rows a call", what, ntok);
     return SI_OK;
 }
 

@@ -269,7 +269,8 @@ __global__ void __launch_bounds__(2 * D) k_kv4_read(Kv4Cache c, int ntok, int po
     if (!is_k) vw[t] = *(const uint32_t *)(page + kv4_v_dword(D, in_page >> 3, t));
     __syncthreads();
     if (j < un.lo || j >= un.hi) return;
-    const float d = h2f_fast(*(const uint16_t *)(page + kv4_scale(D, page_size, i, o >> 2))) * 16.0f;
+    const uint16_t h = *(const uint16_t *)(page + kv4_scale(D, page_size, i, o >> 2));
+    const float d = h2f_fast(h) * 16.0f;
     uint32_t w = 0;
     if (is_k) {
         w = *(const uint32_t *)(page + kv4_k_dword(D, i, o));
@@ -629,8 +630,9 @@ __global__ void __launch_bounds__(64 * NW, NW > 4 ? NW / 4 : MODE ? 2 : 3) k_att
         big = fmaxf(big, swap16_f(big));
         big = fmaxf(big, swap32_f(big));
         const int ex = big == 0.0f ? 0 : (int)(f2u(big) >> 23) - 127;
-        // the scores' units: 2^24 of the subnormals, 16 of the scale, q's
-        fac = __builtin_amdgcn_ldexpf(scale2, 28 + ex - 10);
+        // the scores' units: 2^24 of the subnormals, 16 of the scale, q's (finite for
+        // the largest q too, whose weights are then 0 or 1 either way)
+        fac = fminf(__builtin_amdgcn_ldexpf(scale2, 28 + ex - 10), 0x1.fffffep127f);
         if (wave < KS) {
             float hi[8], lo[8];
 #pragma unroll
@@ -751,20 +753,22 @@ __global__ void __launch_bounds__(64 * NW, NW > 4 ? NW / 4 : MODE ? 2 : 3) k_att
             const h2 hi = __builtin_convertvector(x, h2);
             if constexpr (WIDE) {
                 pa[i] = as_u(hi);
-                pb[i] = as_u((h2){(_Float16)(x[0] - (float)hi[0]), (_Float16)(x[1] - (float)hi[1])});
+                pb[i] = as_u((h2){(_Float16)(x[0] - (float)hi[0]),
+                                  (_Float16)(x[1] - (float)hi[1])});
             } else {
                 pa[i] = as_u((h2){(_Float16)fmaf(-(float)hi[0], lo_col, x[0]),
                                   (_Float16)fmaf(-(float)hi[1], lo_col, x[1])});
             }
         }
         const h8 ph = __builtin_bit_cast(h8, pa), pl = __builtin_bit_cast(h8, pb);
-        const u4 one = {0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u};
-        if constexpr (WIDE)
-            ol = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, one), pl, ol, 0, 0, 0);
-        ol = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, one), ph, ol, 0, 0, 0);
+        const u4 ones = {0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u};
+        const h8 one = __builtin_bit_cast(h8, ones);
+        if constexpr (WIDE) ol = __builtin_amdgcn_mfma_f32_16x16x32_f16(one, pl, ol, 0, 0, 0);
+        ol = __builtin_amdgcn_mfma_f32_16x16x32_f16(one, ph, ol, 0, 0, 0);
 #pragma unroll
         for (int b = 0; b < KS; ++b) {
-            const u4 hv = *(const u4 *)&sl[1][16 * g + 4 * b], off = *(const u4 *)&sl[2][16 * g + 4 * b];
+            const u4 hv = *(const u4 *)&sl[1][16 * g + 4 * b];
+            const u4 off = *(const u4 *)&sl[2][16 * g + 4 * b];
 #pragma unroll
             for (int dt = 2 * b; dt < 2 * b + 2; ++dt) {
                 const uint32_t w = t.v[dt];
@@ -862,7 +866,8 @@ __global__ void __launch_bounds__(64 * NW, NW > 4 ? NW / 4 : MODE ? 2 : 3) k_att
         if (whole) {
             const float r = linv[h];
             const float y[4] = {acc[i][0] * r, acc[i][1] * r, acc[i][2] * r, acc[i][3] * r};
-            kv4_store(y, row * D + dd, e4 & 7, attn, qs, qd8, bsum, tq, td, qheads * D, qi);
+            kv4_store(y, row * D + dd, e4 & 7, attn, qs, qd8, bsum, ROWS ? nullptr : tq, td,
+                      qheads * D, qi);
         } else {
             *(f4 *)(ws_o + (row * ns + sp) * D + dd) = acc[i];
         }
@@ -879,9 +884,9 @@ template <int G>
 __global__ void __launch_bounds__(8 * G) k_kv4_merge(
     int qheads, int hdim, int ns, const int *__restrict__ ctx_dev, const int *__restrict__ parts,
     const float *__restrict__ ws_u, const float *__restrict__ ws_m,
-    const float *__restrict__ ws_l, const float *__restrict__ ws_o, float *__restrict__ attn, int8_t *__restrict__ qs,
-    uint16_t *__restrict__ d, int16_t *__restrict__ bsum, int8_t *__restrict__ tq,
-    uint16_t *__restrict__ td) {
+    const float *__restrict__ ws_l, const float *__restrict__ ws_o, float *__restrict__ attn,
+    int8_t *__restrict__ qs, uint16_t *__restrict__ d, int16_t *__restrict__ bsum,
+    int8_t *__restrict__ tq, uint16_t *__restrict__ td) {
     constexpr int W = G / 8;  // wavefronts
     __shared__ float red_m[W], red_l[W];
     __shared__ f4 red_o[W][8];
@@ -986,7 +991,8 @@ void launch_rope_kv4(const float *qkv, int ldqkv, int ntok, int qheads, int hdim
     if (ntok <= 0) return;
     const int limit = (int)min((long long)max_pos, (long long)c.max_pages << c.shift);
     const int qy = (qheads * hdim / 2 + 2 * hdim - 1) / (2 * hdim);
-    const bool wide = ldqkv % 4 == 0 && (((uintptr_t)qkv | (uintptr_t)rc | (uintptr_t)rs) & 15) == 0;
+    const bool wide =
+        ldqkv % 4 == 0 && (((uintptr_t)qkv | (uintptr_t)rc | (uintptr_t)rs) & 15) == 0;
     const dim3 grid(kv4_units(ntok, pos0, pos_step), c.kvheads + qy);
 #define CALL(DIM)                                                                               \
     SI_LAUNCH((k_kv4_append<DIM, false>), grid, dim3(2 * DIM), 0, st, qkv, ldqkv, nullptr,      \
@@ -1041,7 +1047,7 @@ struct A4Plan {
     int nw, ns, slots;
 };
 static A4Plan a4_plan(int hdim, long long base, int max_ctx, bool ragged) {
-    const long long steps = (max_ctx + 4 * A4_GROUP - 1) / (4 * A4_GROUP);
+    const long long steps = ((long long)max_ctx + 4 * A4_GROUP - 1) / (4 * A4_GROUP);
     const int slots = hdim > 64 ? 768 : 1024;
     if (base >= slots || steps <= 5 + base / 32) return {4, 1, slots};
     if (base > 192 && base <= 256 && steps <= 32) return {a4_big(hdim), 1, slots};
@@ -1056,8 +1062,9 @@ static A4Plan a4_plan(int hdim, long long base, int max_ctx, bool ragged) {
 // 8 | 13, 18 | 81; 256 14 | 17, 89 | 87; 333 18 | 19, 106 | 97; 512 25 | 23, 144 | 118.
 // 14/2 of 64, 512 queries 11 | 14, 56 | 58; 768 16 | 16, 77 | 64.  24/8 of 96, 333 12 | 16,
 // 72 | 80; 512 18 | 20, 93 | 93.  8/8 of 32, 1024 12 | 15, 44 | 56; 2000 22 | 23, 79 | 66.
-static bool kv4_by_rows(int qheads, int nq, int ctx_step) {
-    return ctx_step == 1 && (long long)nq * qheads > 9000;
+// (Past 2^26 positions the rows would be a launch of 2^31 threads and more.)
+static bool kv4_by_rows(int qheads, int nq, int ctx_step, int max_ctx) {
+    return ctx_step == 1 && (long long)nq * qheads > 9000 && max_ctx <= 1 << 26;
 }
 
 // Workgroups of a call that splits no context
@@ -1067,7 +1074,7 @@ static long long a4_base(int qheads, int kvheads, int nq, int ctx_step) {
 }
 
 size_t attn_kv4_workspace(int qheads, int kvheads, int hdim, int nq, int ctx_step, int max_ctx) {
-    if (kv4_by_rows(qheads, nq, ctx_step))
+    if (kv4_by_rows(qheads, nq, ctx_step, max_ctx))
         return (size_t)max_ctx * kvheads * hdim * 2 * sizeof(uint16_t);
     const long long base = a4_base(qheads, kvheads, nq, ctx_step);
     const int ns = max(a4_plan(hdim, base, max_ctx, false).ns,
@@ -1082,7 +1089,7 @@ void launch_attention_kv4(const float *q, int nq, int qheads, int hdim, const Kv
                           int8_t *qs, uint16_t *d, int16_t *bsum, void *ws, hipStream_t st,
                           int8_t *tq, uint16_t *td) {
     if (nq <= 0) return;
-    if (kv4_by_rows(qheads, nq, ctx_step)) {
+    if (kv4_by_rows(qheads, nq, ctx_step, max_ctx)) {
         uint16_t *k = (uint16_t *)ws, *v = k + (size_t)max_ctx * c.kvheads * hdim;
         launch_kv4_read(c, ctx0 - 1 + nq, hdim, 0, 1, nullptr, k, v, st);
         launch_attn_prefill(q, nq, qheads, c.kvheads, hdim, ctx0 - 1, k, v, attn, qs, d, bsum, st);

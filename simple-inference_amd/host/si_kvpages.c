@@ -146,7 +146,8 @@ int si_kv_seq_grow(si_kv_pages_t *p, int seq, int len) {
      * sequence holds it too, into a copy */
     int *last = row + old / p->page_size;
     const int shared = len > old && old % p->page_size && p->seqs[*last] > 1;
-    if (need > p->max_pages || need - p->npg[seq] + shared > p->nfree) return -1; /* nothing taken */
+    if (need > p->max_pages || need - p->npg[seq] + shared > p->nfree)
+        return -1; /* nothing taken */
     if (shared) {
         int from = *last;
         /* copies run at once: of a page that is itself a pending copy, what that reads */

@@ -517,3 +517,35 @@ def test_every_plan(name, nq, longest):
         c.dpages = pages[i:i + 1]
         one = _attention(c, dev(q[i:i + 1]), 1, dev(ctx[i:i + 1]), 0, 0, longest)
         _close(got[i:i + 1], one.astype(np.float64), (name, i))
+
+
+@pytest.mark.parametrize("name", ["g7_d128", "g9_d32", "g1_d32"])
+@pytest.mark.parametrize("big", [1e34, 1e38, 3.4e38])
+def test_largest_queries(name, big):
+    """Queries up to fp32's largest: every weight 0 or 1 (the two best scores of 40 differ by far
+    more than a rounding of either), which no unit's overflow may turn into NaN."""
+    rng = np.random.default_rng(5)
+    c = Cache(rng, name, 3, 300, 32)
+    q = (np.clip(rng.standard_normal((3, c.q, c.D)), -1, 1) * big).astype(np.float32)
+    for ctx in (40, 300):
+        got = _attention(c, dev(q), 3, None, ctx, 0, 300)
+        _close(got, _want(c, q, range(3), np.full(3, ctx)), (name, big, ctx))
+    got = _attention(c, dev(q), 3, None, 38, 1, 300)
+    _close(got, _want(c, q, [0] * 3, np.arange(38, 41)), (name, big))
+
+
+def test_prompts_of_a_very_long_cache():
+    """More rows than go over the pages, in lists of 2^27 positions: no fp16 rows of them all."""
+    rng = np.random.default_rng(6)
+    c = Cache(rng, "g1_d32", 1, 2048, 2048)
+    n, first = 1200, 7
+    q = rng.standard_normal((n, c.q, c.D)).astype(np.float32)
+    some = np.array([0, 1, 600, n - 1])
+    want = _want(c, q[some], [0] * len(some), first + some)
+    by_rows = _attention(c, dev(q), n, None, first, 1, 2048)
+    _close(by_rows[some], want, "rows")
+    c.max_pages = (1 << 27) // 2048
+    c.dpages = dev(np.full((1, c.max_pages), c.pages[0, 0], np.int32))
+    ws = si_amd.lib().si_attention_kv4_workspace(c.s(), n, 1, 1 << 27)
+    assert ws < 1 << 28
+    _close(_attention(c, dev(q), n, None, first, 1, 1 << 27)[some], want, "pages")

@@ -53,6 +53,7 @@ ROW_CASES = [
     (dict(step=1), b"ctx_dev goes with"), (dict(ctx=None, pos0=64), b"exceed 64"),
     (dict(ctx=None, step=1, pos0=63), b"exceed 64"),
     (dict(ctx=None, step=1, ntok=2 ** 31 - 1, pos0=2 ** 31 - 1), b"exceed"),
+    (dict(ntok=1 << 24), b"2^24 - 1 rows"),
 ]
 
 
@@ -109,6 +110,18 @@ def test_attention_workspace():
         for bad in (dict(ws_bytes=need - 1), dict(ws=None), dict(ws=(1 << 16) + 16)):
             assert attention(ctx=None, ctx0=1, step=1, **bad) == si_amd.SI_ERR_ARG
             assert b"workspace" in L.si_last_error()
+
+
+def test_workspace_of_long_prompts():
+    """A prompt of more than 9000 (query, head) rows takes fp16 rows of max_ctx positions, but
+    not past 2^26 of them; the largest contexts do not wrap."""
+    L = si_amd.lib()
+    rows = lambda n: L.si_attention_kv4_workspace(S, 400, 1, n)
+    assert rows(1 << 16) == (1 << 16) * 4 * 128 * 4 and rows(1 << 26) == (1 << 26) * 4 * 128 * 4
+    assert rows((1 << 26) + 1) < 1 << 28
+    for nq, step in ((1, 0), (64, 0), (400, 1)):
+        a, b = (L.si_attention_kv4_workspace(S, nq, step, n) for n in (1 << 30, 2 ** 31 - 1))
+        assert a == b > 0
 
 
 def test_no_rows_is_no_work():
