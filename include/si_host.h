@@ -279,7 +279,10 @@ int si_stack_nseq(const si_stack_t *st);
  * else 0. */
 int si_stack_prepare(si_stack_t *st, const int *seqs, int nseq);
 /* si_kv_seq_fork of the stack's pages: the next si_stack_prepare with one of
- * them copies the page they would both append to, in every pool. */
+ * them copies the page they would both append to, in every pool.  That copy and
+ * si_stack_compact's run in order with the stack's decodes; a caller that reads
+ * or writes the pools on a stream of its own (si_kv4_write, si_kv4_read) has
+ * finished that work before either call, and starts more after it returns. */
 int si_stack_fork(si_stack_t *st, int seq);
 /* si_kv_compact with its copies in every pool (waits for them, and for the
  * stream of the last decode); a si_stack_prepare has to follow. */

@@ -134,8 +134,12 @@ static int kv4_units(int ntok, int pos0, int pos_step) {
 // whose dword holds the unit's 8 positions (one that is not written whole keeps
 // its other nibbles).  (V by a thread per dim with all 8 positions took 8
 // reductions over 32 lanes one after another: 5000 fp16 rows of 2 heads of 128
-// 7.0 us, 5.2 so.)
+// 7.0 us, 5.0 so.)
 // HALF_IN: the rows are fp16 cache rows (kin, vin), copied in without RoPE.
+// Many rows are bound by memory: 1999 rows of 28/4 heads of 128, 69 MB with q in
+// and out, 14.1 us (4.9 TB/s; a large copy reaches 4.8).  Few by their launch and one
+// chain of loads, reduction and store: 64 rows 4.1 us, 1 row 3.3, 5000 fp16 rows
+// of 2 heads of 128 (6.6 MB) 5.0.
 // ---------------------------------------------------------------------------
 // 8 floats, 16 bytes a load where the call's buffers allow it
 __device__ __forceinline__ void load8(const float *p, bool wide, float (&v)[8]) {
@@ -247,7 +251,9 @@ __global__ void __launch_bounds__(2 * D) k_kv4_append(
 }
 
 // ---------------------------------------------------------------------------
-// rows back as fp16, exactly: the same units and threads
+// rows back as fp16, exactly: the same units and threads.  A launch and one chain
+// of loads (page id, nibbles and scale): 1 row 2.2 us, 1999 rows of 4 heads of 128
+// (5.2 MB) 4.4, 5000 of 2 (6.6 MB) 4.1.
 // ---------------------------------------------------------------------------
 template <int D>
 __global__ void __launch_bounds__(2 * D) k_kv4_read(Kv4Cache c, int ntok, int pos0, int pos_step,
@@ -290,8 +296,9 @@ __global__ void __launch_bounds__(2 * D) k_kv4_read(Kv4Cache c, int ntok, int po
 }
 
 // ---------------------------------------------------------------------------
-// attention over the pages: a workgroup per (context chunk, KV head, query), its
-// four wavefronts take every fourth group of 32 positions.  Per group
+// attention over the pages: a workgroup per (KV head, query, context chunk), or per
+// 16 rows (query, head) of a prompt, whose NW wavefronts take every NW-th group of
+// 32 positions.  Per group
 //     S^T[pos][head] = K[pos][:] . q[head][:]        (v_mfma_f32_16x16x32_f16)
 //     O^T[dim][head] += V^T[dim][pos] . P[pos][head]
 // with the group's two score tiles' rows placed so that lane (col, g) gets the
@@ -315,6 +322,15 @@ __global__ void __launch_bounds__(2 * D) k_kv4_read(Kv4Cache c, int ntok, int po
 //
 // The running maximum is moved only when a score passes it by 2^8 (weights up to
 // 256 fit the fp16 pair as well as weights up to 1), a wavefront-uniform branch.
+//
+// What bounds it: a step of 32 positions is about 230 vector operations and 17 matrix
+// instructions (two products: 260 and 34), which hardly overlap, 0.7 us of a SIMD at
+// 128 dims, about as long as its 4.6 KB take to arrive.  64 queries x 4096 of 28/4 heads
+// of 128, 153 MB: 34 us (4.4 TB/s; a large copy reaches 4.8); its loads alone 30, its
+// arithmetic alone 28.  Fewer bytes leave 5 us of launch, page id, first group, last
+// step and the wavefronts' meeting, and the merge of chunks: 48 x 200-4096 (62 MB) 20.7
+// + 3.9 us, 2 queries of 12/2 heads over 60000-131072 (65 MB) 18.9 + 4.0, one query of
+// 14/2 heads of 64 over 1024 5.6 + 3.0.
 // ---------------------------------------------------------------------------
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
@@ -556,7 +572,7 @@ __global__ void __launch_bounds__(64 * NW, NW > 4 ? NW / 4 : MODE ? 2 : 3) k_att
     // positions that the lane's column sees end at `end`, every column's at `all` or past it
     const int end = ROWS ? min(ctx0 + (row0 + min(col, rows - 1)) / per, p1) : p1;
     const int all = ROWS ? uniform(min(ctx0 + row0 / per, p1)) : p1;
-    // groups of this wavefront: s0 = p0 + 32 wave, + 128, ...
+    // groups of this wavefront: s0 = p0 + 32 wave, + STEP, ...
     const int page_size = 1 << c.shift, nib = page_size * (D / 2);
     const size_t hb = (size_t)kv4_head_bytes(D, page_size);
     // (constant memory: scalar loads, which the vector loads' order does not wait for)
@@ -877,7 +893,8 @@ __global__ void __launch_bounds__(64 * NW, NW > 4 ? NW / 4 : MODE ? 2 : 3) k_att
 // ---------------------------------------------------------------------------
 // The chunks' states of a (query, head) to its output: a workgroup per 32 dims
 // (one Q8_0 block), 8 lanes a state, G states at once, at most 8 G in all, so
-// that every load is in flight at once.  tq/td (optional): the Q8_0 also
+// that every load is in flight at once: 2.9-4.0 us, a launch, one round trip and the
+// stores.  tq/td (optional): the Q8_0 also
 // operand-tiled (q8_tiled_byte).
 // ---------------------------------------------------------------------------
 template <int G>
@@ -962,7 +979,9 @@ __global__ void __launch_bounds__(8 * G) k_kv4_merge(
 
 // ---------------------------------------------------------------------------
 // page copies: grid (pieces of a page, moves, pools); the pools' addresses and
-// the moves travel in the kernel's arguments, so the call needs no upload
+// the moves travel in the kernel's arguments, so the call needs no upload.  500
+// pages of 64 KB in 16 pools (1.05 GB read and written) 210 us, 5.0 TB/s; 3 pages of
+// 18 KB in 56 pools 3.1 us.
 // ---------------------------------------------------------------------------
 template <class T>
 __global__ void __launch_bounds__(256) k_kv_copy(KvMoves mv, size_t page_bytes) {
@@ -1027,8 +1046,8 @@ void launch_kv4_read(const Kv4Cache &c, int ntok, int hdim, int pos0, int pos_st
 
 // How a call runs: wavefronts a workgroup, the most chunks of a context, and the
 // workgroups that the GPU holds at once.  By base, the (query, KV head) pairs or
-// blocks of 16 rows, and
-// the steps of 128 positions of the longest context (device contexts: of max_ctx);
+// blocks of 16 rows, and the steps of 128 positions of the longest context (device
+// contexts: of max_ctx);
 // us a call, split | whole | whole in big workgroups, contexts equal (, 1/16 to all
 // of the longest):
 //   - whole in four wavefronts up to 5 + base / 32 steps: the merge and its launch

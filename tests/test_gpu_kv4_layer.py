@@ -376,3 +376,59 @@ def test_decode_captured(oracle):
         assert torch.equal(out, want)
         assert all(torch.equal(a, b) for a, b in zip(pools, held))
     L.close()
+
+
+def test_prompt_through_rows_then_decode(oracle):
+    """A prompt in two pieces through an fp16 cache of its own, the second over the first's rows
+    read back from the pages, then tokens decoded over them."""
+    torch = _torch()
+    sd = si_amd.SHAPES["0.5b"]
+    s, os_ = si_amd.make_shape(**sd), or_shape(**sd)
+    D, kvd, qd = s.hdim, s.kvheads * s.hdim, s.qheads * s.hdim
+    rng, ps, mp, npages = np.random.default_rng(8), 16, 5, 9
+    L = si_amd.Layer(s, make_layer(oracle, os_, 8), 32, 80)
+    page = si_amd.lib().si_kv4_page_bytes(ctypes.byref(s), ps)
+    pools = [torch.zeros(npages * page, dtype=torch.uint8, device="cuda") for _ in "kv"]
+    table = rng.permutation(npages)[:mp].astype(np.int32)
+    dt = dev(table.reshape(1, mp))
+    cache = (si_amd.ptr(pools[0]), si_amd.ptr(pools[1]), npages, ps, si_amd.ptr(dt), mp)
+    shape = ctypes.byref(s)
+
+    def rows(n):
+        return [ref.rows(host(t).reshape(npages, s.kvheads, -1), table, np.arange(n), s.kvheads, D,
+                         ps, k) for t, k in zip(pools, (True, False))]
+
+    done = 0
+    for n in (21, 24):
+        k, v = (torch.zeros(done + n, kvd, dtype=torch.float16, device="cuda") for _ in "kv")
+        si_amd.call("si_kv4_read", shape, *cache, done, 0, 1, None, si_amd.ptr(k), si_amd.ptr(v),
+                    None)
+        torch.cuda.synchronize()
+        before = rows(done)
+        for t, want in zip((k, v), before):
+            assert np.array_equal(host(t)[:done].reshape(want.shape), want)
+        x = dev(rng.standard_normal((n, s.hidden)).astype(np.float32))
+        L.prefill(x, n, done, k, v, empty((n, s.hidden), torch.float32))
+        torch.cuda.synchronize()
+        q = host(_buf(L, "Q", n, qd)).reshape(n, s.qheads, D)
+        kk, vv = (host(t).astype(np.float64).reshape(-1, s.kvheads, D) for t in (k, v))
+        want = np.stack([ref.attend(q[i], kk[:done + i + 1], vv[:done + i + 1]) for i in range(n)])
+        _close(host(_buf(L, "ATTN", n, qd)).reshape(n, s.qheads, D), want, n)
+        si_amd.call("si_kv4_write", shape, si_amd.ptr(k[done:]), si_amd.ptr(v[done:]), n, done, 1,
+                    None, *cache, None)
+        torch.cuda.synchronize()
+        for now, old, t in zip(rows(done + n), before, (k, v)):
+            assert np.array_equal(now[:done], old)
+            assert np.array_equal(now[done:], ref.held(
+                host(t)[done:].astype(np.float32).reshape(n, s.kvheads, D)))
+        done += n
+    for _ in range(3):
+        done += 1
+        x = dev(rng.standard_normal((1, s.hidden)).astype(np.float32))
+        L.decode_kv4(x, 1, *pools, npages, ps, dt, mp, dev(np.array([done], np.int32)), 80,
+                     empty((1, s.hidden), torch.float32))
+        torch.cuda.synchronize()
+        q = host(_buf(L, "Q", 1, qd)).reshape(1, s.qheads, D)
+        _close(host(_buf(L, "ATTN", 1, qd)).reshape(1, s.qheads, D),
+               ref.attend(q[0], *rows(done))[None], done)
+    L.close()

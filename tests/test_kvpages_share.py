@@ -244,7 +244,13 @@ def test_random_workload_keeps_every_sequence(H, seed):
 @pytest.mark.parametrize("code,msg", [
     ("H.si_kv_seq_fork(p, 1)", "unknown sequence"), ("H.si_kv_seq_truncate(p, 0, 6)", "length"),
     ("H.si_kv_seq_truncate(p, 0, -1)", "length"), ("H.si_kv_pages_resize(p, 0)", "npages"),
-    ("H.si_kv_seq_fork(p, 0); H.si_kv_seq_grow(p, 1, 6); H.si_kv_compact(p)", "pending")])
+    ("H.si_kv_seq_fork(p, 0); H.si_kv_seq_grow(p, 1, 6); H.si_kv_compact(p)", "pending"),
+    ("H.si_stack_create_kv(si_amd.make_shape(**si_amd.SHAPES['0.5b']), None, 1, 1, 64, 4, 16, 2)",
+     "unknown K/V format"),
+    ("H.si_stack_create_kv(si_amd.make_shape(**si_amd.SHAPES['0.5b']), None, 1, 1, 64, 4, 8, 1)",
+     "16..65536"),
+    ("H.si_stack_create_kv(si_amd.make_shape(896, 14, 2, 48), None, 1, 1, 64, 4, 16, 1)",
+     "16..65536")])
 def test_misuse_dies(code, msg):
     import subprocess
     import sys
