@@ -320,8 +320,9 @@ __global__ void __launch_bounds__(2 * D) k_kv4_read(Kv4Cache c, int ntok, int po
 // columns 0-7 carry hi, 8-15 lo, and their results are added across (WIDE: 9 to
 // 16 heads, two products).
 //
-// The running maximum is moved only when a score passes it by 2^8 (weights up to
-// 256 fit the fp16 pair as well as weights up to 1), a wavefront-uniform branch.
+// A column's running maximum is moved only when a score of its own passes it by 2^8
+// (weights up to 256 fit the fp16 pair as well as weights up to 1), in a branch that
+// the wavefront takes together: no head's bits depend on the other heads'.
 //
 // What bounds it: a step of 32 positions is about 230 vector operations and 17 matrix
 // instructions (two products: 260 and 34), which hardly overlap, 0.7 us of a SIMD at
@@ -339,8 +340,6 @@ typedef float f2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 
 constexpr int A4_GROUP = 32;  // positions of a wavefront's step
-// Wavefronts of a workgroup that has a CU to itself (3 or 4 a SIMD by its registers)
-constexpr int a4_big(int hdim) { return hdim > 64 ? 12 : 16; }
 
 __device__ __forceinline__ float ror8_add(float v) { return v + dpp_f<DPP_ROR8>(v); }
 
@@ -525,7 +524,7 @@ __device__ __forceinline__ A4Item a4_item(int w, const int *ctx_dev, int nq, int
 enum A4Mode { A4_NARROW, A4_WIDE, A4_ROWS };
 
 template <int D, int MODE, bool PAGE16, int NW>
-__global__ void __launch_bounds__(64 * NW, NW > 4 ? NW / 4 : MODE ? 2 : 3) k_attn_kv4(
+__global__ void __launch_bounds__(64 * NW, NW > 4 || MODE ? 2 : 3) k_attn_kv4(
     const float *__restrict__ q, int qheads, Kv4Cache c, const int *__restrict__ ctx_dev, int ctx0,
     int ctx_step, int nq, int max_ctx, int ns, int chunk, int slots, float scale2,
     int *__restrict__ parts, float *__restrict__ ws_u, float *__restrict__ ws_m,
@@ -752,7 +751,7 @@ __global__ void __launch_bounds__(64 * NW, NW > 4 ? NW / 4 : MODE ? 2 : 3) k_att
         if (__ballot(mx > lim)) {
             mx = fmaxf(mx, swap16_f(mx));
             mx = fmaxf(mx, swap32_f(mx));
-            const float mn = fmaxf(m, mx);
+            const float mn = mx > lim ? mx : m;  // the column's own, whatever the others do
             const float al = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - mn) * fac);
             m = mn;
             ref = mn == -INFINITY ? 0.0f : mn;
@@ -1048,18 +1047,22 @@ void launch_kv4_read(const Kv4Cache &c, int ntok, int hdim, int pos0, int pos_st
 // workgroups that the GPU holds at once.  By base, the (query, KV head) pairs or
 // blocks of 16 rows, and the steps of 128 positions of the longest context (device
 // contexts: of max_ctx);
-// us a call, split | whole | whole in big workgroups, contexts equal (, 1/16 to all
-// of the longest):
-//   - whole in four wavefronts up to 5 + base / 32 steps: the merge and its launch
-//     cost about 4 us, and a wavefront alone on its SIMD steps twice as fast as one
-//     of three.  28/4 heads of 128: 1 query of 512 9 | 8, of 1024 9 | 11; 32 of 1024 15
-//     | 14; 48 of 1024 18 | 14, of 2048 22 | 22; 128 of 2048 41 | 36, of 4096 70 | 69.
-//     14/2 of 64: 64 of 1024 13 | 10, of 2048 15 | 16.
-//   - whole in a workgroup as large as a CU holds where those about fill the GPU,
-//     and up to 32 steps, past which a ragged batch waits for its longest: 28/4 heads of
-//     128, 64 queries of 2048 25 | 23 | 21, of 4096 41 | 46 | 37 (29 | 39 | 29); 48 of 4096
-//     33 | 42 | 31 (25 | 37 | 28).  14/2 of 64, 128 of 4096 26 | 28 | 21 (21 | 27 | 20), of
-//     16384 73 | 112 | 69 (46 | 105 | 58).
+// us a call in a graph, split | whole in four | in eight, contexts equal (1/16 to all of
+// the longest):
+//   - whole in four wavefronts up to 4 steps: the merge and its launch cost about 4 us.
+//     28/4 heads of 128, 1 query of 512 9.1 | 8.1 | 8.2, 48 of 384 13.8 | 8.2 | 8.5.
+//   - with at most one workgroup a CU, whole in eight up to the steps below: they share
+//     a context's steps, and step faster than three wavefronts a SIMD.  28/4 heads of
+//     128: 1 query of 768 8.9 | 9.7 | 9.4, of 1024 9.1 | 11.5 | 10.7; 16 of 1536 14.3 | 16.9 |
+//     14.3; 48 of 2048 21.7 | 21.5 | 18.4; 64 of 4096 40.5 | 45.2 | 35.9 (28.8 | 38.6 | 29.8), of
+//     8192 70.1 | 81.9 | 63.6 (49.0 | 74.9 | 54.6).  14/2 of 64: 1 of 1024 8.3 | 9.4 | 8.7, but
+//     10.6 | 8.8 | 8.1 from Python, whose two launches take longer; 64 of 3000 16.6 | 21.6 |
+//     16.9 (14.8 | 21.2 | 16.4); 128 of 4096 26.1 | 27.2 | 21.4 (20.6 | 27.0 | 20.7).  8/8 of 32: 6
+//     of 1536 8.8 | 10 | 8.5; 32 of 4096 19.6 | 23.1 | 17.2 (15.9 | 22.7 | 16.7).  (Workgroups of
+//     12 or 16: 64 of 4096 38.4; no better below 4096 positions and 5 % so past them.)
+//   - with more, whole in four up to 5 + base / 32 steps: 28/4 heads of 128, 80 queries of 1024
+//     23.6 | 17.8 | 22.4, of 2048 33.2 | 30.2 | 34.9 (25.8 | 23.7 | 25.9), of 3000 43.2 | 42.9 |
+//     48.0 (30.2 | 33.8 | 31.6); 128 of 2048 41 | 36, of 4096 70 | 69.
 //   - else split into chunks: as many as fill the GPU, twice that for contexts on the
 //     device, which the kernel uses as they are ragged.
 struct A4Plan {
@@ -1068,8 +1071,9 @@ struct A4Plan {
 static A4Plan a4_plan(int hdim, long long base, int max_ctx, bool ragged) {
     const long long steps = ((long long)max_ctx + 4 * A4_GROUP - 1) / (4 * A4_GROUP);
     const int slots = hdim > 64 ? 768 : 1024;
-    if (base >= slots || steps <= 5 + base / 32) return {4, 1, slots};
-    if (base > 192 && base <= 256 && steps <= 32) return {a4_big(hdim), 1, slots};
+    if (base >= slots || steps <= 4) return {4, 1, slots};
+    if (base <= 256 ? steps <= 4 + 256 / hdim + base / 8 : steps <= 5 + base / 32)
+        return {base <= 256 ? 8 : 4, 1, slots};
     const long long want = (slots + base - 1) / base * (ragged ? 2 : 1);
     return {4, (int)min(min(steps, want), 256ll), slots};
 }
@@ -1133,8 +1137,8 @@ void launch_attention_kv4(const float *q, int nq, int qheads, int hdim, const Kv
 #define CALL2(DIM, M)                                                  \
     if (plan.nw == 4 && page16) CALL3(DIM, M, true, 4);                \
     else if (plan.nw == 4) CALL3(DIM, M, false, 4);                    \
-    else if (page16) CALL3(DIM, M, true, a4_big(DIM));                 \
-    else CALL3(DIM, M, false, a4_big(DIM))
+    else if (page16) CALL3(DIM, M, true, 8);                           \
+    else CALL3(DIM, M, false, 8)
 #define CALL(DIM)                           \
     if (rows) { CALL2(DIM, A4_ROWS); }      \
     else if (wide) { CALL2(DIM, A4_WIDE); } \

@@ -497,7 +497,10 @@ def test_prompts_both_ways(name, n, first):
     ("g7_d128", 1, 640), ("g7_d128", 1, 641), ("g7_d128", 49, 1500), ("g7_d128", 64, 2047),
     ("g7_d128", 65, 1700), ("g7_d64", 97, 2000), ("g16_d64", 128, 1900), ("g16_d64", 300, 300),
     ("g3_d96", 30, 1801), ("g3_d96", 96, 33), ("g1_d32", 32, 2000), ("g1_d32", 25, 4096),
-    ("g16_d128", 193, 1500), ("g16_d128", 70, 3000), ("g9_d32", 200, 1700)])
+    ("g16_d128", 193, 1500), ("g16_d128", 70, 3000), ("g9_d32", 200, 1700),
+    ("g7_d128", 1, 512), ("g7_d128", 1, 768), ("g7_d128", 1, 769), ("g7_d64", 1, 1024),
+    ("g7_d64", 1, 1025), ("g3_d96", 4, 1280), ("g3_d96", 4, 1281), ("g1_d32", 3, 1984),
+    ("g16_d128", 256, 700), ("g16_d128", 257, 700), ("g8_d96", 20, 1400)])
 def test_every_plan(name, nq, longest):
     """Calls on both sides of the rules that choose workgroups and chunks, with contexts from
     none to the longest: a few rows against 64 bits, all of them against calls of one query
