@@ -413,7 +413,9 @@ int si_kv4_read(const si_shape_t *s, const uint8_t *k_pool, const uint8_t *v_poo
  * to max_ctx; <= 0 gives zeros) or ctx0.  ctx_step 1: nq queries of the first
  * sequence with contexts ctx0, ctx0 + 1, ... (a causal prompt whose rows are in
  * place).  At most 65535 queries.  Outputs as si_attention's; workspace:
- * si_attention_kv4_workspace bytes, 256-byte aligned. */
+ * si_attention_kv4_workspace bytes, 256-byte aligned (calls that overlap need one
+ * each; a prompt of more than 9000 (query, head) rows takes fp16 rows of max_ctx
+ * positions there, so max_ctx is best the last query's context). */
 int si_attention_kv4(const si_shape_t *s, const float *q, int nq, const uint8_t *k_pool,
                      const uint8_t *v_pool, int npages, int page_size, const int *pages,
                      int max_pages, const int *ctx_dev, int ctx0, int ctx_step, int max_ctx,

@@ -327,11 +327,10 @@ __global__ void __launch_bounds__(2 * D) k_kv4_read(Kv4Cache c, int ntok, int po
 // What bounds it: a step of 32 positions is about 230 vector operations and 17 matrix
 // instructions (two products: 260 and 34), which hardly overlap, 0.7 us of a SIMD at
 // 128 dims, about as long as its 4.6 KB take to arrive.  64 queries x 4096 of 28/4 heads
-// of 128, 153 MB: 34 us (4.4 TB/s; a large copy reaches 4.8); its loads alone 30, its
-// arithmetic alone 28.  Fewer bytes leave 5 us of launch, page id, first group, last
-// step and the wavefronts' meeting, and the merge of chunks: 48 x 200-4096 (62 MB) 20.7
-// + 3.9 us, 2 queries of 12/2 heads over 60000-131072 (65 MB) 18.9 + 4.0, one query of
-// 14/2 heads of 64 over 1024 5.6 + 3.0.
+// of 128, 153 MB: 34 us (4.5 TB/s; a large copy reaches 4.8).  Fewer bytes leave 5 us of
+// launch, page id, first group, last step and the wavefronts' meeting, and the merge of
+// chunks: 48 x 200-4096 (62 MB) 21 + 4 us, 2 queries of 12/2 heads over 60000-131072 (65
+// MB) 19 + 4, one query of 14/2 heads of 64 over 1024 (no merge) 7.7.
 // ---------------------------------------------------------------------------
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
@@ -892,7 +891,7 @@ __global__ void __launch_bounds__(64 * NW, NW > 4 || MODE ? 2 : 3) k_attn_kv4(
 // ---------------------------------------------------------------------------
 // The chunks' states of a (query, head) to its output: a workgroup per 32 dims
 // (one Q8_0 block), 8 lanes a state, G states at once, at most 8 G in all, so
-// that every load is in flight at once: 2.9-4.0 us, a launch, one round trip and the
+// that every load is in flight at once: 3.9-4.0 us, a launch, one round trip and the
 // stores.  tq/td (optional): the Q8_0 also
 // operand-tiled (q8_tiled_byte).
 // ---------------------------------------------------------------------------
