@@ -1062,17 +1062,22 @@ void launch_kv4_read(const Kv4Cache &c, int ntok, int hdim, int pos0, int pos_st
 //   - with more, whole in four up to 5 + base / 32 steps: 28/4 heads of 128, 80 queries of 1024
 //     23.6 | 17.8 | 22.4, of 2048 33.2 | 30.2 | 34.9 (25.8 | 23.7 | 25.9), of 3000 43.2 | 42.9 |
 //     48.0 (30.2 | 33.8 | 31.6); 128 of 2048 41 | 36, of 4096 70 | 69.
-//   - else split into chunks: as many as fill the GPU, twice that for contexts on the
-//     device, which the kernel uses as they are ragged.
+//   - else split into chunks: as many as fill the GPU (three, four or five workgroups a
+//     CU by their registers), or fill it twice where they would be two or fewer a pair,
+//     too coarse to end together: once | twice, 93 to 6000 positions (6000), 24/8 heads
+//     of 96: 40 queries 36.4 | 34.2 (54.2 | 53.0), 48 42.9 | 38.7 (58.8 | 60.7), 75 76.2 |
+//     64.6 (91.6 | 91.5); 26 22.6 | 25.9 (38.9 | 40.3).  A context on the device may get
+//     twice its share, which the kernel uses as they are ragged.
 struct A4Plan {
     int nw, ns, slots;
 };
 static A4Plan a4_plan(int hdim, long long base, int max_ctx, bool ragged) {
     const long long steps = ((long long)max_ctx + 4 * A4_GROUP - 1) / (4 * A4_GROUP);
-    const int slots = hdim > 64 ? 768 : 1024;
+    int slots = hdim > 64 ? 768 : hdim > 32 ? 1024 : 1280;
     if (base >= slots || steps <= 4) return {4, 1, slots};
     if (base <= 256 ? steps <= 4 + 256 / hdim + base / 8 : steps <= 5 + base / 32)
         return {base <= 256 ? 8 : 4, 1, slots};
+    if (base > slots * 2 / 5) slots *= 2;
     const long long want = (slots + base - 1) / base * (ragged ? 2 : 1);
     return {4, (int)min(min(steps, want), 256ll), slots};
 }

@@ -500,7 +500,9 @@ def test_prompts_both_ways(name, n, first):
     ("g16_d128", 193, 1500), ("g16_d128", 70, 3000), ("g9_d32", 200, 1700),
     ("g7_d128", 1, 512), ("g7_d128", 1, 768), ("g7_d128", 1, 769), ("g7_d64", 1, 1024),
     ("g7_d64", 1, 1025), ("g3_d96", 4, 1280), ("g3_d96", 4, 1281), ("g1_d32", 3, 1984),
-    ("g16_d128", 256, 700), ("g16_d128", 257, 700), ("g8_d96", 20, 1400)])
+    ("g16_d128", 256, 700), ("g16_d128", 257, 700), ("g8_d96", 20, 1400),
+    ("g7_d128", 76, 2000), ("g7_d128", 77, 2000), ("g3_d96", 39, 1950), ("g1_d32", 65, 2750),
+    ("g1_d32", 160, 700), ("g16_d64", 205, 2300)])
 def test_every_plan(name, nq, longest):
     """Calls on both sides of the rules that choose workgroups and chunks, with contexts from
     none to the longest: a few rows against 64 bits, all of them against calls of one query
