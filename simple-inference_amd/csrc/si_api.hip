@@ -1845,6 +1845,8 @@ int si_kv_copy_pages(void *const *pools, int npools, size_t page_bytes, int npag
         return fail(SI_ERR_NOMEM, "%s: no host memory for %d moves", what, n);
     }
     if (n == 0 || npools == 0) return SI_OK;
+    // bytes read and written past the cache (k_kv_copy)
+    const bool once = 2.0 * npools * n * page_bytes > 256e6;
     KvMoves mv;
     for (int p0 = 0; p0 < npools; p0 += KvMoves::POOLS) {
         const int np = std::min(npools - p0, KvMoves::POOLS);
@@ -1853,7 +1855,7 @@ int si_kv_copy_pages(void *const *pools, int npools, size_t page_bytes, int npag
             const int nm = std::min(n - i0, KvMoves::MOVES);
             std::copy(src + i0, src + i0 + nm, mv.src);
             std::copy(dst + i0, dst + i0 + nm, mv.dst);
-            launch_kv_copy(mv, np, nm, page_bytes, wide, S(stream));
+            launch_kv_copy(mv, np, nm, page_bytes, wide, once, S(stream));
         }
     }
     return check_launch("si_kv_copy_pages");

@@ -360,5 +360,5 @@ struct KvMoves {
     int src[MOVES], dst[MOVES];
 };
 void launch_kv_copy(const KvMoves &mv, int npools, int nmoves, size_t page_bytes, bool wide,
-                    hipStream_t st);
+                    bool once, hipStream_t st);
 }  // namespace si

@@ -346,40 +346,45 @@ __device__ __forceinline__ float ror8_add(float v) { return v + dpp_f<DPP_ROR8>(
 // (the group's place in it is the load's scalar offset, so a step computes no
 // addresses in vector registers, and nothing past the page is touched), or, for
 // pages of half a group, the lane's own address.
+// ONCE: no other workgroup reads the bytes soon (every query but a prompt's), so they
+// are loaded past the caches: 64 queries x 4096 of 28/4 heads of 128 from memory 35.6 ->
+// 32.5 us, 200 x 2000 60.8 -> 54.0, 128 x 4000 of 14/2 of 64 23.7 -> 21.7; a prompt, whose
+// blocks of rows share them, 83.9 -> 89.1.
 struct Kv4InPage {
     __amdgpu_buffer_rsrc_t r;
     int at;
-    template <int N>
+    template <int N, bool ONCE>
     __device__ __forceinline__ void load(int off, uint32_t *w) const {
+        constexpr int AUX = ONCE ? 2 : 0;  // nt
         if constexpr (N == 1) {
-            w[0] = __builtin_amdgcn_raw_buffer_load_b32(r, off, at, 0);
+            w[0] = __builtin_amdgcn_raw_buffer_load_b32(r, off, at, AUX);
         } else if constexpr (N == 2) {
-            const auto t = __builtin_amdgcn_raw_buffer_load_b64(r, off, at, 0);
+            const auto t = __builtin_amdgcn_raw_buffer_load_b64(r, off, at, AUX);
             w[0] = t[0], w[1] = t[1];
         } else if constexpr (N == 3) {
-            const auto t = __builtin_amdgcn_raw_buffer_load_b96(r, off, at, 0);
+            const auto t = __builtin_amdgcn_raw_buffer_load_b96(r, off, at, AUX);
             w[0] = t[0], w[1] = t[1], w[2] = t[2];
         } else {
-            const auto t = __builtin_amdgcn_raw_buffer_load_b128(r, off, at, 0);
+            const auto t = __builtin_amdgcn_raw_buffer_load_b128(r, off, at, AUX);
             w[0] = t[0], w[1] = t[1], w[2] = t[2], w[3] = t[3];
         }
     }
 };
 struct Kv4InHalf {
     const uint8_t *p;
-    template <int N>
+    template <int N, bool ONCE>
     __device__ __forceinline__ void load(int off, uint32_t *w) const {
-        if constexpr (N == 1) {
-            w[0] = *(const uint32_t *)(p + off);
-        } else if constexpr (N == 2) {
-            const uint2 t = *(const uint2 *)(p + off);
-            w[0] = t.x, w[1] = t.y;
-        } else if constexpr (N == 3) {
-            const uint3 t = *(const uint3 *)(p + off);
-            w[0] = t.x, w[1] = t.y, w[2] = t.z;
-        } else {
-            const uint4 t = *(const uint4 *)(p + off);
-            w[0] = t.x, w[1] = t.y, w[2] = t.z, w[3] = t.w;
+        // (three dwords as such: rows of 12 bytes are 4-byte aligned)
+        typedef uint32_t vec __attribute__((ext_vector_type(N == 3 ? 1 : N)));
+        constexpr int PER = N == 3 ? 1 : N;
+#pragma unroll
+        for (int e = 0; e < N; e += PER) {
+            const vec *a = (const vec *)(p + off + 4 * e);
+            vec t;
+            if constexpr (ONCE) t = __builtin_nontemporal_load(a);
+            else t = *a;
+#pragma unroll
+            for (int i = 0; i < PER; ++i) w[e + i] = t[i];
         }
     }
 };
@@ -390,7 +395,7 @@ struct Kv4InHalf {
 // wavefront's own room in LDS (as DPP broadcasts they were 48 of a step's 275
 // vector operations, what bounds the kernel; loaded by every lane, 32 registers
 // and 8 of the 14 loads).
-template <int D>
+template <int D, bool ONCE>
 struct Kv4Group {
     static constexpr int KS = D / 32, DT = D / 16;
     uint32_t k[2][KS], v[DT], kh, vh;
@@ -400,16 +405,18 @@ struct Kv4Group {
                                          int ku, int vu, int lane) {
         const int r = lane & 15, g = lane >> 4;
         const int so = vu * KS * 16 + min(r, 4 * KS - 1) * 4;
-        ks.template load<1>(so, &kh);
-        vs.template load<1>(so, &vh);
+        ks.template load<1, false>(so, &kh);  // (a line holds several groups')
+        vs.template load<1, false>(so, &vh);
 #pragma unroll
         for (int t = 0; t < 2; ++t)
-            kk.template load<KS>(ku * 4 * D + t * 2 * D + g * (D / 2) + (r & 3) * (D / 8), k[t]);
+            kk.template load<KS, ONCE>(ku * 4 * D + t * 2 * D + g * (D / 2) + (r & 3) * (D / 8),
+                                       k[t]);
         constexpr int FULL = D / 64;
 #pragma unroll
         for (int f = 0; f < FULL; ++f)
-            vv.template load<4>(vu * 4 * D + f * 256 + r * 16, v + 4 * f);
-        if constexpr (DT % 4) vv.template load<2>(vu * 4 * D + FULL * 256 + r * 8, v + 4 * FULL);
+            vv.template load<4, ONCE>(vu * 4 * D + f * 256 + r * 16, v + 4 * f);
+        if constexpr (DT % 4)
+            vv.template load<2, ONCE>(vu * 4 * D + FULL * 256 + r * 8, v + 4 * FULL);
     }
 };
 
@@ -531,6 +538,7 @@ __global__ void __launch_bounds__(64 * NW, NW > 4 || MODE ? 2 : 3) k_attn_kv4(
     int8_t *__restrict__ qs, uint16_t *__restrict__ qd8, int16_t *__restrict__ bsum,
     int8_t *__restrict__ tq, uint16_t *__restrict__ td) {
     constexpr bool WIDE = MODE != A4_NARROW, ROWS = MODE == A4_ROWS;
+    typedef Kv4Group<D, !ROWS> Group;
     constexpr int KS = D / 32, DT = D / 16, COLS = WIDE ? 16 : 8, STEP = NW * A4_GROUP;
     __shared__ __attribute__((aligned(16))) float mo[4][COLS][D];
     __shared__ __attribute__((aligned(16))) u4 qop[(WIDE ? 2 : 1) * KS * 64];  // hi (, lo)
@@ -587,7 +595,7 @@ __global__ void __launch_bounds__(64 * NW, NW > 4 || MODE ? 2 : 3) k_attn_kv4(
     auto head_at = [&](int pg) {
         return ((size_t)min(max(pg, 0), c.npages - 1) * c.kvheads + g0) * hb;
     };
-    auto load = [&](Kv4Group<D> &t, int s0, Ids id) {
+    auto load = [&](Group &t, int s0, Ids id) {
         const size_t a = head_at(id.a);
         if constexpr (PAGE16) {
             // two pages a group: units 0, 1 and 2, 3
@@ -603,7 +611,7 @@ __global__ void __launch_bounds__(64 * NW, NW > 4 || MODE ? 2 : 3) k_attn_kv4(
         }
     };
     int s0 = p0 + A4_GROUP * wave;
-    Kv4Group<D> ta, tb;
+    Group ta, tb;
     {
         const Ids ia = ids_of(s0), ib = ids_of(s0 + STEP);
         if (s0 < p1) load(ta, s0, ia);
@@ -687,7 +695,7 @@ __global__ void __launch_bounds__(64 * NW, NW > 4 || MODE ? 2 : 3) k_attn_kv4(
     asm("" : "+s"(mask));
     asm("" : "+v"(magic));
 
-    auto step = [&](Kv4Group<D> &t, int s) {
+    auto step = [&](Group &t, int s) {
         float p[2][4];
         f4 d[2][KS];
         // lane (col, g)'s dword to [g][col]; a wavefront's LDS operations keep their
@@ -977,18 +985,33 @@ __global__ void __launch_bounds__(8 * G) k_kv4_merge(
 
 // ---------------------------------------------------------------------------
 // page copies: grid (pieces of a page, moves, pools); the pools' addresses and
-// the moves travel in the kernel's arguments, so the call needs no upload.  500
-// pages of 64 KB in 16 pools (1.05 GB read and written) 210 us, 5.0 TB/s; 3 pages of
-// 18 KB in 56 pools 3.1 us.
+// the moves travel in the kernel's arguments, so the call needs no upload.  Four
+// loads of a thread are in flight.  ONCE: a call past the 256 MB cache goes past it
+// both ways (500 pages of 64 KB in 16 pools, 1.05 GB read and written: 178 us, 5.9
+// TB/s, else 190, and 209 with a load at a time; 700 of 36 KB 156, else 167), a
+// smaller one may find its pages there (100 of 18 KB in 16 pools 12.2, else 10.9).
+// 3 pages of 18 KB in 56 pools 3.1 us.
 // ---------------------------------------------------------------------------
-template <class T>
+template <class T, bool ONCE>
 __global__ void __launch_bounds__(256) k_kv_copy(KvMoves mv, size_t page_bytes) {
     uint8_t *pool = mv.pool[blockIdx.z];
     const T *src = (const T *)(pool + (size_t)mv.src[blockIdx.y] * page_bytes);
     T *dst = (T *)(pool + (size_t)mv.dst[blockIdx.y] * page_bytes);
-    const size_t n = page_bytes / sizeof(T);
-    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (size_t)gridDim.x * 256)
-        dst[i] = src[i];
+    const size_t n = page_bytes / sizeof(T), step = (size_t)gridDim.x * 256;
+    auto get = [&](size_t i) { return ONCE ? __builtin_nontemporal_load(src + i) : src[i]; };
+    auto put = [&](T v, size_t i) {
+        if constexpr (ONCE) __builtin_nontemporal_store(v, dst + i);
+        else dst[i] = v;
+    };
+    size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
+    for (; i + 3 * step < n; i += 4 * step) {
+        T t[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) t[k] = get(i + k * step);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) put(t[k], i + k * step);
+    }
+    for (; i < n; i += step) put(get(i), i);
 }
 
 // ---------------------------------------------------------------------------
@@ -1162,11 +1185,12 @@ void launch_attention_kv4(const float *q, int nq, int qheads, int hdim, const Kv
 }
 
 void launch_kv_copy(const KvMoves &mv, int npools, int nmoves, size_t page_bytes, bool wide,
-                    hipStream_t st) {
+                    bool once, hipStream_t st) {
     const size_t unit = wide ? 16 : 1;
     const size_t want = (page_bytes / unit + 256 * 4 - 1) / (256 * 4);
     const dim3 grid((unsigned)min(want, (size_t)64), nmoves, npools);
-    if (wide) SI_LAUNCH(k_kv_copy<uint4>, grid, dim3(256), 0, st, mv, page_bytes);
-    else SI_LAUNCH(k_kv_copy<uint8_t>, grid, dim3(256), 0, st, mv, page_bytes);
+    if (wide && once) SI_LAUNCH((k_kv_copy<u4, true>), grid, dim3(256), 0, st, mv, page_bytes);
+    else if (wide) SI_LAUNCH((k_kv_copy<u4, false>), grid, dim3(256), 0, st, mv, page_bytes);
+    else SI_LAUNCH((k_kv_copy<uint8_t, false>), grid, dim3(256), 0, st, mv, page_bytes);
 }
 }  // namespace si

@@ -396,7 +396,8 @@ def test_attention_repeats_its_bits():
 # ---------------------------------------------------------------------------
 @pytest.mark.parametrize("npools,page_bytes,npages,n", [
     (1, 4096, 5, 1), (56, 1152, 40, 7), (3, 18432, 30, 15), (65, 64, 1000, 500), (2, 20, 9, 4),
-    (1, 7, 12, 5), (2, 65536, 12, 6), (1, 16, 900, 450)])
+    (1, 7, 12, 5), (2, 65536, 12, 6), (1, 16, 900, 450),
+    (2, 1000016, 150, 70), (2, 65536, 2100, 1024), (1, 2000001, 140, 70)])  # past 256 MB
 def test_copy_pages(npools, page_bytes, npages, n):
     torch = _torch()
     rng = np.random.default_rng(n)
