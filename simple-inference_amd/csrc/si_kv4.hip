@@ -327,10 +327,10 @@ __global__ void __launch_bounds__(2 * D) k_kv4_read(Kv4Cache c, int ntok, int po
 // What bounds it: a step of 32 positions is about 230 vector operations and 17 matrix
 // instructions (two products: 260 and 34), which hardly overlap, 0.7 us of a SIMD at
 // 128 dims, about as long as its 4.6 KB take to arrive.  64 queries x 4096 of 28/4 heads
-// of 128, 153 MB: 34 us (4.5 TB/s; a large copy reaches 4.8).  Fewer bytes leave 5 us of
+// of 128, 153 MB: 32 us (4.8 TB/s, a large copy's rate).  Fewer bytes leave 5 us of
 // launch, page id, first group, last step and the wavefronts' meeting, and the merge of
 // chunks: 48 x 200-4096 (62 MB) 21 + 4 us, 2 queries of 12/2 heads over 60000-131072 (65
-// MB) 19 + 4, one query of 14/2 heads of 64 over 1024 (no merge) 7.7.
+// MB) 19 + 4, one query of 14/2 heads of 64 over 1024 (no merge) 7.8.
 // ---------------------------------------------------------------------------
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
@@ -348,8 +348,10 @@ __device__ __forceinline__ float ror8_add(float v) { return v + dpp_f<DPP_ROR8>(
 // pages of half a group, the lane's own address.
 // ONCE: no other workgroup reads the bytes soon (every query but a prompt's), so they
 // are loaded past the caches: 64 queries x 4096 of 28/4 heads of 128 from memory 35.6 ->
-// 32.5 us, 200 x 2000 60.8 -> 54.0, 128 x 4000 of 14/2 of 64 23.7 -> 21.7; a prompt, whose
-// blocks of rows share them, 83.9 -> 89.1.
+// 32.6 us, 200 x 2000 61.0 -> 53.7, 8 x 4096 15.3 -> 14.3, 128 x 4000 of 14/2 of 64 23.7 ->
+// 22.9 (as a model's layers come, other pages between; the same pages again and again from
+// the 256 MB cache 33.5 -> 34.5, 15.2 -> 15.5).  A prompt, whose blocks of rows share them,
+// 83.9 -> 89.1.
 struct Kv4InPage {
     __amdgpu_buffer_rsrc_t r;
     int at;
