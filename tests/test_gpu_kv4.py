@@ -555,3 +555,114 @@ def test_prompts_of_a_very_long_cache():
     ws = si_amd.lib().si_attention_kv4_workspace(c.s(), n, 1, 1 << 27)
     assert ws < 1 << 28
     _close(_attention(c, dev(q), n, None, first, 1, 1 << 27)[some], want, "pages")
+
+
+def test_pools_past_4_gib():
+    """Pages more than 2^32 bytes into their pools: written, read, attended to and copied; and a
+    prompt whose fp16 rows of max_ctx positions take 8 GiB of workspace."""
+    torch = _torch()
+    rng = np.random.default_rng(9)
+    q, kv, D = SHAPES["g1_d32"]
+    ps, npages, n = 65536, 480, 66000
+    shape = si_amd.make_shape(32, q, kv, D)
+    s = ctypes.byref(shape)
+    page = si_amd.lib().si_kv4_page_bytes(s, ps)
+    pools = [torch.empty(npages * page, dtype=torch.uint8, device="cuda") for _ in "kv"]
+    assert pools[0].numel() > 1 << 32
+    x = [rng.standard_normal((n, kv, D)).astype(np.float16) for _ in "kv"]
+    held = [ref.held(t.astype(np.float32)) for t in x]
+    dx = [dev(t) for t in x]
+    lists = dev(np.array([[479, 470], [3, 478]], np.int32))
+
+    def cache(seq):
+        return (si_amd.ptr(pools[0]), si_amd.ptr(pools[1]), npages, ps, si_amd.ptr(lists[seq]), 2)
+
+    def rows(seq, first, count):
+        out = [torch.empty(count, kv, D, dtype=torch.float16, device="cuda") for _ in "kv"]
+        si_amd.call("si_kv4_read", s, *cache(seq), count, first, 1, None, si_amd.ptr(out[0]),
+                    si_amd.ptr(out[1]), None)
+        return [host(t).astype(np.float64) for t in out]
+
+    si_amd.call("si_kv4_write", s, si_amd.ptr(dx[0]), si_amd.ptr(dx[1]), n, 0, 1, None, *cache(0),
+                None)
+    addr = (ctypes.c_void_p * 2)(*(t.data_ptr() for t in pools))
+    src, dst = np.array([479, 470], np.int32), np.array([3, 478], np.int32)
+    si_amd.call("si_kv_copy_pages", addr, 2, page, npages, si_amd.ptr(src), si_amd.ptr(dst), 2, None)
+    qs = rng.standard_normal((3, q, D)).astype(np.float32)
+    want = np.stack([ref.attend(qs[i], held[0][:n - 2 + i], held[1][:n - 2 + i])
+                     for i in range(3)])
+    for seq in (0, 1):
+        for got, w in zip(rows(seq, 0, n), held):
+            assert np.array_equal(got, w)
+        need = si_amd.lib().si_attention_kv4_workspace(s, 3, 1, n)
+        ws, out = empty((max(need, 1),), torch.uint8), empty((3, q, D), torch.float32)
+        si_amd.call("si_attention_kv4", s, si_amd.ptr(dev(qs)), 3, *cache(seq), None, n - 2, 1, n,
+                    si_amd.ptr(out), None, None, None, si_amd.ptr(ws), need, None)
+        _close(host(out), want, seq)
+    nq, max_ctx = 1130, 1 << 23
+    long_list = dev(np.full((1, max_ctx // ps), 479, np.int32))
+    need = si_amd.lib().si_attention_kv4_workspace(s, nq, 1, max_ctx)
+    assert need == max_ctx * kv * D * 4
+    ws = torch.empty(need, dtype=torch.uint8, device="cuda")
+    q2 = dev(np.repeat(qs[:1], nq, 0))
+    out = empty((nq, q, D), torch.float32)
+    si_amd.call("si_attention_kv4", s, si_amd.ptr(q2), nq, si_amd.ptr(pools[0]),
+                si_amd.ptr(pools[1]), npages, ps, si_amd.ptr(long_list), max_ctx // ps, None, 1, 1,
+                max_ctx, si_amd.ptr(out), None, None, None, si_amd.ptr(ws), need, None)
+    some = np.array([0, 1, 700, nq - 1])
+    _close(host(out)[some], np.stack([ref.attend(qs[0], held[0][:i + 1], held[1][:i + 1])
+                                      for i in some]), "rows")
+
+
+def test_attention_captured_and_on_a_stream():
+    """Split calls of ragged batches: two captured graphs that share a workspace, replayed in turn
+    with contexts and queries changed between and eager calls beside, and a call on a stream of the
+    caller's, give the eager bits."""
+    torch = _torch()
+    rng = np.random.default_rng(12)
+    nq, longest = 20, 3000
+    c = Cache(rng, "g7_d128", nq, longest, 64)
+    need = si_amd.lib().si_attention_kv4_workspace(c.s(), nq, 0, longest)
+    assert need > 0
+    ws = torch.full((need,), 255, dtype=torch.uint8, device="cuda")
+    sets = []
+    for i in range(2):
+        sets.append([torch.zeros(nq, c.q, c.D, device="cuda"),
+                     torch.ones(nq, dtype=torch.int32, device="cuda"),
+                     torch.empty(nq, c.q, c.D, device="cuda")])
+
+    def call(q, ctx, out, stream=None):
+        si_amd.call("si_attention_kv4", c.s(), si_amd.ptr(q), nq, *c.args(), si_amd.ptr(ctx), 0, 0,
+                    longest, si_amd.ptr(out), None, None, None, si_amd.ptr(ws), need,
+                    si_amd.stream_handle(stream))
+
+    graphs = []
+    for s in sets:
+        call(*s)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            call(*s)
+        graphs.append(g)
+    side = torch.cuda.Stream()
+    for turn in range(4):
+        for s, g in zip(sets, graphs):
+            s[0].copy_(dev(rng.standard_normal((nq, c.q, c.D)).astype(np.float32)))
+            ctx = rng.integers(0, longest + 1, nq).astype(np.int32)
+            if turn == 1:
+                ctx[:] = longest
+            s[1].copy_(dev(ctx))
+            call(*s)
+            torch.cuda.synchronize()
+            want = s[2].clone()
+            s[2].zero_()
+            g.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(s[2], want), turn
+            s[2].zero_()
+            side.wait_stream(torch.cuda.current_stream())
+            call(*s, side)
+            side.synchronize()
+            assert torch.equal(s[2], want), turn
+    some = [0, 7, nq - 1]
+    _close(host(want)[some], _want(c, host(s[0])[some], some, ctx[some]), "last")
