@@ -527,7 +527,16 @@ __device__ __forceinline__ void pf_barrier() {
 // ASYNC: kc and vc are 16-byte aligned (and so is every row, a multiple of 64
 // bytes).  Otherwise the tiles come through registers, by loads that take any
 // address, and are in LDS when copy() returns.
-template <int D, int RT, int KW, bool ASYNC>
+//
+// FAR (prompts over a cache held in 4 bits): positions far below a row's largest
+// score keep their bits, where that one's V row is zero or small (an attention
+// sink).  Weights are against a maximum that follows the running one within 2^4, in
+// units of 2^-11, their lo halves 2^11 higher and in sums of their own: 22 bits down
+// to 2^-25 and an error of at most 2^-47 below.  (Else lo, in hi's units and sums, is an
+// fp16 subnormal from 2^-3 down, and weights below 2^-25 are 0.)  The second sums take
+// D / 2 registers, which past 64 dims come from q's lo halves: those wait in LDS.
+constexpr float PF_SLACK = 4.0f, PF_UP = 11.0f, PF_LO = 2048.0f;
+template <int D, int RT, int KW, bool ASYNC, bool FAR = false>
 __global__ void __launch_bounds__(RT * KW * 64) __attribute__((amdgpu_waves_per_eu(2)))
 k_attn_prefill(const float *__restrict__ q, int ntok, int qheads, int kvheads, int pos0,
                const uint16_t *__restrict__ kc, const uint16_t *__restrict__ vc, float scale2,
@@ -548,6 +557,12 @@ k_attn_prefill(const float *__restrict__ q, int ntok, int qheads, int kvheads, i
     constexpr int HALF_W = (NWV + 1) / 2, MRG = HALF_W * PF_T * OROW * 4;
     __shared__ __attribute__((aligned(16))) uint8_t sb0[STAGE > MRG ? STAGE : MRG];
     __shared__ __attribute__((aligned(16))) uint8_t sb1[STAGE > MRG ? STAGE : MRG];
+    constexpr bool QLDS = FAR && D > 64;  // q's lo halves: [RT][KS][64 lanes]
+    constexpr int QL = QLDS ? RT * KS * 1024 : 0;
+    // behind the stage buffer where the outputs, which come last, leave the room
+    constexpr bool QL_IN = STAGE + QL <= MRG;
+    __shared__ __attribute__((aligned(16))) uint8_t qlo[QL && !QL_IN ? QL : 16];
+    uint8_t *const ql_at = QL_IN ? sb0 + STAGE : qlo;
     __shared__ float mrg_m[NWV][PF_T], mrg_l[NWV][PF_T];
     __shared__ int64_t rowoff[32 * RT];  // output offset of a row, -1 past the last
 
@@ -615,7 +630,7 @@ k_attn_prefill(const float *__restrict__ q, int ntok, int qheads, int kvheads, i
     // past the last row repeat it and are never stored)
     const size_t qoff = ((size_t)(myrow / per) * qheads + g * per + myrow % per) * D;
     if (kw == 0 && hh == 0) rowoff[32 * rt + t] = wr0 + t < nrows ? (int64_t)qoff : -1;
-    h8 qh[KS], ql[KS];
+    h8 qh[KS], ql[QLDS ? 1 : KS];
     {
         const float *qrow = q + qoff + 8 * hh;
         float4 a[KS], b[KS];
@@ -628,17 +643,21 @@ k_attn_prefill(const float *__restrict__ q, int ntok, int qheads, int kvheads, i
         for (int ks = 0; ks < KS; ++ks) {
             const float x[8] = {a[ks].x, a[ks].y, a[ks].z, a[ks].w,
                                 b[ks].x, b[ks].y, b[ks].z, b[ks].w};
+            h8 &l = ql[QLDS ? 0 : ks];
 #pragma unroll
             for (int e = 0; e < 8; e += 2) {
                 pf_h2 hi, lo;
                 split_pair(x[e], x[e + 1], hi, lo);
                 qh[ks][e] = hi[0];
                 qh[ks][e + 1] = hi[1];
-                ql[ks][e] = lo[0];
-                ql[ks][e + 1] = lo[1];
+                l[e] = lo[0];
+                l[e + 1] = lo[1];
             }
+            // (the KW wavefronts of a row tile have the same rows)
+            if (QLDS && kw == 0) *(h8 *)(ql_at + ((rt * KS + ks) * 64 + lane) * 16) = l;
         }
     }
+    if constexpr (QLDS) __syncthreads();
 
     // operand addresses within a stage: K row t, chunk 2 ks + hh; V rows
     // 16 s2 + 8 e + 4 hh + s / 4 (s = lane % 16), columns 32 dt + 16 (lane /
@@ -654,9 +673,13 @@ k_attn_prefill(const float *__restrict__ q, int ntok, int qheads, int kvheads, i
                  (s16 & 1) * 8;
 
     float m = -INFINITY, lsum = 0.0f;  // row t's running max; this lane's share of the sum
-    f16v o[DT];
+    const float over = PF_SLACK * __builtin_amdgcn_rcpf(scale2);  // (FAR)
+    constexpr int LO = FAR ? DT : 0;
+    f16v o[DT], o2[LO + 1];  // FAR: o2, the lo halves' sums
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) o[dt] = (f16v){};
+#pragma unroll
+    for (int dt = 0; dt < LO; ++dt) o2[dt] = (f16v){};
 
     const auto load_k = [&](const uint8_t *kt, h8 (&a)[KS]) {
 #pragma unroll
@@ -667,7 +690,10 @@ k_attn_prefill(const float *__restrict__ q, int ntok, int qheads, int kvheads, i
         f16v s = (f16v){};
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks)
-            s = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[ks], ql[ks], s, 0, 0, 0);
+            s = __builtin_amdgcn_mfma_f32_32x32x16_f16(
+                a[ks],
+                QLDS ? *(const h8 *)(ql_at + ((rt * KS + ks) * 64 + lane) * 16) : ql[QLDS ? 0 : ks],
+                s, 0, 0, 0);
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks)
             s = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[ks], qh[ks], s, 0, 0, 0);
@@ -693,25 +719,36 @@ k_attn_prefill(const float *__restrict__ q, int ntok, int qheads, int kvheads, i
         // rescale of the sums, which some row of the 32 would otherwise ask
         // for in most tiles, becomes rare.  A wavefront's first tiles can lie
         // past a row's limit: its state stays (-inf, 0, 0), no NaN.
-        const float mnew = fmaxf(m, mx * scale2);
-        if (__ballot(mnew > m + 8.0f)) {
-            const float alpha = __builtin_amdgcn_exp2f(m - mnew);
+        // (FAR: by a row of its own only: 2^4 over m, raw scores.)
+        const float mnew = FAR ? (mx - m > over ? mx : m) : fmaxf(m, mx * scale2);
+        if (FAR ? __ballot(mnew > m) : __ballot(mnew > m + 8.0f)) {
+            const float alpha = __builtin_amdgcn_exp2f(FAR ? (m - mnew) * scale2 : m - mnew);
             const float a0 = mnew == -INFINITY ? 1.0f : alpha;
             lsum *= a0;
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt) o[dt] *= a0;
+#pragma unroll
+            for (int dt = 0; dt < LO; ++dt) o2[dt] *= a0;
             m = mnew;
         }
         const float mref = m == -INFINITY ? 0.0f : m;
         float ps = 0.0f;
 #pragma unroll
         for (int r = 0; r < 16; r += 2) {
-            const float p0 = __builtin_amdgcn_exp2f(fmaf(s[r], scale2, -mref));
-            const float p1 = __builtin_amdgcn_exp2f(fmaf(s[r + 1], scale2, -mref));
+            const float p0 = __builtin_amdgcn_exp2f(FAR ? fmaf(s[r] - mref, scale2, PF_UP)
+                                                        : fmaf(s[r], scale2, -mref));
+            const float p1 = __builtin_amdgcn_exp2f(FAR ? fmaf(s[r + 1] - mref, scale2, PF_UP)
+                                                        : fmaf(s[r + 1], scale2, -mref));
             ps += p0;
             ps += p1;
             pf_h2 hi, lo;
-            split_pair(p0, p1, hi, lo);
+            if constexpr (FAR) {
+                hi = __builtin_convertvector((pf_f2){p0, p1}, pf_h2);
+                lo = (pf_h2){(_Float16)fmaf(-(float)hi[0], PF_LO, p0 * PF_LO),
+                             (_Float16)fmaf(-(float)hi[1], PF_LO, p1 * PF_LO)};
+            } else {
+                split_pair(p0, p1, hi, lo);
+            }
             ph[r >> 3][r & 7] = hi[0];
             ph[r >> 3][(r & 7) + 1] = hi[1];
             pl[r >> 3][r & 7] = lo[0];
@@ -730,8 +767,9 @@ k_attn_prefill(const float *__restrict__ q, int ntok, int qheads, int kvheads, i
                 const h4 v1 =
                     __builtin_bit_cast(h4, lds_read_tr16(vt + va[dt] + (16 * s2 + 8) * D * 2));
                 const h8 a = (h8){v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]};
+                f16v &low = FAR ? o2[FAR ? dt : 0] : o[dt];
                 o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, ph[s2], o[dt], 0, 0, 0);
-                o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, pl[s2], o[dt], 0, 0, 0);
+                low = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, pl[s2], low, 0, 0, 0);
             }
     };
     if constexpr (DB) {
@@ -776,6 +814,9 @@ k_attn_prefill(const float *__restrict__ q, int ntok, int qheads, int kvheads, i
             if (more) copy(vc, sb1, st + 1, cv);
         }
     }
+    if constexpr (FAR)
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) o[dt] += o2[dt] * (1.0f / PF_LO);
     lsum += swap32_f(lsum);
     pf_wait<0>();  // no copy in flight (a wavefront without tiles never waited for its own)
     __syncthreads();  // every wavefront is done with the stage buffers
@@ -803,7 +844,7 @@ k_attn_prefill(const float *__restrict__ q, int ntok, int qheads, int kvheads, i
         for (int k = 0; k < KW; ++k) M = fmaxf(M, mrg_m[k * RT + w0][tr]);
 #pragma unroll
         for (int k = 0; k < KW; ++k) {
-            f[k] = __builtin_amdgcn_exp2f(mrg_m[k * RT + w0][tr] - M);
+            f[k] = __builtin_amdgcn_exp2f((mrg_m[k * RT + w0][tr] - M) * (FAR ? scale2 : 1.0f));
             l = fmaf(mrg_l[k * RT + w0][tr], f[k], l);
         }
         const float inv = 1.0f / l;
@@ -861,7 +902,7 @@ size_t attn_prefill_workspace_bytes(int qheads, int hdim, int ntok) {
 
 void launch_attn_prefill(const float *q, int ntok, int qheads, int kvheads, int hdim, int pos0,
                          const uint16_t *kc, const uint16_t *vc, float *attn, int8_t *qs,
-                         uint16_t *qd, int16_t *bsum, hipStream_t st) {
+                         uint16_t *qd, int16_t *bsum, hipStream_t st, bool far) {
     if (ntok <= 0) return;
     const int per = qheads / kvheads;
     const float scale2 = softmax_scale2(hdim);
@@ -890,6 +931,30 @@ void launch_attn_prefill(const float *q, int ntok, int qheads, int kvheads, int 
                    : hdim <= 64 || tiles < 1280        ? 2
                                                        : 4;
     const dim3 grid((unsigned)((rows + 32 * rt - 1) / (32 * rt) * kvheads));
+#define PF_FAR(DIM, RT, KW)                                                                      \
+    SI_LAUNCH((k_attn_prefill<DIM, RT, KW, true, true>), far_grid(RT), dim3(RT * KW * 64), 0, st, q, \
+              ntok, qheads, kvheads, pos0, kc, vc, scale2, attn, qs, qd, bsum)
+    if (far) {
+        const auto far_grid = [&](int rt) {
+            return dim3((unsigned)((rows + 32 * rt - 1) / (32 * rt) * kvheads));
+        };
+        switch (hdim) {
+            case 32: if (rt == 1) PF_FAR(32, 1, 4); else PF_FAR(32, 2, 2); break;
+            case 64: if (rt == 1) PF_FAR(64, 1, 4); else PF_FAR(64, 2, 2); break;
+            case 96:
+                if (rt == 1) PF_FAR(96, 1, 4);
+                else if (rt == 2) PF_FAR(96, 2, 2);
+                else PF_FAR(96, 4, 2);
+                break;
+            default:
+                // (two tiles and their q take more than half of the LDS)
+                if (rt < 4) PF_FAR(128, 1, 4);
+                else PF_FAR(128, 4, 2);
+                break;
+        }
+        return;
+    }
+#undef PF_FAR
 #define PF_CALL(DIM, RT, KW, ASYNC)                                                         \
     SI_LAUNCH((k_attn_prefill<DIM, RT, KW, ASYNC>), grid, dim3(RT * KW * 64), 0, st, q, ntok, \
               qheads, kvheads, pos0, kc, vc, scale2, attn, qs, qd, bsum)

@@ -315,14 +315,19 @@ __global__ void __launch_bounds__(2 * D) k_kv4_read(Kv4Cache c, int ntok, int po
 // unit, 12 bits each of the head's largest value: every sum of 32 products (20
 // bits) is then exact in the matrix core, whose own rounding of a sum with an
 // offset of 8 sum q would show (24 bits of the head's largest q in all; as
-// fp16 roundings of q the result was off by up to 2.7e-5).  The weights' pair
-// has 22 bits.  With at most 8 heads a KV head both halves share one product:
-// columns 0-7 carry hi, 8-15 lo, and their results are added across (WIDE: 9 to
-// 16 heads, two products).
+// fp16 roundings of q the result was off by up to 2.7e-5).  With at most 8 heads a
+// KV head both halves share one product: columns 0-7 carry hi, 8-15 lo, and their
+// results are added across (WIDE: 9 to 16 heads, two products).
 //
-// A column's running maximum is moved only when a score of its own passes it by 2^8
-// (weights up to 256 fit the fp16 pair as well as weights up to 1), in a branch that
-// the wavefront takes together: no head's bits depend on the other heads'.
+// A column's running maximum is moved only when a score of its own passes it by 2^4,
+// in a branch that the wavefront takes together: no head's bits depend on the other
+// heads'.  A weight w against it, up to 2^4, goes in as w 2^11 (fp16 holds 2^16),
+// its lo half 2^11 higher still and in sums of its own (the lo columns', or WIDE's
+// second accumulators), so that the pair has 22 bits down to w = 2^-25 and an error of
+// at most 2^-47 below: a position with all the weight and a zero V row leaves the
+// others their bits up to 20 nats under it.  (In the same units and sums as hi, lo
+// was an fp16 subnormal from w = 2^-3 down and weights below 2^-25 were 0: 1.6e-5 of
+// the result 10 nats under such a position, all of a wavefront's at 18.)
 //
 // What bounds it: a step of 32 positions is about 230 vector operations and 17 matrix
 // instructions (two products: 260 and 34), which hardly overlap, 0.7 us of a SIMD at
@@ -339,6 +344,9 @@ typedef float f2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 
 constexpr int A4_GROUP = 32;  // positions of a wavefront's step
+constexpr float A4_SLACK = 4.0f;  // log2 of the largest weight
+constexpr float A4_UP = 11.0f;    // log2 of a weight's unit in hi
+constexpr float A4_LO = 2048.0f;  // and of lo's in hi's
 
 __device__ __forceinline__ float ror8_add(float v) { return v + dpp_f<DPP_ROR8>(v); }
 
@@ -630,7 +638,7 @@ __global__ void __launch_bounds__(64 * NW, NW > 4 || MODE ? 2 : 3) k_attn_kv4(
     // difference between three wavefronts a SIMD and two).
     float fac;
     const bool lo_half = !WIDE && col >= 8;
-    const float lo_col = lo_half ? 1.0f : 0.0f;
+    const float lo_col = lo_half ? A4_LO : 0.0f, lo_mul = lo_half ? A4_LO : 1.0f;
     {
         float *qmax = &mo[0][0][0];  // [KS][64]
         const int hc = WIDE ? col : col & 7;
@@ -682,16 +690,20 @@ __global__ void __launch_bounds__(64 * NW, NW > 4 || MODE ? 2 : 3) k_attn_kv4(
         }
         __syncthreads();
     }
-    // The running maximum m and its limit lim stay in the scores' raw units (fac
-    // makes them powers of two): weights are 2^((s - m) fac), whose error goes with
-    // the difference, not with the scores.  The sums of the weights are one more
-    // product's rows (ones . P), like the outputs in hi and lo columns.
-    const float over = 8.0f * __builtin_amdgcn_rcpf(fac);
+    // The running maximum m stays in the scores' raw units (fac makes them powers of
+    // two): weights are 2^((s - m) fac), whose error goes with the difference, not
+    // with the scores, and a score passes m by a difference too (m + over would round
+    // up to 2 over where that is about m's last place).  The sums of the weights are
+    // one more product's rows (ones . P), like the outputs in hi and lo.
+    const float over = A4_SLACK * __builtin_amdgcn_rcpf(fac);
     // ref: m, or 0 while a column has seen no position.
-    float m = -INFINITY, ref = 0.0f, lim = -INFINITY;
-    f4 o[DT], ol = {0.0f, 0.0f, 0.0f, 0.0f};
+    float m = -INFINITY, ref = 0.0f;
+    constexpr int LO = WIDE ? DT : 0;  // WIDE: the lo halves' sums
+    f4 o[DT], ol = {0.0f, 0.0f, 0.0f, 0.0f}, o2[LO + 1], ol2 = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) o[dt] = (f4){0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int dt = 0; dt < LO; ++dt) o2[dt] = (f4){0.0f, 0.0f, 0.0f, 0.0f};
     // constants held in registers, so that (n & mask) | magic is one operation
     uint32_t mask = 0x00f000f0u, magic = 0x54005400u;
     asm("" : "+s"(mask));
@@ -757,37 +769,39 @@ __global__ void __launch_bounds__(64 * NW, NW > 4 || MODE ? 2 : 3) k_attn_kv4(
         }
         float mx = fmaxf(fmaxf(fmaxf(p[0][0], p[0][1]), fmaxf(p[0][2], p[0][3])),
                          fmaxf(fmaxf(p[1][0], p[1][1]), fmaxf(p[1][2], p[1][3])));
-        if (__ballot(mx > lim)) {
+        if (__ballot(mx - m > over)) {
             mx = fmaxf(mx, swap16_f(mx));
             mx = fmaxf(mx, swap32_f(mx));
-            const float mn = mx > lim ? mx : m;  // the column's own, whatever the others do
+            const float mn = mx - m > over ? mx : m;  // the column's own, whatever the others do
             const float al = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - mn) * fac);
             m = mn;
             ref = mn == -INFINITY ? 0.0f : mn;
-            lim = mn + over;
             ol *= al;
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt) o[dt] *= al;
+            if constexpr (WIDE) ol2 *= al;
+#pragma unroll
+            for (int dt = 0; dt < LO; ++dt) o2[dt] *= al;
         }
         u4 pa, pb;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const f2 x = {__builtin_amdgcn_exp2f((p[0][i] - ref) * fac),
-                          __builtin_amdgcn_exp2f((p[1][i] - ref) * fac)};
+            const f2 x = {__builtin_amdgcn_exp2f(fmaf(p[0][i] - ref, fac, A4_UP)),
+                          __builtin_amdgcn_exp2f(fmaf(p[1][i] - ref, fac, A4_UP))};
             const h2 hi = __builtin_convertvector(x, h2);
             if constexpr (WIDE) {
                 pa[i] = as_u(hi);
-                pb[i] = as_u((h2){(_Float16)(x[0] - (float)hi[0]),
-                                  (_Float16)(x[1] - (float)hi[1])});
+                pb[i] = as_u((h2){(_Float16)fmaf(-(float)hi[0], A4_LO, x[0] * A4_LO),
+                                  (_Float16)fmaf(-(float)hi[1], A4_LO, x[1] * A4_LO)});
             } else {
-                pa[i] = as_u((h2){(_Float16)fmaf(-(float)hi[0], lo_col, x[0]),
-                                  (_Float16)fmaf(-(float)hi[1], lo_col, x[1])});
+                pa[i] = as_u((h2){(_Float16)fmaf(-(float)hi[0], lo_col, x[0] * lo_mul),
+                                  (_Float16)fmaf(-(float)hi[1], lo_col, x[1] * lo_mul)});
             }
         }
         const h8 ph = __builtin_bit_cast(h8, pa), pl = __builtin_bit_cast(h8, pb);
         const u4 ones = {0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u};
         const h8 one = __builtin_bit_cast(h8, ones);
-        if constexpr (WIDE) ol = __builtin_amdgcn_mfma_f32_16x16x32_f16(one, pl, ol, 0, 0, 0);
+        if constexpr (WIDE) ol2 = __builtin_amdgcn_mfma_f32_16x16x32_f16(one, pl, ol2, 0, 0, 0);
         ol = __builtin_amdgcn_mfma_f32_16x16x32_f16(one, ph, ol, 0, 0, 0);
 #pragma unroll
         for (int b = 0; b < KS; ++b) {
@@ -804,7 +818,7 @@ __global__ void __launch_bounds__(64 * NW, NW > 4 || MODE ? 2 : 3) k_attn_kv4(
                                                            as_h2(hv[i]), as_h2(off[i])));
                 const h8 vv = __builtin_bit_cast(h8, va);
                 if constexpr (WIDE)
-                    o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vv, pl, o[dt], 0, 0, 0);
+                    o2[dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vv, pl, o2[dt], 0, 0, 0);
                 o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vv, ph, o[dt], 0, 0, 0);
             }
         }
@@ -822,7 +836,8 @@ __global__ void __launch_bounds__(64 * NW, NW > 4 || MODE ? 2 : 3) k_attn_kv4(
     }
     // The wavefronts' states meet in LDS: maxima and sums, then the outputs, four
     // wavefronts at a time, added by a thread per four dims in wavefront order.
-    const float lsum = WIDE ? ol[0] : ror8_add(ol[0]);
+    const float lo_unit = lo_half ? 1.0f / A4_LO : 1.0f;
+    const float lsum = WIDE ? fmaf(ol2[0], 1.0f / A4_LO, ol[0]) : ror8_add(ol[0] * lo_unit);
     if (lsum != lsum) m = 0.0f;  // no score of a NaN query passes a limit: not an empty state
     if (g == 0 && col < rows) {
         mm[wave][col] = m;
@@ -861,9 +876,11 @@ __global__ void __launch_bounds__(64 * NW, NW > 4 || MODE ? 2 : 3) k_attn_kv4(
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt) {
                 f4 v = o[dt];
-                if constexpr (!WIDE)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) v[i] = ror8_add(v[i]);
+                for (int i = 0; i < 4; ++i) {
+                    if constexpr (WIDE) v[i] = fmaf(o2[dt][i], 1.0f / A4_LO, v[i]);
+                    else v[i] = ror8_add(v[i] * lo_unit);
+                }
                 if (col < rows) *(f4 *)&mo[wave - w0][col][16 * dt + 4 * g] = v * 16.0f;
             }
         }
@@ -1144,7 +1161,8 @@ void launch_attention_kv4(const float *q, int nq, int qheads, int hdim, const Kv
     if (kv4_by_rows(qheads, nq, ctx_step, max_ctx)) {
         uint16_t *k = (uint16_t *)ws, *v = k + (size_t)max_ctx * c.kvheads * hdim;
         launch_kv4_read(c, ctx0 - 1 + nq, hdim, 0, 1, nullptr, k, v, st);
-        launch_attn_prefill(q, nq, qheads, c.kvheads, hdim, ctx0 - 1, k, v, attn, qs, d, bsum, st);
+        launch_attn_prefill(q, nq, qheads, c.kvheads, hdim, ctx0 - 1, k, v, attn, qs, d, bsum, st,
+                            true);
         return;
     }
     const long long base = a4_base(qheads, c.kvheads, nq, ctx_step);

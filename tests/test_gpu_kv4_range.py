@@ -1,0 +1,81 @@
+"""Attention over the 4-bit cache where a position far above the others has no part in the
+output (an attention sink whose V row is zero), by every way a call runs.
+
+The bound stays 2e-5 of a row's largest value.  A weight is held against the largest that its
+wavefront has seen, w, as an fp16 pair of w 2^11 whose low half is held 2^11 higher: w >= 2^-25 to
+2^-22 of itself, less to 2^-47.  At 20 nats (2^-28.9) that is at most 2^-18 = 3.8e-6 of a weight,
+should all of them be off to the same side; the scores' own error at a score S is S 4 2^-24, at
+30 7e-6."""
+import numpy as np
+import pytest
+
+from tests import kv4_ref as ref
+from tests.gpu_helpers import dev
+from tests.test_gpu_kv4 import Cache, _attention, _close, _want
+
+pytestmark = pytest.mark.gpu
+
+
+def _sinks(rng, name, nseq, longest, sinks, gap, spread):
+    """A cache whose sequences hold at positions `sinks` a K row that scores `gap` above the
+    others' mean (the others spread by `spread`) and a zero V row; and the query for it."""
+    c = Cache(rng, name, nseq, longest, 64)
+    n = c.npages * 64
+    k = np.zeros((n, c.kv, c.D), np.float32)
+    k[:, :, 0] = 8.0  # the first block's scale is 1: dim 1 holds whole numbers
+    k[:, :, 32:] = rng.standard_normal((n, c.kv, c.D - 32))
+    if c.D == 32:
+        k[:, :, 2:] = rng.integers(-1, 2, (n, c.kv, 30))
+    v = rng.standard_normal((n, c.kv, c.D)).astype(np.float32)
+    for pages in c.pages:
+        for p in sinks:
+            row = pages[p // 64] * 64 + p % 64
+            k[row, :, 1:] = 0
+            k[row, :, 1] = 7
+            v[row] = 0
+    c.k0, c.v0 = ref.pack(k, c.kv, c.D, 64, True), ref.pack(v, c.kv, c.D, 64, False)
+    c.k, c.v = dev(c.k0), dev(c.v0)
+
+    def queries(nq):
+        q = rng.standard_normal((nq, c.q, c.D)).astype(np.float32) * spread
+        q[:, :, 0] = 0
+        q[:, :, 1] = gap * np.sqrt(c.D) / 7
+        return q
+    return c, queries
+
+
+GAPS = [(10, 0.3), (14, 0.3), (17, 0.0), (20, 0.0), (20, 0.3)]
+
+
+@pytest.mark.parametrize("gap,spread", GAPS)
+@pytest.mark.parametrize("name,nq,n", [
+    ("g7_d128", 1, 512), ("g7_d128", 16, 1500), ("g7_d128", 1, 5000), ("g7_d128", 200, 800),
+    ("g7_d64", 3, 1100), ("g1_d32", 1, 3000), ("g3_d96", 4, 700),
+    ("g16_d64", 1, 500), ("g16_d64", 2, 4000), ("g9_d32", 30, 900), ("g16_d128", 5, 2500)])
+def test_sinks_of_queries(name, nq, n, gap, spread):
+    """One query a sequence: whole contexts in four and in eight wavefronts, and split."""
+    rng = np.random.default_rng(n + nq)
+    c, queries = _sinks(rng, name, nq, n, [3], gap, spread)
+    q = queries(nq)
+    some = sorted({0, nq // 2, nq - 1})
+    want = _want(c, q[some], some, [n] * len(some))
+    _close(_attention(c, dev(q), nq, None, n, 0, n)[some], want, (name, "host contexts"))
+    ctx = np.full(nq, n, np.int32)
+    _close(_attention(c, dev(q), nq, dev(ctx), 0, 0, n)[some], want, (name, "device contexts"))
+
+
+@pytest.mark.parametrize("gap,spread", GAPS)
+@pytest.mark.parametrize("name,nq,first", [
+    ("g7_d128", 2, 700), ("g7_d128", 20, 1500), ("g16_d64", 40, 300), ("g9_d32", 3, 4000),
+    ("g1_d32", 60, 900), ("g3_d96", 33, 600),
+    # by fp16 rows: every kernel that takes them
+    ("g7_d128", 322, 700), ("g7_d128", 1500, 100), ("g7_d64", 700, 500), ("g16_d64", 1030, 64),
+    ("g3_d96", 400, 900), ("g3_d96", 1000, 50), ("g3_d96", 1800, 50), ("g1_d32", 1200, 300),
+    ("g1_d32", 4100, 100)])
+def test_sinks_of_prompts(name, nq, first, gap, spread):
+    rng = np.random.default_rng(first + nq)
+    c, queries = _sinks(rng, name, 1, first + nq, [0, 37], gap, spread)
+    q = queries(nq)
+    some = sorted({0, 1, nq // 2, nq - 1})
+    got = _attention(c, dev(q), nq, None, first + 1, 1, first + nq)
+    _close(got[some], _want(c, q[some], [0] * len(some), first + 1 + np.array(some)), name)
