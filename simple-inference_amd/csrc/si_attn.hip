@@ -535,6 +535,8 @@ __device__ __forceinline__ void pf_barrier() {
 // to 2^-25 and an error of at most 2^-47 below.  (Else lo, in hi's units and sums, is an
 // fp16 subnormal from 2^-3 down, and weights below 2^-25 are 0.)  The second sums take
 // D / 2 registers, which past 64 dims come from q's lo halves: those wait in LDS.
+// And each row of q is scaled by a power of two, which its scores' unit gives back:
+// fp16 halves of q as it comes are infinite from 65520 and lose bits below 2^-14.
 constexpr float PF_SLACK = 4.0f, PF_UP = 11.0f, PF_LO = 2048.0f;
 template <int D, int RT, int KW, bool ASYNC, bool FAR = false>
 __global__ void __launch_bounds__(RT * KW * 64) __attribute__((amdgpu_waves_per_eu(2)))
@@ -564,6 +566,7 @@ k_attn_prefill(const float *__restrict__ q, int ntok, int qheads, int kvheads, i
     __shared__ __attribute__((aligned(16))) uint8_t qlo[QL && !QL_IN ? QL : 16];
     uint8_t *const ql_at = QL_IN ? sb0 + STAGE : qlo;
     __shared__ float mrg_m[NWV][PF_T], mrg_l[NWV][PF_T];
+    __shared__ float row_unit[FAR ? 32 * RT : 1];  // of a row's scores, in powers of two
     __shared__ int64_t rowoff[32 * RT];  // output offset of a row, -1 past the last
 
     const int per = qheads / kvheads, nrows = ntok * per;
@@ -631,6 +634,7 @@ k_attn_prefill(const float *__restrict__ q, int ntok, int qheads, int kvheads, i
     const size_t qoff = ((size_t)(myrow / per) * qheads + g * per + myrow % per) * D;
     if (kw == 0 && hh == 0) rowoff[32 * rt + t] = wr0 + t < nrows ? (int64_t)qoff : -1;
     h8 qh[KS], ql[QLDS ? 1 : KS];
+    float fac = scale2;
     {
         const float *qrow = q + qoff + 8 * hh;
         float4 a[KS], b[KS];
@@ -639,10 +643,28 @@ k_attn_prefill(const float *__restrict__ q, int ntok, int qheads, int kvheads, i
             a[ks] = *(const float4 *)(qrow + 16 * ks);
             b[ks] = *(const float4 *)(qrow + 16 * ks + 4);
         }
+        int up = 0;  // the row's largest value to 2^14 (one below 2^-60 makes no score)
+        if constexpr (FAR) {
+            float big = 0.0f;
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks)
+                big = fmaxf(big, fmaxf(fmaxf(fmaxf(fabsf(a[ks].x), fabsf(a[ks].y)),
+                                             fmaxf(fabsf(a[ks].z), fabsf(a[ks].w))),
+                                       fmaxf(fmaxf(fabsf(b[ks].x), fabsf(b[ks].y)),
+                                             fmaxf(fabsf(b[ks].z), fabsf(b[ks].w)))));
+            big = fmaxf(big, swap32_f(big));
+            up = 14 - max((int)(f2u(big) >> 23) - 127, -60);
+            // (finite for the largest q too, whose weights are then 0 or 1 either way)
+            fac = fminf(__builtin_amdgcn_ldexpf(scale2, -up), 0x1.fffffep127f);
+            if (kw == 0 && hh == 0) row_unit[32 * rt + t] = fac;
+        }
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
-            const float x[8] = {a[ks].x, a[ks].y, a[ks].z, a[ks].w,
-                                b[ks].x, b[ks].y, b[ks].z, b[ks].w};
+            float x[8] = {a[ks].x, a[ks].y, a[ks].z, a[ks].w,
+                          b[ks].x, b[ks].y, b[ks].z, b[ks].w};
+            if constexpr (FAR)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[e] = __builtin_amdgcn_ldexpf(x[e], up);
             h8 &l = ql[QLDS ? 0 : ks];
 #pragma unroll
             for (int e = 0; e < 8; e += 2) {
@@ -673,7 +695,7 @@ k_attn_prefill(const float *__restrict__ q, int ntok, int qheads, int kvheads, i
                  (s16 & 1) * 8;
 
     float m = -INFINITY, lsum = 0.0f;  // row t's running max; this lane's share of the sum
-    const float over = PF_SLACK * __builtin_amdgcn_rcpf(scale2);  // (FAR)
+    const float over = PF_SLACK * __builtin_amdgcn_rcpf(fac);  // (FAR)
     constexpr int LO = FAR ? DT : 0;
     f16v o[DT], o2[LO + 1];  // FAR: o2, the lo halves' sums
 #pragma unroll
@@ -722,7 +744,7 @@ k_attn_prefill(const float *__restrict__ q, int ntok, int qheads, int kvheads, i
         // (FAR: by a row of its own only: 2^4 over m, raw scores.)
         const float mnew = FAR ? (mx - m > over ? mx : m) : fmaxf(m, mx * scale2);
         if (FAR ? __ballot(mnew > m) : __ballot(mnew > m + 8.0f)) {
-            const float alpha = __builtin_amdgcn_exp2f(FAR ? (m - mnew) * scale2 : m - mnew);
+            const float alpha = __builtin_amdgcn_exp2f(FAR ? (m - mnew) * fac : m - mnew);
             const float a0 = mnew == -INFINITY ? 1.0f : alpha;
             lsum *= a0;
 #pragma unroll
@@ -735,9 +757,9 @@ k_attn_prefill(const float *__restrict__ q, int ntok, int qheads, int kvheads, i
         float ps = 0.0f;
 #pragma unroll
         for (int r = 0; r < 16; r += 2) {
-            const float p0 = __builtin_amdgcn_exp2f(FAR ? fmaf(s[r] - mref, scale2, PF_UP)
+            const float p0 = __builtin_amdgcn_exp2f(FAR ? fmaf(s[r] - mref, fac, PF_UP)
                                                         : fmaf(s[r], scale2, -mref));
-            const float p1 = __builtin_amdgcn_exp2f(FAR ? fmaf(s[r + 1] - mref, scale2, PF_UP)
+            const float p1 = __builtin_amdgcn_exp2f(FAR ? fmaf(s[r + 1] - mref, fac, PF_UP)
                                                         : fmaf(s[r + 1], scale2, -mref));
             ps += p0;
             ps += p1;
@@ -844,7 +866,7 @@ k_attn_prefill(const float *__restrict__ q, int ntok, int qheads, int kvheads, i
         for (int k = 0; k < KW; ++k) M = fmaxf(M, mrg_m[k * RT + w0][tr]);
 #pragma unroll
         for (int k = 0; k < KW; ++k) {
-            f[k] = __builtin_amdgcn_exp2f((mrg_m[k * RT + w0][tr] - M) * (FAR ? scale2 : 1.0f));
+            f[k] = __builtin_amdgcn_exp2f((mrg_m[k * RT + w0][tr] - M) * (FAR ? row_unit[FAR ? tid : 0] : 1.0f));
             l = fmaf(mrg_l[k * RT + w0][tr], f[k], l);
         }
         const float inv = 1.0f / l;
