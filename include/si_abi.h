@@ -519,9 +519,10 @@ int si_layer_decode_paged(si_layer_t *l, const float *x, int nseq, uint16_t *k_p
                           int max_pages, const int *ctx_dev, int context, int max_ctx,
                           float *out, int flags, void *stream);
 
-/* si_layer_decode_paged over a 4-bit cache (pools, page lists and contexts as
- * for si_kv4_write with pos_step 0: sequence i's new token at ctx_dev[i] - 1, or
- * context - 1); at most 65535 sequences.  RoPE and the append run as
+/* si_layer_decode_paged over a 4-bit cache (pools and page lists as for
+ * si_kv4_write with pos_step 0: sequence i's new token at ctx_dev[i] - 1, or
+ * context - 1; ctx_dev[i] past max_ctx is max_ctx, below 1 the sequence attends
+ * to nothing and its pages are left as they are); at most 65535 sequences.  RoPE and the append run as
  * si_rope_kv4_append (the rope_kv phase), attention as si_attention_kv4. */
 int si_layer_decode_kv4(si_layer_t *l, const float *x, int nseq, uint8_t *k_pool, uint8_t *v_pool,
                         int npages, int page_size, const int *pages, int max_pages,

@@ -1396,7 +1396,7 @@ static int run_rows(si_layer *L, const float *x, int rows, uint16_t *kc, uint16_
         // attention over the pages -> Q8
         mark(L, SI_PHASE_ROPE_KV, st);
         launch_rope_kv4(L->qkv, NQKV, rows, s.qheads, s.hdim, pos0, 0, max_ctx, ctx_dev,
-                        L->rope_cos, L->rope_sin, L->q, *kv4, st);
+                        L->rope_cos, L->rope_sin, L->q, *kv4, st, true);
         mark(L, SI_PHASE_ATTENTION_Q8, st);
         tl_att = tl_x;
         launch_attention_kv4(L->q, rows, s.qheads, s.hdim, *kv4, ctx_dev, ctx0, 0, max_ctx,

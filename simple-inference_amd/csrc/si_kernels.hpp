@@ -339,10 +339,12 @@ struct Kv4Cache {
 };
 // RoPE of q|k|v rows, q to q_out, K and V quantized into the pages: tokens at
 // pos0 + t of sequence 0 (pos_step 1), or token t of sequence t at ctx_dev[t] - 1
-// (or pos0).  Positions outside the page lists or max_pos are skipped.
+// (or pos0).  Positions outside the page lists or max_pos are skipped; with clamp,
+// ctx_dev[t] past them is the last one (as attention takes it).
 void launch_rope_kv4(const float *qkv, int ldqkv, int ntok, int qheads, int hdim, int pos0,
                      int pos_step, int max_pos, const int *ctx_dev, const float *rc,
-                     const float *rs, float *q_out, const Kv4Cache &c, hipStream_t st);
+                     const float *rs, float *q_out, const Kv4Cache &c, hipStream_t st,
+                     bool clamp = false);
 // fp16 rows [ntok][kvheads * hdim] into the pages, and back
 void launch_kv4_write(const uint16_t *k, const uint16_t *v, int ntok, int hdim, int pos0,
                       int pos_step, const int *ctx_dev, const Kv4Cache &c, hipStream_t st);

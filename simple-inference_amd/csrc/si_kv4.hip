@@ -99,11 +99,12 @@ struct Kv4Scale {
 // Which tokens of a call fall into a workgroup's unit, 8 positions aligned at 8
 // of one sequence: with pos_step 1 the call's tokens are positions pos0 + t of
 // sequence 0, else token t is one position of sequence t (ctx_dev[t] - 1, or
-// pos0).  Tokens t0 + j sit at base + j for j in [lo, hi).
+// pos0).  Tokens t0 + j sit at base + j for j in [lo, hi).  A device context past
+// `limit` is skipped, or taken as limit (clamp).
 struct Kv4Unit {
     int seq, base, t0, lo, hi;
     __device__ __forceinline__ Kv4Unit(int x, int ntok, int pos0, int pos_step,
-                                       const int *ctx_dev, int limit) {
+                                       const int *ctx_dev, int limit, bool clamp = false) {
         if (pos_step) {
             seq = 0;
             base = (pos0 & ~7) + 8 * x;
@@ -111,7 +112,8 @@ struct Kv4Unit {
             lo = max(-t0, 0);
             hi = min(min(ntok - t0, limit - base), 8);
         } else {
-            const int ctx = ctx_dev ? ctx_dev[x] : pos0 + 1;
+            int ctx = ctx_dev ? ctx_dev[x] : pos0 + 1;
+            if (clamp) ctx = min(ctx, limit);
             const bool live = ctx >= 1 && ctx <= limit;  // device contexts: not host-checked
             const int pos = live ? ctx - 1 : 0;
             seq = x;
@@ -158,9 +160,9 @@ __global__ void __launch_bounds__(2 * D) k_kv4_append(
     const float *__restrict__ qkv, int ldqkv, const uint16_t *__restrict__ kin,
     const uint16_t *__restrict__ vin, int qheads, int ntok, int pos0, int pos_step, int limit,
     const int *__restrict__ ctx_dev, const float *__restrict__ rc, const float *__restrict__ rs,
-    float *__restrict__ q_out, bool wide, Kv4Cache c) {
+    float *__restrict__ q_out, bool wide, bool clamp, Kv4Cache c) {
     constexpr int HALF = D / 2;
-    const Kv4Unit un((int)blockIdx.x, ntok, pos0, pos_step, ctx_dev, limit);
+    const Kv4Unit un((int)blockIdx.x, ntok, pos0, pos_step, ctx_dev, limit, clamp);
     if (un.lo >= un.hi) return;
     const int tid = threadIdx.x, kvh = c.kvheads, qd = qheads * D, kvd = kvh * D;
     const int g = blockIdx.y;
@@ -1046,7 +1048,8 @@ __global__ void __launch_bounds__(256) k_kv_copy(KvMoves mv, size_t page_bytes) 
 
 void launch_rope_kv4(const float *qkv, int ldqkv, int ntok, int qheads, int hdim, int pos0,
                      int pos_step, int max_pos, const int *ctx_dev, const float *rc,
-                     const float *rs, float *q_out, const Kv4Cache &c, hipStream_t st) {
+                     const float *rs, float *q_out, const Kv4Cache &c, hipStream_t st,
+                     bool clamp) {
     if (ntok <= 0) return;
     const int limit = (int)min((long long)max_pos, (long long)c.max_pages << c.shift);
     const int qy = (qheads * hdim / 2 + 2 * hdim - 1) / (2 * hdim);
@@ -1055,7 +1058,7 @@ void launch_rope_kv4(const float *qkv, int ldqkv, int ntok, int qheads, int hdim
     const dim3 grid(kv4_units(ntok, pos0, pos_step), c.kvheads + qy);
 #define CALL(DIM)                                                                               \
     SI_LAUNCH((k_kv4_append<DIM, false>), grid, dim3(2 * DIM), 0, st, qkv, ldqkv, nullptr,      \
-              nullptr, qheads, ntok, pos0, pos_step, limit, ctx_dev, rc, rs, q_out, wide, c)
+              nullptr, qheads, ntok, pos0, pos_step, limit, ctx_dev, rc, rs, q_out, wide, clamp, c)
     KV4_DIM(hdim, CALL)
 #undef CALL
 }
@@ -1067,7 +1070,7 @@ void launch_kv4_write(const uint16_t *k, const uint16_t *v, int ntok, int hdim, 
     const dim3 grid(kv4_units(ntok, pos0, pos_step), c.kvheads);
 #define CALL(DIM)                                                                            \
     SI_LAUNCH((k_kv4_append<DIM, true>), grid, dim3(2 * DIM), 0, st, nullptr, 0, k, v, 0, ntok, \
-              pos0, pos_step, limit, ctx_dev, nullptr, nullptr, nullptr, false, c)
+              pos0, pos_step, limit, ctx_dev, nullptr, nullptr, nullptr, false, false, c)
     KV4_DIM(hdim, CALL)
 #undef CALL
 }
