@@ -273,7 +273,9 @@ int si_stack_nseq(const si_stack_t *st);
 /* Grows each of the nseq distinct sequences seqs[] by one position (the
  * token about to be decoded) and uploads their page lists and contexts in
  * batch order (synchronous copies, after waiting for the stream of the
- * previous si_stack_decode, whose kernels read them).  -1 when the pool is exhausted (the
+ * previous si_stack_decode, whose kernels read them; for the device, once a
+ * decode has been captured, as its replays run on streams of the caller's, or
+ * when decodes ran on several).  -1 when the pool is exhausted (the
  * lengths are left as before; pages already taken stay with their
  * sequences, and si_stack_decode dies until a later prepare succeeds),
  * else 0. */
@@ -284,11 +286,13 @@ int si_stack_prepare(si_stack_t *st, const int *seqs, int nseq);
  * or writes the pools on a stream of its own (si_kv4_write, si_kv4_read) has
  * finished that work before either call, and starts more after it returns. */
 int si_stack_fork(si_stack_t *st, int seq);
-/* si_kv_compact with its copies in every pool (waits for them, and for the
- * stream of the last decode); a si_stack_prepare has to follow. */
+/* si_kv_compact with its copies in every pool (waits for them, and before for
+ * the decodes as si_stack_prepare does); a si_stack_prepare has to follow. */
 int si_stack_compact(si_stack_t *st);
 /* x [nseq][hidden] (device) through every layer -> out [nseq][hidden]: the
- * residual stream of a decode step; kernel launches only (capturable). */
+ * residual stream of a decode step; kernel launches only (capturable: a replay
+ * decodes the sequences of the last si_stack_prepare, of as many as when it
+ * was captured). */
 void si_stack_decode(si_stack_t *st, const float *x, float *out, int flags, void *stream);
 
 /* Offline weight preparation (host memory): ggml's Q4_0 rule, the format

@@ -306,6 +306,8 @@ struct si_stack {
     int nseq;       /* rows of the last prepare */
     void *stream;   /* stream of the last si_stack_decode */
     int pending;    /* a decode was enqueued since the last prepare */
+    int streams;    /* and another before it, on another stream */
+    int captured;   /* a decode was captured: its replays run on any stream, unseen */
 };
 
 si_stack_t *si_stack_create(const si_shape_t *s, const si_layer_host_t *layers, int nlayers,
@@ -387,9 +389,17 @@ int si_stack_nseq(const si_stack_t *st) { return st->nseq; }
 
 /* The previous step's kernels, which read the pools and the device table. */
 static void wait_decode(si_stack_t *st) {
-    if (st->pending)
+    if (st->captured || st->streams)
+        hip_check(hipDeviceSynchronize(), "si_stack: wait");
+    else if (st->pending)
         hip_check(hipStreamSynchronize((hipStream_t)st->stream), "si_stack: wait");
-    st->pending = 0;
+    st->pending = st->streams = 0;
+}
+
+static int is_capturing(void *stream) {
+    hipStreamCaptureStatus s = hipStreamCaptureStatusNone;
+    return stream && hipStreamIsCapturing((hipStream_t)stream, &s) == hipSuccess &&
+           s != hipStreamCaptureStatusNone;
 }
 
 /* The bookkeeping's copies in every pool (after wait_decode), and until done. */
@@ -478,6 +488,11 @@ void si_stack_decode(si_stack_t *st, const float *x, float *out, int flags, void
                   "si_layer_decode_paged");
         in = o;
     }
+    if (is_capturing(stream)) {
+        st->captured = 1;
+        return;
+    }
+    if (st->pending && st->stream != stream) st->streams = 1;
     st->stream = stream;
     st->pending = 1;
 }
