@@ -292,7 +292,8 @@ int si_stack_compact(si_stack_t *st);
 /* x [nseq][hidden] (device) through every layer -> out [nseq][hidden]: the
  * residual stream of a decode step; kernel launches only (capturable: a replay
  * decodes the sequences of the last si_stack_prepare, of as many as when it
- * was captured). */
+ * was captured; over fp16 pools up to the longest context at the capture, past
+ * which the step is to be captured again; over 4-bit pools any). */
 void si_stack_decode(si_stack_t *st, const float *x, float *out, int flags, void *stream);
 
 /* Offline weight preparation (host memory): ggml's Q4_0 rule, the format

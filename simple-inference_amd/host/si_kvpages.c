@@ -468,9 +468,12 @@ int si_stack_prepare(si_stack_t *st, const int *seqs, int nseq) {
 
 void si_stack_decode(si_stack_t *st, const float *x, float *out, int flags, void *stream) {
     if (st->nseq < 1) die("si_stack_decode: no si_stack_prepare call");
+    const int capturing = is_capturing(stream);
     int max_ctx = 1;
     for (int i = 0; i < st->nseq; ++i)
         if (st->host_ctx[i] > max_ctx) max_ctx = st->host_ctx[i];
+    /* the contexts of its replays are any */
+    if (capturing && st->format == SI_KV_Q4) max_ctx = st->max_ctx;
     const float *in = x;
     for (int l = 0; l < st->nlayers; ++l) {
         float *o = l == st->nlayers - 1 ? out : st->act[l & 1];
@@ -488,7 +491,7 @@ void si_stack_decode(si_stack_t *st, const float *x, float *out, int flags, void
                   "si_layer_decode_paged");
         in = o;
     }
-    if (is_capturing(stream)) {
+    if (capturing) {
         st->captured = 1;
         return;
     }

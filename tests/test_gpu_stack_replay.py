@@ -98,3 +98,43 @@ def test_prepare_waits_for_replays(oracle, fmt):
     torch.cuda.synchronize()
     assert torch.isfinite(out).all()
     S.close()
+
+
+def test_replays_of_growing_contexts(oracle):
+    """A 4-bit step captured once, replayed as its sequences grow past every context that it was
+    captured with: the bits of its layers called for the stack's longest contexts."""
+    import torch
+    S = Stack(oracle, si_amd.SI_KV_Q4, 200)
+    layers = [si_amd.Layer(S.s, lay, SEQS, S.max_ctx) for lay in S.lays]
+    mem = [[t.clone() for t in pair] for pair in S.pools]
+    rng = np.random.default_rng(2)
+    seqs = [S.H.si_kv_seq_add(S.pg) for _ in range(3)]
+    x, out = empty((3, S.s.hidden), torch.float32), empty((3, S.s.hidden), torch.float32)
+    graph = None
+    for step in range(40):
+        if step == 20:
+            S.H.si_kv_seq_truncate(S.pg, seqs[1], 4)
+        S.prepare(seqs)
+        x.copy_(dev(rng.standard_normal((3, S.s.hidden)).astype(np.float32)))
+        torch.cuda.synchronize()
+        if graph is None:
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                S.decode(x, out)
+        graph.replay()
+        table = np.ctypeslib.as_array(S.H.si_kv_page_table(S.pg), shape=(SEQS * S.mp,)).reshape(
+            SEQS, S.mp)
+        tab = dev(table[seqs].copy())
+        ctx = dev(np.array([S.H.si_kv_seq_len(S.pg, i) for i in seqs], np.int32))
+        cur = x
+        for L, (k, v) in zip(layers, mem):
+            o = empty((3, S.s.hidden), torch.float32)
+            L.decode_kv4(cur, 3, k, v, NPAGES, PS, tab, S.mp, ctx, S.max_ctx, o, capture=False)
+            cur = o
+        torch.cuda.synchronize()
+        assert torch.equal(out, cur), step
+        for a, b in zip(S.pools, mem):
+            assert all(torch.equal(s, t) for s, t in zip(a, b)), step
+    S.close()
+    for L in layers:
+        L.close()

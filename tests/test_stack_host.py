@@ -113,6 +113,18 @@ BODIES = {
     running[4] = 1;
     CHECK(si_stack_prepare(st, seqs + 1, 1) == 0);
 """,
+    # contexts grow between a captured 4-bit step's replays
+    "capture": """
+    CHECK(si_stack_prepare(st, seqs, 1) == 0);
+    si_stack_decode(st, x, out, 0, S(1));
+    CHECK(last_max == 6);
+    capturing = 3;
+    si_stack_decode(st, x, out, 0, S(3));
+    CHECK(last_max == (format == SI_KV_Q4 ? 96 : 6));
+    capturing = 0;
+    si_stack_decode(st, x, out, 0, S(1));
+    CHECK(last_max == 6);
+""",
     "streams": """
     si_stack_decode(st, x, out, 0, S(2));         /* the same step again, on another stream */
     seqs[1] = si_stack_fork(st, seqs[0]);
