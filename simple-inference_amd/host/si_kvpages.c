@@ -294,6 +294,7 @@ const int *si_kv_page_table(const si_kv_pages_t *p) { return p->table; }
 struct si_stack {
     si_shape_t shape;
     int nlayers, max_seqs, max_ctx, page_size, npages, format;
+    int device;     /* current when it was created: its pools' and tables' */
     size_t page_bytes;
     si_workspace_t *ws;
     si_layer_t **layers;
@@ -329,6 +330,7 @@ si_stack_t *si_stack_create_kv(const si_shape_t *s, const si_layer_host_t *layer
     st->max_ctx = max_ctx;
     st->page_size = page_size;
     st->npages = npages;
+    hip_check(hipGetDevice(&st->device), "hipGetDevice");
     const int max_pages = (max_ctx + page_size - 1) / page_size;
     st->pages = si_kv_pages_create(npages, page_size, max_seqs, max_pages);
     check(si_workspace_create(s, max_seqs, max_ctx, &st->ws), "si_workspace_create");
@@ -387,12 +389,22 @@ const int *si_stack_dev_table(const si_stack_t *st) { return st->dev_table; }
 const int *si_stack_dev_ctx(const si_stack_t *st) { return st->dev_ctx; }
 int si_stack_nseq(const si_stack_t *st) { return st->nseq; }
 
+/* Makes `device` current, if it is not: the one that was. */
+static int switch_device(int device) {
+    int was = device;
+    hip_check(hipGetDevice(&was), "hipGetDevice");
+    if (was != device) hip_check(hipSetDevice(device), "hipSetDevice");
+    return was;
+}
+
 /* The previous step's kernels, which read the pools and the device table. */
 static void wait_decode(si_stack_t *st) {
+    const int was = switch_device(st->device); /* (a null stream is the current device's) */
     if (st->captured || st->streams)
         hip_check(hipDeviceSynchronize(), "si_stack: wait");
     else if (st->pending)
         hip_check(hipStreamSynchronize((hipStream_t)st->stream), "si_stack: wait");
+    switch_device(was);
     st->pending = st->streams = 0;
 }
 
@@ -413,10 +425,12 @@ static void run_copies(si_stack_t *st) {
         pools[2 * l] = st->kpool[l];
         pools[2 * l + 1] = st->vpool[l];
     }
+    const int was = switch_device(st->device);
     check(si_kv_copy_pages(pools, 2 * st->nlayers, st->page_bytes, st->npages, src, dst, n, NULL),
           "si_kv_copy_pages");
     free(pools);
     hip_check(hipStreamSynchronize(NULL), "si_stack: page copies");
+    switch_device(was);
     si_kv_copies_done(st->pages);
 }
 

@@ -29,7 +29,10 @@ hipError_t hipMemcpy(void *d, const void *s, size_t n, hipMemcpyKind k) {
     (void)k; none_running("the tables were written below a running step"); memcpy(d, s, n);
     return hipSuccess;
 }
-hipError_t hipStreamSynchronize(hipStream_t s) { running[ID(s)] = 0; return hipSuccess; }
+hipError_t hipStreamSynchronize(hipStream_t s) {
+    if (s || device == 0) running[ID(s)] = 0;   /* a null stream is the current device's */
+    return hipSuccess;
+}
 hipError_t hipDeviceSynchronize(void) {
     if (device == 0) memset(running, 0, sizeof running);
     ++waits; return hipSuccess;
@@ -124,6 +127,25 @@ BODIES = {
     capturing = 0;
     si_stack_decode(st, x, out, 0, S(1));
     CHECK(last_max == 6);
+""",
+    # the caller's current device is another one
+    "device": """
+    si_stack_decode(st, x, out, 0, S(0));
+    si_stack_prepare(st, seqs, 1);
+    si_stack_decode(st, x, out, 0, S(0));
+    device = 1;
+    seqs[1] = si_stack_fork(st, seqs[0]);
+    CHECK(si_stack_prepare(st, seqs, 2) == 0);
+    CHECK(copies == 1 && copy_device == 0 && device == 1);
+    running[4] = 1;
+    capturing = 3;
+    si_stack_decode(st, x, out, 0, S(3));
+    capturing = 0;
+    CHECK(si_stack_prepare(st, seqs, 2) == 0 && device == 1);
+    si_kv_seq_free(pg, seqs[0]);
+    copy_device = -1;
+    si_stack_compact(st);
+    CHECK((copy_device == 0 || copy_device == -1) && device == 1);
 """,
     "streams": """
     si_stack_decode(st, x, out, 0, S(2));         /* the same step again, on another stream */
