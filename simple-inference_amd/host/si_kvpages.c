@@ -136,11 +136,16 @@ static void drop_page(si_kv_pages_t *p, int pg) {
     release_page(p, pg);
 }
 
+/* pages of len positions (len + page_size may pass an int) */
+static int pages_of(const si_kv_pages_t *p, int len) {
+    return (int)(((long long)len + p->page_size - 1) / p->page_size);
+}
+
 int si_kv_seq_grow(si_kv_pages_t *p, int seq, int len) {
     check_seq(p, seq);
     const int old = p->len[seq];
     if (len < old) die("si_kv_seq_grow: sequences only grow");
-    const long long need = ((long long)len + p->page_size - 1) / p->page_size;
+    const long long need = pages_of(p, len);
     int *row = p->table + (size_t)seq * p->max_pages;
     /* positions are about to be written into the last one's page: where another
      * sequence holds it too, into a copy */
@@ -176,7 +181,7 @@ int si_kv_seq_fork(si_kv_pages_t *p, int seq) {
     p->len[to] = p->len[seq];
     /* the pages with its positions (a sequence may hold more, after a prepare
      * that failed) */
-    p->npg[to] = (p->len[seq] + p->page_size - 1) / p->page_size;
+    p->npg[to] = pages_of(p, p->len[seq]);
     for (int i = 0; i < p->npg[to]; ++i) {
         row[i] = from[i];
         ++p->seqs[row[i]];
@@ -188,7 +193,7 @@ void si_kv_seq_truncate(si_kv_pages_t *p, int seq, int len) {
     check_seq(p, seq);
     if (len < 0 || len > p->len[seq]) die("si_kv_seq_truncate: length outside 0..its own");
     int *row = p->table + (size_t)seq * p->max_pages;
-    const int keep = (len + p->page_size - 1) / p->page_size;
+    const int keep = pages_of(p, len);
     while (p->npg[seq] > keep) {
         const int i = --p->npg[seq];
         drop_page(p, row[i]);
