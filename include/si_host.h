@@ -242,7 +242,8 @@ void si_kv_copies_done(si_kv_pages_t *p);
  * the copies are done.  The page tables change. */
 int si_kv_compact(si_kv_pages_t *p);
 /* The pool now has npages pages: 0, or -1 (unchanged) when a page past them is
- * held.  The tail of a smaller pool is the caller's again. */
+ * held, or a stack's pools end before them (they keep their size: fewer pages
+ * only set the others aside).  The tail of a smaller pool is the caller's again. */
 int si_kv_pages_resize(si_kv_pages_t *p, int npages);
 int si_kv_seq_len(const si_kv_pages_t *p, int seq);
 int si_kv_pages_free(const si_kv_pages_t *p);

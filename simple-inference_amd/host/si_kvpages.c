@@ -41,6 +41,7 @@ static void hip_check(hipError_t e, const char *what) {
 
 struct si_kv_pages {
     int npages, page_size, max_seqs, max_pages;
+    int most;       /* pages that the pools have, 0: the caller's concern */
     int *free_list; /* stack of free page ids */
     int nfree;
     int *seqs;      /* per page: sequences that hold it, */
@@ -265,6 +266,7 @@ int si_kv_compact(si_kv_pages_t *p) {
 
 int si_kv_pages_resize(si_kv_pages_t *p, int npages) {
     if (npages < 1) die("si_kv_pages_resize: npages must be >= 1");
+    if (p->most && npages > p->most) return -1;
     for (int pg = npages; pg < p->npages; ++pg)
         if (p->seqs[pg] || p->reads[pg]) return -1;
     if (npages > p->npages) {
@@ -338,6 +340,7 @@ si_stack_t *si_stack_create_kv(const si_shape_t *s, const si_layer_host_t *layer
     hip_check(hipGetDevice(&st->device), "hipGetDevice");
     const int max_pages = (max_ctx + page_size - 1) / page_size;
     st->pages = si_kv_pages_create(npages, page_size, max_seqs, max_pages);
+    st->pages->most = npages;
     check(si_workspace_create(s, max_seqs, max_ctx, &st->ws), "si_workspace_create");
     st->layers = calloc((size_t)nlayers, sizeof *st->layers);
     st->kpool = calloc((size_t)nlayers, sizeof *st->kpool);

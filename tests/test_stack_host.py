@@ -147,6 +147,15 @@ BODIES = {
     si_stack_compact(st);
     CHECK((copy_device == 0 || copy_device == -1) && device == 1);
 """,
+    # the stack's pools stay as they are: its bookkeeping may set pages aside, no more
+    "resize": """
+    CHECK(si_kv_pages_resize(pg, 13) == -1 && si_kv_pages_free(pg) == 11);
+    CHECK(si_kv_pages_resize(pg, 2) == 0 && si_kv_pages_free(pg) == 1);
+    CHECK(si_kv_pages_resize(pg, 1 << 20) == -1 && si_kv_pages_free(pg) == 1);
+    CHECK(si_kv_pages_resize(pg, 12) == 0 && si_kv_pages_free(pg) == 11);
+    CHECK(si_kv_seq_grow(pg, seqs[0], 96) == 0 && si_kv_pages_free(pg) == 6);
+    for (int i = 0; i < 6; ++i) CHECK(si_kv_page_table(pg)[i] < 12);
+""",
     "streams": """
     si_stack_decode(st, x, out, 0, S(2));         /* the same step again, on another stream */
     seqs[1] = si_stack_fork(st, seqs[0]);
