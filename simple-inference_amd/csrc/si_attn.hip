@@ -528,7 +528,7 @@ __device__ __forceinline__ void pf_barrier() {
 // bytes).  Otherwise the tiles come through registers, by loads that take any
 // address, and are in LDS when copy() returns.
 //
-// FAR (prompts over a cache held in 4 bits): positions far below a row's largest
+// FAR (k_attn_prefill_far, prompts over a cache held in 4 bits): positions far below a row's largest
 // score keep their bits, where that one's V row is zero or small (an attention
 // sink).  Weights are against a maximum that follows the running one within 2^4, in
 // units of 2^-11, their lo halves 2^11 higher and in sums of their own: 22 bits down
@@ -538,12 +538,12 @@ __device__ __forceinline__ void pf_barrier() {
 // And each row of q is scaled by a power of two, which its scores' unit gives back:
 // fp16 halves of q as it comes are infinite from 65520 and lose bits below 2^-14.
 constexpr float PF_SLACK = 4.0f, PF_UP = 11.0f, PF_LO = 2048.0f;
-template <int D, int RT, int KW, bool ASYNC, bool FAR = false>
-__global__ void __launch_bounds__(RT * KW * 64) __attribute__((amdgpu_waves_per_eu(2)))
-k_attn_prefill(const float *__restrict__ q, int ntok, int qheads, int kvheads, int pos0,
-               const uint16_t *__restrict__ kc, const uint16_t *__restrict__ vc, float scale2,
-               float *__restrict__ attn, int8_t *__restrict__ qs, uint16_t *__restrict__ qd,
-               int16_t *__restrict__ bsum) {
+template <int D, int RT, int KW, bool ASYNC, bool FAR>
+__device__ __forceinline__ void
+attn_prefill(const float *__restrict__ q, int ntok, int qheads, int kvheads, int pos0,
+             const uint16_t *__restrict__ kc, const uint16_t *__restrict__ vc, float scale2,
+             float *__restrict__ attn, int8_t *__restrict__ qs, uint16_t *__restrict__ qd,
+             int16_t *__restrict__ bsum) {
     constexpr int NWV = RT * KW, NT = NWV * 64, KS = D / 16, DT = D / 32, CH = D / 8;
     constexpr int TB = PF_T * D * 2;            // bytes of a K (or V) tile
     constexpr int TI = TB / 1024;               // copy instructions per tile
@@ -907,6 +907,25 @@ k_attn_prefill(const float *__restrict__ q, int ntok, int qheads, int kvheads, i
     }
 }
 
+template <int D, int RT, int KW, bool ASYNC>
+__global__ void __launch_bounds__(RT * KW * 64) __attribute__((amdgpu_waves_per_eu(2)))
+k_attn_prefill(const float *__restrict__ q, int ntok, int qheads, int kvheads, int pos0,
+               const uint16_t *__restrict__ kc, const uint16_t *__restrict__ vc, float scale2,
+               float *__restrict__ attn, int8_t *__restrict__ qs, uint16_t *__restrict__ qd,
+               int16_t *__restrict__ bsum) {
+    attn_prefill<D, RT, KW, ASYNC, false>(q, ntok, qheads, kvheads, pos0, kc, vc, scale2, attn, qs,
+                                          qd, bsum);
+}
+template <int D, int RT, int KW>
+__global__ void __launch_bounds__(RT * KW * 64) __attribute__((amdgpu_waves_per_eu(2)))
+k_attn_prefill_far(const float *__restrict__ q, int ntok, int qheads, int kvheads, int pos0,
+                   const uint16_t *__restrict__ kc, const uint16_t *__restrict__ vc, float scale2,
+                   float *__restrict__ attn, int8_t *__restrict__ qs, uint16_t *__restrict__ qd,
+                   int16_t *__restrict__ bsum) {
+    attn_prefill<D, RT, KW, true, true>(q, ntok, qheads, kvheads, pos0, kc, vc, scale2, attn, qs,
+                                        qd, bsum);
+}
+
 // Causal prefill of ntok tokens at positions pos0.. of one sequence whose
 // cache rows 0..pos0+ntok-1 are in place (RoPE'd K, V).
 bool attn_prefill_supported(int qheads, int kvheads, int hdim) {
@@ -954,8 +973,8 @@ void launch_attn_prefill(const float *q, int ntok, int qheads, int kvheads, int 
                                                        : 4;
     const dim3 grid((unsigned)((rows + 32 * rt - 1) / (32 * rt) * kvheads));
 #define PF_FAR(DIM, RT, KW)                                                                      \
-    SI_LAUNCH((k_attn_prefill<DIM, RT, KW, true, true>), far_grid(RT), dim3(RT * KW * 64), 0, st, q, \
-              ntok, qheads, kvheads, pos0, kc, vc, scale2, attn, qs, qd, bsum)
+    SI_LAUNCH((k_attn_prefill_far<DIM, RT, KW>), far_grid(RT), dim3(RT * KW * 64), 0, st, q, ntok, \
+              qheads, kvheads, pos0, kc, vc, scale2, attn, qs, qd, bsum)
     if (far) {
         const auto far_grid = [&](int rt) {
             return dim3((unsigned)((rows + 32 * rt - 1) / (32 * rt) * kvheads));
