@@ -542,7 +542,7 @@ __device__ __forceinline__ A4Item a4_item(int w, const int *ctx_dev, int nq, int
 enum A4Mode { A4_NARROW, A4_WIDE, A4_ROWS };
 
 template <int D, int MODE, bool PAGE16, int NW>
-__global__ void __launch_bounds__(64 * NW, NW > 4 || MODE ? 2 : 3) k_attn_kv4(
+__global__ void __launch_bounds__(64 * NW, 3) k_attn_kv4(
     const float *__restrict__ q, int qheads, Kv4Cache c, const int *__restrict__ ctx_dev, int ctx0,
     int ctx_step, int nq, int max_ctx, int ns, int chunk, int slots, float scale2,
     int *__restrict__ parts, float *__restrict__ ws_u, float *__restrict__ ws_m,
@@ -713,7 +713,6 @@ __global__ void __launch_bounds__(64 * NW, NW > 4 || MODE ? 2 : 3) k_attn_kv4(
 
     auto step = [&](Group &t, int s) {
         float p[2][4];
-        f4 d[2][KS];
         // lane (col, g)'s dword to [g][col]; a wavefront's LDS operations keep their
         // order, the compiler is to keep it too (and to read q here, not before the
         // loop)
@@ -730,31 +729,31 @@ __global__ void __launch_bounds__(64 * NW, NW > 4 || MODE ? 2 : 3) k_attn_kv4(
         sl[1][lane] = t.vh;
         sl[2][lane] = as_u(as_h2(t.vh) * (h2){(_Float16)-72.0f, (_Float16)-72.0f});
         asm volatile("" ::: "memory");
+        f4 acc[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
 #pragma unroll
         for (int b = 0; b < KS; ++b) {
+            // (q read as it is needed, or the registers are not three wavefronts' a SIMD)
+            if constexpr (WIDE && D == 128) asm volatile("" ::: "memory");
             const h8 qa = __builtin_bit_cast(h8, qop[b * 64 + lane]);
             const f4 c8 = qc[b * 64 + lane];
+            f4 d[2];
 #pragma unroll
             for (int tl = 0; tl < 2; ++tl) {
                 const uint32_t w = t.k[tl][b], w8 = w >> 8;
                 const u4 a = {w & 0x000f000fu, w & 0x00f000f0u, w8 & 0x000f000fu, w8 & 0x00f000f0u};
                 const h8 ka = __builtin_bit_cast(h8, a);
-                d[tl][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, qa, c8, 0, 0, 0);
+                d[tl] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, qa, c8, 0, 0, 0);
                 if constexpr (WIDE)
-                    d[tl][b] += __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                    d[tl] += __builtin_amdgcn_mfma_f32_16x16x32_f16(
                         ka, __builtin_bit_cast(h8, qop[(KS + b) * 64 + lane]),
                         qc[(KS + b) * 64 + lane], 0, 0, 0);
             }
-        }
-        f4 acc[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
-#pragma unroll
-        for (int b = 0; b < KS; ++b) {
             const u4 hk = *(const u4 *)&sl[0][16 * g + 4 * b];
 #pragma unroll
             for (int tl = 0; tl < 2; ++tl)
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    acc[tl][i] = fmaf((float)as_h2(hk[i])[tl], d[tl][b][i], acc[tl][i]);
+                    acc[tl][i] = fmaf((float)as_h2(hk[i])[tl], d[tl][i], acc[tl][i]);
         }
 #pragma unroll
         for (int tl = 0; tl < 2; ++tl)
@@ -825,10 +824,11 @@ __global__ void __launch_bounds__(64 * NW, NW > 4 || MODE ? 2 : 3) k_attn_kv4(
             }
         }
     };
-    while (s0 < p1) {
+    // (two whole steps a turn: with an exit between them the sums moved to other
+    // registers and back each turn, which were then a third more)
+    while (s0 + STEP < p1) {
         step(ta, s0);
         s0 += STEP;
-        if (s0 >= p1) break;
         if (s0 + STEP < p1) load(ta, s0 + STEP, id);
         id = ids_of(s0 + 2 * STEP);
         step(tb, s0);
@@ -836,6 +836,7 @@ __global__ void __launch_bounds__(64 * NW, NW > 4 || MODE ? 2 : 3) k_attn_kv4(
         if (s0 + STEP < p1) load(tb, s0 + STEP, id);
         id = ids_of(s0 + 2 * STEP);
     }
+    if (s0 < p1) step(ta, s0);
     // The wavefronts' states meet in LDS: maxima and sums, then the outputs, four
     // wavefronts at a time, added by a thread per four dims in wavefront order.
     const float lo_unit = lo_half ? 1.0f / A4_LO : 1.0f;
