@@ -412,7 +412,9 @@ int si_kv4_read(const si_shape_t *s, const uint8_t *k_pool, const uint8_t *v_poo
  * cache.  ctx_step 0: query i over sequence i, its context ctx_dev[i] (clamped
  * to max_ctx; <= 0 gives zeros) or ctx0.  ctx_step 1: nq queries of the first
  * sequence with contexts ctx0, ctx0 + 1, ... (a causal prompt whose rows are in
- * place).  At most 65535 queries.  Outputs as si_attention's; workspace:
+ * place).  At most 65535 queries, of any size up to fp32's largest: a head's q is
+ * held to 2^-24 of its largest value, a weight to 2^-22 of itself down to 2^-25 of
+ * its row's largest and to 2^-47 of that one below.  Outputs as si_attention's; workspace:
  * si_attention_kv4_workspace bytes, 256-byte aligned (calls that overlap need one
  * each; a prompt of more than 9000 (query, head) rows takes fp16 rows of max_ctx
  * positions there, so max_ctx is best the last query's context). */

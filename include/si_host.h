@@ -285,7 +285,9 @@ int si_stack_prepare(si_stack_t *st, const int *seqs, int nseq);
  * them copies the page they would both append to, in every pool.  That copy and
  * si_stack_compact's run in order with the stack's decodes; a caller that reads
  * or writes the pools on a stream of its own (si_kv4_write, si_kv4_read) has
- * finished that work before either call, and starts more after it returns. */
+ * finished that work before either call, and starts more after it returns.  A
+ * fork between a prepare and its decode has the position that the decode writes;
+ * the decode comes before the next prepare. */
 int si_stack_fork(si_stack_t *st, int seq);
 /* si_kv_compact with its copies in every pool (waits for them, and before for
  * the decodes as si_stack_prepare does); a si_stack_prepare has to follow. */

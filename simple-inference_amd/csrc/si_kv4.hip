@@ -138,10 +138,10 @@ static int kv4_units(int ntok, int pos0, int pos_step) {
 // reductions over 32 lanes one after another: 5000 fp16 rows of 2 heads of 128
 // 7.0 us, 5.0 so.)
 // HALF_IN: the rows are fp16 cache rows (kin, vin), copied in without RoPE.
-// Many rows are bound by memory: 1999 rows of 28/4 heads of 128, 69 MB with q in
-// and out, 14.1 us (4.9 TB/s; a large copy reaches 4.8).  Few by their launch and one
-// chain of loads, reduction and store: 64 rows 4.1 us, 1 row 3.3, 5000 fp16 rows
-// of 2 heads of 128 (6.6 MB) 5.0.
+// Many rows are bound by memory: 1999 rows of 28/4 heads of 128, 68 MB with q in
+// and out, 13.8 us; 77 MB move, as each XCD reads the tables for itself, at 5.6 TB/s
+// (k_kv_copy reaches 5.9).  Few by their launch and one chain of loads, reduction and
+// store: 64 rows 4.3 us, 1 row 3.4, 5000 fp16 rows of 2 heads of 128 (6.6 MB) 5.0.
 // ---------------------------------------------------------------------------
 // 8 floats, 16 bytes a load where the call's buffers allow it
 __device__ __forceinline__ void load8(const float *p, bool wide, float (&v)[8]) {
@@ -254,8 +254,8 @@ __global__ void __launch_bounds__(2 * D) k_kv4_append(
 
 // ---------------------------------------------------------------------------
 // rows back as fp16, exactly: the same units and threads.  A launch and one chain
-// of loads (page id, nibbles and scale): 1 row 2.2 us, 1999 rows of 4 heads of 128
-// (5.2 MB) 4.4, 5000 of 2 (6.6 MB) 4.1.
+// of loads (page id, nibbles and scale): 1 row 2.3 us, 1999 rows of 4 heads of 128
+// (5.2 MB) 4.2, 5000 of 2 (6.6 MB) 4.2.
 // ---------------------------------------------------------------------------
 template <int D>
 __global__ void __launch_bounds__(2 * D) k_kv4_read(Kv4Cache c, int ntok, int pos0, int pos_step,
@@ -331,13 +331,14 @@ __global__ void __launch_bounds__(2 * D) k_kv4_read(Kv4Cache c, int ntok, int po
 // was an fp16 subnormal from w = 2^-3 down and weights below 2^-25 were 0: 1.6e-5 of
 // the result 10 nats under such a position, all of a wavefront's at 18.)
 //
-// What bounds it: a step of 32 positions is about 230 vector operations and 17 matrix
-// instructions (two products: 260 and 34), which hardly overlap, 0.7 us of a SIMD at
+// What bounds it: a step of 32 positions is about 240 vector operations and 17 matrix
+// instructions (two products: 270 and 34), which hardly overlap, 0.7 us of a SIMD at
 // 128 dims, about as long as its 4.6 KB take to arrive.  64 queries x 4096 of 28/4 heads
-// of 128, 153 MB: 32 us (4.8 TB/s, a large copy's rate).  Fewer bytes leave 5 us of
-// launch, page id, first group, last step and the wavefronts' meeting, and the merge of
-// chunks: 48 x 200-4096 (62 MB) 21 + 4 us, 2 queries of 12/2 heads over 60000-131072 (65
-// MB) 19 + 4, one query of 14/2 heads of 64 over 1024 (no merge) 7.8.
+// of 128, 153 MB: 32.6 us (4.7 TB/s; a plain read takes 28), vector issue busy half of it
+// and the matrix cores an eighth.  Fewer bytes leave 5 us of launch, page id, first
+// group, last step and the wavefronts' meeting, and the merge of chunks: 48 x 200-4096
+// (62 MB) 21 + 4 us, 2 queries of 12/2 heads over 60000-131072 (65 MB) 19 + 4, one query
+// of 14/2 heads of 64 over 1024 (no merge) 7.9.
 // ---------------------------------------------------------------------------
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
@@ -357,11 +358,11 @@ __device__ __forceinline__ float ror8_add(float v) { return v + dpp_f<DPP_ROR8>(
 // addresses in vector registers, and nothing past the page is touched), or, for
 // pages of half a group, the lane's own address.
 // ONCE: no other workgroup reads the bytes soon (every query but a prompt's), so they
-// are loaded past the caches: 64 queries x 4096 of 28/4 heads of 128 from memory 35.6 ->
-// 32.6 us, 200 x 2000 61.0 -> 53.7, 8 x 4096 15.3 -> 14.3, 128 x 4000 of 14/2 of 64 23.7 ->
-// 22.9 (as a model's layers come, other pages between; the same pages again and again from
-// the 256 MB cache 33.5 -> 34.5, 15.2 -> 15.5).  A prompt, whose blocks of rows share them,
-// 83.9 -> 89.1.
+// are loaded past the caches, which the next layers' pages then find as they were: 64
+// queries x 4096 of 28/4 heads of 128 from memory 37.8 -> 37.5 us, 200 x 2000 59.3 -> 56.2,
+// 8 x 4096 14.3 -> 14.5, 128 x 4000 of 14/2 of 64 24.7 -> 23.2 (2.5 GB of other pages
+// between; the same pages again and again from the 256 MB cache 31.3 -> 34.0, 50.2 -> 55.0,
+// 12.7 -> 13.1, 21.4 -> 22.4).  A prompt, whose blocks of rows share them, 85.5 -> 88.7.
 struct Kv4InPage {
     __amdgpu_buffer_rsrc_t r;
     int at;
@@ -1095,24 +1096,26 @@ void launch_kv4_read(const Kv4Cache &c, int ntok, int hdim, int pos0, int pos_st
 // us a call in a graph, split | whole in four | in eight, contexts equal (1/16 to all of
 // the longest):
 //   - whole in four wavefronts up to 4 steps: the merge and its launch cost about 4 us.
-//     28/4 heads of 128, 1 query of 512 9.1 | 8.1 | 8.2, 48 of 384 13.8 | 8.2 | 8.5.
+//     28/4 heads of 128, 1 query of 512 8.7 | 7.7 | 8.0, 48 of 384 13.0 | 7.4 | 7.7.
 //   - with at most one workgroup a CU, whole in eight up to the steps below: they share
 //     a context's steps, and step faster than three wavefronts a SIMD.  28/4 heads of
-//     128: 1 query of 768 8.9 | 9.7 | 9.4, of 1024 9.1 | 11.5 | 10.7; 16 of 1536 14.3 | 16.9 |
-//     14.3; 48 of 2048 21.7 | 21.5 | 18.4; 64 of 4096 40.5 | 45.2 | 35.9 (28.8 | 38.6 | 29.8), of
-//     8192 70.1 | 81.9 | 63.6 (49.0 | 74.9 | 54.6).  14/2 of 64: 1 of 1024 8.3 | 9.4 | 8.7, but
-//     10.6 | 8.8 | 8.1 from Python, whose two launches take longer; 64 of 3000 16.6 | 21.6 |
-//     16.9 (14.8 | 21.2 | 16.4); 128 of 4096 26.1 | 27.2 | 21.4 (20.6 | 27.0 | 20.7).  8/8 of 32: 6
-//     of 1536 8.8 | 10 | 8.5; 32 of 4096 19.6 | 23.1 | 17.2 (15.9 | 22.7 | 16.7).  (Workgroups of
-//     12 or 16: 64 of 4096 38.4; no better below 4096 positions and 5 % so past them.)
+//     128: 16 of 1536 13.1 | 16.6 | 14.2; 48 of 2048 21.8 | 22.1 | 18.4; 64 of 4096 36.0 | 39.0 |
+//     31.1 (25.5 | 37.2 | 28.3), of 8192 64.1 | 72.7 | 57.9 (39.5 | 69.7 | 50.2).  14/2 of 64: 64 of
+//     3000 15.7 | 22.5 | 16.9 (13.7 | 21.4 | 16.2); 128 of 4096 26.3 | 29.5 | 21.5 (19.4 | 28.4 |
+//     20.7).  8/8 of 32: 6 of 1536 8.9 | 10.1 | 8.5; 32 of 4096 19.5 | 24.4 | 17.0 (16.2 | 23.5 |
+//     16.4).  One query's border is set by calls one by one, whose second launch the host
+//     is late with: 14/2 of 64, 1 of 1024 9.6 | 8.9 | 8.3 from Python, 7.9 | 8.9 | 8.3 in a graph;
+//     28/4 of 128, 1 of 768 8.5 | 9.6 | 9.2 there, of 1024 8.8 | 10.9 | 10.4.
 //   - with more, whole in four up to 5 + base / 32 steps: 28/4 heads of 128, 80 queries of 1024
-//     23.6 | 17.8 | 22.4, of 2048 33.2 | 30.2 | 34.9 (25.8 | 23.7 | 25.9), of 3000 43.2 | 42.9 |
-//     48.0 (30.2 | 33.8 | 31.6); 128 of 2048 41 | 36, of 4096 70 | 69.
+//     26.3 | 17.0 | 21.3, of 2048 34.0 | 28.0 | 33.0 (28.3 | 25.2 | 22.8), of 3000 41.6 | 38.7 |
+//     43.8 (32.0 | 35.0 | 29.7); 128 of 2048 46.2 | 30.5 | 36.0, of 4096 68.9 | 58.6 | 63.5.
+//   - from `slots` pairs on (and not by their lengths) whole in four: contexts of about one
+//     length; one far longer than the others is walked by its one workgroup.
 //   - else split into chunks: as many as fill the GPU (three, four or five workgroups a
 //     CU by their registers), or fill it twice where they would be two or fewer a pair,
 //     too coarse to end together: once | twice, 93 to 6000 positions (6000), 24/8 heads
-//     of 96: 40 queries 36.4 | 34.2 (54.2 | 53.0), 48 42.9 | 38.7 (58.8 | 60.7), 75 76.2 |
-//     64.6 (91.6 | 91.5); 26 22.6 | 25.9 (38.9 | 40.3).  A context on the device may get
+//     of 96: 40 queries 34.9 | 34.2 (49.1 | 46.5), 48 36.6 | 34.7 (51.5 | 52.0), 75 63.2 |
+//     50.2 (84.7 | 81.5); 26 26.9 | 26.0 (35.3 | 34.1).  A context on the device may get
 //     twice its share, which the kernel uses as they are ragged.
 struct A4Plan {
     int nw, ns, slots;
@@ -1130,11 +1133,13 @@ static A4Plan a4_plan(int hdim, long long base, int max_ctx, bool ragged) {
 
 // Whether a prompt's pages are read into fp16 rows for the prefill kernel, which
 // unpacks nothing and takes 32 rows a tile, but walks a tile's context in one
-// workgroup: it pays once its tiles fill the GPU.  Both ways (us a call, over the
-// pages | by rows, after 300 and after 6000 positions): 28/4 heads of 128, 16 queries
-// 8 | 13, 18 | 81; 256 14 | 17, 89 | 87; 333 18 | 19, 106 | 97; 512 25 | 23, 144 | 118.
-// 14/2 of 64, 512 queries 11 | 14, 56 | 58; 768 16 | 16, 77 | 64.  24/8 of 96, 333 12 | 16,
-// 72 | 80; 512 18 | 20, 93 | 93.  8/8 of 32, 1024 12 | 15, 44 | 56; 2000 22 | 23, 79 | 66.
+// workgroup: it pays once its tiles fill the GPU, whatever the context.  Both ways (us a
+// call in a graph, over the pages | by rows, after 300, 1500 and 6000 positions): 28/4
+// heads of 128, 16 queries 9 | 15, 12 | 31, 19 | 91; 256 15 | 19, 29 | 34, 86 | 93; 333 17 |
+// 21, 37 | 41, 108 | 107; 512 26 | 25, 53 | 46, 156 | 130; 2048 130 | 101, 220 | 171, 559 | 428.
+// 14/2 of 64, 512 11 | 14, 21 | 22, 54 | 52; 768 16 | 16, 28 | 26, 77 | 68.  16/1 of 128, 600 21 |
+// 23, 40 | 38, 117 | 100.  24/8 of 96, 512 18 | 21, 34 | 37, 95 | 101; 1000 37 | 36, 67 | 62, 184
+// | 167.  8/8 of 32, 1024 12 | 14, 19 | 21, 42 | 46; 2000 22 | 20, 32 | 29, 81 | 65.
 // (Past 2^26 positions the rows would be a launch of 2^31 threads and more.)
 static bool kv4_by_rows(int qheads, int nq, int ctx_step, int max_ctx) {
     return ctx_step == 1 && (long long)nq * qheads > 9000 && max_ctx <= 1 << 26;
