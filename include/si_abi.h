@@ -435,6 +435,74 @@ int si_kv_copy_pages(void *const *pools, int npools, size_t page_bytes, int npag
                      const int *src, const int *dst, int n, void *stream);
 
 /* ------------------------------------------------------------------ */
+/* A step whose sequences bring any number of rows each                */
+/* ------------------------------------------------------------------ */
+
+/* No counterpart in the reference, which runs one sequence (qwen_one_layer.c:
+ * 237-281).  A step's rows (a token, drafted tokens or a prompt's piece of each of
+ * nseq sequences, in sequence order) run over a paged fp16 cache, with the lengths,
+ * the page lists and the free pages in device memory, so that a captured step needs
+ * no host.  Per sequence start[i] .. start[i+1] - 1 are its rows and ctx[i] its
+ * positions with them; per row seq, pos and slot (pool row, page * page_size +
+ * offset) say where it belongs, -1 each behind the last row.  Rows there, up to
+ * max_rows (fewer than 2^24), are left as they are by every call.
+ *
+ * si_kv_step makes them from have[i] (positions in place, -1: the sequence has
+ * ended) and add[i] (its rows of the step; below 0 is 0):
+ *   pages      [nseq][max_pages], the sequences' page lists (at most 2^30
+ *              positions each): pages for have + add positions are taken into them;
+ *   held       [nseq][2], per sequence the pages its list has taken and how many of
+ *              them have been given back (0, 0: none yet).  The list's first
+ *              ceil(sinks / page_size) pages stay; those behind them of which no row
+ *              from position have on sees anything (all positions <= have - window)
+ *              are given back: their entries are stale from then on.  A later have
+ *              may be lower (drafts that were not accepted), down to this one.  An
+ *              ended sequence gives all of its pages back, and has (0, 0) again;
+ *   free_ring  [npages], the free ids: free[1] of them from entry free[0] on, round
+ *              the end.  Pages are taken from its front, sequence by sequence, and
+ *              given back to its end in the same order (in use from the next step on);
+ *   taken      [nseq + 1], pages taken before sequence i;
+ *   status     [4]: {code, rows, pages taken, pages given back}.
+ * Code 0 is success; otherwise the sum of 1 (more rows than max_rows), 2 (too few free
+ * pages) and 4 (positions past max_pages pages, or have past the taken ones: that
+ * sequence counts as one without rows); the step then has no rows and pages, held and
+ * free stay as they are.  held_out may be held_in, free_out free_in; nothing else
+ * may overlap.  window >= 1 (INT_MAX: none is given back).  page_size: a power of two in 1..2^20. */
+int si_kv_step(int nseq, const int *have, const int *add, int max_rows, int window, int sinks,
+               int page_size, int npages, int max_pages, int *pages, int *free_ring,
+               const int *free_in, int *free_out, const int *held_in, int *held_out, int *start,
+               int *ctx, int *seq, int *pos, int64_t *slot, int *taken, int *status,
+               void *stream);
+
+/* si_rope_kv_append of a step's rows: row r of qkv at position pos[r] to row slot[r]
+ * of the pools ([pool_rows][kvheads*hdim]), the rotated q to q_out; the same bits.  A
+ * row whose position is outside 0..max_pos-1 or slot outside the pools is left out.
+ * rope tables, q_out and pools 16-byte aligned; two rows of one slot are an error
+ * that is not detected. */
+int si_rope_kv_append_rows(const si_shape_t *s, const float *qkv, int ldqkv, int max_rows,
+                           int max_pos, const int *pos, const int64_t *slot,
+                           const float *rope_cos, const float *rope_sin, float *q_out,
+                           uint16_t *k_pool, uint16_t *v_pool, size_t pool_rows, void *stream);
+
+/* Attention (attention_flash, attention_kernels.h:80-164) of a step's rows: the row
+ * of sequence i at position p, ctx[i] - 1 for its last one, sees position t <= p of
+ * the sequence where t > p - window or t < sinks (a sliding window, and a few first
+ * positions that stay visible); what it does not see has no influence, infinities and
+ * NaN included.  window >= 1 (INT_MAX: all of them), sinks >= 0.  Contexts above
+ * max_ctx are max_ctx; rows before position 0 are zeros; a sequence's rows past the
+ * first max_new are left as they are.  q, pools, attn 16-byte aligned, qs 4-byte.
+ * Of the shape qheads, kvheads and hdim are read; outputs as si_attention's.
+ * workspace: si_attention_rows_workspace bytes, 256-byte aligned (calls that
+ * overlap need one each). */
+int si_attention_rows(const si_shape_t *s, const float *q, int nseq, int max_rows, int max_new,
+                      int max_ctx, int window, int sinks, const int *start, const int *ctx,
+                      const uint16_t *k_pool, const uint16_t *v_pool, int npages, int page_size,
+                      const int *pages, int max_pages, float *attn, int8_t *qs, uint16_t *d,
+                      int16_t *bsum, void *workspace, size_t workspace_bytes, void *stream);
+size_t si_attention_rows_workspace(const si_shape_t *s, int nseq, int max_rows, int max_new,
+                                   int max_ctx, int window, int sinks);
+
+/* ------------------------------------------------------------------ */
 /* Layer level (run_layer / run_layer_fused / pf_run_batch)            */
 /* ------------------------------------------------------------------ */
 

@@ -1862,3 +1862,168 @@ int si_kv_copy_pages(void *const *pools, int npools, size_t page_bytes, int npag
 }
 
 }  // extern "C"
+
+// ---------------------------------------------------------------------------
+// A step whose sequences bring any number of rows each (si_step.hip, si_rows.hip)
+// ---------------------------------------------------------------------------
+constexpr int kMaxRows = (1 << 24) - 1, kMaxSeqs = (1 << 20);
+
+static int step_sizes(const char *what, int nseq, int max_rows, int window, int sinks) {
+    SI_REQUIRE(nseq >= 0 && nseq <= kMaxSeqs, "%s: nseq %d outside 0..2^20", what, nseq);
+    SI_REQUIRE(max_rows >= 0 && max_rows <= kMaxRows, "%s: max_rows %d outside 0..2^24 - 1", what,
+               max_rows);
+    SI_REQUIRE(window >= 1 && sinks >= 0, "%s: bad window %d / sinks %d", what, window, sinks);
+    return SI_OK;
+}
+
+// page sizes of fp16 pools: their shift, or -1
+static int page_shift(int page_size) {
+    if (page_size < 1 || page_size > (1 << 20) || (page_size & (page_size - 1))) return -1;
+    return __builtin_ctz((unsigned)page_size);
+}
+
+static int step_pages(const char *what, int npages, int page_size, int max_pages, int *shift) {
+    *shift = page_shift(page_size);
+    SI_REQUIRE(*shift >= 0, "%s: page_size %d must be a power of two in 1..2^20", what, page_size);
+    SI_REQUIRE(npages >= 1 && max_pages >= 1, "%s: npages and max_pages must be >= 1", what);
+    SI_REQUIRE((long long)max_pages << *shift <= (1 << 30),
+               "%s: %d pages of %d a sequence exceed 2^30 positions", what, max_pages, page_size);
+    return SI_OK;
+}
+
+static bool aligned(const void *p, unsigned to) { return ((uintptr_t)p & (to - 1)) == 0; }
+
+// The sizes of an attention over a step's rows, as the kernels take them.
+static RowsArgs rows_sizes(const si_shape_t *s, int nseq, int max_rows, int max_new, int max_ctx,
+                           int window, int sinks) {
+    RowsArgs a = {};
+    a.qheads = s->qheads;
+    a.kvheads = s->kvheads;
+    a.hdim = s->hdim;
+    a.nseq = nseq;
+    a.max_rows = max_rows;
+    a.max_new = std::min(max_new, max_rows);
+    a.max_ctx = max_ctx;
+    a.window = std::min(window, max_ctx);
+    a.sinks = std::min(sinks, max_ctx);
+    a.scale2 = softmax_scale2(s->hdim);
+    return a;
+}
+
+extern "C" {
+
+int si_kv_step(int nseq, const int *have, const int *add, int max_rows, int window, int sinks,
+               int page_size, int npages, int max_pages, int *pages, int *free_ring,
+               const int *free_in, int *free_out, const int *held_in, int *held_out, int *start,
+               int *ctx, int *seq, int *pos, int64_t *slot, int *taken, int *status,
+               void *stream) {
+    const char *what = "si_kv_step";
+    KvStep a = {};
+    int r = step_sizes(what, nseq, max_rows, window, sinks);
+    if (!r) r = step_pages(what, npages, page_size, max_pages, &a.shift);
+    if (r) return r;
+    SI_REQUIRE(free_ring && free_in && free_out && start && taken && status &&
+                   (nseq == 0 || (have && add && pages && held_in && held_out && ctx)) &&
+                   (max_rows == 0 || (seq && pos && slot)),
+               "%s: NULL pointer", what);
+    a.nseq = nseq;
+    a.max_rows = max_rows;
+    a.window = window;
+    a.kept = (int)(((long long)sinks + page_size - 1) >> a.shift);
+    a.npages = npages;
+    a.max_pages = max_pages;
+    a.have = have;
+    a.add = add;
+    a.pages = pages;
+    a.ring = free_ring;
+    a.free_in = free_in;
+    a.held_in = held_in;
+    a.free_out = free_out;
+    a.held_out = held_out;
+    a.start = start;
+    a.ctx = ctx;
+    a.seq = seq;
+    a.pos = pos;
+    a.slot = (long long *)slot;
+    a.taken = taken;
+    a.status = status;
+    launch_kv_step(a, S(stream));
+    return check_launch(what);
+}
+
+int si_rope_kv_append_rows(const si_shape_t *s, const float *qkv, int ldqkv, int max_rows,
+                           int max_pos, const int *pos, const int64_t *slot, const float *rc,
+                           const float *rs, float *q_out, uint16_t *k_pool, uint16_t *v_pool,
+                           size_t pool_rows, void *stream) {
+    const char *what = "si_rope_kv_append_rows";
+    int r = check_heads(what, s);
+    if (!r) r = step_sizes(what, 0, max_rows, 1, 0);
+    if (r) return r;
+    SI_REQUIRE(max_pos >= 1, "%s: max_pos must be >= 1", what);
+    SI_REQUIRE(ldqkv >= (s->qheads + 2 * s->kvheads) * s->hdim, "%s: ldqkv too small", what);
+    SI_REQUIRE(pool_rows >= 1 && pool_rows < (1ull << 51), "%s: %zu pool rows", what, pool_rows);
+    if (max_rows == 0) return SI_OK;
+    SI_REQUIRE(qkv && pos && slot && rc && rs && q_out && k_pool && v_pool, "%s: NULL pointer",
+               what);
+    SI_REQUIRE(aligned(rc, 16) && aligned(rs, 16) && aligned(q_out, 16) && aligned(k_pool, 16) &&
+                   aligned(v_pool, 16),
+               "%s: the RoPE tables, q_out and the pools must be 16-byte aligned", what);
+    launch_rope_kv_rows(qkv, ldqkv, max_rows, s->qheads, s->kvheads, s->hdim, max_pos, pos,
+                        (const long long *)slot, rc, rs, q_out, k_pool, v_pool,
+                        (long long)pool_rows, S(stream));
+    return check_launch(what);
+}
+
+size_t si_attention_rows_workspace(const si_shape_t *s, int nseq, int max_rows, int max_new,
+                                   int max_ctx, int window, int sinks) {
+    if (check_heads("si_attention_rows_workspace", s) ||
+        step_sizes("si_attention_rows_workspace", nseq, max_rows, window, sinks) || max_new < 1 ||
+        max_ctx < 1 || max_ctx > (1 << 30))
+        return 0;
+    return attn_rows_workspace(rows_sizes(s, nseq, max_rows, max_new, max_ctx, window, sinks));
+}
+
+int si_attention_rows(const si_shape_t *s, const float *q, int nseq, int max_rows, int max_new,
+                      int max_ctx, int window, int sinks, const int *start, const int *ctx,
+                      const uint16_t *k_pool, const uint16_t *v_pool, int npages, int page_size,
+                      const int *pages, int max_pages, float *attn, int8_t *qs, uint16_t *d,
+                      int16_t *bsum, void *ws, size_t ws_bytes, void *stream) {
+    const char *what = "si_attention_rows";
+    KvPages pg;
+    int r = check_heads(what, s);
+    if (!r) r = step_sizes(what, nseq, max_rows, window, sinks);
+    if (!r) r = step_pages(what, npages, page_size, max_pages, &pg.shift);
+    if (r) return r;
+    SI_REQUIRE(max_new >= 1, "%s: max_new must be >= 1", what);
+    SI_REQUIRE(max_ctx >= 1 && (long long)max_pages << pg.shift >= max_ctx,
+               "%s: max_ctx %d outside 1..max_pages * page_size", what, max_ctx);
+    SI_REQUIRE(((long long)npages << pg.shift) * s->kvheads * s->hdim < (1LL << 40),
+               "%s: KV pool too large", what);
+    if (nseq == 0 || max_rows == 0) return SI_OK;
+    SI_REQUIRE(q && start && ctx && k_pool && v_pool && pages && attn, "%s: NULL pointer", what);
+    SI_REQUIRE(aligned(q, 16) && aligned(attn, 16) && aligned(k_pool, 16) && aligned(v_pool, 16),
+               "%s: q, attn and the pools must be 16-byte aligned", what);
+    SI_REQUIRE(!qs || d, "%s: qs without d", what);
+    SI_REQUIRE(aligned(qs, 4), "%s: qs must be 4-byte aligned", what);
+    RowsArgs a = rows_sizes(s, nseq, max_rows, max_new, max_ctx, window, sinks);
+    const size_t need = attn_rows_workspace(a);
+    SI_REQUIRE(ws_bytes >= need && (ws || !need), "%s: workspace too small", what);
+    SI_REQUIRE(aligned(ws, 256), "%s: the workspace must be 256-byte aligned", what);
+    pg.pages = pages;
+    pg.max_pages = max_pages;
+    pg.npages = npages;
+    a.q = q;
+    a.start = start;
+    a.ctx = ctx;
+    a.k = k_pool;
+    a.v = v_pool;
+    a.pg = pg;
+    a.attn = attn;
+    a.qs = qs;
+    a.d = d;
+    a.bsum = bsum;
+    launch_attn_rows_paged(a, ws, S(stream));
+    return check_launch(what);
+}
+
+}  // extern "C"

@@ -363,4 +363,35 @@ struct KvMoves {
 };
 void launch_kv_copy(const KvMoves &mv, int npools, int nmoves, size_t page_bytes, bool wide,
                     bool once, hipStream_t st);
+// A ragged step's page lists and slot maps (si_step.hip): si_kv_step's arguments.
+struct KvStep {
+    int nseq, max_rows, window, kept, shift, npages, max_pages;  // kept: pages of the sinks
+    const int *have, *add;
+    int *pages, *ring;
+    const int *free_in, *held_in;
+    int *free_out, *held_out, *start, *ctx, *seq, *pos;
+    long long *slot;
+    int *taken, *status;
+};
+void launch_kv_step(const KvStep &a, hipStream_t st);
+void launch_rope_kv_rows(const float *qkv, int ldqkv, int rows, int qheads, int kvheads, int hdim,
+                         int max_pos, const int *pos, const long long *slot, const float *rc,
+                         const float *rs, float *q_out, uint16_t *kc, uint16_t *vc,
+                         long long pool_rows, hipStream_t st);
+// Attention of a ragged step's rows over pages (si_rows.hip): si_attention_rows'
+// arguments, window and sinks at most max_ctx.
+struct RowsArgs {
+    const float *q;
+    int qheads, kvheads, hdim, nseq, max_rows, max_new, max_ctx, window, sinks;
+    const int *start, *ctx;
+    const uint16_t *k, *v;
+    KvPages pg;
+    float scale2;  // softmax_scale2
+    float *attn;
+    int8_t *qs;
+    uint16_t *d;
+    int16_t *bsum;
+};
+size_t attn_rows_workspace(const RowsArgs &a);  // (reads sizes only)
+void launch_attn_rows_paged(const RowsArgs &a, void *workspace, hipStream_t st);
 }  // namespace si

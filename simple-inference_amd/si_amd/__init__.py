@@ -136,6 +136,12 @@ _SIGS = {
     "si_attention_kv4_workspace": (_Z, [ctypes.POINTER(Shape), _I, _I, _I]),
     "si_layer_decode_kv4": (_I, [_P, _P, _I, _P, _P, _I, _I, _P, _I, _P, _I, _I, _P, _I, _P]),
     "si_kv_copy_pages": (_I, [_P, _I, _Z, _I, _P, _P, _I, _P]),
+    "si_kv_step": (_I, [_I, _P, _P] + [_I] * 6 + [_P] * 14),
+    "si_rope_kv_append_rows": (_I, [ctypes.POINTER(Shape), _P, _I, _I, _I, _P, _P, _P, _P, _P, _P,
+                                    _P, _Z, _P]),
+    "si_attention_rows": (_I, [ctypes.POINTER(Shape), _P] + [_I] * 6 + [_P] * 4 +
+                          [_I, _I, _P, _I, _P, _P, _P, _P, _P, _Z, _P]),
+    "si_attention_rows_workspace": (_Z, [ctypes.POINTER(Shape)] + [_I] * 6),
     "si_layer_buffer": (_P, [_P, _I]),
     "si_layer_set_timing": (_I, [_P, _I]),
     "si_layer_phase_ms": (_I, [_P, _P]),
