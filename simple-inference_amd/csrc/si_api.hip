@@ -2006,6 +2006,8 @@ int si_attention_rows(const si_shape_t *s, const float *q, int nseq, int max_row
     SI_REQUIRE(!qs || d, "%s: qs without d", what);
     SI_REQUIRE(aligned(qs, 4), "%s: qs must be 4-byte aligned", what);
     RowsArgs a = rows_sizes(s, nseq, max_rows, max_new, max_ctx, window, sinks);
+    SI_REQUIRE(attn_rows_fits(a), "%s: %d rows of %d heads are too many", what, max_rows,
+               s->qheads);
     const size_t need = attn_rows_workspace(a);
     SI_REQUIRE(ws_bytes >= need && (ws || !need), "%s: workspace too small", what);
     SI_REQUIRE(aligned(ws, 256), "%s: the workspace must be 256-byte aligned", what);

@@ -16,6 +16,7 @@
 // step, qwen_one_layer.c:272).
 #include "si_device.hpp"
 #include "si_kernels.hpp"
+#include "si_tiles.hpp"
 
 namespace si {
 
@@ -250,9 +251,6 @@ static void combine(int qheads, int hdim, int nq, int nsplit, bool pow2, const A
 // would take 0.1-0.4 us less of 5-8 at 2-7 queries of 256 positions, 0.1-1.5
 // of 5-24 at 4096.
 // ===========================================================================
-typedef _Float16 h8 __attribute__((ext_vector_type(8)));
-typedef _Float16 h4 __attribute__((ext_vector_type(4)));
-typedef float f4 __attribute__((ext_vector_type(4)));
 
 constexpr int MA_TILE = 16;            // positions per wavefront tile
 constexpr int MA_SUPER = 4 * MA_TILE;  // positions per workgroup step
@@ -458,71 +456,8 @@ __global__ void __launch_bounds__(256) k_attn_decode_mfma(
 // l/32.  A and B use the same k assignment, so any consistent assignment of
 // reduction indices to (slice, element) is exact.
 // ===========================================================================
-typedef float f16v __attribute__((ext_vector_type(16)));
-typedef _Float16 pf_h2 __attribute__((ext_vector_type(2)));
-typedef float pf_f2 __attribute__((ext_vector_type(2)));
 typedef uint32_t pf_u4 __attribute__((ext_vector_type(4)));
 typedef pf_u4 pf_u4u __attribute__((aligned(2)));  // at any fp16 address
-
-constexpr int PF_T = 32;      // query rows per wavefront, positions per K/V tile
-constexpr int PF_OPAD = 4;    // floats of padding per merged output row
-
-// LDS slot (16-byte unit within the row) of chunk c of tile row r: the 16
-// rows a score operand read takes together, and the 4 rows x 4 chunks of a
-// transposing read, spread over the 64 banks
-template <int D>
-__device__ __forceinline__ int pf_k_slot(int r, int c) {
-    if (D == 128) return c ^ (r & 15);
-    if (D == 64) return c ^ ((r >> 1) & 7);
-    if (D == 32) return c ^ ((r >> 2) & 3);
-    const int s = c + ((r >> 2) & 3);  // 12 chunks: a rotation
-    return s >= D / 8 ? s - D / 8 : s;
-}
-template <int D>
-__device__ __forceinline__ int pf_v_slot(int r, int c) {
-    if (D == 128) return c ^ ((r & 3) << 2);
-    if (D == 64) return c ^ (((r >> 1) & 1) << 2);
-    return c;  // 4 rows already cover the banks
-}
-// the chunk whose slot is s
-template <int D>
-__device__ __forceinline__ int pf_k_chunk(int r, int s) {
-    if (D != 96) return pf_k_slot<D>(r, s);  // an XOR
-    const int c = s - ((r >> 2) & 3);
-    return c < 0 ? c + D / 8 : c;
-}
-
-// (fmaxf of matrix results would first canonicalise each; a must come from an
-// ordinary operation on those results)
-__device__ __forceinline__ float max3_f(float a, float b, float c) {
-    float r;
-    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
-    return r;
-}
-// two values as fp16 hi + lo halves (hi rounded to nearest, lo = x - hi by a
-// mixed-precision fma; the plain conversion to hi reads both values first)
-__device__ __forceinline__ void split_pair(float x0, float x1, pf_h2 &hi, pf_h2 &lo) {
-    hi = __builtin_convertvector((pf_f2){x0, x1}, pf_h2);
-    float l0, l1;
-    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(l0) : "v"(hi), "v"(x0));
-    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]"
-        : "=v"(l1)
-        : "v"(hi), "v"(x1));
-    lo = __builtin_convertvector((pf_f2){l0, l1}, pf_h2);
-}
-
-// at most VM vector-memory operations of this wavefront outstanding, its LDS
-// reads complete
-template <int VM>
-__device__ __forceinline__ void pf_wait() {
-    static_assert(VM <= 63, "vmcnt holds 6 bits");
-    __builtin_amdgcn_s_waitcnt((VM & 15) | ((VM >> 4) << 14) | (7 << 4));
-    asm volatile("" ::: "memory");
-}
-__device__ __forceinline__ void pf_barrier() {
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-}
 
 // ASYNC: kc and vc are 16-byte aligned (and so is every row, a multiple of 64
 // bytes).  Otherwise the tiles come through registers, by loads that take any

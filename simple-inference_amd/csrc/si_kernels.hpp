@@ -392,6 +392,8 @@ struct RowsArgs {
     uint16_t *d;
     int16_t *bsum;
 };
-size_t attn_rows_workspace(const RowsArgs &a);  // (reads sizes only)
+// (both read sizes only; fits: whether one launch takes the call's workgroups)
+size_t attn_rows_workspace(const RowsArgs &a);
+bool attn_rows_fits(const RowsArgs &a);
 void launch_attn_rows_paged(const RowsArgs &a, void *workspace, hipStream_t st);
 }  // namespace si

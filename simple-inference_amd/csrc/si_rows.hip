@@ -3,84 +3,770 @@
 // attention_kernels.h:80-164, has one query and sees everything).
 //
 // A row at position p of its sequence sees position t <= p where t > p - window or
-// t < sinks.
+// t < sinks.  The (row, head) pairs of a sequence and KV group, row-major, are cut into
+// tiles of 32 RT; what a tile's rows see are whole 32-position tiles of K and V, the
+// sinks' and then the window's (RowTile), which a workgroup of RT x KW wavefronts walks:
+// KW of them side by side, each met by the RT wavefronts' 32 rows.  Long walks are cut
+// into chunks, a workgroup each, whose states (maximum, sum, unnormalised output) meet in
+// a second kernel.
+//
+// Per K/V tile a wavefront computes, as the causal prefill kernel does,
+//     S^T[pos][row] = K[pos][:] . Q[row][:]          (v_mfma_f32_32x32x16_f16)
+//     O^T[d][row] += V^T[d][pos] . P^T[pos][row]
+// with Q and P as two fp16 halves each.  A weight is 2^(fac (s - m) + 11) for raw scores s
+// and a reference m that follows the row's running maximum within 2^4; its lo half, 2^11
+// higher, is summed apart: 22 bits down to 2^-25 of the largest weight and an error of at
+// most 2^-47 of it below, for rows whose first position outweighs the rest (a sink).  A
+// row of q is scaled by a power of two to 2^14, fac takes it back.
+//
+// Where a mask cuts a tile its hidden scores are replaced (not added to), and V's values
+// there are looked at: 0 x infinity would be NaN.  Only if one is not finite, the rows
+// that see it are found first (exact counts, by the matrix cores), get their infinity or
+// NaN, and the tile in LDS has zeros in such places from then on.
+#include <algorithm>
+
 #include "si_device.hpp"
 #include "si_kernels.hpp"
+#include "si_tiles.hpp"
 
 namespace si {
 
-// A wavefront for each (row, head): lane l scores position l of each group of 64 visible
-// ones, then the group's weights meet V, a lane holding two or one of the head's values.
-__global__ void __launch_bounds__(64) k_attn_rows_plain(RowsArgs a) {
-    __shared__ float w_lds[64];
-    __shared__ size_t at_lds[64];
-    const int r = blockIdx.x, h = blockIdx.y, lane = threadIdx.x, D = a.hdim;
-    int lo = 0, hi = a.nseq;
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (a.start[mid] <= r) lo = mid;
-        else hi = mid;
+constexpr float RW_SLACK = 4.0f, RW_UP = 11.0f, RW_LO = 2048.0f;
+
+// ---------------------------------------------------------------------------
+// What a tile's rows see
+// ---------------------------------------------------------------------------
+struct RowTile {
+    int seq, row0;      // the sequence; its first row in q (row0 + t / per is pair t's)
+    int p0;             // position of row0
+    int pair0, pairs;   // the tile's (row, head) pairs of this KV group
+    int sink_tiles, w0; // K/V tiles of the sinks; the window's first one (not below them)
+    int ntiles;         // of both
+    // the v-th of them
+    __device__ __forceinline__ int tile(int v) const {
+        return v < sink_tiles ? v : w0 + v - sink_tiles;
     }
-    const int first = a.start[lo], n = a.start[lo + 1] - first;
-    if (r < first || r - first >= min(n, a.max_new)) return;
-    const int p = min(a.ctx[lo], a.max_ctx) - n + r - first;
-    const int w0 = max(p - a.window + 1, 0), ns = min(a.sinks, w0);
-    const int seen = p < 0 ? 0 : ns + p + 1 - w0;
-    const float *q = a.q + ((size_t)r * a.qheads + h) * D;
-    const int g = h / (a.qheads / a.kvheads), kvd = a.kvheads * D;
-    float m = -INFINITY, l = 0.0f, o0 = 0.0f, o1 = 0.0f;
-    for (int j0 = 0; j0 < seen; j0 += 64) {
-        const int j = min(j0 + lane, seen - 1), t = j < ns ? j : w0 + j - ns;
-        const size_t at = a.pg.at<true>(lo, t, 0, kvd) + (size_t)g * D;
-        float s = 0.0f;
-        for (int d = 0; d < D; ++d) s = fmaf(q[d], h2f(a.k[at + d]), s);
-        s = j0 + lane < seen ? s * a.scale2 : -INFINITY;
-        float mx = m;
-        for (int k = 0; k < 64; ++k) mx = fmaxf(mx, __shfl(s, k, 64));
-        const float ref = mx == -INFINITY ? 0.0f : mx;
-        const float w = exp2f(s - ref), alpha = exp2f(m - ref);
-        m = mx;
-        float sum = 0.0f;
-        for (int k = 0; k < 64; ++k) sum += __shfl(w, k, 64);
-        l = l * alpha + sum;
-        o0 *= alpha;
-        o1 *= alpha;
-        __syncthreads();
-        w_lds[lane] = w;
-        at_lds[lane] = at;
-        __syncthreads();
-        for (int k = 0; k < min(64, seen - j0); ++k) {
-            if (lane < D) o0 = fmaf(w_lds[k], h2f(a.v[at_lds[k] + lane]), o0);
-            if (lane + 64 < D) o1 = fmaf(w_lds[k], h2f(a.v[at_lds[k] + lane + 64]), o1);
+};
+
+// rows of sequence i within the call's limits, the first and its position
+__device__ __forceinline__ int seq_rows(const RowsArgs &a, int i, int &row0, int &p0) {
+    const int s0 = max(a.start[i], 0), s1 = max(a.start[i + 1], 0);
+    row0 = min(s0, a.max_rows);
+    // (rows are fewer than 2^24: what lies further before position 0 is all hidden)
+    p0 = max(min(a.ctx[i], a.max_ctx) - (s1 - s0), -(1 << 24));
+    return min(max(min(s1, a.max_rows) - row0, 0), a.max_new);
+}
+
+__device__ __forceinline__ void row_tile(const RowsArgs &a, int tile_rows, int i, int k,
+                                         RowTile &t) {
+    const int per = a.qheads / a.kvheads;
+    const int n = seq_rows(a, i, t.row0, t.p0);
+    t.seq = i;
+    t.pair0 = k * tile_rows;
+    t.pairs = min(n * per - t.pair0, tile_rows);
+    if (t.pairs <= 0) {
+        t.pairs = t.ntiles = 0;
+        return;
+    }
+    const int first = t.p0 + t.pair0 / per, last = t.p0 + (t.pair0 + t.pairs - 1) / per;
+    t.w0 = max(first - a.window + 1, 0) / PF_T;
+    t.sink_tiles = min((a.sinks + PF_T - 1) / PF_T, t.w0);
+    t.ntiles = last < 0 ? 0 : t.sink_tiles + last / PF_T - t.w0 + 1;
+}
+
+// Tile number `tile` of the call: one a sequence (ONE: max_new rows fill no more), or the
+// sequences' tiles one after another, found by a prefix sum over the sequences.  Every
+// thread of the workgroup; false past the last.
+template <bool ONE, int NT>
+__device__ __forceinline__ bool find_tile(const RowsArgs &a, int tile_rows, int tile, RowTile &t) {
+    if constexpr (ONE) {
+        row_tile(a, tile_rows, tile, 0, t);
+        return t.pairs > 0;
+    } else {
+        __shared__ int red[NT / 64], found[2];
+        const int per = a.qheads / a.kvheads, tid = threadIdx.x;
+        const auto tiles = [&](int i) {
+            int r, p;
+            return (seq_rows(a, i, r, p) * per + tile_rows - 1) / tile_rows;
+        };
+        const int each = (a.nseq + NT - 1) / NT;
+        const int i0 = min(tid * each, a.nseq), i1 = min(i0 + each, a.nseq);
+        int sum = 0;
+        for (int i = i0; i < i1; ++i) sum += tiles(i);
+        int x = sum;
+        for (int d = 1; d < 64; d <<= 1) {
+            const int y = __shfl_up(x, d, 64);
+            if ((tid & 63) >= d) x += y;
         }
+        if (tid == 0) found[0] = -1;
+        if ((tid & 63) == 63) red[tid >> 6] = x;
+        __syncthreads();
+        int base = x - sum;
+        for (int w = 0; w < (tid >> 6); ++w) base += red[w];
+        if (tile >= base && tile < base + sum)
+            for (int i = i0; i < i1; ++i) {
+                const int n = tiles(i);
+                if (tile < base + n) {
+                    found[0] = i;
+                    found[1] = tile - base;
+                    break;
+                }
+                base += n;
+            }
+        __syncthreads();
+        if (found[0] < 0) return false;
+        row_tile(a, tile_rows, __builtin_amdgcn_readfirstlane(found[0]),
+                 __builtin_amdgcn_readfirstlane(found[1]), t);
+        return t.pairs > 0;
     }
-    const size_t off = ((size_t)r * a.qheads + h) * D;
+}
+
+// ---------------------------------------------------------------------------
+// The chunks' states in the workspace: [tile][KV group][chunk] blocks of rows x (D
+// outputs), then as many rows x (maximum, sum, unit)
+// ---------------------------------------------------------------------------
+struct RowsParts {
+    float *o, *m;
+    int chunks, rows;  // rows of a block that may be used
+    size_t blocks;
+};
+
+__device__ __forceinline__ size_t part_row(const RowsParts &pt, int kvheads, int tile, int g,
+                                           int chunk, int row) {
+    return (((size_t)tile * kvheads + g) * pt.chunks + chunk) * pt.rows + row;
+}
+
+// 4 values of a row's head (8 lanes hold a Q8_0 block), zeros before position 0
+template <int D>
+__device__ __forceinline__ void rows_store(const RowsArgs &a, int row, int head, int dd, int pos,
+                                           float (&y)[4]) {
+    if (pos < 0)
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-        const int d = lane + 64 * e;
-        const float y = d < D && seen ? (e ? o1 : o0) / l : 0.0f;
-        uint16_t dbits;
-        int sum;
-        const int qv = quant_block_lane(y, dbits, sum);  // every lane
-        if (d >= D) continue;
-        a.attn[off + d] = y;
-        if (!a.qs) continue;
-        a.qs[off + d] = (int8_t)qv;
-        if ((d & 31) == 0) {
-            a.d[(off + d) / SI_QK] = dbits;
-            if (a.bsum) a.bsum[(off + d) / SI_QK] = (int16_t)sum;
+        for (int i = 0; i < 4; ++i) y[i] = 0.0f;
+    const size_t off = ((size_t)row * a.qheads + head) * D + dd;
+    *(f4 *)(a.attn + off) = (f4){y[0], y[1], y[2], y[3]};
+    if (!a.qs) return;
+    uint16_t dbits;
+    int sum;
+    *(uint32_t *)(a.qs + off) = quant_block_oct(y, dbits, sum);
+    if ((threadIdx.x & 7) == 0) {
+        a.d[off / SI_QK] = dbits;
+        if (a.bsum) a.bsum[off / SI_QK] = (int16_t)sum;
+    }
+}
+
+template <int D, int RT, int KW, bool ONE, bool PAGE32>
+__global__ void __launch_bounds__(RT * KW * 64) __attribute__((amdgpu_waves_per_eu(2)))
+k_attn_rows(RowsArgs a, RowsParts pt, int chunk_tiles) {
+    constexpr int NWV = RT * KW, NT = NWV * 64, KS = D / 16, DT = D / 32, CH = D / 8;
+    constexpr int TB = PF_T * D * 2;         // bytes of a K (or V) tile
+    constexpr int TI = TB / 1024;            // copy instructions per tile
+    constexpr int TIW = (TI + RT - 1) / RT;  // of one wavefront
+    constexpr int OROW = D + PF_OPAD;
+    // RT > 1: two stage buffers (K tiles, then V tiles) used in turn, one barrier per
+    // step.  RT == 1: each wavefront stages its own tiles, K in sb0 and V in sb1, each
+    // refilled as soon as it has been read (no barrier).  At the end the wavefronts'
+    // outputs: the first half in sb0, the others in sb1.
+    constexpr bool DB = RT > 1;
+    constexpr int STAGE = DB ? 2 * KW * TB : KW * TB;
+    constexpr int HALF_W = (NWV + 1) / 2, MRG = HALF_W * PF_T * OROW * 4;
+    __shared__ __attribute__((aligned(16))) uint8_t sb0[STAGE > MRG ? STAGE : MRG];
+    __shared__ __attribute__((aligned(16))) uint8_t sb1[STAGE > MRG ? STAGE : MRG];
+    constexpr bool QLDS = D > 64;  // q's lo halves: [RT][KS][64 lanes]
+    constexpr int QL = QLDS ? RT * KS * 1024 : 0;
+    // behind the stage buffer where the outputs, which come last, leave the room
+    constexpr bool QL_IN = STAGE + QL <= MRG;
+    __shared__ __attribute__((aligned(16))) uint8_t qlo[QL && !QL_IN ? QL : 16];
+    uint8_t *const ql_at = QL_IN ? sb0 + STAGE : qlo;
+    __shared__ float mrg_m[NWV][PF_T], mrg_l[NWV][PF_T];
+    __shared__ float row_unit[32 * RT];  // of a row's scores, in powers of two
+    __shared__ int bad_step[2];          // whether a cut step's V holds infinities or NaN
+
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int kw = wave / RT, rt = wave % RT;
+    const int t = lane & 31, hh = lane >> 5;
+    // KV groups side by side: one group's tiles on the same XCDs where their count
+    // divides 8
+    const int g = blockIdx.x % a.kvheads;
+    const int tile_id = blockIdx.x / a.kvheads / pt.chunks;
+    const int chunk = blockIdx.x / a.kvheads % pt.chunks;
+    RowTile rw;
+    if (!find_tile<ONE, NT>(a, 32 * RT, tile_id, rw)) return;
+    const int v0 = chunk * chunk_tiles, v1 = min(rw.ntiles, v0 + chunk_tiles);
+    if (chunk > 0 && v0 >= v1) return;
+    const bool whole = rw.ntiles <= chunk_tiles;  // the results themselves, not a part
+
+    const int per = a.qheads / a.kvheads, kvd = a.kvheads * D;
+    const int steps = (v1 - v0 + KW - 1) / KW;
+    // this wavefront's rows: positions of the first, the last and lane t's own
+    const int wp0 = rw.pair0 + min(32 * rt, rw.pairs - 1);
+    const int wp1 = rw.pair0 + min(32 * rt + 31, rw.pairs - 1);
+    const bool rows_here = 32 * rt < rw.pairs;
+    const int wfirst = rw.p0 + wp0 / per, wlast = rw.p0 + wp1 / per;
+    const int mypair = min(rw.pair0 + 32 * rt + t, wp1);
+    const int prow = rw.p0 + mypair / per;
+
+    // this wavefront's copies of a tile: instruction i takes the 16-byte units
+    // 64 n .. 64 n + 63 of the tile (LDS order), n = rt + RT i.  Where these are whole rows
+    // (RPI of them) the lane's offset within them is one number for V, and for K one that
+    // an XOR turns into each instruction's (a row's bytes are a multiple of its D 2).
+    constexpr bool WHOLE = 64 % CH == 0;
+    constexpr int RPI = WHOLE ? 64 / CH : 1;
+    const int lrow = lane / CH, lslot = lane % CH;
+    const int kcol = pf_k_chunk<D>(lrow, lslot) * 16, vcol = pf_v_slot<D>(lrow, lslot) * 16;
+    // row of the lane's unit of instruction i within the tile, and its bytes from the row's start
+    const auto unit = [&](int i, bool is_k, int &row, int &col) {
+        const int n = rt + RT * i;
+        if constexpr (WHOLE) {
+            row = RPI * n + lrow;
+            col = is_k ? kcol ^ (pf_k_slot<D>(RPI * n, 0) * 16) : vcol;
+        } else {
+            const int p = n * 64 + lane;
+            row = p / CH;
+            col = (is_k ? pf_k_chunk<D>(row, p % CH) : pf_v_slot<D>(row, p % CH)) * 16;
+        }
+    };
+    // the page of a step's tile (past the chunk: its last one again): of its first
+    // position, or (PAGE32 false: several pages a tile) of position t
+    const int *list = a.pg.pages + (size_t)rw.seq * a.pg.max_pages;
+    const auto kv_tile = [&](int st) { return rw.tile(min(v0 + st * KW + kw, v1 - 1)); };
+    const auto page_of = [&](int st) {
+        const int pos = kv_tile(st) * PF_T + (PAGE32 ? 0 : t);
+        const int id = list[min(pos >> a.pg.shift, a.pg.max_pages - 1)];
+        return min(max(id, 0), a.pg.npages - 1);
+    };
+    const auto copy = [&](const uint16_t *pool, uint8_t *dst, int st, int page, bool is_k) {
+        const int pos0 = kv_tile(st) * PF_T, mask = (1 << a.pg.shift) - 1;
+        uint8_t *const to = dst + kw * TB + 1024 * rt;
+        if constexpr (PAGE32) {
+            const size_t row0 = ((size_t)__builtin_amdgcn_readfirstlane(page) << a.pg.shift) |
+                                (size_t)(pos0 & mask);
+            const __amdgpu_buffer_rsrc_t rs = buf_rsrc(pool + row0 * kvd + g * D, 0x7fffffffu);
+#pragma unroll
+            for (int i = 0; i < TIW; ++i)
+                if (TI % RT == 0 || rt + RT * i < TI) {
+                    if constexpr (WHOLE) {
+                        const int x = is_k ? pf_k_slot<D>(RPI * (rt + RT * i), 0) * 16 : 0;
+                        lds_copy16(rs, to + 1024 * RT * i,
+                                   (uint32_t)(lrow * (kvd * 2) + ((is_k ? kcol : vcol) ^ x)),
+                                   RPI * (rt + RT * i) * (kvd * 2));
+                    } else {
+                        int row, col;
+                        unit(i, is_k, row, col);
+                        lds_copy16(rs, to + 1024 * RT * i, (uint32_t)(row * (kvd * 2) + col), 0);
+                    }
+                }
+        } else {
+#pragma unroll
+            for (int i = 0; i < TIW; ++i)
+                if (TI % RT == 0 || rt + RT * i < TI) {
+                    int r, col;
+                    unit(i, is_k, r, col);
+                    const int id = __shfl(page, r, 64);
+                    const size_t row = ((size_t)id << a.pg.shift) | (size_t)((pos0 + r) & mask);
+                    lds_copy16_at((const uint8_t *)(pool + row * kvd + g * D) + col,
+                                  to + 1024 * RT * i);
+                }
+        }
+    };
+    int page = 0;
+    if (steps > 0) {
+        page = page_of(0);
+        copy(a.k, sb0, 0, page, true);
+        copy(a.v, DB ? sb0 + KW * TB : sb1, 0, page, false);
+        page = page_of(1);
+    }
+
+    // Q^T as the B operand of the score MFMA: column t, k-slice hh (columns past the last
+    // row repeat it and are never stored)
+    const size_t qoff =
+        ((size_t)(rw.row0 + mypair / per) * a.qheads + g * per + mypair % per) * D;
+    h8 qh[KS], ql[QLDS ? 1 : KS];
+    float fac;
+    {
+        const float *qrow = a.q + qoff + 8 * hh;
+        float4 x0[KS], x1[KS];
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            x0[ks] = *(const float4 *)(qrow + 16 * ks);
+            x1[ks] = *(const float4 *)(qrow + 16 * ks + 4);
+        }
+        float big = 0.0f;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+            big = fmaxf(big, fmaxf(fmaxf(fmaxf(fabsf(x0[ks].x), fabsf(x0[ks].y)),
+                                         fmaxf(fabsf(x0[ks].z), fabsf(x0[ks].w))),
+                                   fmaxf(fmaxf(fabsf(x1[ks].x), fabsf(x1[ks].y)),
+                                         fmaxf(fabsf(x1[ks].z), fabsf(x1[ks].w)))));
+        big = fmaxf(big, swap32_f(big));
+        // the row's largest value to 2^14 (one below 2^-60 makes no score)
+        const int up = 14 - max((int)(f2u(big) >> 23) - 127, -60);
+        // (finite for the largest q too, whose weights are then 0 or 1 either way)
+        fac = fminf(__builtin_amdgcn_ldexpf(a.scale2, -up), 0x1.fffffep127f);
+        if (kw == 0 && hh == 0) row_unit[32 * rt + t] = fac;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            float x[8] = {x0[ks].x, x0[ks].y, x0[ks].z, x0[ks].w,
+                          x1[ks].x, x1[ks].y, x1[ks].z, x1[ks].w};
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = __builtin_amdgcn_ldexpf(x[e], up);
+            h8 &l = ql[QLDS ? 0 : ks];
+#pragma unroll
+            for (int e = 0; e < 8; e += 2) {
+                pf_h2 hi, lo;
+                split_pair(x[e], x[e + 1], hi, lo);
+                qh[ks][e] = hi[0];
+                qh[ks][e + 1] = hi[1];
+                l[e] = lo[0];
+                l[e + 1] = lo[1];
+            }
+            // (the KW wavefronts of a row tile have the same rows)
+            if (QLDS && kw == 0) *(h8 *)(ql_at + ((rt * KS + ks) * 64 + lane) * 16) = l;
         }
     }
+    __syncthreads();
+
+    // operand addresses within a stage: K row t, chunk 2 ks + hh; V rows
+    // 16 s2 + 8 e + 4 hh + s / 4 (s = lane % 16), columns 32 dt + 16 (lane / 16 % 2) +
+    // 4 (s % 4), as the transposing read takes them
+    const int s16 = lane & 15;
+    int ka[KS], va[DT];
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) ka[ks] = kw * TB + t * D * 2 + pf_k_slot<D>(t, 2 * ks + hh) * 16;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+        va[dt] = kw * TB + (4 * hh + (s16 >> 2)) * D * 2 +
+                 pf_v_slot<D>(s16 >> 2, 4 * dt + 2 * ((lane >> 4) & 1) + ((s16 & 3) >> 1)) * 16 +
+                 (s16 & 1) * 8;
+
+    float m = -INFINITY, lsum = 0.0f;  // row t's reference; this lane's share of the sum
+    const float over = RW_SLACK * __builtin_amdgcn_rcpf(fac);
+    f16v o[DT], o2[DT];  // o2: the lo halves' sums
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) o[dt] = o2[dt] = (f16v){};
+
+    const auto load_k = [&](const uint8_t *kt, h8 (&x)[KS]) {
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) x[ks] = *(const h8 *)(kt + ka[ks]);
+    };
+    const auto scores = [&](const h8 (&x)[KS]) {
+        // the lo products first: they round at their own small magnitude
+        f16v s = (f16v){};
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+            s = __builtin_amdgcn_mfma_f32_32x32x16_f16(
+                x[ks],
+                QLDS ? *(const h8 *)(ql_at + ((rt * KS + ks) * 64 + lane) * 16) : ql[QLDS ? 0 : ks],
+                s, 0, 0, 0);
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+            s = __builtin_amdgcn_mfma_f32_32x32x16_f16(x[ks], qh[ks], s, 0, 0, 0);
+        return s;
+    };
+    // whether lane t's row sees position kv0 + 8 (r / 4) + 4 hh + r % 4
+    const auto sees = [&](int kv0, int r) {
+        const int pos = kv0 + 8 * (r >> 2) + 4 * hh + (r & 3), back = prow - pos;
+        return ((unsigned)back < (unsigned)a.window) | ((pos < a.sinks) & (back >= 0));
+    };
+    h8 ph[2], pl[2];  // the tile's weights
+    const auto softmax = [&](f16v s, int kv0, bool cut) {
+        if (cut) {  // wavefront-uniform
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[r] = sees(kv0, r) ? s[r] : -INFINITY;
+        }
+        // (a plain operation reads the matrix results first: the compiler puts the wait
+        // states they need before it, which it would not before the inline instructions
+        // that follow from it)
+        float mx = fmaxf(s[0], s[1]);
+#pragma unroll
+        for (int r = 2; r < 16; r += 2) mx = max3_f(mx, s[r], s[r + 1]);
+        mx = fmaxf(mx, swap32_f(mx));
+        // the reference moves when a row's own maximum has passed it by 2^4
+        const float mnew = mx - m > over ? mx : m;
+        if (__ballot(mnew > m)) {
+            const float alpha = __builtin_amdgcn_exp2f((m - mnew) * fac);
+            const float a0 = mnew == -INFINITY ? 1.0f : alpha;
+            lsum *= a0;
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) o[dt] *= a0;
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) o2[dt] *= a0;
+            m = mnew;
+        }
+        const float mref = m == -INFINITY ? 0.0f : m;
+        float ps = 0.0f;
+#pragma unroll
+        for (int r = 0; r < 16; r += 2) {
+            const float p0 = __builtin_amdgcn_exp2f(fmaf(s[r] - mref, fac, RW_UP));
+            const float p1 = __builtin_amdgcn_exp2f(fmaf(s[r + 1] - mref, fac, RW_UP));
+            ps += p0;
+            ps += p1;
+            const pf_h2 hi = __builtin_convertvector((pf_f2){p0, p1}, pf_h2);
+            ph[r >> 3][r & 7] = hi[0];
+            ph[r >> 3][(r & 7) + 1] = hi[1];
+            pl[r >> 3][r & 7] = (_Float16)fmaf(-(float)hi[0], RW_LO, p0 * RW_LO);
+            pl[r >> 3][(r & 7) + 1] = (_Float16)fmaf(-(float)hi[1], RW_LO, p1 * RW_LO);
+        }
+        lsum += ps;
+    };
+    // k-step s2 covers positions 16 s2 + 8 (e / 4) + 4 hh + e % 4 (e = element 0..7), the
+    // positions of registers 8 s2 + e of the score output
+    const auto v_operand = [&](const uint8_t *vt, int dt, int s2) {
+        const h4 x0 = __builtin_bit_cast(h4, lds_read_tr16(vt + va[dt] + 16 * s2 * D * 2));
+        const h4 x1 = __builtin_bit_cast(h4, lds_read_tr16(vt + va[dt] + (16 * s2 + 8) * D * 2));
+        return (h8){x0[0], x0[1], x0[2], x0[3], x1[0], x1[1], x1[2], x1[3]};
+    };
+    const auto weigh = [&](const uint8_t *vt) {
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+            for (int s2 = 0; s2 < 2; ++s2) {
+                const h8 x = v_operand(vt, dt, s2);
+                o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, ph[s2], o[dt], 0, 0, 0);
+                o2[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, pl[s2], o2[dt], 0, 0, 0);
+            }
+    };
+    // whether a V operand holds an infinity or NaN (exponents of all ones)
+    typedef uint32_t w4 __attribute__((ext_vector_type(4)));
+    const auto any_bad = [&](const uint8_t *vt) {
+        uint32_t bad = 0;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+            for (int s2 = 0; s2 < 2; ++s2) {
+                const w4 w = __builtin_bit_cast(w4, v_operand(vt, dt, s2));
+#pragma unroll
+                for (int e = 0; e < 4; ++e) bad |= (w[e] & 0x7c007c00u) + 0x04000400u;
+            }
+        return __ballot((bad & 0x80008000u) != 0) != 0;
+    };
+    // the rows that see such values: how many infinities (1 each), negative ones (64) and
+    // NaN (both) each output meets, exactly, and the infinity or NaN that follows
+    typedef uint16_t u8v __attribute__((ext_vector_type(8)));
+    const auto meet_bad = [&](const uint8_t *vt, int kv0) {
+        h8 seen[2];
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+            seen[r >> 3][r & 7] = sees(kv0, r) ? (_Float16)1.0f : (_Float16)0.0f;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) {
+            f16v n = (f16v){};
+#pragma unroll
+            for (int s2 = 0; s2 < 2; ++s2) {
+                const u8v x = __builtin_bit_cast(u8v, v_operand(vt, dt, s2));
+                h8 c;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const uint16_t b = x[e];
+                    const float k = (b & 0x3ffu) ? 65.0f : b >> 15 ? 64.0f : 1.0f;
+                    c[e] = (_Float16)((b & 0x7c00u) == 0x7c00u ? k : 0.0f);
+                }
+                n = __builtin_amdgcn_mfma_f32_32x32x16_f16(c, seen[s2], n, 0, 0, 0);
+            }
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const int k = (int)n[e];
+                const float up = (k & 63) ? __builtin_inff() : 0.0f;
+                const float down = (k >> 6) ? -__builtin_inff() : 0.0f;
+                o[dt][e] += up + down;
+            }
+        }
+    };
+    // this wavefront's share of a V tile with zeros in their places
+    const auto drop_bad = [&](uint8_t *vt) {
+#pragma unroll
+        for (int i = 0; i < TIW; ++i)
+            if (TI % RT == 0 || rt + RT * i < TI) {
+                w4 *at = (w4 *)(vt + kw * TB + 1024 * (rt + RT * i) + 16 * lane);
+                w4 w = *at;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const uint32_t bad = (((w[e] & 0x7c007c00u) + 0x04000400u) >> 15) & 0x10001u;
+                    w[e] &= ~(bad * 0xffffu);
+                }
+                *at = w;
+            }
+    };
+    // whether this wavefront's rows see anything of the tile, and all of it
+    const auto touches = [&](int kv0) {
+        return rows_here && kv0 <= wlast && (kv0 + PF_T - 1 > wfirst - a.window || kv0 < a.sinks);
+    };
+    const auto inside = [&](int kv0) {
+        return kv0 + PF_T - 1 <= wfirst && (kv0 > wlast - a.window || kv0 + PF_T <= a.sinks);
+    };
+    if constexpr (DB) {
+        // one step: the stage is complete and the other buffer free after the barrier; the
+        // next stage's copies run during the whole step
+        const int first = rw.p0 + rw.pair0 / per, last = rw.p0 + (rw.pair0 + rw.pairs - 1) / per;
+        if (tid < 2) bad_step[tid] = 0;
+        for (int st = 0; st < steps; ++st) {
+            uint8_t *const cur = st & 1 ? sb1 : sb0, *const nxt = st & 1 ? sb0 : sb1;
+            pf_wait<0>();
+            pf_barrier();
+            if (st + 1 < steps) {
+                copy(a.k, nxt, st + 1, page, true);
+                copy(a.v, nxt + KW * TB, st + 1, page, false);
+                page = page_of(st + 2);
+            }
+            const int kv0 = kv_tile(st) * PF_T;
+            const bool use = v0 + st * KW + kw < v1 && touches(kv0);  // wavefront-uniform
+            if (use) {
+                h8 x[KS];
+                load_k(cur, x);
+                softmax(scores(x), kv0, !inside(kv0));
+            }
+            uint8_t *const vt = cur + KW * TB;
+            // a step with a tile that some row of the workgroup sees in part
+            bool cut = false;
+#pragma unroll
+            for (int k = 0; k < KW; ++k) {
+                const int p = rw.tile(min(v0 + st * KW + k, v1 - 1)) * PF_T;
+                cut |= !(p + PF_T - 1 <= first && (p > last - a.window || p + PF_T <= a.sinks));
+            }
+            if (cut) {  // workgroup-uniform
+                if (any_bad(vt)) {
+                    if (use) meet_bad(vt, kv0);
+                    if (lane == 0) bad_step[st & 1] = 1;
+                }
+                __syncthreads();
+                if (bad_step[st & 1]) {
+                    drop_bad(vt);
+                    __syncthreads();
+                    if (tid == 0) bad_step[st & 1] = 0;  // (next set two barriers from here)
+                }
+            }
+            if (use) weigh(vt);
+        }
+    } else {
+        for (int st = 0; st < steps; ++st) {
+            if (v0 + st * KW + kw >= v1) break;  // wavefront-uniform
+            const int kv0 = kv_tile(st) * PF_T;
+            const bool more = v0 + (st + 1) * KW + kw < v1, use = touches(kv0);
+            // outstanding: this tile's K and V copies, in this order (a page's load may
+            // stand anywhere: it only makes a wait longer)
+            const int next = page;
+            pf_wait<TIW>();  // K is in; V may still be on its way
+            h8 x[KS];
+            load_k(sb0, x);
+            pf_wait<TIW>();  // K has been read
+            if (more) {
+                page = page_of(st + 2);
+                copy(a.k, sb0, st + 1, next, true);
+            }
+            const bool cut = !inside(kv0);
+            if (use) softmax(scores(x), kv0, cut);
+            if (more)
+                pf_wait<TIW>();  // V is in; the next K may still be on its way
+            else
+                pf_wait<0>();
+            if (use) {
+                if (cut && any_bad(sb1)) {
+                    meet_bad(sb1, kv0);
+                    pf_wait<63>();  // (its reads are done)
+                    drop_bad(sb1);
+                    pf_wait<63>();
+                }
+                weigh(sb1);
+            }
+            pf_wait<TIW>();  // V has been read
+            if (more) copy(a.v, sb1, st + 1, next, false);
+        }
+    }
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) o[dt] += o2[dt] * (1.0f / RW_LO);
+    lsum += swap32_f(lsum);
+    pf_wait<0>();  // no copy in flight (a wavefront without tiles never waited for its own)
+    __syncthreads();  // every wavefront is done with the stage buffers
+
+    // lane (t, hh) holds O[row t][32 dt + 8 (r / 4) + 4 hh + r % 4] in o[dt][r]
+    {
+        float *mo = (float *)(wave < HALF_W ? sb0 : sb1) + (wave % HALF_W) * (PF_T * OROW);
+        if (hh == 0) {
+            mrg_m[wave][t] = m;
+            mrg_l[wave][t] = lsum;
+        }
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+            for (int r4 = 0; r4 < 4; ++r4)
+                *(f4 *)(mo + t * OROW + 32 * dt + 8 * r4 + 4 * hh) =
+                    (f4){o[dt][4 * r4], o[dt][4 * r4 + 1], o[dt][4 * r4 + 2], o[dt][4 * r4 + 3]};
+    }
+    __syncthreads();
+    // a row's factors for its KW states, in mrg_m: 2^(unit (m_k - max)), over the sum
+    // where the results come from this workgroup alone
+    if (tid < rw.pairs) {
+        const int w0 = tid >> 5, tr = tid & 31;
+        const float u = row_unit[tid];
+        float M = -INFINITY, l = 0.0f, f[KW];
+#pragma unroll
+        for (int k = 0; k < KW; ++k) M = fmaxf(M, mrg_m[k * RT + w0][tr]);
+        const float ref = M == -INFINITY ? 0.0f : M;
+#pragma unroll
+        for (int k = 0; k < KW; ++k) {
+            f[k] = __builtin_amdgcn_exp2f((mrg_m[k * RT + w0][tr] - ref) * u);
+            l = fmaf(mrg_l[k * RT + w0][tr], f[k], l);
+        }
+        if (!whole) {
+            float *to = pt.m + 3 * part_row(pt, a.kvheads, tile_id, g, chunk, tid);
+            to[0] = M;
+            to[1] = l;
+            to[2] = u;
+        }
+        const float inv = whole ? 1.0f / l : 1.0f;
+#pragma unroll
+        for (int k = 0; k < KW; ++k) mrg_m[k * RT + w0][tr] = f[k] * inv;
+    }
+    __syncthreads();
+    // 4 consecutive elements of a row per thread: merge the KW states, quantize (8 lanes
+    // hold one Q8_0 block, qwen_one_layer.c:272)
+    for (int e = tid; e < rw.pairs * (D / 4); e += NT) {
+        const int lr = e / (D / 4), dd = 4 * (e % (D / 4)), w0 = lr >> 5, tr = lr & 31;
+        float y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int k = 0; k < KW; ++k) {
+            const int w = k * RT + w0;
+            const float *mo = (const float *)(w < HALF_W ? sb0 : sb1) + (w % HALF_W) * (PF_T * OROW);
+            const f4 v = *(const f4 *)(mo + tr * OROW + dd);
+            const float f = mrg_m[w][tr];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) y[i] = fmaf(v[i], f, y[i]);
+        }
+        if (!whole) {
+            *(f4 *)(pt.o + part_row(pt, a.kvheads, tile_id, g, chunk, lr) * D + dd) =
+                (f4){y[0], y[1], y[2], y[3]};
+            continue;
+        }
+        const int pair = rw.pair0 + lr;
+        rows_store<D>(a, rw.row0 + pair / per, g * per + pair % per, dd, rw.p0 + pair / per, y);
+    }
+}
+
+// ---------------------------------------------------------------------------
+// The chunks' states of tiles that were cut: grid (tiles x KV groups, rows), 4 values of a
+// row per thread
+// ---------------------------------------------------------------------------
+constexpr int RM_T = 256;
+template <int D, bool ONE>
+__global__ void __launch_bounds__(RM_T) k_attn_rows_merge(RowsArgs a, RowsParts pt, int tile_rows,
+                                                          int chunk_tiles) {
+    const int g = blockIdx.x % a.kvheads, tile_id = blockIdx.x / a.kvheads;
+    RowTile rw;
+    if (!find_tile<ONE, RM_T>(a, tile_rows, tile_id, rw) || rw.ntiles <= chunk_tiles) return;
+    const int e = blockIdx.y * RM_T + threadIdx.x;
+    const int lr = e / (D / 4), dd = 4 * (e % (D / 4));
+    if (lr >= rw.pairs) return;  // whole groups of 8 lanes
+    const int n = (rw.ntiles + chunk_tiles - 1) / chunk_tiles;
+    float M = -INFINITY;
+#pragma unroll 4
+    for (int c = 0; c < n; ++c)
+        M = fmaxf(M, pt.m[3 * part_row(pt, a.kvheads, tile_id, g, c, lr)]);
+    const float u = pt.m[3 * part_row(pt, a.kvheads, tile_id, g, 0, lr) + 2];
+    const float ref = M == -INFINITY ? 0.0f : M;
+    float l = 0.0f, y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+    for (int c = 0; c < n; ++c) {
+        const size_t at = part_row(pt, a.kvheads, tile_id, g, c, lr);
+        const float f = __builtin_amdgcn_exp2f((pt.m[3 * at] - ref) * u);
+        const f4 v = *(const f4 *)(pt.o + at * D + dd);
+        l = fmaf(pt.m[3 * at + 1], f, l);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) y[i] = fmaf(v[i], f, y[i]);
+    }
+    const float inv = 1.0f / l;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) y[i] *= inv;
+    const int per = a.qheads / a.kvheads, pair = rw.pair0 + lr;
+    rows_store<D>(a, rw.row0 + pair / per, g * per + pair % per, dd, rw.p0 + pair / per, y);
+}
+
+// ---------------------------------------------------------------------------
+// How a call is cut
+// ---------------------------------------------------------------------------
+struct RowsPlan {
+    bool one;       // a tile a sequence at most
+    int rt, kw;     // wavefronts of a workgroup: 32-row tiles x K/V tiles
+    int tiles;      // at most
+    int chunks, chunk_tiles, rows;
+};
+
+static RowsPlan rows_plan(const RowsArgs &a) {
+    RowsPlan p;
+    const int per = a.qheads / a.kvheads;
+    const long long pairs = (long long)a.max_new * per;
+    p.one = pairs <= 64;
+    p.rt = pairs <= 32 ? 1 : pairs <= 64 ? 2 : 4;
+    p.kw = p.rt == 4 ? 2 : 4;
+    const int rows = 32 * p.rt;
+    p.tiles = p.one ? a.nseq : (int)((long long)a.max_rows * per / rows) + a.nseq;
+    p.rows = (int)std::min<long long>(rows, pairs);
+    // K/V tiles that a tile's rows can see: the sinks', and a window's of every row
+    const long long span = std::min<long long>(a.max_ctx, (long long)a.window + rows / per + 1);
+    const int most = (int)std::min<long long>((a.max_ctx + PF_T - 1) / PF_T,
+                                              span / PF_T + 2 + (a.sinks + PF_T - 1) / PF_T);
+    const long long base =
+        (long long)a.kvheads *
+        (p.one ? a.nseq : std::max<long long>(1, (long long)a.max_rows * per / rows));
+    const long long want = p.rt == 1 ? 512 : 256;
+    long long chunks = std::max(1LL, want / base);
+    chunks = std::min<long long>(chunks, std::max(1, most / (2 * p.kw)));
+    p.chunk_tiles = (int)((most + chunks - 1) / chunks);
+    p.chunks = (most + p.chunk_tiles - 1) / p.chunk_tiles;
+    return p;
 }
 
 size_t attn_rows_workspace(const RowsArgs &a) {
-    (void)a;
-    return 0;
+    const RowsPlan p = rows_plan(a);
+    if (p.chunks == 1) return 0;
+    return (size_t)p.tiles * a.kvheads * p.chunks * p.rows * (a.hdim + 3) * sizeof(float);
+}
+
+bool attn_rows_fits(const RowsArgs &a) {
+    const RowsPlan p = rows_plan(a);
+    // (a launch's threads are counted in 32 bits)
+    return (long long)p.tiles * a.kvheads * p.chunks * p.rt * p.kw * 64 < (1LL << 32);
 }
 
 void launch_attn_rows_paged(const RowsArgs &a, void *workspace, hipStream_t st) {
-    (void)workspace;
-    SI_LAUNCH(k_attn_rows_plain, dim3(a.max_rows, a.qheads), dim3(64), 0, st, a);
+    const RowsPlan p = rows_plan(a);
+    RowsParts pt = {};
+    pt.chunks = p.chunks;
+    pt.rows = p.rows;
+    pt.blocks = (size_t)p.tiles * a.kvheads * p.chunks;
+    pt.o = (float *)workspace;
+    pt.m = pt.o + pt.blocks * p.rows * a.hdim;
+    const dim3 grid((unsigned)(p.tiles * a.kvheads * p.chunks)), block(p.rt * p.kw * 64);
+    const bool page32 = a.pg.shift >= 5;
+#define CALL(DIM, RT, KW, ONE, P32) \
+    SI_LAUNCH((k_attn_rows<DIM, RT, KW, ONE, P32>), grid, block, 0, st, a, pt, p.chunk_tiles)
+#define PAGES(DIM, RT, KW, ONE) \
+    if (page32) CALL(DIM, RT, KW, ONE, true); \
+    else CALL(DIM, RT, KW, ONE, false)
+#define DIMS(DIM)                                  \
+    if (p.rt == 1) { PAGES(DIM, 1, 4, true); }     \
+    else if (p.rt == 2) { PAGES(DIM, 2, 4, true); } \
+    else { PAGES(DIM, 4, 2, false); }
+#define MERGE(DIM, ONE)                                                                         \
+    SI_LAUNCH((k_attn_rows_merge<DIM, ONE>),                                                    \
+              dim3((unsigned)(p.tiles * a.kvheads), (p.rows * (DIM / 4) + RM_T - 1) / RM_T),    \
+              dim3(RM_T), 0, st, a, pt, 32 * p.rt, p.chunk_tiles)
+#define MERGES(DIM)                  \
+    if (p.chunks > 1) {              \
+        if (p.one) MERGE(DIM, true); \
+        else MERGE(DIM, false);      \
+    }
+    switch (a.hdim) {
+        case 32: DIMS(32); MERGES(32); break;
+        case 64: DIMS(64); MERGES(64); break;
+        case 96: DIMS(96); MERGES(96); break;
+        default: DIMS(128); MERGES(128); break;
+    }
+#undef MERGES
+#undef MERGE
+#undef DIMS
+#undef PAGES
+#undef CALL
 }
 
 }  // namespace si
