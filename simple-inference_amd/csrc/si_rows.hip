@@ -4,20 +4,22 @@
 //
 // A row at position p of its sequence sees position t <= p where t > p - window or
 // t < sinks.  The (row, head) pairs of a sequence and KV group, row-major, are cut into
-// tiles of 32 RT; what a tile's rows see are whole 32-position tiles of K and V, the
-// sinks' and then the window's (RowTile), which a workgroup of RT x KW wavefronts walks:
-// KW of them side by side, each met by the RT wavefronts' 32 rows.  Long walks are cut
-// into chunks, a workgroup each, whose states (maximum, sum, unnormalised output) meet in
-// a second kernel.
+// tiles of 32 RT; what a tile's rows see are 32-position tiles of K and V, the sinks' and
+// then the window's (RowTile), which a workgroup of RT x KW wavefronts walks: KW of them
+// side by side, each met by the RT wavefronts' 32 rows.  Long walks are cut into chunks,
+// a workgroup each, whose states (reference, sum, unnormalised output) meet in a second
+// kernel.
 //
 // Per K/V tile a wavefront computes, as the causal prefill kernel does,
 //     S^T[pos][row] = K[pos][:] . Q[row][:]          (v_mfma_f32_32x32x16_f16)
 //     O^T[d][row] += V^T[d][pos] . P^T[pos][row]
-// with Q and P as two fp16 halves each.  A weight is 2^(fac (s - m) + 11) for raw scores s
-// and a reference m that follows the row's running maximum within 2^4; its lo half, 2^11
-// higher, is summed apart: 22 bits down to 2^-25 of the largest weight and an error of at
-// most 2^-47 of it below, for rows whose first position outweighs the rest (a sink).  A
-// row of q is scaled by a power of two to 2^14, fac takes it back.
+// with Q and P as two fp16 halves each.  A row of q is scaled by a power of two to 2^14,
+// fac takes it back: a weight is 2^(fac s - c + 11), c a reference near the scores of the
+// tile at hand: it moves when the tile's largest lies more than 2^4 over it, or 2^12
+// under.  So a weight keeps 22 bits down to 2^-14 of its tile's largest and has an error
+// of at most 2^-24 of that one below, also behind a position that outweighs the rest (an
+// attention sink, whose values are small): sums in 32 bits hold both.  The sinks' tiles
+// have no other positions in them (a window's tile that they share is met twice).
 //
 // Where a mask cuts a tile its hidden scores are replaced (not added to), and V's values
 // there are looked at: 0 x infinity would be NaN.  Only if one is not finite, the rows
@@ -31,7 +33,10 @@
 
 namespace si {
 
-constexpr float RW_SLACK = 4.0f, RW_UP = 11.0f, RW_LO = 2048.0f;
+constexpr float RW_UP = 11.0f;    // log2 of a weight's unit
+constexpr float RW_OVER = 4.0f;   // how far a tile's largest may lie over the reference
+constexpr float RW_UNDER = 12.0f; // and under it
+constexpr float RW_ROOM = 100.0f; // log2 of a sum's largest value (times V's, 2^16)
 
 // ---------------------------------------------------------------------------
 // What a tile's rows see
@@ -40,11 +45,23 @@ struct RowTile {
     int seq, row0;      // the sequence; its first row in q (row0 + t / per is pair t's)
     int p0;             // position of row0
     int pair0, pairs;   // the tile's (row, head) pairs of this KV group
-    int sink_tiles, w0; // K/V tiles of the sinks; the window's first one (not below them)
+    int first, last;    // positions of the first and the last of them
+    int sink_tiles, w0; // K/V tiles of the sinks; the window's first one
     int ntiles;         // of both
     // the v-th of them
     __device__ __forceinline__ int tile(int v) const {
         return v < sink_tiles ? v : w0 + v - sink_tiles;
+    }
+    // whether rows at positions p0 to p1 see anything of the v-th, and all of it (of a
+    // sinks' tile the sinks, of a window's tile the others)
+    __device__ __forceinline__ bool touches(const RowsArgs &a, int v, int p0, int p1) const {
+        const int kv0 = tile(v) * PF_T;
+        return kv0 <= p1 && (v < sink_tiles || kv0 + PF_T - 1 > p0 - a.window);
+    }
+    __device__ __forceinline__ bool inside(const RowsArgs &a, int v, int p0, int p1) const {
+        const int kv0 = tile(v) * PF_T;
+        return kv0 + PF_T - 1 <= p0 && (v < sink_tiles ? kv0 + PF_T <= a.sinks
+                                                       : kv0 >= a.sinks && kv0 > p1 - a.window);
     }
 };
 
@@ -68,10 +85,12 @@ __device__ __forceinline__ void row_tile(const RowsArgs &a, int tile_rows, int i
         t.pairs = t.ntiles = 0;
         return;
     }
-    const int first = t.p0 + t.pair0 / per, last = t.p0 + (t.pair0 + t.pairs - 1) / per;
-    t.w0 = max(first - a.window + 1, 0) / PF_T;
-    t.sink_tiles = min((a.sinks + PF_T - 1) / PF_T, t.w0);
-    t.ntiles = last < 0 ? 0 : t.sink_tiles + last / PF_T - t.w0 + 1;
+    t.first = t.p0 + t.pair0 / per;
+    t.last = t.p0 + (t.pair0 + t.pairs - 1) / per;
+    const int from = max(t.first - a.window + 1, a.sinks);
+    t.w0 = from / PF_T;
+    t.sink_tiles = min((a.sinks + PF_T - 1) / PF_T, t.last < 0 ? 0 : t.last / PF_T + 1);
+    t.ntiles = t.sink_tiles + (t.last < from ? 0 : t.last / PF_T - t.w0 + 1);
 }
 
 // Tile number `tile` of the call: one a sequence (ONE: max_new rows fill no more), or the
@@ -122,13 +141,12 @@ __device__ __forceinline__ bool find_tile(const RowsArgs &a, int tile_rows, int 
 }
 
 // ---------------------------------------------------------------------------
-// The chunks' states in the workspace: [tile][KV group][chunk] blocks of rows x (D
-// outputs), then as many rows x (maximum, sum, unit)
+// The chunks' states in the workspace: [tile][KV group][chunk] blocks of rows x D outputs,
+// then as many rows x (reference, sum)
 // ---------------------------------------------------------------------------
 struct RowsParts {
     float *o, *m;
     int chunks, rows;  // rows of a block that may be used
-    size_t blocks;
 };
 
 __device__ __forceinline__ size_t part_row(const RowsParts &pt, int kvheads, int tile, int g,
@@ -163,24 +181,15 @@ k_attn_rows(RowsArgs a, RowsParts pt, int chunk_tiles) {
     constexpr int TI = TB / 1024;            // copy instructions per tile
     constexpr int TIW = (TI + RT - 1) / RT;  // of one wavefront
     constexpr int OROW = D + PF_OPAD;
-    // RT > 1: two stage buffers (K tiles, then V tiles) used in turn, one barrier per
-    // step.  RT == 1: each wavefront stages its own tiles, K in sb0 and V in sb1, each
-    // refilled as soon as it has been read (no barrier).  At the end the wavefronts'
-    // outputs: the first half in sb0, the others in sb1.
+    // RT > 1: two stages (K tiles, then V tiles) used in turn, one barrier per step.
+    // RT == 1: each wavefront stages its own tiles, K and V, each refilled as soon as it
+    // has been read (no barrier).  KW > 1: at the end the wavefronts' outputs.
     constexpr bool DB = RT > 1;
-    constexpr int STAGE = DB ? 2 * KW * TB : KW * TB;
-    constexpr int HALF_W = (NWV + 1) / 2, MRG = HALF_W * PF_T * OROW * 4;
-    __shared__ __attribute__((aligned(16))) uint8_t sb0[STAGE > MRG ? STAGE : MRG];
-    __shared__ __attribute__((aligned(16))) uint8_t sb1[STAGE > MRG ? STAGE : MRG];
-    constexpr bool QLDS = D > 64;  // q's lo halves: [RT][KS][64 lanes]
-    constexpr int QL = QLDS ? RT * KS * 1024 : 0;
-    // behind the stage buffer where the outputs, which come last, leave the room
-    constexpr bool QL_IN = STAGE + QL <= MRG;
-    __shared__ __attribute__((aligned(16))) uint8_t qlo[QL && !QL_IN ? QL : 16];
-    uint8_t *const ql_at = QL_IN ? sb0 + STAGE : qlo;
-    __shared__ float mrg_m[NWV][PF_T], mrg_l[NWV][PF_T];
-    __shared__ float row_unit[32 * RT];  // of a row's scores, in powers of two
-    __shared__ int bad_step[2];          // whether a cut step's V holds infinities or NaN
+    constexpr int STAGE = 2 * KW * TB, NSTAGE = DB ? 2 : 1;
+    constexpr int MRG = KW > 1 ? NWV * PF_T * OROW * 4 : 0;
+    __shared__ __attribute__((aligned(16))) uint8_t sb[NSTAGE * STAGE > MRG ? NSTAGE * STAGE : MRG];
+    __shared__ float mrg_m[KW > 1 ? NWV : 1][PF_T], mrg_l[KW > 1 ? NWV : 1][PF_T];
+    __shared__ int bad_step[2];  // whether a cut step's V holds infinities or NaN
 
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -205,6 +214,7 @@ k_attn_rows(RowsArgs a, RowsParts pt, int chunk_tiles) {
     const bool rows_here = 32 * rt < rw.pairs;
     const int wfirst = rw.p0 + wp0 / per, wlast = rw.p0 + wp1 / per;
     const int mypair = min(rw.pair0 + 32 * rt + t, wp1);
+    const int myrow = rw.row0 + mypair / per, myhead = g * per + mypair % per;
     const int prow = rw.p0 + mypair / per;
 
     // this wavefront's copies of a tile: instruction i takes the 16-byte units
@@ -230,14 +240,14 @@ k_attn_rows(RowsArgs a, RowsParts pt, int chunk_tiles) {
     // the page of a step's tile (past the chunk: its last one again): of its first
     // position, or (PAGE32 false: several pages a tile) of position t
     const int *list = a.pg.pages + (size_t)rw.seq * a.pg.max_pages;
-    const auto kv_tile = [&](int st) { return rw.tile(min(v0 + st * KW + kw, v1 - 1)); };
+    const auto nth = [&](int st) { return min(v0 + st * KW + kw, v1 - 1); };
     const auto page_of = [&](int st) {
-        const int pos = kv_tile(st) * PF_T + (PAGE32 ? 0 : t);
+        const int pos = rw.tile(nth(st)) * PF_T + (PAGE32 ? 0 : t);
         const int id = list[min(pos >> a.pg.shift, a.pg.max_pages - 1)];
         return min(max(id, 0), a.pg.npages - 1);
     };
     const auto copy = [&](const uint16_t *pool, uint8_t *dst, int st, int page, bool is_k) {
-        const int pos0 = kv_tile(st) * PF_T, mask = (1 << a.pg.shift) - 1;
+        const int pos0 = rw.tile(nth(st)) * PF_T, mask = (1 << a.pg.shift) - 1;
         uint8_t *const to = dst + kw * TB + 1024 * rt;
         if constexpr (PAGE32) {
             const size_t row0 = ((size_t)__builtin_amdgcn_readfirstlane(page) << a.pg.shift) |
@@ -273,19 +283,17 @@ k_attn_rows(RowsArgs a, RowsParts pt, int chunk_tiles) {
     int page = 0;
     if (steps > 0) {
         page = page_of(0);
-        copy(a.k, sb0, 0, page, true);
-        copy(a.v, DB ? sb0 + KW * TB : sb1, 0, page, false);
+        copy(a.k, sb, 0, page, true);
+        copy(a.v, sb + KW * TB, 0, page, false);
         page = page_of(1);
     }
 
     // Q^T as the B operand of the score MFMA: column t, k-slice hh (columns past the last
     // row repeat it and are never stored)
-    const size_t qoff =
-        ((size_t)(rw.row0 + mypair / per) * a.qheads + g * per + mypair % per) * D;
-    h8 qh[KS], ql[QLDS ? 1 : KS];
+    h8 qh[KS], ql[KS];
     float fac;
     {
-        const float *qrow = a.q + qoff + 8 * hh;
+        const float *qrow = a.q + ((size_t)myrow * a.qheads + myhead) * D + 8 * hh;
         float4 x0[KS], x1[KS];
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
@@ -302,30 +310,25 @@ k_attn_rows(RowsArgs a, RowsParts pt, int chunk_tiles) {
         big = fmaxf(big, swap32_f(big));
         // the row's largest value to 2^14 (one below 2^-60 makes no score)
         const int up = 14 - max((int)(f2u(big) >> 23) - 127, -60);
-        // (finite for the largest q too, whose weights are then 0 or 1 either way)
-        fac = fminf(__builtin_amdgcn_ldexpf(a.scale2, -up), 0x1.fffffep127f);
-        if (kw == 0 && hh == 0) row_unit[32 * rt + t] = fac;
+        // (past 2^80 a weight is 0 or 1 either way, and a score, 2^38 at most, times it finite)
+        fac = fminf(__builtin_amdgcn_ldexpf(a.scale2, -up), 0x1p80f);
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
             float x[8] = {x0[ks].x, x0[ks].y, x0[ks].z, x0[ks].w,
                           x1[ks].x, x1[ks].y, x1[ks].z, x1[ks].w};
 #pragma unroll
             for (int e = 0; e < 8; ++e) x[e] = __builtin_amdgcn_ldexpf(x[e], up);
-            h8 &l = ql[QLDS ? 0 : ks];
 #pragma unroll
             for (int e = 0; e < 8; e += 2) {
                 pf_h2 hi, lo;
                 split_pair(x[e], x[e + 1], hi, lo);
                 qh[ks][e] = hi[0];
                 qh[ks][e + 1] = hi[1];
-                l[e] = lo[0];
-                l[e + 1] = lo[1];
+                ql[ks][e] = lo[0];
+                ql[ks][e + 1] = lo[1];
             }
-            // (the KW wavefronts of a row tile have the same rows)
-            if (QLDS && kw == 0) *(h8 *)(ql_at + ((rt * KS + ks) * 64 + lane) * 16) = l;
         }
     }
-    __syncthreads();
 
     // operand addresses within a stage: K row t, chunk 2 ks + hh; V rows
     // 16 s2 + 8 e + 4 hh + s / 4 (s = lane % 16), columns 32 dt + 16 (lane / 16 % 2) +
@@ -340,40 +343,46 @@ k_attn_rows(RowsArgs a, RowsParts pt, int chunk_tiles) {
                  pf_v_slot<D>(s16 >> 2, 4 * dt + 2 * ((lane >> 4) & 1) + ((s16 & 3) >> 1)) * 16 +
                  (s16 & 1) * 8;
 
-    float m = -INFINITY, lsum = 0.0f;  // row t's reference; this lane's share of the sum
-    const float over = RW_SLACK * __builtin_amdgcn_rcpf(fac);
-    f16v o[DT], o2[DT];  // o2: the lo halves' sums
+    float c = -INFINITY, lsum = 0.0f;  // row t's reference; this lane's share of the sum
+    f16v o[DT];
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt) o[dt] = o2[dt] = (f16v){};
+    for (int dt = 0; dt < DT; ++dt) o[dt] = (f16v){};
 
-    const auto load_k = [&](const uint8_t *kt, h8 (&x)[KS]) {
+    const auto scores = [&](const uint8_t *kt) {
+        h8 x[KS];
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) x[ks] = *(const h8 *)(kt + ka[ks]);
-    };
-    const auto scores = [&](const h8 (&x)[KS]) {
         // the lo products first: they round at their own small magnitude
         f16v s = (f16v){};
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks)
-            s = __builtin_amdgcn_mfma_f32_32x32x16_f16(
-                x[ks],
-                QLDS ? *(const h8 *)(ql_at + ((rt * KS + ks) * 64 + lane) * 16) : ql[QLDS ? 0 : ks],
-                s, 0, 0, 0);
+            s = __builtin_amdgcn_mfma_f32_32x32x16_f16(x[ks], ql[ks], s, 0, 0, 0);
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks)
             s = __builtin_amdgcn_mfma_f32_32x32x16_f16(x[ks], qh[ks], s, 0, 0, 0);
         return s;
     };
-    // whether lane t's row sees position kv0 + 8 (r / 4) + 4 hh + r % 4
-    const auto sees = [&](int kv0, int r) {
-        const int pos = kv0 + 8 * (r >> 2) + 4 * hh + (r & 3), back = prow - pos;
-        return ((unsigned)back < (unsigned)a.window) | ((pos < a.sinks) & (back >= 0));
+    // the positions of the v-th tile that lane t's row sees: those from `from` on, `width`
+    // more, counted from the lane's first, kv0 + 4 hh (register r: 8 (r / 4) + r % 4 behind it)
+    struct Seen {
+        int from, width;
+        __device__ __forceinline__ bool at(int r) const {
+            return (unsigned)(8 * (r >> 2) + (r & 3) - from) <= (unsigned)width;
+        }
+    };
+    const auto seen_of = [&](int v) {
+        const bool sink = v < rw.sink_tiles;
+        const int lo = sink ? 0 : max(prow - a.window + 1, a.sinks);
+        const int hi = sink ? min(prow, a.sinks - 1) : prow;
+        const int at = rw.tile(v) * PF_T + 4 * hh;
+        return hi < lo ? Seen{64, 0} : Seen{lo - at, hi - lo};
     };
     h8 ph[2], pl[2];  // the tile's weights
-    const auto softmax = [&](f16v s, int kv0, bool cut) {
+    const auto softmax = [&](f16v s, int v, bool cut) {
         if (cut) {  // wavefront-uniform
+            const Seen seen = seen_of(v);
 #pragma unroll
-            for (int r = 0; r < 16; ++r) s[r] = sees(kv0, r) ? s[r] : -INFINITY;
+            for (int r = 0; r < 16; ++r) s[r] = seen.at(r) ? s[r] : -INFINITY;
         }
         // (a plain operation reads the matrix results first: the compiler puts the wait
         // states they need before it, which it would not before the inline instructions
@@ -381,32 +390,36 @@ k_attn_rows(RowsArgs a, RowsParts pt, int chunk_tiles) {
         float mx = fmaxf(s[0], s[1]);
 #pragma unroll
         for (int r = 2; r < 16; r += 2) mx = max3_f(mx, s[r], s[r + 1]);
-        mx = fmaxf(mx, swap32_f(mx));
-        // the reference moves when a row's own maximum has passed it by 2^4
-        const float mnew = mx - m > over ? mx : m;
-        if (__ballot(mnew > m)) {
-            const float alpha = __builtin_amdgcn_exp2f((m - mnew) * fac);
-            const float a0 = mnew == -INFINITY ? 1.0f : alpha;
-            lsum *= a0;
+        mx = fmaxf(mx, swap32_f(mx)) * fac;
+        const float d = mx - c;
+        if (__ballot((d > RW_OVER) | (d < -RW_UNDER))) {
+            // up to the tile's largest; or down to it, as far as the sums have room
+            // (both halves of a row take the same step)
+            const float l = fmaxf(lsum, swap32_f(lsum));
+            const float room = RW_ROOM - (float)((int)(f2u(l) >> 23) - 127);
+            float to = c;
+            if (d > RW_OVER) to = mx;
+            else if (d < -RW_UNDER && mx > -INFINITY) to = c - fminf(-d, fmaxf(room, 0.0f));
+            const float alpha = to == c ? 1.0f : __builtin_amdgcn_exp2f(c - to);
+            c = to;
+            lsum *= alpha;
 #pragma unroll
-            for (int dt = 0; dt < DT; ++dt) o[dt] *= a0;
-#pragma unroll
-            for (int dt = 0; dt < DT; ++dt) o2[dt] *= a0;
-            m = mnew;
+            for (int dt = 0; dt < DT; ++dt) o[dt] *= alpha;
         }
-        const float mref = m == -INFINITY ? 0.0f : m;
+        const float up = RW_UP - (c == -INFINITY ? 0.0f : c);
         float ps = 0.0f;
 #pragma unroll
         for (int r = 0; r < 16; r += 2) {
-            const float p0 = __builtin_amdgcn_exp2f(fmaf(s[r] - mref, fac, RW_UP));
-            const float p1 = __builtin_amdgcn_exp2f(fmaf(s[r + 1] - mref, fac, RW_UP));
+            const float p0 = __builtin_amdgcn_exp2f(fmaf(s[r], fac, up));
+            const float p1 = __builtin_amdgcn_exp2f(fmaf(s[r + 1], fac, up));
             ps += p0;
             ps += p1;
-            const pf_h2 hi = __builtin_convertvector((pf_f2){p0, p1}, pf_h2);
+            pf_h2 hi, lo;
+            split_pair(p0, p1, hi, lo);
             ph[r >> 3][r & 7] = hi[0];
             ph[r >> 3][(r & 7) + 1] = hi[1];
-            pl[r >> 3][r & 7] = (_Float16)fmaf(-(float)hi[0], RW_LO, p0 * RW_LO);
-            pl[r >> 3][(r & 7) + 1] = (_Float16)fmaf(-(float)hi[1], RW_LO, p1 * RW_LO);
+            pl[r >> 3][r & 7] = lo[0];
+            pl[r >> 3][(r & 7) + 1] = lo[1];
         }
         lsum += ps;
     };
@@ -424,7 +437,7 @@ k_attn_rows(RowsArgs a, RowsParts pt, int chunk_tiles) {
             for (int s2 = 0; s2 < 2; ++s2) {
                 const h8 x = v_operand(vt, dt, s2);
                 o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, ph[s2], o[dt], 0, 0, 0);
-                o2[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, pl[s2], o2[dt], 0, 0, 0);
+                o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, pl[s2], o[dt], 0, 0, 0);
             }
     };
     // whether a V operand holds an infinity or NaN (exponents of all ones)
@@ -444,25 +457,26 @@ k_attn_rows(RowsArgs a, RowsParts pt, int chunk_tiles) {
     // the rows that see such values: how many infinities (1 each), negative ones (64) and
     // NaN (both) each output meets, exactly, and the infinity or NaN that follows
     typedef uint16_t u8v __attribute__((ext_vector_type(8)));
-    const auto meet_bad = [&](const uint8_t *vt, int kv0) {
+    const auto meet_bad = [&](const uint8_t *vt, int v) {
         h8 seen[2];
+        const Seen sn = seen_of(v);
 #pragma unroll
         for (int r = 0; r < 16; ++r)
-            seen[r >> 3][r & 7] = sees(kv0, r) ? (_Float16)1.0f : (_Float16)0.0f;
+            seen[r >> 3][r & 7] = sn.at(r) ? (_Float16)1.0f : (_Float16)0.0f;
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) {
             f16v n = (f16v){};
 #pragma unroll
             for (int s2 = 0; s2 < 2; ++s2) {
                 const u8v x = __builtin_bit_cast(u8v, v_operand(vt, dt, s2));
-                h8 c;
+                h8 k;
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     const uint16_t b = x[e];
-                    const float k = (b & 0x3ffu) ? 65.0f : b >> 15 ? 64.0f : 1.0f;
-                    c[e] = (_Float16)((b & 0x7c00u) == 0x7c00u ? k : 0.0f);
+                    const float f = (b & 0x3ffu) ? 65.0f : b >> 15 ? 64.0f : 1.0f;
+                    k[e] = (_Float16)((b & 0x7c00u) == 0x7c00u ? f : 0.0f);
                 }
-                n = __builtin_amdgcn_mfma_f32_32x32x16_f16(c, seen[s2], n, 0, 0, 0);
+                n = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, seen[s2], n, 0, 0, 0);
             }
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
@@ -488,20 +502,12 @@ k_attn_rows(RowsArgs a, RowsParts pt, int chunk_tiles) {
                 *at = w;
             }
     };
-    // whether this wavefront's rows see anything of the tile, and all of it
-    const auto touches = [&](int kv0) {
-        return rows_here && kv0 <= wlast && (kv0 + PF_T - 1 > wfirst - a.window || kv0 < a.sinks);
-    };
-    const auto inside = [&](int kv0) {
-        return kv0 + PF_T - 1 <= wfirst && (kv0 > wlast - a.window || kv0 + PF_T <= a.sinks);
-    };
     if constexpr (DB) {
-        // one step: the stage is complete and the other buffer free after the barrier; the
+        // one step: the stage is complete and the other one free after the barrier; the
         // next stage's copies run during the whole step
-        const int first = rw.p0 + rw.pair0 / per, last = rw.p0 + (rw.pair0 + rw.pairs - 1) / per;
         if (tid < 2) bad_step[tid] = 0;
         for (int st = 0; st < steps; ++st) {
-            uint8_t *const cur = st & 1 ? sb1 : sb0, *const nxt = st & 1 ? sb0 : sb1;
+            uint8_t *const cur = sb + (st & 1) * STAGE, *const nxt = sb + (~st & 1) * STAGE;
             pf_wait<0>();
             pf_barrier();
             if (st + 1 < steps) {
@@ -509,24 +515,19 @@ k_attn_rows(RowsArgs a, RowsParts pt, int chunk_tiles) {
                 copy(a.v, nxt + KW * TB, st + 1, page, false);
                 page = page_of(st + 2);
             }
-            const int kv0 = kv_tile(st) * PF_T;
-            const bool use = v0 + st * KW + kw < v1 && touches(kv0);  // wavefront-uniform
-            if (use) {
-                h8 x[KS];
-                load_k(cur, x);
-                softmax(scores(x), kv0, !inside(kv0));
-            }
+            const int v = nth(st);
+            const bool use = v0 + st * KW + kw < v1 && rows_here &&
+                             rw.touches(a, v, wfirst, wlast);  // wavefront-uniform
+            if (use) softmax(scores(cur), v, !rw.inside(a, v, wfirst, wlast));
             uint8_t *const vt = cur + KW * TB;
             // a step with a tile that some row of the workgroup sees in part
             bool cut = false;
 #pragma unroll
-            for (int k = 0; k < KW; ++k) {
-                const int p = rw.tile(min(v0 + st * KW + k, v1 - 1)) * PF_T;
-                cut |= !(p + PF_T - 1 <= first && (p > last - a.window || p + PF_T <= a.sinks));
-            }
+            for (int k = 0; k < KW; ++k)
+                cut |= !rw.inside(a, min(v0 + st * KW + k, v1 - 1), rw.first, rw.last);
             if (cut) {  // workgroup-uniform
                 if (any_bad(vt)) {
-                    if (use) meet_bad(vt, kv0);
+                    if (use) meet_bad(vt, v);
                     if (lane == 0) bad_step[st & 1] = 1;
                 }
                 __syncthreads();
@@ -539,80 +540,119 @@ k_attn_rows(RowsArgs a, RowsParts pt, int chunk_tiles) {
             if (use) weigh(vt);
         }
     } else {
-        for (int st = 0; st < steps; ++st) {
-            if (v0 + st * KW + kw >= v1) break;  // wavefront-uniform
-            const int kv0 = kv_tile(st) * PF_T;
-            const bool more = v0 + (st + 1) * KW + kw < v1, use = touches(kv0);
+        // (the workgroup's rows are the wavefront's: every tile of the walk touches them)
+        uint8_t *const vt = sb + KW * TB;
+        for (int v = v0 + kw, st = 0; v < v1; v += KW, ++st) {  // wavefront-uniform
+            const bool more = v + KW < v1, cut = !rw.inside(a, v, wfirst, wlast);
             // outstanding: this tile's K and V copies, in this order (a page's load may
             // stand anywhere: it only makes a wait longer)
             const int next = page;
             pf_wait<TIW>();  // K is in; V may still be on its way
-            h8 x[KS];
-            load_k(sb0, x);
+            const f16v s = scores(sb);
             pf_wait<TIW>();  // K has been read
             if (more) {
                 page = page_of(st + 2);
-                copy(a.k, sb0, st + 1, next, true);
+                copy(a.k, sb, st + 1, next, true);
             }
-            const bool cut = !inside(kv0);
-            if (use) softmax(scores(x), kv0, cut);
+            softmax(s, v, cut);
             if (more)
                 pf_wait<TIW>();  // V is in; the next K may still be on its way
             else
                 pf_wait<0>();
-            if (use) {
-                if (cut && any_bad(sb1)) {
-                    meet_bad(sb1, kv0);
-                    pf_wait<63>();  // (its reads are done)
-                    drop_bad(sb1);
-                    pf_wait<63>();
-                }
-                weigh(sb1);
+            if (cut && any_bad(vt)) {
+                meet_bad(vt, v);
+                pf_wait<63>();  // (its reads are done)
+                drop_bad(vt);
+                pf_wait<63>();
             }
+            weigh(vt);
             pf_wait<TIW>();  // V has been read
-            if (more) copy(a.v, sb1, st + 1, next, false);
+            if (more) copy(a.v, vt, st + 1, next, false);
         }
     }
-#pragma unroll
-    for (int dt = 0; dt < DT; ++dt) o[dt] += o2[dt] * (1.0f / RW_LO);
     lsum += swap32_f(lsum);
-    pf_wait<0>();  // no copy in flight (a wavefront without tiles never waited for its own)
-    __syncthreads();  // every wavefront is done with the stage buffers
 
     // lane (t, hh) holds O[row t][32 dt + 8 (r / 4) + 4 hh + r % 4] in o[dt][r]
-    {
-        float *mo = (float *)(wave < HALF_W ? sb0 : sb1) + (wave % HALF_W) * (PF_T * OROW);
-        if (hh == 0) {
-            mrg_m[wave][t] = m;
-            mrg_l[wave][t] = lsum;
+    if constexpr (KW == 1) {
+        // each lane its row's halves of 8: 16-byte stores, the Q8_0 of a block from the pair
+        // of lanes that holds it
+        const int lr = 32 * rt + t;
+        if (!whole) {
+            const size_t at = part_row(pt, a.kvheads, tile_id, g, chunk, min(lr, pt.rows - 1));
+            if (lr < rw.pairs) {
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                    for (int r4 = 0; r4 < 4; ++r4)
+                        *(f4 *)(pt.o + at * D + 32 * dt + 8 * r4 + 4 * hh) =
+                            (f4){o[dt][4 * r4], o[dt][4 * r4 + 1], o[dt][4 * r4 + 2],
+                                 o[dt][4 * r4 + 3]};
+                if (hh == 0) {
+                    pt.m[2 * at] = c;
+                    pt.m[2 * at + 1] = lsum;
+                }
+            }
+            return;
         }
+        const float inv = 1.0f / lsum;
+        const size_t off = ((size_t)myrow * a.qheads + myhead) * D;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) {
+            float y[16];
+#pragma unroll
+            for (int r = 0; r < 16; ++r) y[r] = prow < 0 ? 0.0f : o[dt][r] * inv;
+            uint32_t q[4];
+            uint16_t dbits;
+            int sum;
+            if (a.qs) quant_block_pair16(y, q, dbits, sum);  // every lane
+            if (lr >= rw.pairs) continue;
+#pragma unroll
+            for (int r4 = 0; r4 < 4; ++r4)
+                *(f4 *)(a.attn + off + 32 * dt + 8 * r4 + 4 * hh) =
+                    (f4){y[4 * r4], y[4 * r4 + 1], y[4 * r4 + 2], y[4 * r4 + 3]};
+            if (!a.qs) continue;
+#pragma unroll
+            for (int r4 = 0; r4 < 4; ++r4)
+                *(uint32_t *)(a.qs + off + 32 * dt + 8 * r4 + 4 * hh) = q[r4];
+            if (hh == 0) {
+                a.d[off / SI_QK + dt] = dbits;
+                if (a.bsum) a.bsum[off / SI_QK + dt] = (int16_t)sum;
+            }
+        }
+        return;
+    }
+    pf_wait<0>();  // no copy in flight (a wavefront without tiles never waited for its own)
+    __syncthreads();  // every wavefront is done with the stages
+    float *const mo = (float *)sb;  // [wavefront][row][OROW]
+    if (hh == 0 && KW > 1) {
+        mrg_m[wave][t] = c;
+        mrg_l[wave][t] = lsum;
+    }
+    if (32 * rt + t < rw.pairs)
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
             for (int r4 = 0; r4 < 4; ++r4)
-                *(f4 *)(mo + t * OROW + 32 * dt + 8 * r4 + 4 * hh) =
+                *(f4 *)(mo + (wave * PF_T + t) * OROW + 32 * dt + 8 * r4 + 4 * hh) =
                     (f4){o[dt][4 * r4], o[dt][4 * r4 + 1], o[dt][4 * r4 + 2], o[dt][4 * r4 + 3]};
-    }
     __syncthreads();
-    // a row's factors for its KW states, in mrg_m: 2^(unit (m_k - max)), over the sum
-    // where the results come from this workgroup alone
-    if (tid < rw.pairs) {
+    // a row's factors for its KW states, in mrg_m: 2^(c_k - largest), over the sum where
+    // the results come from this workgroup alone
+    if (tid < rw.pairs && KW > 1) {
         const int w0 = tid >> 5, tr = tid & 31;
-        const float u = row_unit[tid];
         float M = -INFINITY, l = 0.0f, f[KW];
 #pragma unroll
         for (int k = 0; k < KW; ++k) M = fmaxf(M, mrg_m[k * RT + w0][tr]);
         const float ref = M == -INFINITY ? 0.0f : M;
 #pragma unroll
         for (int k = 0; k < KW; ++k) {
-            f[k] = __builtin_amdgcn_exp2f((mrg_m[k * RT + w0][tr] - ref) * u);
+            f[k] = __builtin_amdgcn_exp2f(mrg_m[k * RT + w0][tr] - ref);
             l = fmaf(mrg_l[k * RT + w0][tr], f[k], l);
         }
         if (!whole) {
-            float *to = pt.m + 3 * part_row(pt, a.kvheads, tile_id, g, chunk, tid);
-            to[0] = M;
-            to[1] = l;
-            to[2] = u;
+            const size_t at = part_row(pt, a.kvheads, tile_id, g, chunk, tid);
+            pt.m[2 * at] = M;
+            pt.m[2 * at + 1] = l;
         }
         const float inv = whole ? 1.0f / l : 1.0f;
 #pragma unroll
@@ -627,9 +667,8 @@ k_attn_rows(RowsArgs a, RowsParts pt, int chunk_tiles) {
 #pragma unroll
         for (int k = 0; k < KW; ++k) {
             const int w = k * RT + w0;
-            const float *mo = (const float *)(w < HALF_W ? sb0 : sb1) + (w % HALF_W) * (PF_T * OROW);
-            const f4 v = *(const f4 *)(mo + tr * OROW + dd);
-            const float f = mrg_m[w][tr];
+            const f4 v = *(const f4 *)(mo + (w * PF_T + tr) * OROW + dd);
+            const float f = mrg_m[KW > 1 ? w : 0][tr];
 #pragma unroll
             for (int i = 0; i < 4; ++i) y[i] = fmaf(v[i], f, y[i]);
         }
@@ -660,17 +699,16 @@ __global__ void __launch_bounds__(RM_T) k_attn_rows_merge(RowsArgs a, RowsParts 
     const int n = (rw.ntiles + chunk_tiles - 1) / chunk_tiles;
     float M = -INFINITY;
 #pragma unroll 4
-    for (int c = 0; c < n; ++c)
-        M = fmaxf(M, pt.m[3 * part_row(pt, a.kvheads, tile_id, g, c, lr)]);
-    const float u = pt.m[3 * part_row(pt, a.kvheads, tile_id, g, 0, lr) + 2];
+    for (int k = 0; k < n; ++k)
+        M = fmaxf(M, pt.m[2 * part_row(pt, a.kvheads, tile_id, g, k, lr)]);
     const float ref = M == -INFINITY ? 0.0f : M;
     float l = 0.0f, y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 4
-    for (int c = 0; c < n; ++c) {
-        const size_t at = part_row(pt, a.kvheads, tile_id, g, c, lr);
-        const float f = __builtin_amdgcn_exp2f((pt.m[3 * at] - ref) * u);
+    for (int k = 0; k < n; ++k) {
+        const size_t at = part_row(pt, a.kvheads, tile_id, g, k, lr);
+        const float f = __builtin_amdgcn_exp2f(pt.m[2 * at] - ref);
         const f4 v = *(const f4 *)(pt.o + at * D + dd);
-        l = fmaf(pt.m[3 * at + 1], f, l);
+        l = fmaf(pt.m[2 * at + 1], f, l);
 #pragma unroll
         for (int i = 0; i < 4; ++i) y[i] = fmaf(v[i], f, y[i]);
     }
@@ -697,18 +735,18 @@ static RowsPlan rows_plan(const RowsArgs &a) {
     const long long pairs = (long long)a.max_new * per;
     p.one = pairs <= 64;
     p.rt = pairs <= 32 ? 1 : pairs <= 64 ? 2 : 4;
-    p.kw = p.rt == 4 ? 2 : 4;
+    p.kw = p.rt == 4 ? 1 : p.rt == 2 ? 2 : 4;
     const int rows = 32 * p.rt;
     p.tiles = p.one ? a.nseq : (int)((long long)a.max_rows * per / rows) + a.nseq;
     p.rows = (int)std::min<long long>(rows, pairs);
     // K/V tiles that a tile's rows can see: the sinks', and a window's of every row
     const long long span = std::min<long long>(a.max_ctx, (long long)a.window + rows / per + 1);
-    const int most = (int)std::min<long long>((a.max_ctx + PF_T - 1) / PF_T,
-                                              span / PF_T + 2 + (a.sinks + PF_T - 1) / PF_T);
+    const int most = (int)std::min<long long>((a.max_ctx + PF_T - 1) / PF_T, span / PF_T + 2) +
+                     (a.sinks + PF_T - 1) / PF_T;
     const long long base =
         (long long)a.kvheads *
         (p.one ? a.nseq : std::max<long long>(1, (long long)a.max_rows * per / rows));
-    const long long want = p.rt == 1 ? 512 : 256;
+    const long long want = 512;
     long long chunks = std::max(1LL, want / base);
     chunks = std::min<long long>(chunks, std::max(1, most / (2 * p.kw)));
     p.chunk_tiles = (int)((most + chunks - 1) / chunks);
@@ -719,7 +757,7 @@ static RowsPlan rows_plan(const RowsArgs &a) {
 size_t attn_rows_workspace(const RowsArgs &a) {
     const RowsPlan p = rows_plan(a);
     if (p.chunks == 1) return 0;
-    return (size_t)p.tiles * a.kvheads * p.chunks * p.rows * (a.hdim + 3) * sizeof(float);
+    return (size_t)p.tiles * a.kvheads * p.chunks * p.rows * (a.hdim + 2) * sizeof(float);
 }
 
 bool attn_rows_fits(const RowsArgs &a) {
@@ -733,9 +771,8 @@ void launch_attn_rows_paged(const RowsArgs &a, void *workspace, hipStream_t st) 
     RowsParts pt = {};
     pt.chunks = p.chunks;
     pt.rows = p.rows;
-    pt.blocks = (size_t)p.tiles * a.kvheads * p.chunks;
     pt.o = (float *)workspace;
-    pt.m = pt.o + pt.blocks * p.rows * a.hdim;
+    pt.m = pt.o + (size_t)p.tiles * a.kvheads * p.chunks * p.rows * a.hdim;
     const dim3 grid((unsigned)(p.tiles * a.kvheads * p.chunks)), block(p.rt * p.kw * 64);
     const bool page32 = a.pg.shift >= 5;
 #define CALL(DIM, RT, KW, ONE, P32) \
@@ -745,8 +782,8 @@ void launch_attn_rows_paged(const RowsArgs &a, void *workspace, hipStream_t st) 
     else CALL(DIM, RT, KW, ONE, false)
 #define DIMS(DIM)                                  \
     if (p.rt == 1) { PAGES(DIM, 1, 4, true); }     \
-    else if (p.rt == 2) { PAGES(DIM, 2, 4, true); } \
-    else { PAGES(DIM, 4, 2, false); }
+    else if (p.rt == 2) { PAGES(DIM, 2, 2, true); } \
+    else { PAGES(DIM, 4, 1, false); }
 #define MERGE(DIM, ONE)                                                                         \
     SI_LAUNCH((k_attn_rows_merge<DIM, ONE>),                                                    \
               dim3((unsigned)(p.tiles * a.kvheads), (p.rows * (DIM / 4) + RM_T - 1) / RM_T),    \
