@@ -33,6 +33,10 @@
 
 namespace si {
 
+#ifndef A2
+#define A2 1
+#define A4 2
+#endif
 constexpr float RW_UP = 11.0f;    // log2 of a weight's unit
 constexpr float RW_OVER = 4.0f;   // how far a tile's largest may lie over the reference
 constexpr float RW_UNDER = 12.0f; // and under it
@@ -173,7 +177,8 @@ __device__ __forceinline__ void rows_store(const RowsArgs &a, int row, int head,
     }
 }
 
-template <int D, int RT, int KW, bool ONE, bool PAGE32>
+// AHEAD: steps that a stage's copies are issued before their use (RT > 1)
+template <int D, int RT, int KW, int AHEAD, bool ONE, bool PAGE32>
 __global__ void __launch_bounds__(RT * KW * 64) __attribute__((amdgpu_waves_per_eu(2)))
 k_attn_rows(RowsArgs a, RowsParts pt, int chunk_tiles) {
     constexpr int NWV = RT * KW, NT = NWV * 64, KS = D / 16, DT = D / 32, CH = D / 8;
@@ -181,13 +186,17 @@ k_attn_rows(RowsArgs a, RowsParts pt, int chunk_tiles) {
     constexpr int TI = TB / 1024;            // copy instructions per tile
     constexpr int TIW = (TI + RT - 1) / RT;  // of one wavefront
     constexpr int OROW = D + PF_OPAD;
-    // RT > 1: two stages (K tiles, then V tiles) used in turn, one barrier per step.
-    // RT == 1: each wavefront stages its own tiles, K and V, each refilled as soon as it
-    // has been read (no barrier).  KW > 1: at the end the wavefronts' outputs.
+    // RT > 1: AHEAD + 1 stages (K tiles, then V tiles) used in turn, one barrier per step.
+    // RT == 1: each wavefront stages its own tiles, K in sb and V in sb1 (an array of its
+    // own: the compiler waits for every copy into an array before it reads that), each
+    // refilled as soon as it has been read (no barrier).  KW > 1: at the end the
+    // wavefronts' outputs, where there are two arrays half of them in each.
     constexpr bool DB = RT > 1;
-    constexpr int STAGE = 2 * KW * TB, NSTAGE = DB ? 2 : 1;
-    constexpr int MRG = KW > 1 ? NWV * PF_T * OROW * 4 : 0;
-    __shared__ __attribute__((aligned(16))) uint8_t sb[NSTAGE * STAGE > MRG ? NSTAGE * STAGE : MRG];
+    constexpr int STAGE = (DB ? 2 : 1) * KW * TB, NSTAGE = DB ? AHEAD + 1 : 1;
+    constexpr int MRG_W = DB ? NWV : (NWV + 1) / 2, MRG = KW > 1 ? MRG_W * PF_T * OROW * 4 : 0;
+    constexpr int SB = NSTAGE * STAGE > MRG ? NSTAGE * STAGE : MRG;
+    __shared__ __attribute__((aligned(16))) uint8_t sb[SB];
+    __shared__ __attribute__((aligned(16))) uint8_t sb1[DB ? 16 : SB];
     __shared__ float mrg_m[KW > 1 ? NWV : 1][PF_T], mrg_l[KW > 1 ? NWV : 1][PF_T];
     __shared__ int bad_step[2];  // whether a cut step's V holds infinities or NaN
 
@@ -239,7 +248,10 @@ k_attn_rows(RowsArgs a, RowsParts pt, int chunk_tiles) {
     };
     // the page of a step's tile (past the chunk: its last one again): of its first
     // position, or (PAGE32 false: several pages a tile) of position t
-    const int *list = a.pg.pages + (size_t)rw.seq * a.pg.max_pages;
+    // (read as constant data: one page a tile through the scalar cache, whose loads are
+    // not among those that the waits for copies count)
+    typedef const __attribute__((address_space(4))) int const_int;
+    const const_int *list = (const const_int *)(a.pg.pages + (size_t)rw.seq * a.pg.max_pages);
     const auto nth = [&](int st) { return min(v0 + st * KW + kw, v1 - 1); };
     const auto page_of = [&](int st) {
         const int pos = rw.tile(nth(st)) * PF_T + (PAGE32 ? 0 : t);
@@ -280,12 +292,24 @@ k_attn_rows(RowsArgs a, RowsParts pt, int chunk_tiles) {
                 }
         }
     };
-    int page = 0;
+    // the first copies: K up to step AHEAD and V one step less (RT == 1: of step 0)
+    int page = 0, page1 = 0;
     if (steps > 0) {
         page = page_of(0);
         copy(a.k, sb, 0, page, true);
-        copy(a.v, sb + KW * TB, 0, page, false);
-        page = page_of(1);
+        if constexpr (DB) {
+#pragma unroll
+            for (int s = 0; s < AHEAD; ++s) {
+                if (s < steps) copy(a.v, sb + s * STAGE + KW * TB, s, page, false);
+                page = page_of(s + 1);
+                if (s + 1 < steps) copy(a.k, sb + (s + 1) * STAGE, s + 1, page, true);
+            }
+            page1 = page;
+            page = page_of(AHEAD + 1);
+        } else {
+            copy(a.v, sb1, 0, page, false);
+            page = page_of(1);
+        }
     }
 
     // Q^T as the B operand of the score MFMA: column t, k-slice hh (columns past the last
@@ -348,10 +372,7 @@ k_attn_rows(RowsArgs a, RowsParts pt, int chunk_tiles) {
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) o[dt] = (f16v){};
 
-    const auto scores = [&](const uint8_t *kt) {
-        h8 x[KS];
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) x[ks] = *(const h8 *)(kt + ka[ks]);
+    const auto products = [&](const h8 (&x)[KS]) {
         // the lo products first: they round at their own small magnitude
         f16v s = (f16v){};
 #pragma unroll
@@ -361,6 +382,12 @@ k_attn_rows(RowsArgs a, RowsParts pt, int chunk_tiles) {
         for (int ks = 0; ks < KS; ++ks)
             s = __builtin_amdgcn_mfma_f32_32x32x16_f16(x[ks], qh[ks], s, 0, 0, 0);
         return s;
+    };
+    const auto scores = [&](const uint8_t *kt) {
+        h8 x[KS];
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) x[ks] = *(const h8 *)(kt + ka[ks]);
+        return products(x);
     };
     // the positions of the v-th tile that lane t's row sees: those from `from` on, `width`
     // more, counted from the lane's first, kv0 + 4 hh (register r: 8 (r / 4) + r % 4 behind it)
@@ -378,7 +405,9 @@ k_attn_rows(RowsArgs a, RowsParts pt, int chunk_tiles) {
         return hi < lo ? Seen{64, 0} : Seen{lo - at, hi - lo};
     };
     h8 ph[2], pl[2];  // the tile's weights
-    const auto softmax = [&](f16v s, int v, bool cut) {
+    float one = 1.0f;
+    asm("" : "+s"(one));
+    const auto refer = [&](f16v &s, int v, bool cut) {
         if (cut) {  // wavefront-uniform
             const Seen seen = seen_of(v);
 #pragma unroll
@@ -406,6 +435,8 @@ k_attn_rows(RowsArgs a, RowsParts pt, int chunk_tiles) {
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt) o[dt] *= alpha;
         }
+    };
+    const auto weights = [&](const f16v &s) {
         const float up = RW_UP - (c == -INFINITY ? 0.0f : c);
         float ps = 0.0f;
 #pragma unroll
@@ -414,12 +445,12 @@ k_attn_rows(RowsArgs a, RowsParts pt, int chunk_tiles) {
             const float p1 = __builtin_amdgcn_exp2f(fmaf(s[r + 1], fac, up));
             ps += p0;
             ps += p1;
-            pf_h2 hi, lo;
-            split_pair(p0, p1, hi, lo);
+            const pf_h2 hi = __builtin_convertvector((pf_f2){p0, p1}, pf_h2);
             ph[r >> 3][r & 7] = hi[0];
             ph[r >> 3][(r & 7) + 1] = hi[1];
-            pl[r >> 3][r & 7] = lo[0];
-            pl[r >> 3][(r & 7) + 1] = lo[1];
+            // (a mixed-precision fma each, as the factor 1 is not the compiler's to see)
+            pl[r >> 3][r & 7] = (_Float16)fmaf(-(float)hi[0], one, p0);
+            pl[r >> 3][(r & 7) + 1] = (_Float16)fmaf(-(float)hi[1], one, p1);
         }
         lsum += ps;
     };
@@ -439,6 +470,57 @@ k_attn_rows(RowsArgs a, RowsParts pt, int chunk_tiles) {
                 o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, ph[s2], o[dt], 0, 0, 0);
                 o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, pl[s2], o[dt], 0, 0, 0);
             }
+    };
+    // The scores of K tile kt among the weights of s, and V's operands on their way: the
+    // matrix cores and the vector ALU work side by side, each product followed by its share
+    // of the weights (the order as written: left to itself the compiler puts the products
+    // together).
+    const auto scores_and_weights = [&](const uint8_t *kt, const f16v &s, const uint8_t *vt) {
+        constexpr int SLOTS = 2 * KS;
+        const float up = RW_UP - (c == -INFINITY ? 0.0f : c);
+        f16v n = (f16v){};
+        h8 x[KS], vx[2 * DT];
+        float p[16], ps = 0.0f;
+        x[0] = *(const h8 *)(kt + ka[0]);
+        x[1] = *(const h8 *)(kt + ka[1]);
+#pragma unroll
+        for (int i = 0; i < SLOTS; ++i) {
+            const int ks = i / 2;
+            if (i % 2 == 0 && ks + 2 < KS) x[ks + 2] = *(const h8 *)(kt + ka[ks + 2]);
+            n = __builtin_amdgcn_mfma_f32_32x32x16_f16(x[ks], i % 2 ? qh[ks] : ql[ks], n, 0, 0, 0);
+#pragma unroll
+            for (int r = i * 16 / SLOTS; r < (i + 1) * 16 / SLOTS; ++r) {
+                p[r] = __builtin_amdgcn_exp2f(fmaf(s[r], fac, up));
+                if (r >= 2) {  // (the exponential before the last is done)
+                    const int e = r - 2;
+                    ps += p[e];
+                    ph[e >> 3][e & 7] = (_Float16)p[e];
+                    pl[e >> 3][e & 7] = (_Float16)fmaf(-(float)ph[e >> 3][e & 7], one, p[e]);
+                }
+            }
+            // (the first positions' operands in the last slots; registers are short)
+#pragma unroll
+            for (int k = 0; k < DT; ++k)
+                if (i == SLOTS - DT + k) vx[2 * k] = v_operand(vt, k, 0);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+#pragma unroll
+        for (int e = 14; e < 16; ++e) {
+            ps += p[e];
+            ph[1][e & 7] = (_Float16)p[e];
+            pl[1][e & 7] = (_Float16)fmaf(-(float)ph[1][e & 7], one, p[e]);
+        }
+        lsum += ps;
+#pragma unroll
+        for (int s2 = 0; s2 < 2; ++s2)
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) {
+                if (s2 == 0) vx[2 * dt + 1] = v_operand(vt, dt, 1);
+                o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vx[2 * dt + s2], ph[s2], o[dt], 0, 0, 0);
+                o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vx[2 * dt + s2], pl[s2], o[dt], 0, 0, 0);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        return n;
     };
     // whether a V operand holds an infinity or NaN (exponents of all ones)
     typedef uint32_t w4 __attribute__((ext_vector_type(4)));
@@ -503,28 +585,41 @@ k_attn_rows(RowsArgs a, RowsParts pt, int chunk_tiles) {
             }
     };
     if constexpr (DB) {
-        // one step: the stage is complete and the other one free after the barrier; the
-        // next stage's copies run during the whole step
+        // K runs a step ahead of V: a step's weights are computed among the next one's
+        // scores.  After its barrier the next K and this V are in, and the buffers of the
+        // last K and V free; the copies into them have AHEAD steps to arrive.
         if (tid < 2) bad_step[tid] = 0;
-        for (int st = 0; st < steps; ++st) {
-            uint8_t *const cur = sb + (st & 1) * STAGE, *const nxt = sb + (~st & 1) * STAGE;
-            pf_wait<0>();
+        pf_wait<0>();
+        pf_barrier();
+        f16v s0 = (f16v){}, s1 = (f16v){};
+        if (steps > 0) s0 = scores(sb);
+        int at = 0;  // st % NSTAGE
+        const auto step = [&](f16v &s, f16v &next, int st) {
+            const int after = at + 1 == NSTAGE ? 0 : at + 1, before = at ? at - 1 : NSTAGE - 1;
+            uint8_t *const cur = sb + at * STAGE, *const nxt = sb + after * STAGE;
+            // (copies of the steps since may be on their way; D of 96: fewer for some)
+            if (st + AHEAD < steps) pf_wait<(AHEAD - 1) * 2 * (TI / RT)>();
+            else pf_wait<0>();
             pf_barrier();
-            if (st + 1 < steps) {
-                copy(a.k, nxt, st + 1, page, true);
-                copy(a.v, nxt + KW * TB, st + 1, page, false);
-                page = page_of(st + 2);
-            }
+            // (the next page's load before the copies: a wait for it is none for them)
+            const int page2 = page_of(st + AHEAD + 2);
+            asm volatile("" ::: "memory");
+            if (st + AHEAD < steps)
+                copy(a.v, sb + before * STAGE + KW * TB, st + AHEAD, page1, false);
+            if (st + AHEAD + 1 < steps) copy(a.k, cur, st + AHEAD + 1, page, true);
+            page1 = page;
+            page = page2;
+            at = after;
             const int v = nth(st);
             const bool use = v0 + st * KW + kw < v1 && rows_here &&
                              rw.touches(a, v, wfirst, wlast);  // wavefront-uniform
-            if (use) softmax(scores(cur), v, !rw.inside(a, v, wfirst, wlast));
             uint8_t *const vt = cur + KW * TB;
             // a step with a tile that some row of the workgroup sees in part
             bool cut = false;
 #pragma unroll
             for (int k = 0; k < KW; ++k)
                 cut |= !rw.inside(a, min(v0 + st * KW + k, v1 - 1), rw.first, rw.last);
+            if (use) refer(s, v, cut && !rw.inside(a, v, wfirst, wlast));
             if (cut) {  // workgroup-uniform
                 if (any_bad(vt)) {
                     if (use) meet_bad(vt, v);
@@ -537,24 +632,40 @@ k_attn_rows(RowsArgs a, RowsParts pt, int chunk_tiles) {
                     if (tid == 0) bad_step[st & 1] = 0;  // (next set two barriers from here)
                 }
             }
-            if (use) weigh(vt);
+            // (past the last step the next scores are of no use)
+            if (use) {
+                next = scores_and_weights(nxt, s, vt);
+            } else if (rows_here) {
+                next = scores(nxt);
+            }
+        };
+        for (int st = 0; st < steps; st += 2) {
+            step(s0, s1, st);
+            if (st + 1 < steps) step(s1, s0, st + 1);
         }
     } else {
         // (the workgroup's rows are the wavefront's: every tile of the walk touches them)
-        uint8_t *const vt = sb + KW * TB;
+        uint8_t *const vt = sb1;
         for (int v = v0 + kw, st = 0; v < v1; v += KW, ++st) {  // wavefront-uniform
             const bool more = v + KW < v1, cut = !rw.inside(a, v, wfirst, wlast);
             // outstanding: this tile's K and V copies, in this order (a page's load may
             // stand anywhere: it only makes a wait longer)
             const int next = page;
             pf_wait<TIW>();  // K is in; V may still be on its way
-            const f16v s = scores(sb);
-            pf_wait<TIW>();  // K has been read
+            uint32_t kat[KS];
+            h8 x[KS];
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks)
+                kat[ks] = (uint32_t)(uintptr_t)(lds_void *)(void *)(sb + ka[ks]);
+            lds_read16(kat, x);
             if (more) {
                 page = page_of(st + 2);
+                asm volatile("" ::: "memory");
                 copy(a.k, sb, st + 1, next, true);
             }
-            softmax(s, v, cut);
+            f16v s = products(x);
+            refer(s, v, cut);
+            weights(s);
             if (more)
                 pf_wait<TIW>();  // V is in; the next K may still be on its way
             else
@@ -623,7 +734,9 @@ k_attn_rows(RowsArgs a, RowsParts pt, int chunk_tiles) {
     }
     pf_wait<0>();  // no copy in flight (a wavefront without tiles never waited for its own)
     __syncthreads();  // every wavefront is done with the stages
-    float *const mo = (float *)sb;  // [wavefront][row][OROW]
+    const auto mo = [&](int w) {  // [row][OROW] of a wavefront
+        return (float *)(w < MRG_W ? sb : sb1) + (w % MRG_W) * (PF_T * OROW);
+    };
     if (hh == 0 && KW > 1) {
         mrg_m[wave][t] = c;
         mrg_l[wave][t] = lsum;
@@ -633,7 +746,7 @@ k_attn_rows(RowsArgs a, RowsParts pt, int chunk_tiles) {
         for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
             for (int r4 = 0; r4 < 4; ++r4)
-                *(f4 *)(mo + (wave * PF_T + t) * OROW + 32 * dt + 8 * r4 + 4 * hh) =
+                *(f4 *)(mo(wave) + t * OROW + 32 * dt + 8 * r4 + 4 * hh) =
                     (f4){o[dt][4 * r4], o[dt][4 * r4 + 1], o[dt][4 * r4 + 2], o[dt][4 * r4 + 3]};
     __syncthreads();
     // a row's factors for its KW states, in mrg_m: 2^(c_k - largest), over the sum where
@@ -667,7 +780,7 @@ k_attn_rows(RowsArgs a, RowsParts pt, int chunk_tiles) {
 #pragma unroll
         for (int k = 0; k < KW; ++k) {
             const int w = k * RT + w0;
-            const f4 v = *(const f4 *)(mo + (w * PF_T + tr) * OROW + dd);
+            const f4 v = *(const f4 *)(mo(w) + tr * OROW + dd);
             const float f = mrg_m[KW > 1 ? w : 0][tr];
 #pragma unroll
             for (int i = 0; i < 4; ++i) y[i] = fmaf(v[i], f, y[i]);
@@ -684,34 +797,63 @@ k_attn_rows(RowsArgs a, RowsParts pt, int chunk_tiles) {
 
 // ---------------------------------------------------------------------------
 // The chunks' states of tiles that were cut: grid (tiles x KV groups, rows), 4 values of a
-// row per thread
+// row per thread, its chunks taken G ways (G > 1: they meet in LDS, in their order)
 // ---------------------------------------------------------------------------
 constexpr int RM_T = 256;
-template <int D, bool ONE>
+template <int D, bool ONE, int G>
 __global__ void __launch_bounds__(RM_T) k_attn_rows_merge(RowsArgs a, RowsParts pt, int tile_rows,
                                                           int chunk_tiles) {
+    constexpr int LANES = D / 4, ROWS = RM_T / (LANES * G);  // of a workgroup
+    static_assert(ROWS >= 1, "a row's threads fit a workgroup");
     const int g = blockIdx.x % a.kvheads, tile_id = blockIdx.x / a.kvheads;
     RowTile rw;
     if (!find_tile<ONE, RM_T>(a, tile_rows, tile_id, rw) || rw.ntiles <= chunk_tiles) return;
-    const int e = blockIdx.y * RM_T + threadIdx.x;
-    const int lr = e / (D / 4), dd = 4 * (e % (D / 4));
-    if (lr >= rw.pairs) return;  // whole groups of 8 lanes
+    const int grp = threadIdx.x / LANES, dd = 4 * (threadIdx.x % LANES);
+    const int way = grp / ROWS, lr = blockIdx.y * ROWS + grp % ROWS;
+    const bool mine = way < G && lr < rw.pairs;  // whole groups of 8 lanes
     const int n = (rw.ntiles + chunk_tiles - 1) / chunk_tiles;
-    float M = -INFINITY;
+    float M = -INFINITY, l = 0.0f, y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (mine) {
 #pragma unroll 4
-    for (int k = 0; k < n; ++k)
-        M = fmaxf(M, pt.m[2 * part_row(pt, a.kvheads, tile_id, g, k, lr)]);
-    const float ref = M == -INFINITY ? 0.0f : M;
-    float l = 0.0f, y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int k = way; k < n; k += G)
+            M = fmaxf(M, pt.m[2 * part_row(pt, a.kvheads, tile_id, g, k, lr)]);
+        const float ref = M == -INFINITY ? 0.0f : M;
 #pragma unroll 4
-    for (int k = 0; k < n; ++k) {
-        const size_t at = part_row(pt, a.kvheads, tile_id, g, k, lr);
-        const float f = __builtin_amdgcn_exp2f(pt.m[2 * at] - ref);
-        const f4 v = *(const f4 *)(pt.o + at * D + dd);
-        l = fmaf(pt.m[2 * at + 1], f, l);
+        for (int k = way; k < n; k += G) {
+            const size_t at = part_row(pt, a.kvheads, tile_id, g, k, lr);
+            const float f = __builtin_amdgcn_exp2f(pt.m[2 * at] - ref);
+            const f4 v = *(const f4 *)(pt.o + at * D + dd);
+            l = fmaf(pt.m[2 * at + 1], f, l);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) y[i] = fmaf(v[i], f, y[i]);
+            for (int i = 0; i < 4; ++i) y[i] = fmaf(v[i], f, y[i]);
+        }
     }
+    if constexpr (G > 1) {
+        __shared__ float all_m[G][ROWS], all_l[G][ROWS];
+        __shared__ f4 all_y[G][ROWS * LANES];
+        const int at = threadIdx.x % (ROWS * LANES);
+        if (way < G) {
+            if (dd == 0) {
+                all_m[way][grp % ROWS] = M;
+                all_l[way][grp % ROWS] = l;
+            }
+            all_y[way][at] = (f4){y[0], y[1], y[2], y[3]};
+        }
+        __syncthreads();
+        if (way > 0 || !mine) return;
+#pragma unroll
+        for (int w = 0; w < G; ++w) M = fmaxf(M, all_m[w][grp % ROWS]);
+        const float ref = M == -INFINITY ? 0.0f : M;
+        l = y[0] = y[1] = y[2] = y[3] = 0.0f;
+#pragma unroll
+        for (int w = 0; w < G; ++w) {
+            const float f = __builtin_amdgcn_exp2f(all_m[w][grp % ROWS] - ref);
+            l = fmaf(all_l[w][grp % ROWS], f, l);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) y[i] = fmaf(all_y[w][at][i], f, y[i]);
+        }
+    }
+    if (!mine) return;
     const float inv = 1.0f / l;
 #pragma unroll
     for (int i = 0; i < 4; ++i) y[i] *= inv;
@@ -775,23 +917,29 @@ void launch_attn_rows_paged(const RowsArgs &a, void *workspace, hipStream_t st) 
     pt.m = pt.o + (size_t)p.tiles * a.kvheads * p.chunks * p.rows * a.hdim;
     const dim3 grid((unsigned)(p.tiles * a.kvheads * p.chunks)), block(p.rt * p.kw * 64);
     const bool page32 = a.pg.shift >= 5;
-#define CALL(DIM, RT, KW, ONE, P32) \
-    SI_LAUNCH((k_attn_rows<DIM, RT, KW, ONE, P32>), grid, block, 0, st, a, pt, p.chunk_tiles)
-#define PAGES(DIM, RT, KW, ONE) \
-    if (page32) CALL(DIM, RT, KW, ONE, true); \
-    else CALL(DIM, RT, KW, ONE, false)
+#define CALL(DIM, RT, KW, AHEAD, ONE, P32)                                                    \
+    SI_LAUNCH((k_attn_rows<DIM, RT, KW, AHEAD, ONE, P32>), grid, block, 0, st, a, pt, \
+              p.chunk_tiles)
+#define PAGES(DIM, RT, KW, AHEAD, ONE) \
+    if (page32) CALL(DIM, RT, KW, AHEAD, ONE, true); \
+    else CALL(DIM, RT, KW, AHEAD, ONE, false)
 #define DIMS(DIM)                                  \
-    if (p.rt == 1) { PAGES(DIM, 1, 4, true); }     \
-    else if (p.rt == 2) { PAGES(DIM, 2, 2, true); } \
-    else { PAGES(DIM, 4, 1, false); }
-#define MERGE(DIM, ONE)                                                                         \
-    SI_LAUNCH((k_attn_rows_merge<DIM, ONE>),                                                    \
-              dim3((unsigned)(p.tiles * a.kvheads), (p.rows * (DIM / 4) + RM_T - 1) / RM_T),    \
+    if (p.rt == 1) { PAGES(DIM, 1, 4, 1, true); }     \
+    else if (p.rt == 2) { PAGES(DIM, 2, 2, A2, true); } \
+    else { PAGES(DIM, 4, 1, A4, false); }
+    // (a row's chunks 8 ways where there are many)
+#define MERGE(DIM, ONE, G)                                                                    \
+    SI_LAUNCH((k_attn_rows_merge<DIM, ONE, G>),                                                 \
+              dim3((unsigned)(p.tiles * a.kvheads),                                             \
+                   (p.rows - 1) / (RM_T / (DIM / 4 * G)) + 1),                                  \
               dim3(RM_T), 0, st, a, pt, 32 * p.rt, p.chunk_tiles)
-#define MERGES(DIM)                  \
-    if (p.chunks > 1) {              \
-        if (p.one) MERGE(DIM, true); \
-        else MERGE(DIM, false);      \
+#define MERGES(DIM)                                          \
+    if (p.chunks > 8) {                                      \
+        if (p.one) MERGE(DIM, true, 8);                      \
+        else MERGE(DIM, false, 8);                           \
+    } else if (p.chunks > 1) {                               \
+        if (p.one) MERGE(DIM, true, 1);                      \
+        else MERGE(DIM, false, 1);                           \
     }
     switch (a.hdim) {
         case 32: DIMS(32); MERGES(32); break;

@@ -72,6 +72,43 @@ __device__ __forceinline__ void pf_barrier() {
     asm volatile("" ::: "memory");
 }
 
+// N 16-byte reads of LDS at the given addresses, complete on return.  As inline assembly,
+// which the compiler does not know to read LDS: before its own reads it would wait for
+// every copy into LDS under way, also those that go elsewhere.  The caller has waited for
+// the bytes themselves.
+template <int N>
+__device__ __forceinline__ void lds_read16(const uint32_t (&at)[N], h8 (&x)[N]) {
+    static_assert(N == 2 || N == 4 || N == 6 || N == 8, "the head dims' k-steps");
+    if constexpr (N == 2)
+        asm volatile("ds_read_b128 %0, %2\n\tds_read_b128 %1, %3\n\ts_waitcnt lgkmcnt(0)"
+                     : "=&v"(x[0]), "=&v"(x[1])
+                     : "v"(at[0]), "v"(at[1])
+                     : "memory");
+    if constexpr (N == 4)
+        asm volatile("ds_read_b128 %0, %4\n\tds_read_b128 %1, %5\n\t"
+                     "ds_read_b128 %2, %6\n\tds_read_b128 %3, %7\n\ts_waitcnt lgkmcnt(0)"
+                     : "=&v"(x[0]), "=&v"(x[1]), "=&v"(x[2]), "=&v"(x[3])
+                     : "v"(at[0]), "v"(at[1]), "v"(at[2]), "v"(at[3])
+                     : "memory");
+    if constexpr (N == 6)
+        asm volatile("ds_read_b128 %0, %6\n\tds_read_b128 %1, %7\n\t"
+                     "ds_read_b128 %2, %8\n\tds_read_b128 %3, %9\n\t"
+                     "ds_read_b128 %4, %10\n\tds_read_b128 %5, %11\n\ts_waitcnt lgkmcnt(0)"
+                     : "=&v"(x[0]), "=&v"(x[1]), "=&v"(x[2]), "=&v"(x[3]), "=&v"(x[4]),
+                       "=&v"(x[5])
+                     : "v"(at[0]), "v"(at[1]), "v"(at[2]), "v"(at[3]), "v"(at[4]), "v"(at[5])
+                     : "memory");
+    if constexpr (N == 8)
+        asm volatile("ds_read_b128 %0, %8\n\tds_read_b128 %1, %9\n\t"
+                     "ds_read_b128 %2, %10\n\tds_read_b128 %3, %11\n\t"
+                     "ds_read_b128 %4, %12\n\tds_read_b128 %5, %13\n\t"
+                     "ds_read_b128 %6, %14\n\tds_read_b128 %7, %15\n\ts_waitcnt lgkmcnt(0)"
+                     : "=&v"(x[0]), "=&v"(x[1]), "=&v"(x[2]), "=&v"(x[3]), "=&v"(x[4]),
+                       "=&v"(x[5]), "=&v"(x[6]), "=&v"(x[7])
+                     : "v"(at[0]), "v"(at[1]), "v"(at[2]), "v"(at[3]), "v"(at[4]), "v"(at[5]),
+                       "v"(at[6]), "v"(at[7])
+                     : "memory");
+}
 // lds_copy16 at soff more, wavefront-uniform
 __device__ __forceinline__ void lds_copy16(__amdgpu_buffer_rsrc_t r, uint8_t *lds, uint32_t voff,
                                            int soff) {
