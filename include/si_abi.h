@@ -442,7 +442,7 @@ int si_kv_copy_pages(void *const *pools, int npools, size_t page_bytes, int npag
  * 237-281).  A step's rows (a token, drafted tokens or a prompt's piece of each of
  * nseq sequences, in sequence order) run over a paged fp16 cache, with the lengths,
  * the page lists and the free pages in device memory, so that a captured step needs
- * no host.  Per sequence start[i] .. start[i+1] - 1 are its rows and ctx[i] its
+ * no host.  Per sequence (at most 65535) start[i] .. start[i+1] - 1 are its rows and ctx[i] its
  * positions with them; per row seq, pos and slot (pool row, page * page_size +
  * offset) say where it belongs, -1 each behind the last row.  Rows there, up to
  * max_rows (fewer than 2^24), are left as they are by every call.

@@ -1866,10 +1866,10 @@ int si_kv_copy_pages(void *const *pools, int npools, size_t page_bytes, int npag
 // ---------------------------------------------------------------------------
 // A step whose sequences bring any number of rows each (si_step.hip, si_rows.hip)
 // ---------------------------------------------------------------------------
-constexpr int kMaxRows = (1 << 24) - 1, kMaxSeqs = (1 << 20);
+constexpr int kMaxRows = (1 << 24) - 1, kMaxSeqs = 65535;
 
 static int step_sizes(const char *what, int nseq, int max_rows, int window, int sinks) {
-    SI_REQUIRE(nseq >= 0 && nseq <= kMaxSeqs, "%s: nseq %d outside 0..2^20", what, nseq);
+    SI_REQUIRE(nseq >= 0 && nseq <= kMaxSeqs, "%s: nseq %d outside 0..65535", what, nseq);
     SI_REQUIRE(max_rows >= 0 && max_rows <= kMaxRows, "%s: max_rows %d outside 0..2^24 - 1", what,
                max_rows);
     SI_REQUIRE(window >= 1 && sinks >= 0, "%s: bad window %d / sinks %d", what, window, sinks);

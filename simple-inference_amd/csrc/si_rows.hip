@@ -25,6 +25,7 @@
 // there are looked at: 0 x infinity would be NaN.  Only if one is not finite, the rows
 // that see it are found first (exact counts, by the matrix cores), get their infinity or
 // NaN, and the tile in LDS has zeros in such places from then on.
+#include <limits.h>
 #include <algorithm>
 
 #include "si_device.hpp"
@@ -33,9 +34,11 @@
 
 namespace si {
 
-#ifndef A2
-#define A2 1
-#define A4 2
+#ifndef ONE1
+#define ONE1 256
+#define ONE2 512
+#define MULTI 256
+#define WGSLOTS 512
 #endif
 constexpr float RW_UP = 11.0f;    // log2 of a weight's unit
 constexpr float RW_OVER = 4.0f;   // how far a tile's largest may lie over the reference
@@ -98,8 +101,8 @@ __device__ __forceinline__ void row_tile(const RowsArgs &a, int tile_rows, int i
 }
 
 // Tile number `tile` of the call: one a sequence (ONE: max_new rows fill no more), or the
-// sequences' tiles one after another, found by a prefix sum over the sequences.  Every
-// thread of the workgroup; false past the last.
+// sequences' tiles one after another, the last first (a prompt's last rows see most), found
+// by a prefix sum over the sequences.  Every thread of the workgroup; false past the last.
 template <bool ONE, int NT>
 __device__ __forceinline__ bool find_tile(const RowsArgs &a, int tile_rows, int tile, RowTile &t) {
     if constexpr (ONE) {
@@ -112,6 +115,12 @@ __device__ __forceinline__ bool find_tile(const RowsArgs &a, int tile_rows, int 
             int r, p;
             return (seq_rows(a, i, r, p) * per + tile_rows - 1) / tile_rows;
         };
+        if (a.nseq == 1) {  // (its tiles are the call's)
+            const int k = tiles(0) - 1 - tile;
+            if (k < 0) return false;
+            row_tile(a, tile_rows, 0, k, t);
+            return true;
+        }
         const int each = (a.nseq + NT - 1) / NT;
         const int i0 = min(tid * each, a.nseq), i1 = min(i0 + each, a.nseq);
         int sum = 0;
@@ -121,11 +130,15 @@ __device__ __forceinline__ bool find_tile(const RowsArgs &a, int tile_rows, int 
             const int y = __shfl_up(x, d, 64);
             if ((tid & 63) >= d) x += y;
         }
-        if (tid == 0) found[0] = -1;
         if ((tid & 63) == 63) red[tid >> 6] = x;
         __syncthreads();
-        int base = x - sum;
-        for (int w = 0; w < (tid >> 6); ++w) base += red[w];
+        int base = x - sum, total = 0;
+        for (int w = 0; w < NT / 64; ++w) {
+            if (w < (tid >> 6)) base += red[w];
+            total += red[w];
+        }
+        tile = total - 1 - tile;
+        if (tile < 0) return false;
         if (tile >= base && tile < base + sum)
             for (int i = i0; i < i1; ++i) {
                 const int n = tiles(i);
@@ -137,10 +150,9 @@ __device__ __forceinline__ bool find_tile(const RowsArgs &a, int tile_rows, int 
                 base += n;
             }
         __syncthreads();
-        if (found[0] < 0) return false;
         row_tile(a, tile_rows, __builtin_amdgcn_readfirstlane(found[0]),
                  __builtin_amdgcn_readfirstlane(found[1]), t);
-        return t.pairs > 0;
+        return true;
     }
 }
 
@@ -150,12 +162,14 @@ __device__ __forceinline__ bool find_tile(const RowsArgs &a, int tile_rows, int 
 // ---------------------------------------------------------------------------
 struct RowsParts {
     float *o, *m;
-    int chunks, rows;  // rows of a block that may be used
+    int rows;         // rows of a block that may be used
+    int whole_tiles;  // the call's first tiles, which are not cut
+    int chunks, chunk_tiles;  // of the others
 };
 
 __device__ __forceinline__ size_t part_row(const RowsParts &pt, int kvheads, int tile, int g,
                                            int chunk, int row) {
-    return (((size_t)tile * kvheads + g) * pt.chunks + chunk) * pt.rows + row;
+    return (((size_t)(tile - pt.whole_tiles) * kvheads + g) * pt.chunks + chunk) * pt.rows + row;
 }
 
 // 4 values of a row's head (8 lanes hold a Q8_0 block), zeros before position 0
@@ -180,12 +194,13 @@ __device__ __forceinline__ void rows_store(const RowsArgs &a, int row, int head,
 // AHEAD: steps that a stage's copies are issued before their use (RT > 1)
 template <int D, int RT, int KW, int AHEAD, bool ONE, bool PAGE32>
 __global__ void __launch_bounds__(RT * KW * 64) __attribute__((amdgpu_waves_per_eu(2)))
-k_attn_rows(RowsArgs a, RowsParts pt, int chunk_tiles) {
+k_attn_rows(RowsArgs a, RowsParts pt) {
     constexpr int NWV = RT * KW, NT = NWV * 64, KS = D / 16, DT = D / 32, CH = D / 8;
     constexpr int TB = PF_T * D * 2;         // bytes of a K (or V) tile
     constexpr int TI = TB / 1024;            // copy instructions per tile
     constexpr int TIW = (TI + RT - 1) / RT;  // of one wavefront
     constexpr int OROW = D + PF_OPAD;
+    constexpr int AUX = ONE ? 2 : 0;
     // RT > 1: AHEAD + 1 stages (K tiles, then V tiles) used in turn, one barrier per step.
     // RT == 1: each wavefront stages its own tiles, K in sb and V in sb1 (an array of its
     // own: the compiler waits for every copy into an array before it reads that), each
@@ -207,11 +222,13 @@ k_attn_rows(RowsArgs a, RowsParts pt, int chunk_tiles) {
     // KV groups side by side: one group's tiles on the same XCDs where their count
     // divides 8
     const int g = blockIdx.x % a.kvheads;
-    const int tile_id = blockIdx.x / a.kvheads / pt.chunks;
-    const int chunk = blockIdx.x / a.kvheads % pt.chunks;
+    const int item = blockIdx.x / a.kvheads, later = item - pt.whole_tiles;
+    const int tile_id = later < 0 ? item : pt.whole_tiles + later / pt.chunks;
+    const int chunk = later < 0 ? 0 : later % pt.chunks;
+    const int chunk_tiles = later < 0 ? INT_MAX : pt.chunk_tiles;
     RowTile rw;
     if (!find_tile<ONE, NT>(a, 32 * RT, tile_id, rw)) return;
-    const int v0 = chunk * chunk_tiles, v1 = min(rw.ntiles, v0 + chunk_tiles);
+    const int v0 = chunk * pt.chunk_tiles, v1 = min(rw.ntiles - v0, chunk_tiles) + v0;
     if (chunk > 0 && v0 >= v1) return;
     const bool whole = rw.ntiles <= chunk_tiles;  // the results themselves, not a part
 
@@ -226,6 +243,16 @@ k_attn_rows(RowsArgs a, RowsParts pt, int chunk_tiles) {
     const int myrow = rw.row0 + mypair / per, myhead = g * per + mypair % per;
     const int prow = rw.p0 + mypair / per;
 
+    // lane (t, hh) has k-slice hh of row t of q: on its way while the pages are looked up
+    float4 x0[KS], x1[KS];
+    {
+        const float *qrow = a.q + ((size_t)myrow * a.qheads + myhead) * D + 8 * hh;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            x0[ks] = *(const float4 *)(qrow + 16 * ks);
+            x1[ks] = *(const float4 *)(qrow + 16 * ks + 4);
+        }
+    }
     // this wavefront's copies of a tile: instruction i takes the 16-byte units
     // 64 n .. 64 n + 63 of the tile (LDS order), n = rt + RT i.  Where these are whole rows
     // (RPI of them) the lane's offset within them is one number for V, and for K one that
@@ -270,13 +297,13 @@ k_attn_rows(RowsArgs a, RowsParts pt, int chunk_tiles) {
                 if (TI % RT == 0 || rt + RT * i < TI) {
                     if constexpr (WHOLE) {
                         const int x = is_k ? pf_k_slot<D>(RPI * (rt + RT * i), 0) * 16 : 0;
-                        lds_copy16(rs, to + 1024 * RT * i,
+                        lds_copy16<AUX>(rs, to + 1024 * RT * i,
                                    (uint32_t)(lrow * (kvd * 2) + ((is_k ? kcol : vcol) ^ x)),
                                    RPI * (rt + RT * i) * (kvd * 2));
                     } else {
                         int row, col;
                         unit(i, is_k, row, col);
-                        lds_copy16(rs, to + 1024 * RT * i, (uint32_t)(row * (kvd * 2) + col), 0);
+                        lds_copy16<AUX>(rs, to + 1024 * RT * i, (uint32_t)(row * (kvd * 2) + col), 0);
                     }
                 }
         } else {
@@ -312,18 +339,11 @@ k_attn_rows(RowsArgs a, RowsParts pt, int chunk_tiles) {
         }
     }
 
-    // Q^T as the B operand of the score MFMA: column t, k-slice hh (columns past the last
-    // row repeat it and are never stored)
+    // Q^T as the B operand of the score MFMA (columns past the last row repeat it and are
+    // never stored)
     h8 qh[KS], ql[KS];
     float fac;
     {
-        const float *qrow = a.q + ((size_t)myrow * a.qheads + myhead) * D + 8 * hh;
-        float4 x0[KS], x1[KS];
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-            x0[ks] = *(const float4 *)(qrow + 16 * ks);
-            x1[ks] = *(const float4 *)(qrow + 16 * ks + 4);
-        }
         float big = 0.0f;
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks)
@@ -522,15 +542,15 @@ k_attn_rows(RowsArgs a, RowsParts pt, int chunk_tiles) {
             }
         return n;
     };
-    // whether a V operand holds an infinity or NaN (exponents of all ones)
+    // whether this wavefront's share of a V tile holds an infinity or NaN (exponents of all
+    // ones)
     typedef uint32_t w4 __attribute__((ext_vector_type(4)));
     const auto any_bad = [&](const uint8_t *vt) {
         uint32_t bad = 0;
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-            for (int s2 = 0; s2 < 2; ++s2) {
-                const w4 w = __builtin_bit_cast(w4, v_operand(vt, dt, s2));
+        for (int i = 0; i < TIW; ++i)
+            if (TI % RT == 0 || rt + RT * i < TI) {
+                const w4 w = *(const w4 *)(vt + kw * TB + 1024 * (rt + RT * i) + 16 * lane);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) bad |= (w[e] & 0x7c007c00u) + 0x04000400u;
             }
@@ -621,12 +641,11 @@ k_attn_rows(RowsArgs a, RowsParts pt, int chunk_tiles) {
                 cut |= !rw.inside(a, min(v0 + st * KW + k, v1 - 1), rw.first, rw.last);
             if (use) refer(s, v, cut && !rw.inside(a, v, wfirst, wlast));
             if (cut) {  // workgroup-uniform
-                if (any_bad(vt)) {
-                    if (use) meet_bad(vt, v);
-                    if (lane == 0) bad_step[st & 1] = 1;
-                }
+                if (any_bad(vt) && lane == 0) bad_step[st & 1] = 1;
                 __syncthreads();
                 if (bad_step[st & 1]) {
+                    if (use) meet_bad(vt, v);
+                    __syncthreads();
                     drop_bad(vt);
                     __syncthreads();
                     if (tid == 0) bad_step[st & 1] = 0;  // (next set two barriers from here)
@@ -801,17 +820,17 @@ k_attn_rows(RowsArgs a, RowsParts pt, int chunk_tiles) {
 // ---------------------------------------------------------------------------
 constexpr int RM_T = 256;
 template <int D, bool ONE, int G>
-__global__ void __launch_bounds__(RM_T) k_attn_rows_merge(RowsArgs a, RowsParts pt, int tile_rows,
-                                                          int chunk_tiles) {
+__global__ void __launch_bounds__(RM_T) k_attn_rows_merge(RowsArgs a, RowsParts pt,
+                                                          int tile_rows) {
     constexpr int LANES = D / 4, ROWS = RM_T / (LANES * G);  // of a workgroup
     static_assert(ROWS >= 1, "a row's threads fit a workgroup");
-    const int g = blockIdx.x % a.kvheads, tile_id = blockIdx.x / a.kvheads;
+    const int g = blockIdx.x % a.kvheads, tile_id = pt.whole_tiles + blockIdx.x / a.kvheads;
     RowTile rw;
-    if (!find_tile<ONE, RM_T>(a, tile_rows, tile_id, rw) || rw.ntiles <= chunk_tiles) return;
+    if (!find_tile<ONE, RM_T>(a, tile_rows, tile_id, rw) || rw.ntiles <= pt.chunk_tiles) return;
     const int grp = threadIdx.x / LANES, dd = 4 * (threadIdx.x % LANES);
     const int way = grp / ROWS, lr = blockIdx.y * ROWS + grp % ROWS;
     const bool mine = way < G && lr < rw.pairs;  // whole groups of 8 lanes
-    const int n = (rw.ntiles + chunk_tiles - 1) / chunk_tiles;
+    const int n = (rw.ntiles + pt.chunk_tiles - 1) / pt.chunk_tiles;
     float M = -INFINITY, l = 0.0f, y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
     if (mine) {
 #pragma unroll 4
@@ -867,8 +886,9 @@ __global__ void __launch_bounds__(RM_T) k_attn_rows_merge(RowsArgs a, RowsParts 
 struct RowsPlan {
     bool one;       // a tile a sequence at most
     int rt, kw;     // wavefronts of a workgroup: 32-row tiles x K/V tiles
-    int tiles;      // at most
-    int chunks, chunk_tiles, rows;
+    int tiles;      // at most; the first whole_tiles are not cut, the others into chunks
+    int whole_tiles, chunks, chunk_tiles, rows;
+    size_t parts() const { return chunks > 1 ? (size_t)(tiles - whole_tiles) * chunks : 0; }
 };
 
 static RowsPlan rows_plan(const RowsArgs &a) {
@@ -879,18 +899,29 @@ static RowsPlan rows_plan(const RowsArgs &a) {
     p.rt = pairs <= 32 ? 1 : pairs <= 64 ? 2 : 4;
     p.kw = p.rt == 4 ? 1 : p.rt == 2 ? 2 : 4;
     const int rows = 32 * p.rt;
+    // (of a batch of several sequences the tiles are about max_rows' and at most one more each)
+    const int about = p.one ? a.nseq
+                            : std::max(1, (int)(((long long)a.max_rows * per + rows - 1) / rows));
     p.tiles = p.one ? a.nseq : (int)((long long)a.max_rows * per / rows) + a.nseq;
     p.rows = (int)std::min<long long>(rows, pairs);
     // K/V tiles that a tile's rows can see: the sinks', and a window's of every row
     const long long span = std::min<long long>(a.max_ctx, (long long)a.window + rows / per + 1);
     const int most = (int)std::min<long long>((a.max_ctx + PF_T - 1) / PF_T, span / PF_T + 2) +
                      (a.sinks + PF_T - 1) / PF_T;
-    const long long base =
-        (long long)a.kvheads *
-        (p.one ? a.nseq : std::max<long long>(1, (long long)a.max_rows * per / rows));
-    const long long want = 512;
-    long long chunks = std::max(1LL, want / base);
-    chunks = std::min<long long>(chunks, std::max(1, most / (2 * p.kw)));
+    const long long base = (long long)a.kvheads * about;
+    p.whole_tiles = 0;
+    long long chunks;
+    if (p.one) {
+        chunks = (p.rt == 1 ? ONE1 : ONE2) / base;
+    } else if (base < MULTI) {
+        chunks = MULTI / base;
+    } else {
+        // full rounds of workgroups whole, the rest cut so that it takes the same time
+        p.whole_tiles = (int)(base / WGSLOTS * WGSLOTS / a.kvheads);
+        const long long rest = base - (long long)p.whole_tiles * a.kvheads;
+        chunks = rest > 0 ? WGSLOTS / rest : 1;
+    }
+    chunks = std::max(1LL, std::min<long long>(chunks, most / (2 * p.kw)));
     p.chunk_tiles = (int)((most + chunks - 1) / chunks);
     p.chunks = (most + p.chunk_tiles - 1) / p.chunk_tiles;
     return p;
@@ -898,41 +929,45 @@ static RowsPlan rows_plan(const RowsArgs &a) {
 
 size_t attn_rows_workspace(const RowsArgs &a) {
     const RowsPlan p = rows_plan(a);
-    if (p.chunks == 1) return 0;
-    return (size_t)p.tiles * a.kvheads * p.chunks * p.rows * (a.hdim + 2) * sizeof(float);
+    return p.parts() * a.kvheads * p.rows * (a.hdim + 2) * sizeof(float);
+}
+
+static long long rows_items(const RowsPlan &p) {
+    return p.whole_tiles + (long long)(p.tiles - p.whole_tiles) * p.chunks;
 }
 
 bool attn_rows_fits(const RowsArgs &a) {
     const RowsPlan p = rows_plan(a);
     // (a launch's threads are counted in 32 bits)
-    return (long long)p.tiles * a.kvheads * p.chunks * p.rt * p.kw * 64 < (1LL << 32);
+    return rows_items(p) * a.kvheads * p.rt * p.kw * 64 < (1LL << 32);
 }
 
 void launch_attn_rows_paged(const RowsArgs &a, void *workspace, hipStream_t st) {
     const RowsPlan p = rows_plan(a);
     RowsParts pt = {};
+    pt.whole_tiles = p.whole_tiles;
     pt.chunks = p.chunks;
+    pt.chunk_tiles = p.chunk_tiles;
     pt.rows = p.rows;
     pt.o = (float *)workspace;
-    pt.m = pt.o + (size_t)p.tiles * a.kvheads * p.chunks * p.rows * a.hdim;
-    const dim3 grid((unsigned)(p.tiles * a.kvheads * p.chunks)), block(p.rt * p.kw * 64);
+    pt.m = pt.o + p.parts() * a.kvheads * p.rows * a.hdim;
+    const dim3 grid((unsigned)(rows_items(p) * a.kvheads)), block(p.rt * p.kw * 64);
     const bool page32 = a.pg.shift >= 5;
-#define CALL(DIM, RT, KW, AHEAD, ONE, P32)                                                    \
-    SI_LAUNCH((k_attn_rows<DIM, RT, KW, AHEAD, ONE, P32>), grid, block, 0, st, a, pt, \
-              p.chunk_tiles)
+#define CALL(DIM, RT, KW, AHEAD, ONE, P32) \
+    SI_LAUNCH((k_attn_rows<DIM, RT, KW, AHEAD, ONE, P32>), grid, block, 0, st, a, pt)
 #define PAGES(DIM, RT, KW, AHEAD, ONE) \
     if (page32) CALL(DIM, RT, KW, AHEAD, ONE, true); \
     else CALL(DIM, RT, KW, AHEAD, ONE, false)
 #define DIMS(DIM)                                  \
     if (p.rt == 1) { PAGES(DIM, 1, 4, 1, true); }     \
-    else if (p.rt == 2) { PAGES(DIM, 2, 2, A2, true); } \
-    else { PAGES(DIM, 4, 1, A4, false); }
+    else if (p.rt == 2) { PAGES(DIM, 2, 2, 1, true); } \
+    else { PAGES(DIM, 4, 1, 2, false); }
     // (a row's chunks 8 ways where there are many)
 #define MERGE(DIM, ONE, G)                                                                    \
     SI_LAUNCH((k_attn_rows_merge<DIM, ONE, G>),                                                 \
-              dim3((unsigned)(p.tiles * a.kvheads),                                             \
+              dim3((unsigned)((p.tiles - p.whole_tiles) * a.kvheads),                           \
                    (p.rows - 1) / (RM_T / (DIM / 4 * G)) + 1),                                  \
-              dim3(RM_T), 0, st, a, pt, 32 * p.rt, p.chunk_tiles)
+              dim3(RM_T), 0, st, a, pt, 32 * p.rt)
 #define MERGES(DIM)                                          \
     if (p.chunks > 8) {                                      \
         if (p.one) MERGE(DIM, true, 8);                      \

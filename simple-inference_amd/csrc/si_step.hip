@@ -2,6 +2,8 @@
 // lists and slot maps from the sequences' lengths, and the RoPE + K/V append by slot.
 // No counterpart in the reference (one sequence, one contiguous cache,
 // qwen_one_layer.c:262-266).
+#include <algorithm>
+
 #include "si_device.hpp"
 #include "si_kernels.hpp"
 
@@ -38,6 +40,17 @@ __device__ __forceinline__ StepSeq step_seq(const KvStep &a, int i) {
     s.now = s.ended || s.bad ? s.gone : max(s.gone, min(behind, s.taken) - a.kept);
     return s;
 }
+// its state after the step, and the ring's
+__device__ __forceinline__ void step_state(const KvStep &a, int i, const StepSeq &s, int code) {
+    a.held_out[2 * i] = code ? s.taken : s.ended ? 0 : s.taken + s.more;
+    a.held_out[2 * i + 1] = code ? s.gone : s.ended ? 0 : s.now;
+}
+__device__ __forceinline__ void ring_state(const KvStep &a, int begin, int count, int code,
+                                           long long more, long long back) {
+    const long long to = begin + more;  // (of a step that succeeds at most npages more)
+    a.free_out[0] = code ? begin : (int)(to >= a.npages ? to - a.npages : to);
+    a.free_out[1] = code ? count : (int)min(count - more + back, (long long)a.npages);
+}
 // ids that the sequence puts back into the ring, in the order of its list
 __device__ __forceinline__ int step_back(const KvStep &a, const StepSeq &s) {
     return s.ended ? min(a.kept, s.taken) + max(s.taken - a.kept - s.gone, 0) : s.now - s.gone;
@@ -48,107 +61,198 @@ __device__ __forceinline__ int step_back_page(const KvStep &a, const StepSeq &s,
     return k < first ? k : a.kept + s.gone + k - first;
 }
 
-// exclusive prefix sum over the workgroup of one value a thread; total: its sum
-__device__ __forceinline__ long long block_scan(long long v, long long *red, long long &total) {
-    long long x = v;
-    for (int d = 1; d < 64; d <<= 1) {
-        const long long y = __shfl_up(x, d, 64);
-        if ((int)(threadIdx.x & 63) >= d) x += y;
-    }
-    __syncthreads();  // red may still be read from the scan before
-    if ((threadIdx.x & 63) == 63) red[threadIdx.x >> 6] = x;
-    __syncthreads();
-    long long base = 0;
-    total = 0;
-    for (int w = 0; w < (int)(blockDim.x >> 6); ++w) {
-        if (w < (int)(threadIdx.x >> 6)) base += red[w];
-        total += red[w];
-    }
-    return base + x - v;
-}
-
-constexpr int STEP_T = 1024;
-__global__ void __launch_bounds__(STEP_T) k_kv_step(KvStep a) {
-    __shared__ long long red[STEP_T / 64];
-    const int tid = threadIdx.x;
-    const int per = (a.nseq + STEP_T - 1) / STEP_T;
-    const int i0 = min(tid * per, a.nseq), i1 = min(i0 + per, a.nseq);
-    const int begin = min(max(a.free_in[0], 0), a.npages - 1);
-    const int count = min(max(a.free_in[1], 0), a.npages);
+// what the sequences of a thread add up to, before (of) and in (the sums) the workgroup
+struct StepSums {
     long long rows = 0, more = 0, back = 0, bad = 0;
-    for (int i = i0; i < i1; ++i) {
-        const StepSeq s = step_seq(a, i);
+    __device__ __forceinline__ void add(const KvStep &a, const StepSeq &s) {
         rows += s.add;
         more += s.more;
         back += step_back(a, s);
         bad += s.bad;
     }
-    long long nrows, nmore, nback, nbad;
-    rows = block_scan(rows, red, nrows);
-    more = block_scan(more, red, nmore);
-    back = block_scan(back, red, nback);
-    block_scan(bad, red, nbad);
-    const int code = (nrows > a.max_rows ? 1 : 0) | (nmore > count ? 2 : 0) | (nbad ? 4 : 0);
-    const auto wrap = [&](long long k) { return (int)((begin + k) % a.npages); };
-    for (int i = i0; i < i1; ++i) {
-        const StepSeq s = step_seq(a, i);
-        int *list = a.pages + (size_t)i * a.max_pages;
-        if (code) {
-            a.start[i] = a.taken[i] = 0;
-            a.ctx[i] = s.have;
-            a.held_out[2 * i] = s.taken;
-            a.held_out[2 * i + 1] = s.gone;
-            continue;
-        }
-        a.start[i] = (int)rows;
-        a.taken[i] = (int)more;
-        a.ctx[i] = s.ended ? 0 : s.have + s.add;
-        for (int k = 0; k < s.more; ++k) list[s.taken + k] = a.ring[wrap(more + k)];
-        const int nb = step_back(a, s);
-        for (int k = 0; k < nb; ++k)
-            a.ring[wrap(count + back + k)] = list[step_back_page(a, s, k)];
-        a.held_out[2 * i] = s.ended ? 0 : s.taken + s.more;
-        a.held_out[2 * i + 1] = s.ended ? 0 : s.now;
-        rows += s.add;
-        more += s.more;
-        back += nb;
+};
+
+constexpr int STEP_T = 1024, STEP_FEW = 256;  // threads of a workgroup; of one for few rows
+
+// exclusive prefix sums over the workgroup's threads (of rows, more and back); the totals
+template <int T>
+__device__ __forceinline__ void step_scan(StepSums &v, StepSums &total) {
+    __shared__ long long part[4][T / 64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    StepSums x = v;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const long long r = __shfl_up(x.rows, d, 64), m = __shfl_up(x.more, d, 64),
+                        k = __shfl_up(x.back, d, 64), e = __shfl_up(x.bad, d, 64);
+        if (lane >= d) x.rows += r, x.more += m, x.back += k, x.bad += e;
     }
-    if (tid == 0) {
-        a.start[a.nseq] = code ? 0 : (int)nrows;
-        a.taken[a.nseq] = code ? 0 : (int)nmore;
-        a.free_out[0] = code ? begin : wrap(nmore);
-        a.free_out[1] = code ? count : (int)min(count - nmore + nback, (long long)a.npages);
-        a.status[0] = code;
-        a.status[1] = (int)min(nrows, (long long)INT_MAX);
-        a.status[2] = (int)min(nmore, (long long)INT_MAX);
-        a.status[3] = code ? 0 : (int)nback;
+    if (lane == 63) {
+        part[0][wave] = x.rows;
+        part[1][wave] = x.more;
+        part[2][wave] = x.back;
+        part[3][wave] = x.bad;
     }
     __syncthreads();
-    const int n = code ? 0 : (int)nrows;
-    for (int r = tid; r < a.max_rows; r += STEP_T) {
+    x.rows -= v.rows, x.more -= v.more, x.back -= v.back;
+    total = StepSums();
+#pragma unroll
+    for (int w = 0; w < T / 64; ++w) {
+        const long long r = part[0][w], m = part[1][w], k = part[2][w];
+        total.rows += r, total.more += m, total.back += k, total.bad += part[3][w];
+        if (w < wave) x.rows += r, x.more += m, x.back += k;
+    }
+    v = x;
+}
+
+// The last of n (at least one) ascending numbers that is not above x, the first of which
+// is not.
+__device__ __forceinline__ int last_not_above(const int *at, int n, int x) {
+    int lo = 0, hi = n;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (at[mid] <= x) lo = mid;
+        else hi = mid;
+    }
+    return lo;
+}
+
+// the ring's entry k behind entry begin, both below npages (a state that no step left may
+// ask for more)
+__device__ __forceinline__ int ring_at(int npages, int begin, int k) {
+    if (k >= npages) k %= npages;
+    const unsigned x = (unsigned)begin + (unsigned)k;
+    return (int)(x >= (unsigned)npages ? x - npages : x);
+}
+
+// Every workgroup adds up all sequences (they are few numbers, from the caches) and then
+// writes its share of the rows, the sequences' entries and the pages given back; so none
+// waits for another.  STATE: it also writes the state that the next step starts from,
+// which may lie where this step's did: one workgroup, after all have read it.  With
+// several a second launch does that.
+//
+// A page is taken by the row at its first position: what the list holds from `taken` on
+// has no other rows, so each page has one.
+template <int T, bool STATE>
+__global__ void __launch_bounds__(T) k_kv_step(KvStep a) {
+    // of each thread's sequences: where they start in the rows, the pages taken and those
+    // given back; the first one itself
+    __shared__ int rows_at[T], more_at[T], back_at[T];
+    __shared__ StepSeq first_of[T];
+    const int tid = threadIdx.x, wg = blockIdx.x, wgs = gridDim.x;
+    const int each = (a.nseq + T - 1) / T;
+    const int i0 = min(tid * each, a.nseq), i1 = min(i0 + each, a.nseq);
+    const int chunks = a.nseq ? (a.nseq + each - 1) / each : 0;
+    const int begin = min(max(a.free_in[0], 0), a.npages - 1);
+    const int count = min(max(a.free_in[1], 0), a.npages);
+    StepSums at, total;
+    if (i0 < i1) {
+        const StepSeq s = step_seq(a, i0);
+        first_of[tid] = s;
+        at.add(a, s);
+    }
+#pragma unroll 4
+    for (int i = i0 + 1; i < i1; ++i) at.add(a, step_seq(a, i));
+    step_scan<T>(at, total);
+    const int code = (total.rows > a.max_rows ? 1 : 0) | (total.more > count ? 2 : 0) |
+                     (total.bad ? 4 : 0);
+    // (a step that succeeds has fewer than 2^31 of each)
+    rows_at[tid] = (int)at.rows;
+    more_at[tid] = (int)at.more;
+    back_at[tid] = (int)at.back;
+    __syncthreads();
+    const int nrows = code ? 0 : (int)total.rows, nback = code ? 0 : (int)total.back;
+    for (int r = wg * T + tid; r < a.max_rows; r += wgs * T) {
         int seq = -1, pos = -1;
         long long slot = -1;
-        if (r < n) {
-            int lo = 0, hi = a.nseq;  // start[lo] <= r < start[hi]
-            while (hi - lo > 1) {
-                const int mid = (lo + hi) >> 1;
-                if (a.start[mid] <= r) lo = mid;
-                else hi = mid;
+        if (r < nrows) {
+            const int c = last_not_above(rows_at, chunks, r);
+            int row = rows_at[c], more = more_at[c], i = c * each;
+            StepSeq s = first_of[c];
+            while (r >= row + s.add) {  // within the chunk: its rows reach past r
+                row += s.add;
+                more += s.more;
+                s = step_seq(a, ++i);
             }
-            seq = lo;
-            pos = a.ctx[lo] - a.start[lo + 1] + r;
-            const int id = a.pages[(size_t)lo * a.max_pages + (pos >> a.shift)];
-            slot = ((long long)min(max(id, 0), a.npages - 1) << a.shift) |
-                   (pos & ((1 << a.shift) - 1));
+            seq = i;
+            pos = s.have + r - row;
+            const int j = pos >> a.shift, in = pos & ((1 << a.shift) - 1);
+            int *const entry = a.pages + (size_t)i * a.max_pages + j;
+            int id;
+            if (j < s.taken) {
+                id = *entry;
+            } else {
+                id = a.ring[ring_at(a.npages, begin, more + j - s.taken)];
+                if (in == 0) *entry = id;
+            }
+            slot = ((long long)min(max(id, 0), a.npages - 1) << a.shift) | in;
         }
         a.seq[r] = seq;
         a.pos[r] = pos;
         a.slot[r] = slot;
     }
+    const int back0 = ring_at(a.npages, begin, count);
+    for (int k = wg * T + tid; k < nback; k += wgs * T) {
+        const int c = last_not_above(back_at, chunks, k);
+        int from = back_at[c], i = c * each;
+        StepSeq s = first_of[c];
+        while (k >= from + step_back(a, s)) {
+            from += step_back(a, s);
+            s = step_seq(a, ++i);
+        }
+        a.ring[ring_at(a.npages, back0, k)] =
+            a.pages[(size_t)i * a.max_pages + step_back_page(a, s, k - from)];
+    }
+    // the sequences' entries: a workgroup's threads that lie together
+    if (tid * wgs / T == wg && i0 < i1) {
+        int rows = (int)at.rows, more = (int)at.more;
+        StepSeq s = first_of[tid];
+        for (int i = i0;;) {
+            a.start[i] = code ? 0 : rows;
+            a.taken[i] = code ? 0 : more;
+            a.ctx[i] = code ? s.have : s.ended ? 0 : s.have + s.add;
+            rows += s.add;
+            more += s.more;
+            if (++i >= i1) break;
+            s = step_seq(a, i);
+        }
+    }
+    if (wg == 0 && tid == 0) {
+        a.start[a.nseq] = code ? 0 : (int)total.rows;
+        a.taken[a.nseq] = code ? 0 : (int)total.more;
+        a.status[0] = code;
+        a.status[1] = (int)min(total.rows, (long long)INT_MAX);
+        a.status[2] = (int)min(total.more, (long long)INT_MAX);
+        a.status[3] = nback;
+    }
+    if constexpr (STATE) {
+        __syncthreads();
+        if (i0 < i1) step_state(a, i0, first_of[tid], code);
+#pragma unroll 4
+        for (int i = i0 + 1; i < i1; ++i) step_state(a, i, step_seq(a, i), code);
+        if (tid == 0) ring_state(a, begin, count, code, total.more, nback);
+    }
+}
+
+// the state after a step of several workgroups, whose status says what it came to
+constexpr int STATE_T = 256;
+__global__ void __launch_bounds__(STATE_T) k_kv_step_state(KvStep a) {
+    const int i = blockIdx.x * STATE_T + threadIdx.x, code = a.status[0];
+    if (i < a.nseq) step_state(a, i, step_seq(a, i), code);
+    if (i == 0)
+        ring_state(a, min(max(a.free_in[0], 0), a.npages - 1),
+                   min(max(a.free_in[1], 0), a.npages), code, a.status[2], a.status[3]);
 }
 
 void launch_kv_step(const KvStep &a, hipStream_t st) {
-    SI_LAUNCH(k_kv_step, dim3(1), dim3(STEP_T), 0, st, a);
+    if (a.max_rows <= STEP_FEW && a.nseq <= STEP_FEW) {
+        SI_LAUNCH((k_kv_step<STEP_FEW, true>), dim3(1), dim3(STEP_FEW), 0, st, a);
+    } else if (a.max_rows <= 8 * STEP_T && a.nseq <= 4 * STEP_T) {
+        SI_LAUNCH((k_kv_step<STEP_T, true>), dim3(1), dim3(STEP_T), 0, st, a);
+    } else {
+        const int wgs = std::min(std::max(a.max_rows / STEP_T, a.nseq / 512), 128);
+        SI_LAUNCH((k_kv_step<STEP_T, false>), dim3(wgs), dim3(STEP_T), 0, st, a);
+        SI_LAUNCH(k_kv_step_state, dim3(a.nseq / STATE_T + 1), dim3(STATE_T), 0, st, a);
+    }
 }
 
 // ---------------------------------------------------------------------------

@@ -109,10 +109,11 @@ __device__ __forceinline__ void lds_read16(const uint32_t (&at)[N], h8 (&x)[N]) 
                        "v"(at[6]), "v"(at[7])
                      : "memory");
 }
-// lds_copy16 at soff more, wavefront-uniform
+// lds_copy16 at soff more, wavefront-uniform; AUX: its cache policy
+template <int AUX>
 __device__ __forceinline__ void lds_copy16(__amdgpu_buffer_rsrc_t r, uint8_t *lds, uint32_t voff,
                                            int soff) {
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void *)lds, 16, voff, soff, 0, 0);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void *)lds, 16, voff, soff, 0, AUX);
 }
 // lds_copy16 from an address of its own for each lane
 typedef __attribute__((address_space(1))) void global_void;
