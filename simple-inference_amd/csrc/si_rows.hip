@@ -34,12 +34,6 @@
 
 namespace si {
 
-#ifndef ONE1
-#define ONE1 256
-#define ONE2 512
-#define MULTI 256
-#define WGSLOTS 512
-#endif
 constexpr float RW_UP = 11.0f;    // log2 of a weight's unit
 constexpr float RW_OVER = 4.0f;   // how far a tile's largest may lie over the reference
 constexpr float RW_UNDER = 12.0f; // and under it
@@ -833,18 +827,33 @@ __global__ void __launch_bounds__(RM_T) k_attn_rows_merge(RowsArgs a, RowsParts 
     const int n = (rw.ntiles + pt.chunk_tiles - 1) / pt.chunk_tiles;
     float M = -INFINITY, l = 0.0f, y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
     if (mine) {
-#pragma unroll 4
-        for (int k = way; k < n; k += G)
-            M = fmaxf(M, pt.m[2 * part_row(pt, a.kvheads, tile_id, g, k, lr)]);
-        const float ref = M == -INFINITY ? 0.0f : M;
-#pragma unroll 4
-        for (int k = way; k < n; k += G) {
-            const size_t at = part_row(pt, a.kvheads, tile_id, g, k, lr);
-            const float f = __builtin_amdgcn_exp2f(pt.m[2 * at] - ref);
-            const f4 v = *(const f4 *)(pt.o + at * D + dd);
-            l = fmaf(pt.m[2 * at + 1], f, l);
+        constexpr int U = 4;  // chunks whose loads are in flight together
+        for (int k0 = way; k0 < n; k0 += U * G) {
+            float m[U], s[U];
+            f4 v[U];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) y[i] = fmaf(v[i], f, y[i]);
+            for (int u = 0; u < U; ++u) {  // (past the last: it again, of no weight)
+                const size_t at = part_row(pt, a.kvheads, tile_id, g, min(k0 + u * G, n - 1), lr);
+                m[u] = k0 + u * G < n ? pt.m[2 * at] : -INFINITY;
+                s[u] = pt.m[2 * at + 1];
+                v[u] = *(const f4 *)(pt.o + at * D + dd);
+            }
+            float to = M;
+#pragma unroll
+            for (int u = 0; u < U; ++u) to = fmaxf(to, m[u]);
+            const float ref = to == -INFINITY ? 0.0f : to, old = __builtin_amdgcn_exp2f(M - ref);
+            M = to;
+            l *= old;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) y[i] *= old;
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const float f = __builtin_amdgcn_exp2f(m[u] - ref);
+                if (m[u] == -INFINITY) continue;  // (a chunk that the row sees nothing of)
+                l = fmaf(s[u], f, l);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) y[i] = fmaf(v[u][i], f, y[i]);
+            }
         }
     }
     if constexpr (G > 1) {
@@ -896,7 +905,15 @@ static RowsPlan rows_plan(const RowsArgs &a) {
     const int per = a.qheads / a.kvheads;
     const long long pairs = (long long)a.max_new * per;
     p.one = pairs <= 64;
-    p.rt = pairs <= 32 ? 1 : pairs <= 64 ? 2 : 4;
+    // Wavefronts of a workgroup.  Rows of a sequence that fill one or two 32-row tiles: a
+    // workgroup for all of them, so that K and V are read once.  More (prompts): while the
+    // 32-row tiles are few each is a workgroup's, its walk taken four ways; past that four
+    // tiles share each staged K/V tile (us, 1x4 | 4x1: 28/4 heads of 128, 1000 rows 39 | 50,
+    // 2048 (1792 tiles) 94 | 97, 3000 in a window of 1024 (2628) 127 | 107, 8000 of 2048
+    // 500 | 422; 14/2 of 64, 2048 rows 31 | 67, 4000 in 1024 (1750) 49 | 58, 8000 of 2048
+    // (3500) 144 | 148).
+    const long long tiles32 = ((long long)a.max_rows * per + 31) / 32 * a.kvheads;
+    p.rt = pairs <= 32 ? 1 : pairs <= 64 ? 2 : tiles32 < (a.hdim <= 64 ? 3500 : 1800) ? 1 : 4;
     p.kw = p.rt == 4 ? 1 : p.rt == 2 ? 2 : 4;
     const int rows = 32 * p.rt;
     // (of a batch of several sequences the tiles are about max_rows' and at most one more each)
@@ -911,16 +928,20 @@ static RowsPlan rows_plan(const RowsArgs &a) {
     const long long base = (long long)a.kvheads * about;
     p.whole_tiles = 0;
     long long chunks;
-    if (p.one) {
-        chunks = (p.rt == 1 ? ONE1 : ONE2) / base;
-    } else if (base < MULTI) {
-        chunks = MULTI / base;
+    if (p.rt < 4) {
+        // Chunks so that there are 256 workgroups of one row tile (one a CU: two halve the
+        // walks but double the states to merge; us, 256 | 512 | 1024 workgroups: 64 x 4096 of
+        // 28/4 heads of 128 90 | 93 | 107, 2 x 65536 of 12/2 28.9 | 30.3 | 39.9, 100 rows
+        // after 1000 19.6 | 21.0 | -), 512 of two, whose fewer wavefronts share a K/V tile
+        // (16 sequences of 1-8 rows 34.8 | 32.3 | 41).
+        chunks = (p.rt == 1 ? 256 : 512) / base;
     } else {
-        // full rounds of workgroups whole, the rest cut so that it takes the same time
-        p.whole_tiles = (int)(base / WGSLOTS * WGSLOTS / a.kvheads);
+        // full rounds of workgroups, two a CU, whole; the rest cut to take a round's share
+        p.whole_tiles = (int)(base / 512 * 512 / a.kvheads);
         const long long rest = base - (long long)p.whole_tiles * a.kvheads;
-        chunks = rest > 0 ? WGSLOTS / rest : 1;
+        chunks = rest > 0 ? 512 / rest : 1;
     }
+    // (two steps of a workgroup at least)
     chunks = std::max(1LL, std::min<long long>(chunks, most / (2 * p.kw)));
     p.chunk_tiles = (int)((most + chunks - 1) / chunks);
     p.chunks = (most + p.chunk_tiles - 1) / p.chunk_tiles;
@@ -958,9 +979,10 @@ void launch_attn_rows_paged(const RowsArgs &a, void *workspace, hipStream_t st) 
 #define PAGES(DIM, RT, KW, AHEAD, ONE) \
     if (page32) CALL(DIM, RT, KW, AHEAD, ONE, true); \
     else CALL(DIM, RT, KW, AHEAD, ONE, false)
-#define DIMS(DIM)                                  \
-    if (p.rt == 1) { PAGES(DIM, 1, 4, 1, true); }     \
-    else if (p.rt == 2) { PAGES(DIM, 2, 2, 1, true); } \
+#define DIMS(DIM)                                              \
+    if (p.rt == 1 && p.one) { PAGES(DIM, 1, 4, 1, true); }    \
+    else if (p.rt == 1) { PAGES(DIM, 1, 4, 1, false); }       \
+    else if (p.rt == 2) { PAGES(DIM, 2, 2, 1, true); }        \
     else { PAGES(DIM, 4, 1, 2, false); }
     // (a row's chunks 8 ways where there are many)
 #define MERGE(DIM, ONE, G)                                                                    \
