@@ -599,6 +599,18 @@ int si_layer_decode_kv4(si_layer_t *l, const float *x, int nseq, uint8_t *k_pool
                         const int *ctx_dev, int context, int max_ctx, float *out, int flags,
                         void *stream);
 
+/* The layer over a ragged step's rows (si_kv_step's start, ctx, pos, slot and
+ * pages): x and out [max_rows][hidden], max_rows up to the workspace's tokens.  K
+ * and V are appended as si_rope_kv_append_rows does it, attention is
+ * si_attention_rows', everything else the other calls' (the sums of max_rows rows).
+ * max_ctx is at most the workspace's max_pos.  What out's rows behind the step's last
+ * one hold is undefined. */
+int si_layer_step(si_layer_t *l, const float *x, int nseq, int max_rows, int max_new, int max_ctx,
+                  int window, int sinks, const int *start, const int *ctx, const int *pos,
+                  const int64_t *slot, uint16_t *k_pool, uint16_t *v_pool, int npages,
+                  int page_size, const int *pages, int max_pages, float *out, int flags,
+                  void *stream);
+
 /* si_attention for nq decode queries over a paged cache (ctx_dev required):
  * the same kernels as the contiguous form, so the result is bit-identical to
  * si_attention on the same rows laid out contiguously. */

@@ -1336,10 +1336,19 @@ static int run_decode_ffn(si_layer *L, float *out, bool exact, bool cap, hipStre
 // positions and attention contexts come either from (pos0, ctx0, ctx_step)
 // or from ctx_dev.  ctx_step 0 is batched decode (one new token per
 // sequence), ctx_step 1 causal prefill.
+// A ragged step's rows (si_layer_step): their places, and the sizes, starts and contexts
+// of their attention.
+struct StepRows {
+    const int *pos;
+    const long long *slot;
+    RowsArgs args;
+};
+
 static int run_rows(si_layer *L, const float *x, int rows, uint16_t *kc, uint16_t *vc,
                     size_t kv_seq_stride, int pos0, const int *ctx_dev, int ctx0, int ctx_step,
                     int max_ctx, float *out, int flags, hipStream_t st,
-                    KvPages pg = KvPages(), const Kv4Cache *kv4 = nullptr) {
+                    KvPages pg = KvPages(), const Kv4Cache *kv4 = nullptr,
+                    const StepRows *step = nullptr) {
     const int pos_step = ctx_step;  // positions advance with the contexts
     const si_shape_t &s = L->s;
     const int H = s.hidden, QD = s.qheads * s.hdim, NQKV = QD + 2 * s.kvheads * s.hdim;
@@ -1402,6 +1411,29 @@ static int run_rows(si_layer *L, const float *x, int rows, uint16_t *kc, uint16_
         launch_attention_kv4(L->q, rows, s.qheads, s.hdim, *kv4, ctx_dev, ctx0, 0, max_ctx,
                              L->attn, L->attq.qs, L->attq.d, L->attq.s, L->attn_ws, st,
                              tl_x ? L->attq.tq : nullptr, tl_x ? L->attq.td : nullptr);
+    } else if (step) {
+        // a ragged step's rows: RoPE + K/V append by slot, then attention over the
+        // pages -> Q8 (rows behind the last one keep what their buffers held)
+        mark(L, SI_PHASE_ROPE_KV, st);
+        launch_rope_kv_rows(L->qkv, NQKV, rows, s.qheads, s.kvheads, s.hdim, L->max_pos,
+                            step->pos, step->slot, L->rope_cos, L->rope_sin, L->q, kc, vc,
+                            (long long)pg.npages << pg.shift, st);
+        mark(L, SI_PHASE_ATTENTION_Q8, st);
+        RowsArgs a = step->args;
+        a.q = L->q;
+        a.k = kc;
+        a.v = vc;
+        a.pg = pg;
+        a.attn = L->attn;
+        a.qs = L->attq.qs;
+        a.d = L->attq.d;
+        a.bsum = L->attq.s;
+        a.ws_most = L->attn_ws_bytes;
+        launch_attn_rows_paged(a, L->attn_ws, st);
+        if (tl_x && full && gemm_streams(rows, L->wo.n, L->wo.k)) {
+            launch_q8_tile(L->attq.qs, L->attq.d, rows, QD, L->attq.tq, L->attq.td, st);
+            tl_att = true;
+        }
     } else if (ctx_step == 0) {
         // batched decode: RoPE + K/V append inside the attention kernel,
         // contiguous caches or a paged pool (pg)
@@ -1907,6 +1939,7 @@ static RowsArgs rows_sizes(const si_shape_t *s, int nseq, int max_rows, int max_
     a.window = std::min(window, max_ctx);
     a.sinks = std::min(sinks, max_ctx);
     a.scale2 = softmax_scale2(s->hdim);
+    a.ws_most = (size_t)-1;
     return a;
 }
 
@@ -2026,6 +2059,44 @@ int si_attention_rows(const si_shape_t *s, const float *q, int nseq, int max_row
     a.bsum = bsum;
     launch_attn_rows_paged(a, ws, S(stream));
     return check_launch(what);
+}
+
+int si_layer_step(si_layer_t *L, const float *x, int nseq, int max_rows, int max_new, int max_ctx,
+                  int window, int sinks, const int *start, const int *ctx, const int *pos,
+                  const int64_t *slot, uint16_t *k_pool, uint16_t *v_pool, int npages,
+                  int page_size, const int *pages, int max_pages, float *out, int flags,
+                  void *stream) {
+    const char *what = "layer_step";
+    SI_REQUIRE(L && x && start && ctx && pos && slot && k_pool && v_pool && pages && out,
+               "%s: NULL pointer", what);
+    SI_REQUIRE((flags & ~(SI_LAYER_ATTN_ONLY | SI_LAYER_EXACT | SI_LAYER_CAPTURE)) == 0,
+               "%s: unsupported flags %d (standard attention is single-token decode only)", what,
+               flags);
+    KvPages pg;
+    TRY(step_sizes(what, nseq, max_rows, window, sinks));
+    TRY(step_pages(what, npages, page_size, max_pages, &pg.shift));
+    SI_REQUIRE(nseq >= 1, "%s: nseq must be >= 1", what);
+    SI_REQUIRE(max_rows >= 1 && max_rows <= L->max_tokens, "%s: max_rows %d outside 1..%d", what,
+               max_rows, L->max_tokens);
+    SI_REQUIRE(max_new >= 1, "%s: max_new must be >= 1", what);
+    SI_REQUIRE(max_ctx >= 1 && max_ctx <= L->max_pos &&
+                   (long long)max_pages << pg.shift >= max_ctx,
+               "%s: max_ctx %d outside 1..%d or max_pages * page_size", what, max_ctx, L->max_pos);
+    SI_REQUIRE(((long long)npages << pg.shift) * L->s.kvheads * L->s.hdim < (1LL << 40),
+               "%s: KV pool too large", what);
+    SI_REQUIRE(aligned(k_pool, 16) && aligned(v_pool, 16),
+               "%s: the pools must be 16-byte aligned", what);
+    pg.pages = pages;
+    pg.max_pages = max_pages;
+    pg.npages = npages;
+    StepRows r;
+    r.pos = pos;
+    r.slot = (const long long *)slot;
+    r.args = rows_sizes(&L->s, nseq, max_rows, max_new, max_ctx, window, sinks);
+    r.args.start = start;
+    r.args.ctx = ctx;
+    return run_rows(L, x, max_rows, k_pool, v_pool, 0, 0, nullptr, 1, 0, max_ctx, out, flags,
+                    S(stream), pg, nullptr, &r);
 }
 
 }  // extern "C"

@@ -391,6 +391,7 @@ struct RowsArgs {
     int8_t *qs;
     uint16_t *d;
     int16_t *bsum;
+    size_t ws_most;  // bytes of workspace: with fewer the walks are cut into fewer chunks
 };
 // (both read sizes only; fits: whether one launch takes the call's workgroups)
 size_t attn_rows_workspace(const RowsArgs &a);

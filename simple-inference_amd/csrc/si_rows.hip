@@ -941,8 +941,13 @@ static RowsPlan rows_plan(const RowsArgs &a) {
         const long long rest = base - (long long)p.whole_tiles * a.kvheads;
         chunks = rest > 0 ? 512 / rest : 1;
     }
-    // (two steps of a workgroup at least)
-    chunks = std::max(1LL, std::min<long long>(chunks, most / (2 * p.kw)));
+    // (two steps of a workgroup at least, and as many states as there is room for)
+    const size_t state = (size_t)(p.tiles - p.whole_tiles) * a.kvheads * p.rows * (a.hdim + 2) *
+                         sizeof(float);
+    chunks = std::min<long long>(chunks, most / (2 * p.kw));
+    if (state > 0) chunks = (long long)std::min<size_t>((size_t)std::max(chunks, 0LL),
+                                                        a.ws_most / state);
+    chunks = std::max(1LL, chunks);
     p.chunk_tiles = (int)((most + chunks - 1) / chunks);
     p.chunks = (most + p.chunk_tiles - 1) / p.chunk_tiles;
     return p;

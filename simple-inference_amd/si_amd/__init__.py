@@ -135,6 +135,7 @@ _SIGS = {
                               _I, _P, _P, _P, _P, _P, _Z, _P]),
     "si_attention_kv4_workspace": (_Z, [ctypes.POINTER(Shape), _I, _I, _I]),
     "si_layer_decode_kv4": (_I, [_P, _P, _I, _P, _P, _I, _I, _P, _I, _P, _I, _I, _P, _I, _P]),
+    "si_layer_step": (_I, [_P, _P] + [_I] * 6 + [_P] * 6 + [_I, _I, _P, _I, _P, _I, _P]),
     "si_kv_copy_pages": (_I, [_P, _I, _Z, _I, _P, _P, _I, _P]),
     "si_kv_step": (_I, [_I, _P, _P] + [_I] * 6 + [_P] * 14),
     "si_rope_kv_append_rows": (_I, [ctypes.POINTER(Shape), _P, _I, _I, _I, _P, _P, _P, _P, _P, _P,
@@ -371,6 +372,14 @@ class Layer:
                    max_ctx, out, flags=SI_LAYER_FULL, stream=None, capture=True):
         call("si_layer_decode_kv4", self.h, ptr(x), nseq, ptr(k_pool), ptr(v_pool), npages,
              page_size, ptr(pages), max_pages, ptr(ctx_dev), max_ctx, max_ctx, ptr(out),
+             flags | (SI_LAYER_CAPTURE if capture else 0), stream_handle(stream))
+
+    def step(self, x, nseq, max_rows, max_new, max_ctx, window, sinks, start, ctx, pos, slot,
+             k_pool, v_pool, npages, page_size, pages, max_pages, out, flags=SI_LAYER_FULL,
+             stream=None, capture=True):
+        call("si_layer_step", self.h, ptr(x), nseq, max_rows, max_new, max_ctx, window, sinks,
+             ptr(start), ptr(ctx), ptr(pos), ptr(slot), ptr(k_pool), ptr(v_pool), npages,
+             page_size, ptr(pages), max_pages, ptr(out),
              flags | (SI_LAYER_CAPTURE if capture else 0), stream_handle(stream))
 
     def prefill(self, x, ntok, prefix, kc, vc, out, flags=SI_LAYER_FULL, stream=None,
