@@ -464,8 +464,9 @@ int si_kv_copy_pages(void *const *pools, int npools, size_t page_bytes, int npag
  *   taken      [nseq + 1], pages taken before sequence i;
  *   status     [4]: {code, rows, pages taken, pages given back}.
  * Code 0 is success; otherwise the sum of 1 (more rows than max_rows), 2 (too few free
- * pages) and 4 (positions past max_pages pages, or have past the taken ones: that
- * sequence counts as one without rows); the step then has no rows and pages, held and
+ * pages) and 4 (positions past max_pages pages, have past the taken ones, which
+ * counts as a sequence without rows, or more pages in held and free than there are);
+ * the step then has no rows and pages, held and
  * free stay as they are.  held_out may be held_in, free_out free_in; nothing else
  * may overlap.  window >= 1 (INT_MAX: none is given back).  page_size: a power of two in 1..2^20. */
 int si_kv_step(int nseq, const int *have, const int *add, int max_rows, int window, int sinks,
@@ -489,7 +490,8 @@ int si_rope_kv_append_rows(const si_shape_t *s, const float *qkv, int ldqkv, int
  * the sequence where t > p - window or t < sinks (a sliding window, and a few first
  * positions that stay visible); what it does not see has no influence, infinities and
  * NaN included.  window >= 1 (INT_MAX: all of them), sinks >= 0.  Contexts above
- * max_ctx are max_ctx; rows before position 0 are zeros; a sequence's rows past the
+ * max_ctx are max_ctx, starts outside 0..max_rows the nearer of these (a last sequence
+ * may reach past max_rows); rows before position 0 are zeros; a sequence's rows past the
  * first max_new are left as they are.  q, pools, attn 16-byte aligned, qs 4-byte.
  * Of the shape qheads, kvheads and hdim are read; outputs as si_attention's.
  * workspace: si_attention_rows_workspace bytes, 256-byte aligned (calls that

@@ -1959,6 +1959,12 @@ int si_kv_step(int nseq, const int *have, const int *add, int max_rows, int wind
                    (nseq == 0 || (have && add && pages && held_in && held_out && ctx)) &&
                    (max_rows == 0 || (seq && pos && slot)),
                "%s: NULL pointer", what);
+    for (const void *in : {(const void *)have, (const void *)add})
+        for (const void *to : {(const void *)start, (const void *)ctx, (const void *)seq,
+                               (const void *)pos, (const void *)taken, (const void *)held_out})
+            SI_REQUIRE(!in || in != to, "%s: have and add may not be outputs", what);
+    SI_REQUIRE(start != taken && (!ctx || (ctx != start && ctx != taken)),
+               "%s: start, taken and ctx are arrays of their own", what);
     a.nseq = nseq;
     a.max_rows = max_rows;
     a.window = window;

@@ -16,9 +16,9 @@
 // with Q and P as two fp16 halves each.  A row of q is scaled by a power of two to 2^14,
 // fac takes it back: a weight is 2^(fac s - c + 11), c a reference near the scores of the
 // tile at hand: it moves when the tile's largest lies more than 2^4 over it, or 2^12
-// under.  So a weight keeps 22 bits down to 2^-14 of its tile's largest and has an error
-// of at most 2^-24 of that one below, also behind a position that outweighs the rest (an
-// attention sink, whose values are small): sums in 32 bits hold both.  The sinks' tiles
+// under.  So a weight is off by at most 2^-23 of itself and 2^-24 of its tile's largest,
+// also behind a position that outweighs the rest (an attention sink, whose values are
+// small): sums in 32 bits hold both.  The sinks' tiles
 // have no other positions in them (a window's tile that they share is met twice).
 //
 // Where a mask cuts a tile its hidden scores are replaced (not added to), and V's values
@@ -103,7 +103,9 @@ __device__ __forceinline__ bool find_tile(const RowsArgs &a, int tile_rows, int 
         row_tile(a, tile_rows, tile, 0, t);
         return t.pairs > 0;
     } else {
-        __shared__ int red[NT / 64], found[2];
+        // (64 bits: starts that are no prefix sums may give every sequence all rows)
+        __shared__ long long red[NT / 64];
+        __shared__ int found[2];
         const int per = a.qheads / a.kvheads, tid = threadIdx.x;
         const auto tiles = [&](int i) {
             int r, p;
@@ -117,28 +119,28 @@ __device__ __forceinline__ bool find_tile(const RowsArgs &a, int tile_rows, int 
         }
         const int each = (a.nseq + NT - 1) / NT;
         const int i0 = min(tid * each, a.nseq), i1 = min(i0 + each, a.nseq);
-        int sum = 0;
+        long long sum = 0;
         for (int i = i0; i < i1; ++i) sum += tiles(i);
-        int x = sum;
+        long long x = sum;
         for (int d = 1; d < 64; d <<= 1) {
-            const int y = __shfl_up(x, d, 64);
+            const long long y = __shfl_up(x, d, 64);
             if ((tid & 63) >= d) x += y;
         }
         if ((tid & 63) == 63) red[tid >> 6] = x;
         __syncthreads();
-        int base = x - sum, total = 0;
+        long long base = x - sum, total = 0;
         for (int w = 0; w < NT / 64; ++w) {
             if (w < (tid >> 6)) base += red[w];
             total += red[w];
         }
-        tile = total - 1 - tile;
-        if (tile < 0) return false;
-        if (tile >= base && tile < base + sum)
+        const long long at = total - 1 - tile;
+        if (at < 0) return false;
+        if (at >= base && at < base + sum)  // (one thread's)
             for (int i = i0; i < i1; ++i) {
                 const int n = tiles(i);
-                if (tile < base + n) {
+                if (at < base + n) {
                     found[0] = i;
-                    found[1] = tile - base;
+                    found[1] = (int)(at - base);
                     break;
                 }
                 base += n;

@@ -49,7 +49,7 @@ __device__ __forceinline__ void ring_state(const KvStep &a, int begin, int count
                                            long long more, long long back) {
     const long long to = begin + more;  // (of a step that succeeds at most npages more)
     a.free_out[0] = code ? begin : (int)(to >= a.npages ? to - a.npages : to);
-    a.free_out[1] = code ? count : (int)min(count - more + back, (long long)a.npages);
+    a.free_out[1] = code ? count : (int)(count - more + back);
 }
 // ids that the sequence puts back into the ring, in the order of its list
 __device__ __forceinline__ int step_back(const KvStep &a, const StepSeq &s) {
@@ -116,10 +116,8 @@ __device__ __forceinline__ int last_not_above(const int *at, int n, int x) {
     return lo;
 }
 
-// the ring's entry k behind entry begin, both below npages (a state that no step left may
-// ask for more)
+// the ring's entry k (at most npages) behind entry begin
 __device__ __forceinline__ int ring_at(int npages, int begin, int k) {
-    if (k >= npages) k %= npages;
     const unsigned x = (unsigned)begin + (unsigned)k;
     return (int)(x >= (unsigned)npages ? x - npages : x);
 }
@@ -153,8 +151,10 @@ __global__ void __launch_bounds__(T) k_kv_step(KvStep a) {
 #pragma unroll 4
     for (int i = i0 + 1; i < i1; ++i) at.add(a, step_seq(a, i));
     step_scan<T>(at, total);
-    const int code = (total.rows > a.max_rows ? 1 : 0) | (total.more > count ? 2 : 0) |
-                     (total.bad ? 4 : 0);
+    // (ids that go back come from the pool: a state that has more is none that a step left)
+    const bool bad = total.bad > 0 || count - total.more + total.back > a.npages;
+    const int code =
+        (total.rows > a.max_rows ? 1 : 0) | (total.more > count ? 2 : 0) | (bad ? 4 : 0);
     // (a step that succeeds has fewer than 2^31 of each)
     rows_at[tid] = (int)at.rows;
     more_at[tid] = (int)at.more;

@@ -164,6 +164,18 @@ def test_tables_state_out_of_range():
     assert 0 <= f[0] < 20 and 0 <= f[1] <= 20
 
 
+def test_tables_more_pages_than_there_are():
+    """A ring and lists that together hold more than the pool: refused, nothing changes."""
+    t, have = filled()
+    t.free.copy_(dev(np.array([3, 20], np.int32)))  # all free, and four taken
+    before = [host(x).copy() for x in (t.pages, t.ring, t.free, t.held)]
+    have[1] = -1
+    t.run(dev(have), dev(np.zeros(4, np.int32)))
+    assert host(t.status).tolist() == [4, 0, 0, 0]
+    for a, b in zip(before, (t.pages, t.ring, t.free, t.held)):
+        assert np.array_equal(a, host(b))
+
+
 def test_tables_long_prompt():
     """One sequence of many pages next to idle ones."""
     t = Tables(70, 1, 300000, 250000, 260000, 1000, 4)
@@ -397,6 +409,38 @@ def test_attention_rows_before_the_start():
     got = b.run()
     assert (got[:2] == 0).all()
     b.check(got)
+
+
+def test_attention_starts_past_the_rows():
+    """A last sequence that reaches past max_rows: the rows that are there, at their positions."""
+    for new in ([3, 40], [3, 5]):
+        b = Batch((14, 2, 64), [60, 90], new, 16, 50, 4, seed=3)
+        b.upload()
+        b.max_rows = b.rows - 3
+        b.out = dev(np.full((b.max_rows + 4, 14 * 64), 7.0, np.float32))
+        b.call(b.out)
+        got = host(b.out).reshape(-1, 14, 64)
+        assert (got[b.max_rows:] == 7.0).all()
+        b.rows = b.max_rows
+        b.new[1] -= 3
+        b.ctx[1] -= 3
+        b.start[2] -= 3
+        b.check(got[:b.max_rows], every=3)
+
+
+def test_attention_starts_that_are_none():
+    """Starts in no order, below 0 and past the rows: every row that is written is one of some
+    sequence (values are the caller's affair), those behind max_rows are left as they are."""
+    rng = np.random.default_rng(6)
+    for max_new in (2, 64):
+        b = Batch((14, 2, 64), [60, 90, 40, 30], [20, 20, 1, 3], 16, 50, 4, max_new=max_new)
+        b.upload()
+        for _ in range(4):
+            b.ds = dev(rng.integers(-50, 100, 5).astype(np.int32))
+            b.dc = dev(rng.integers(-20, 200, 4).astype(np.int32))
+            out = dev(np.full((b.max_rows + 4, 14 * 64), 7.0, np.float32))
+            b.call(out)
+            assert (host(out)[b.max_rows:] == 7.0).all()
 
 
 def test_attention_limits():

@@ -57,6 +57,14 @@ def test_tables_refuse(bad, why):
     refused(tables(**bad), why)
 
 
+@pytest.mark.parametrize("bad", [dict(ctx=16 * A), dict(start=16 * A), dict(held_out=17 * A),
+                                 dict(taken=17 * A), dict(seq=16 * A), dict(pos=17 * A),
+                                 dict(start=18 * A, taken=18 * A), dict(ctx=18 * A, taken=18 * A)])
+def test_tables_refuse_overlaps(bad):
+    apart = dict(have=16 * A, add=17 * A, ctx=2 * A, start=3 * A, taken=4 * A)
+    refused(tables(**dict(apart, **bad)), b"of their own" if 18 * A in bad.values() else b"outputs")
+
+
 @pytest.mark.parametrize("bad,why", HEAD_CASES + [
     (dict(max_rows=-1), b"max_rows"), (dict(max_rows=1 << 24), b"max_rows"),
     (dict(max_pos=0), b"max_pos"), (dict(ld=4607), b"ldqkv"), (dict(pool_rows=0), b"pool rows"),
