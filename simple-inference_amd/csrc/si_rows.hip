@@ -187,8 +187,10 @@ __device__ __forceinline__ void rows_store(const RowsArgs &a, int row, int head,
     }
 }
 
-// AHEAD: steps that a stage's copies are issued before their use (RT > 1)
-template <int D, int RT, int KW, int AHEAD, bool ONE, bool PAGE32>
+// AHEAD: steps that a stage's copies are issued before their use (RT > 1).  PAGE: pages of
+// 32 positions and more, whole tiles (32), of 16 where an instruction's rows are whole (16:
+// two a tile), of any (1: each lane looks up its own row's).
+template <int D, int RT, int KW, int AHEAD, bool ONE, int PAGE>
 __global__ void __launch_bounds__(RT * KW * 64) __attribute__((amdgpu_waves_per_eu(2)))
 k_attn_rows(RowsArgs a, RowsParts pt) {
     constexpr int NWV = RT * KW, NT = NWV * 64, KS = D / 16, DT = D / 32, CH = D / 8;
@@ -269,37 +271,50 @@ k_attn_rows(RowsArgs a, RowsParts pt) {
             col = (is_k ? pf_k_chunk<D>(row, p % CH) : pf_v_slot<D>(row, p % CH)) * 16;
         }
     };
-    // the page of a step's tile (past the chunk: its last one again): of its first
-    // position, or (PAGE32 false: several pages a tile) of position t
-    // (read as constant data: one page a tile through the scalar cache, whose loads are
-    // not among those that the waits for copies count)
+    // the pages of a step's tile (past the chunk: its last one again): of its first
+    // position, of the one 16 behind it too, or of position t
+    // (read as constant data: through the scalar cache, whose loads are not among those
+    // that the waits for copies count)
     typedef const __attribute__((address_space(4))) int const_int;
     const const_int *list = (const const_int *)(a.pg.pages + (size_t)rw.seq * a.pg.max_pages);
+    struct Pages {
+        int id, second;
+    };
     const auto nth = [&](int st) { return min(v0 + st * KW + kw, v1 - 1); };
-    const auto page_of = [&](int st) {
-        const int pos = rw.tile(nth(st)) * PF_T + (PAGE32 ? 0 : t);
+    const auto id_of = [&](int pos) {
         const int id = list[min(pos >> a.pg.shift, a.pg.max_pages - 1)];
         return min(max(id, 0), a.pg.npages - 1);
     };
-    const auto copy = [&](const uint16_t *pool, uint8_t *dst, int st, int page, bool is_k) {
+    const auto page_of = [&](int st) {
+        const int pos = rw.tile(nth(st)) * PF_T;
+        return Pages{id_of(PAGE == 1 ? pos + t : pos), PAGE == 16 ? id_of(pos + 16) : 0};
+    };
+    const auto copy = [&](const uint16_t *pool, uint8_t *dst, int st, Pages page, bool is_k) {
         const int pos0 = rw.tile(nth(st)) * PF_T, mask = (1 << a.pg.shift) - 1;
         uint8_t *const to = dst + kw * TB + 1024 * rt;
-        if constexpr (PAGE32) {
-            const size_t row0 = ((size_t)__builtin_amdgcn_readfirstlane(page) << a.pg.shift) |
-                                (size_t)(pos0 & mask);
-            const __amdgpu_buffer_rsrc_t rs = buf_rsrc(pool + row0 * kvd + g * D, 0x7fffffffu);
+        if constexpr (PAGE > 1) {
+            const auto at = [&](int id, int pos) {
+                const size_t row0 = ((size_t)__builtin_amdgcn_readfirstlane(id) << a.pg.shift) |
+                                    (size_t)(pos & mask);
+                return buf_rsrc(pool + row0 * kvd + g * D, 0x7fffffffu);
+            };
+            const __amdgpu_buffer_rsrc_t rs = at(page.id, pos0);
+            const __amdgpu_buffer_rsrc_t rs2 = PAGE == 16 ? at(page.second, pos0 + 16) : rs;
 #pragma unroll
             for (int i = 0; i < TIW; ++i)
                 if (TI % RT == 0 || rt + RT * i < TI) {
                     if constexpr (WHOLE) {
-                        const int x = is_k ? pf_k_slot<D>(RPI * (rt + RT * i), 0) * 16 : 0;
-                        lds_copy16<AUX>(rs, to + 1024 * RT * i,
-                                   (uint32_t)(lrow * (kvd * 2) + ((is_k ? kcol : vcol) ^ x)),
-                                   RPI * (rt + RT * i) * (kvd * 2));
+                        const int row = RPI * (rt + RT * i);  // the instruction's first
+                        const int x = is_k ? pf_k_slot<D>(row, 0) * 16 : 0;
+                        const bool second = PAGE == 16 && row >= 16;  // wavefront-uniform
+                        lds_copy16<AUX>(second ? rs2 : rs, to + 1024 * RT * i,
+                                        (uint32_t)(lrow * (kvd * 2) + ((is_k ? kcol : vcol) ^ x)),
+                                        (second ? row - 16 : row) * (kvd * 2));
                     } else {
                         int row, col;
                         unit(i, is_k, row, col);
-                        lds_copy16<AUX>(rs, to + 1024 * RT * i, (uint32_t)(row * (kvd * 2) + col), 0);
+                        lds_copy16<AUX>(rs, to + 1024 * RT * i,
+                                        (uint32_t)(row * (kvd * 2) + col), 0);
                     }
                 }
         } else {
@@ -308,7 +323,7 @@ k_attn_rows(RowsArgs a, RowsParts pt) {
                 if (TI % RT == 0 || rt + RT * i < TI) {
                     int r, col;
                     unit(i, is_k, r, col);
-                    const int id = __shfl(page, r, 64);
+                    const int id = __shfl(page.id, r, 64);
                     const size_t row = ((size_t)id << a.pg.shift) | (size_t)((pos0 + r) & mask);
                     lds_copy16_at((const uint8_t *)(pool + row * kvd + g * D) + col,
                                   to + 1024 * RT * i);
@@ -316,7 +331,7 @@ k_attn_rows(RowsArgs a, RowsParts pt) {
         }
     };
     // the first copies: K up to step AHEAD and V one step less (RT == 1: of step 0)
-    int page = 0, page1 = 0;
+    Pages page = {}, page1 = {};
     if (steps > 0) {
         page = page_of(0);
         copy(a.k, sb, 0, page, true);
@@ -618,7 +633,7 @@ k_attn_rows(RowsArgs a, RowsParts pt) {
             else pf_wait<0>();
             pf_barrier();
             // (the next page's load before the copies: a wait for it is none for them)
-            const int page2 = page_of(st + AHEAD + 2);
+            const Pages page2 = page_of(st + AHEAD + 2);
             asm volatile("" ::: "memory");
             if (st + AHEAD < steps)
                 copy(a.v, sb + before * STAGE + KW * TB, st + AHEAD, page1, false);
@@ -665,7 +680,7 @@ k_attn_rows(RowsArgs a, RowsParts pt) {
             const bool more = v + KW < v1, cut = !rw.inside(a, v, wfirst, wlast);
             // outstanding: this tile's K and V copies, in this order (a page's load may
             // stand anywhere: it only makes a wait longer)
-            const int next = page;
+            const Pages next = page;
             pf_wait<TIW>();  // K is in; V may still be on its way
             uint32_t kat[KS];
             h8 x[KS];
@@ -943,10 +958,10 @@ static RowsPlan rows_plan(const RowsArgs &a) {
         const long long rest = base - (long long)p.whole_tiles * a.kvheads;
         chunks = rest > 0 ? 512 / rest : 1;
     }
-    // (two steps of a workgroup at least, and as many states as there is room for)
+    // (a step of a workgroup at least, and as many states as there is room for)
     const size_t state = (size_t)(p.tiles - p.whole_tiles) * a.kvheads * p.rows * (a.hdim + 2) *
                          sizeof(float);
-    chunks = std::min<long long>(chunks, most / (2 * p.kw));
+    chunks = std::min<long long>(chunks, most / p.kw);
     if (state > 0) chunks = (long long)std::min<size_t>((size_t)std::max(chunks, 0LL),
                                                         a.ws_most / state);
     chunks = std::max(1LL, chunks);
@@ -980,12 +995,12 @@ void launch_attn_rows_paged(const RowsArgs &a, void *workspace, hipStream_t st) 
     pt.o = (float *)workspace;
     pt.m = pt.o + p.parts() * a.kvheads * p.rows * a.hdim;
     const dim3 grid((unsigned)(rows_items(p) * a.kvheads)), block(p.rt * p.kw * 64);
-    const bool page32 = a.pg.shift >= 5;
-#define CALL(DIM, RT, KW, AHEAD, ONE, P32) \
-    SI_LAUNCH((k_attn_rows<DIM, RT, KW, AHEAD, ONE, P32>), grid, block, 0, st, a, pt)
-#define PAGES(DIM, RT, KW, AHEAD, ONE) \
-    if (page32) CALL(DIM, RT, KW, AHEAD, ONE, true); \
-    else CALL(DIM, RT, KW, AHEAD, ONE, false)
+#define CALL(DIM, RT, KW, AHEAD, ONE, PAGE) \
+    SI_LAUNCH((k_attn_rows<DIM, RT, KW, AHEAD, ONE, PAGE>), grid, block, 0, st, a, pt)
+#define PAGES(DIM, RT, KW, AHEAD, ONE)                                              \
+    if (a.pg.shift >= 5) CALL(DIM, RT, KW, AHEAD, ONE, 32);                          \
+    else if (a.pg.shift == 4 && DIM != 96) CALL(DIM, RT, KW, AHEAD, ONE, (DIM == 96 ? 1 : 16)); \
+    else CALL(DIM, RT, KW, AHEAD, ONE, 1)
 #define DIMS(DIM)                                              \
     if (p.rt == 1 && p.one) { PAGES(DIM, 1, 4, 1, true); }    \
     else if (p.rt == 1) { PAGES(DIM, 1, 4, 1, false); }       \

@@ -136,7 +136,9 @@ __global__ void __launch_bounds__(T) k_kv_step(KvStep a) {
     // given back; the first one itself
     __shared__ int rows_at[T], more_at[T], back_at[T];
     __shared__ StepSeq first_of[T];
+    // (of several workgroups half write rows, the others what else there is)
     const int tid = threadIdx.x, wg = blockIdx.x, wgs = gridDim.x;
+    const bool do_rows = STATE || blockIdx.y == 0, do_rest = STATE || blockIdx.y == 1;
     const int each = (a.nseq + T - 1) / T;
     const int i0 = min(tid * each, a.nseq), i1 = min(i0 + each, a.nseq);
     const int chunks = a.nseq ? (a.nseq + each - 1) / each : 0;
@@ -161,7 +163,7 @@ __global__ void __launch_bounds__(T) k_kv_step(KvStep a) {
     back_at[tid] = (int)at.back;
     __syncthreads();
     const int nrows = code ? 0 : (int)total.rows, nback = code ? 0 : (int)total.back;
-    for (int r = wg * T + tid; r < a.max_rows; r += wgs * T) {
+    for (int r = wg * T + tid; do_rows && r < a.max_rows; r += wgs * T) {
         int seq = -1, pos = -1;
         long long slot = -1;
         if (r < nrows) {
@@ -190,6 +192,7 @@ __global__ void __launch_bounds__(T) k_kv_step(KvStep a) {
         a.pos[r] = pos;
         a.slot[r] = slot;
     }
+    if (!do_rest) return;
     const int back0 = ring_at(a.npages, begin, count);
     for (int k = wg * T + tid; k < nback; k += wgs * T) {
         const int c = last_not_above(back_at, chunks, k);
@@ -250,7 +253,7 @@ void launch_kv_step(const KvStep &a, hipStream_t st) {
         SI_LAUNCH((k_kv_step<STEP_T, true>), dim3(1), dim3(STEP_T), 0, st, a);
     } else {
         const int wgs = std::min(std::max(a.max_rows / STEP_T, a.nseq / 512), 128);
-        SI_LAUNCH((k_kv_step<STEP_T, false>), dim3(wgs), dim3(STEP_T), 0, st, a);
+        SI_LAUNCH((k_kv_step<STEP_T, false>), dim3(wgs, 2), dim3(STEP_T), 0, st, a);
         SI_LAUNCH(k_kv_step_state, dim3(a.nseq / STATE_T + 1), dim3(STATE_T), 0, st, a);
     }
 }
