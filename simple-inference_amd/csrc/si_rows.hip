@@ -158,14 +158,13 @@ __device__ __forceinline__ bool find_tile(const RowsArgs &a, int tile_rows, int 
 // ---------------------------------------------------------------------------
 struct RowsParts {
     float *o, *m;
-    int rows;         // rows of a block that may be used
-    int whole_tiles;  // the call's first tiles, which are not cut
-    int chunks, chunk_tiles;  // of the others
+    int rows;  // rows of a block that may be used
+    int chunks, chunk_tiles;
 };
 
 __device__ __forceinline__ size_t part_row(const RowsParts &pt, int kvheads, int tile, int g,
                                            int chunk, int row) {
-    return (((size_t)(tile - pt.whole_tiles) * kvheads + g) * pt.chunks + chunk) * pt.rows + row;
+    return (((size_t)tile * kvheads + g) * pt.chunks + chunk) * pt.rows + row;
 }
 
 // 4 values of a row's head (8 lanes hold a Q8_0 block), zeros before position 0
@@ -200,10 +199,9 @@ k_attn_rows(RowsArgs a, RowsParts pt) {
     constexpr int OROW = D + PF_OPAD;
     constexpr int AUX = ONE ? 2 : 0;
     // RT > 1: AHEAD + 1 stages (K tiles, then V tiles) used in turn, one barrier per step.
-    // RT == 1: each wavefront stages its own tiles, K in sb and V in sb1 (an array of its
-    // own: the compiler waits for every copy into an array before it reads that), each
-    // refilled as soon as it has been read (no barrier).  KW > 1: at the end the
-    // wavefronts' outputs, where there are two arrays half of them in each.
+    // RT == 1: each wavefront stages its own tiles, K in sb and V in sb1, both refilled as
+    // soon as they are in registers (no barrier).  KW > 1: at the end the wavefronts'
+    // outputs, where there are two arrays half of them in each.
     constexpr bool DB = RT > 1;
     constexpr int STAGE = (DB ? 2 : 1) * KW * TB, NSTAGE = DB ? AHEAD + 1 : 1;
     constexpr int MRG_W = DB ? NWV : (NWV + 1) / 2, MRG = KW > 1 ? MRG_W * PF_T * OROW * 4 : 0;
@@ -220,15 +218,13 @@ k_attn_rows(RowsArgs a, RowsParts pt) {
     // KV groups side by side: one group's tiles on the same XCDs where their count
     // divides 8
     const int g = blockIdx.x % a.kvheads;
-    const int item = blockIdx.x / a.kvheads, later = item - pt.whole_tiles;
-    const int tile_id = later < 0 ? item : pt.whole_tiles + later / pt.chunks;
-    const int chunk = later < 0 ? 0 : later % pt.chunks;
-    const int chunk_tiles = later < 0 ? INT_MAX : pt.chunk_tiles;
+    const int tile_id = blockIdx.x / a.kvheads / pt.chunks;
+    const int chunk = blockIdx.x / a.kvheads % pt.chunks;
     RowTile rw;
     if (!find_tile<ONE, NT>(a, 32 * RT, tile_id, rw)) return;
-    const int v0 = chunk * pt.chunk_tiles, v1 = min(rw.ntiles - v0, chunk_tiles) + v0;
+    const int v0 = chunk * pt.chunk_tiles, v1 = min(rw.ntiles, v0 + pt.chunk_tiles);
     if (chunk > 0 && v0 >= v1) return;
-    const bool whole = rw.ntiles <= chunk_tiles;  // the results themselves, not a part
+    const bool whole = rw.ntiles <= pt.chunk_tiles;  // the results themselves, not a part
 
     const int per = a.qheads / a.kvheads, kvd = a.kvheads * D;
     const int steps = (v1 - v0 + KW - 1) / KW;
@@ -391,7 +387,8 @@ k_attn_rows(RowsArgs a, RowsParts pt) {
     const int s16 = lane & 15;
     int ka[KS], va[DT];
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) ka[ks] = kw * TB + t * D * 2 + pf_k_slot<D>(t, 2 * ks + hh) * 16;
+    for (int ks = 0; ks < KS; ++ks)
+        ka[ks] = kw * TB + t * D * 2 + pf_k_slot<D>(t, 2 * ks + hh) * 16;
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
         va[dt] = kw * TB + (4 * hh + (s16 >> 2)) * D * 2 +
@@ -492,16 +489,6 @@ k_attn_rows(RowsArgs a, RowsParts pt) {
         const h4 x1 = __builtin_bit_cast(h4, lds_read_tr16(vt + va[dt] + (16 * s2 + 8) * D * 2));
         return (h8){x0[0], x0[1], x0[2], x0[3], x1[0], x1[1], x1[2], x1[3]};
     };
-    const auto weigh = [&](const uint8_t *vt) {
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-            for (int s2 = 0; s2 < 2; ++s2) {
-                const h8 x = v_operand(vt, dt, s2);
-                o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, ph[s2], o[dt], 0, 0, 0);
-                o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, pl[s2], o[dt], 0, 0, 0);
-            }
-    };
     // The scores of K tile kt among the weights of s, and V's operands on their way: the
     // matrix cores and the vector ALU work side by side, each product followed by its share
     // of the weights (the order as written: left to itself the compiler puts the products
@@ -547,8 +534,9 @@ k_attn_rows(RowsArgs a, RowsParts pt) {
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt) {
                 if (s2 == 0) vx[2 * dt + 1] = v_operand(vt, dt, 1);
-                o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vx[2 * dt + s2], ph[s2], o[dt], 0, 0, 0);
-                o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vx[2 * dt + s2], pl[s2], o[dt], 0, 0, 0);
+                const h8 y = vx[2 * dt + s2];
+                o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(y, ph[s2], o[dt], 0, 0, 0);
+                o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(y, pl[s2], o[dt], 0, 0, 0);
                 __builtin_amdgcn_sched_barrier(0);
             }
         return n;
@@ -675,66 +663,52 @@ k_attn_rows(RowsArgs a, RowsParts pt) {
         }
     } else {
         // (the workgroup's rows are the wavefront's: every tile of the walk touches them)
-        uint8_t *const vt = sb1;
         for (int v = v0 + kw, st = 0; v < v1; v += KW, ++st) {  // wavefront-uniform
             const bool more = v + KW < v1, cut = !rw.inside(a, v, wfirst, wlast);
-            // outstanding: this tile's K and V copies, in this order (a page's load may
-            // stand anywhere: it only makes a wait longer)
-            const Pages next = page;
-            pf_wait<TIW>();  // K is in; V may still be on its way
+            pf_wait<0>();  // K and V are in
+            if (cut && any_bad(sb1)) {
+                meet_bad(sb1, v);
+                pf_wait<0>();  // (its reads are done)
+                drop_bad(sb1);
+                pf_wait<0>();
+            }
+            // both into registers, so that the next ones have the whole step to arrive
             uint32_t kat[KS];
-            h8 x[KS];
+            h8 x[KS], vx[2 * DT];
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks)
                 kat[ks] = (uint32_t)(uintptr_t)(lds_void *)(void *)(sb + ka[ks]);
+#pragma unroll
+            for (int k = 0; k < 2 * DT; ++k) vx[k] = v_operand(sb1, k / 2, k % 2);
             lds_read16(kat, x);
+            pf_wait<0>();  // (read)
             if (more) {
+                const Pages next = page;
                 page = page_of(st + 2);
                 asm volatile("" ::: "memory");
                 copy(a.k, sb, st + 1, next, true);
+                copy(a.v, sb1, st + 1, next, false);
             }
             f16v s = products(x);
             refer(s, v, cut);
             weights(s);
-            if (more)
-                pf_wait<TIW>();  // V is in; the next K may still be on its way
-            else
-                pf_wait<0>();
-            if (cut && any_bad(vt)) {
-                meet_bad(vt, v);
-                pf_wait<63>();  // (its reads are done)
-                drop_bad(vt);
-                pf_wait<63>();
-            }
-            weigh(vt);
-            pf_wait<TIW>();  // V has been read
-            if (more) copy(a.v, vt, st + 1, next, false);
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                for (int s2 = 0; s2 < 2; ++s2) {
+                    const h8 y = vx[2 * dt + s2];
+                    o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(y, ph[s2], o[dt], 0, 0, 0);
+                    o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(y, pl[s2], o[dt], 0, 0, 0);
+                }
         }
     }
     lsum += swap32_f(lsum);
 
     // lane (t, hh) holds O[row t][32 dt + 8 (r / 4) + 4 hh + r % 4] in o[dt][r]
     if constexpr (KW == 1) {
-        // each lane its row's halves of 8: 16-byte stores, the Q8_0 of a block from the pair
-        // of lanes that holds it
+        // (never cut) each lane its row's halves of 8: 16-byte stores, the Q8_0 of a block
+        // from the pair of lanes that holds it
         const int lr = 32 * rt + t;
-        if (!whole) {
-            const size_t at = part_row(pt, a.kvheads, tile_id, g, chunk, min(lr, pt.rows - 1));
-            if (lr < rw.pairs) {
-#pragma unroll
-                for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-                    for (int r4 = 0; r4 < 4; ++r4)
-                        *(f4 *)(pt.o + at * D + 32 * dt + 8 * r4 + 4 * hh) =
-                            (f4){o[dt][4 * r4], o[dt][4 * r4 + 1], o[dt][4 * r4 + 2],
-                                 o[dt][4 * r4 + 3]};
-                if (hh == 0) {
-                    pt.m[2 * at] = c;
-                    pt.m[2 * at + 1] = lsum;
-                }
-            }
-            return;
-        }
         const float inv = 1.0f / lsum;
         const size_t off = ((size_t)myrow * a.qheads + myhead) * D;
 #pragma unroll
@@ -835,7 +809,7 @@ __global__ void __launch_bounds__(RM_T) k_attn_rows_merge(RowsArgs a, RowsParts 
                                                           int tile_rows) {
     constexpr int LANES = D / 4, ROWS = RM_T / (LANES * G);  // of a workgroup
     static_assert(ROWS >= 1, "a row's threads fit a workgroup");
-    const int g = blockIdx.x % a.kvheads, tile_id = pt.whole_tiles + blockIdx.x / a.kvheads;
+    const int g = blockIdx.x % a.kvheads, tile_id = blockIdx.x / a.kvheads;
     RowTile rw;
     if (!find_tile<ONE, RM_T>(a, tile_rows, tile_id, rw) || rw.ntiles <= pt.chunk_tiles) return;
     const int grp = threadIdx.x / LANES, dd = 4 * (threadIdx.x % LANES);
@@ -910,11 +884,12 @@ __global__ void __launch_bounds__(RM_T) k_attn_rows_merge(RowsArgs a, RowsParts 
 // How a call is cut
 // ---------------------------------------------------------------------------
 struct RowsPlan {
-    bool one;       // a tile a sequence at most
-    int rt, kw;     // wavefronts of a workgroup: 32-row tiles x K/V tiles
-    int tiles;      // at most; the first whole_tiles are not cut, the others into chunks
-    int whole_tiles, chunks, chunk_tiles, rows;
-    size_t parts() const { return chunks > 1 ? (size_t)(tiles - whole_tiles) * chunks : 0; }
+    bool one;    // a tile a sequence at most
+    int rt, kw;  // wavefronts of a workgroup: 32-row tiles x K/V tiles
+    int tiles;   // at most
+    int chunks, chunk_tiles, rows;
+    size_t parts() const { return chunks > 1 ? (size_t)tiles * chunks : 0; }
+    long long items() const { return (long long)tiles * chunks; }
 };
 
 static RowsPlan rows_plan(const RowsArgs &a) {
@@ -943,23 +918,14 @@ static RowsPlan rows_plan(const RowsArgs &a) {
     const int most = (int)std::min<long long>((a.max_ctx + PF_T - 1) / PF_T, span / PF_T + 2) +
                      (a.sinks + PF_T - 1) / PF_T;
     const long long base = (long long)a.kvheads * about;
-    p.whole_tiles = 0;
-    long long chunks;
-    if (p.rt < 4) {
-        // Chunks so that there are 256 workgroups of one row tile (one a CU: two halve the
-        // walks but double the states to merge; us, 256 | 512 | 1024 workgroups: 64 x 4096 of
-        // 28/4 heads of 128 90 | 93 | 107, 2 x 65536 of 12/2 28.9 | 30.3 | 39.9, 100 rows
-        // after 1000 19.6 | 21.0 | -), 512 of two, whose fewer wavefronts share a K/V tile
-        // (16 sequences of 1-8 rows 34.8 | 32.3 | 41).
-        chunks = (p.rt == 1 ? 256 : 512) / base;
-    } else {
-        // full rounds of workgroups, two a CU, whole; the rest cut to take a round's share
-        p.whole_tiles = (int)(base / 512 * 512 / a.kvheads);
-        const long long rest = base - (long long)p.whole_tiles * a.kvheads;
-        chunks = rest > 0 ? 512 / rest : 1;
-    }
+    // Chunks so that there are 256 workgroups of one row tile (one a CU: two halve the walks
+    // but double the states to merge; us, 256 | 512 | 1024 workgroups: 64 x 4096 of 28/4 heads
+    // of 128 90 | 93 | 107, 2 x 65536 of 12/2 28.9 | 30.3 | 39.9, 100 rows after 1000 19.6 |
+    // 21.0 | -), 512 of two, whose fewer wavefronts share a K/V tile (16 sequences of 1-8 rows
+    // 34.8 | 32.3 | 41).  Workgroups of four tiles are more than that from the start.
+    long long chunks = p.rt == 4 ? 1 : (p.rt == 1 ? 256 : 512) / base;
     // (a step of a workgroup at least, and as many states as there is room for)
-    const size_t state = (size_t)(p.tiles - p.whole_tiles) * a.kvheads * p.rows * (a.hdim + 2) *
+    const size_t state = (size_t)p.tiles * a.kvheads * p.rows * (a.hdim + 2) *
                          sizeof(float);
     chunks = std::min<long long>(chunks, most / p.kw);
     if (state > 0) chunks = (long long)std::min<size_t>((size_t)std::max(chunks, 0LL),
@@ -975,26 +941,21 @@ size_t attn_rows_workspace(const RowsArgs &a) {
     return p.parts() * a.kvheads * p.rows * (a.hdim + 2) * sizeof(float);
 }
 
-static long long rows_items(const RowsPlan &p) {
-    return p.whole_tiles + (long long)(p.tiles - p.whole_tiles) * p.chunks;
-}
-
 bool attn_rows_fits(const RowsArgs &a) {
     const RowsPlan p = rows_plan(a);
     // (a launch's threads are counted in 32 bits)
-    return rows_items(p) * a.kvheads * p.rt * p.kw * 64 < (1LL << 32);
+    return p.items() * a.kvheads * p.rt * p.kw * 64 < (1LL << 32);
 }
 
 void launch_attn_rows_paged(const RowsArgs &a, void *workspace, hipStream_t st) {
     const RowsPlan p = rows_plan(a);
     RowsParts pt = {};
-    pt.whole_tiles = p.whole_tiles;
     pt.chunks = p.chunks;
     pt.chunk_tiles = p.chunk_tiles;
     pt.rows = p.rows;
     pt.o = (float *)workspace;
     pt.m = pt.o + p.parts() * a.kvheads * p.rows * a.hdim;
-    const dim3 grid((unsigned)(rows_items(p) * a.kvheads)), block(p.rt * p.kw * 64);
+    const dim3 grid((unsigned)(p.items() * a.kvheads)), block(p.rt * p.kw * 64);
 #define CALL(DIM, RT, KW, AHEAD, ONE, PAGE) \
     SI_LAUNCH((k_attn_rows<DIM, RT, KW, AHEAD, ONE, PAGE>), grid, block, 0, st, a, pt)
 #define PAGES(DIM, RT, KW, AHEAD, ONE)                                              \
@@ -1009,7 +970,7 @@ void launch_attn_rows_paged(const RowsArgs &a, void *workspace, hipStream_t st) 
     // (a row's chunks 8 ways where there are many)
 #define MERGE(DIM, ONE, G)                                                                    \
     SI_LAUNCH((k_attn_rows_merge<DIM, ONE, G>),                                                 \
-              dim3((unsigned)((p.tiles - p.whole_tiles) * a.kvheads),                           \
+              dim3((unsigned)(p.tiles * a.kvheads),                                             \
                    (p.rows - 1) / (RM_T / (DIM / 4 * G)) + 1),                                  \
               dim3(RM_T), 0, st, a, pt, 32 * p.rt)
 #define MERGES(DIM)                                          \
