@@ -1332,10 +1332,6 @@ static int run_decode_ffn(si_layer *L, float *out, bool exact, bool cap, hipStre
     return check_launch("layer decode");
 }
 
-// Shared schedule of the matrix-core paths.  rows activation rows;
-// positions and attention contexts come either from (pos0, ctx0, ctx_step)
-// or from ctx_dev.  ctx_step 0 is batched decode (one new token per
-// sequence), ctx_step 1 causal prefill.
 // A ragged step's rows (si_layer_step): their places, and the sizes, starts and contexts
 // of their attention.
 struct StepRows {
@@ -1344,6 +1340,10 @@ struct StepRows {
     RowsArgs args;
 };
 
+// Shared schedule of the matrix-core paths.  rows activation rows;
+// positions and attention contexts come either from (pos0, ctx0, ctx_step)
+// or from ctx_dev.  ctx_step 0 is batched decode (one new token per
+// sequence), ctx_step 1 causal prefill.
 static int run_rows(si_layer *L, const float *x, int rows, uint16_t *kc, uint16_t *vc,
                     size_t kv_seq_stride, int pos0, const int *ctx_dev, int ctx0, int ctx_step,
                     int max_ctx, float *out, int flags, hipStream_t st,

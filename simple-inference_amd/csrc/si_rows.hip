@@ -911,7 +911,8 @@ static RowsPlan rows_plan(const RowsArgs &a) {
     // (of a batch of several sequences the tiles are about max_rows' and at most one more each)
     const int about = p.one ? a.nseq
                             : std::max(1, (int)(((long long)a.max_rows * per + rows - 1) / rows));
-    p.tiles = p.one ? a.nseq : (int)((long long)a.max_rows * per / rows) + a.nseq;
+    p.tiles = p.one ? a.nseq
+                    : (int)((long long)a.max_rows * per / rows) + std::min(a.nseq, a.max_rows);
     p.rows = (int)std::min<long long>(rows, pairs);
     // K/V tiles that a tile's rows can see: the sinks', and a window's of every row
     const long long span = std::min<long long>(a.max_ctx, (long long)a.window + rows / per + 1);

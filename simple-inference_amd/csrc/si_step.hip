@@ -153,8 +153,9 @@ __global__ void __launch_bounds__(T) k_kv_step(KvStep a) {
 #pragma unroll 4
     for (int i = i0 + 1; i < i1; ++i) at.add(a, step_seq(a, i));
     step_scan<T>(at, total);
-    // (ids that go back come from the pool: a state that has more is none that a step left)
-    const bool bad = total.bad > 0 || count - total.more + total.back > a.npages;
+    // (ids that go back are none of the free ones: a state whose sum is more than the pool is
+    // none that a step left, and they would be written over ids that are being taken)
+    const bool bad = total.bad > 0 || count + total.back > a.npages;
     const int code =
         (total.rows > a.max_rows ? 1 : 0) | (total.more > count ? 2 : 0) | (bad ? 4 : 0);
     // (a step that succeeds has fewer than 2^31 of each)

@@ -105,3 +105,12 @@ def test_nothing_to_do():
     assert append(max_rows=0, qkv=None, pos=None, slot=None) == 0
     assert attention(max_rows=0, q=None, out=None) == 0
     assert attention(nseq=0, start=None, ctx=None, pages=None) == 0
+
+
+def test_attention_workspace_of_idle_sequences():
+    """Sequences without rows need no room: 40 rows of 7 heads a group are 8 whole tiles of 32, and
+    at most one more for each of 40 sequences, in 7 parts of 32 x 130 numbers (256 workgroups of
+    4 groups x 9 tiles)."""
+    need = si_amd.lib().si_attention_rows_workspace
+    most = (8 + 40) * 4 * 7 * 32 * 130 * 4
+    assert need(S, 65535, 40, 40, 8192, 4096, 4) == need(S, 40, 40, 40, 8192, 4096, 4) <= most
