@@ -25,6 +25,22 @@
 // there are looked at: 0 x infinity would be NaN.  Only if one is not finite, the rows
 // that see it are found first (exact counts, by the matrix cores), get their infinity or
 // NaN, and the tile in LDS has zeros in such places from then on.
+//
+// What bounds it (MI355X; a plain read reaches 6.2 TB/s, a large f16 product 1.18 PFLOP/s):
+//   single tokens, 64 sequences in windows of 4096, 28/4 heads of 128: memory, 539 MB in
+//     88 us, 6.1 TB/s.
+//   few of them (2 x 65536 positions of 12/2 heads, 16 x 4096 of 28/4 with up to 8 rows): the
+//     chunks' start, 129 MB in 23 us and 92 MB in 29 us, and the merge's launch after them, 4.5.
+//   one short window (1024 of 14/2 heads of 64): latency, 6.2 us + 3.0 of the merge.
+//   prompts (8000 rows in a window of 2048, 28/4): 415 us, 205 GFLOP, twice that issued for the
+//     halves: 1.0 PFLOP/s at the 1.9 GHz that the clock keeps.  Matrix cores busy half of the
+//     cycles; without the lo halves 300 us (and errors of 2^-11), without exponentials 366.
+//   pieces of prompts (333 rows after 1500) and pieces among single tokens: 25 and 100 us, the
+//     latency of the steps and of a workgroup's start (6 us: its sequence, pages, q).
+// Why these tiles: a lane holds one row's half of a tile's scores, so that a row's maximum and sum
+// take one exchange and its weights are the next product's operand as they are, without LDS.  One
+// 32-row tile a workgroup leaves a wavefront its own K/V tiles and no barrier; with four a staged
+// tile is read from LDS by four wavefronts and from memory once.
 #include <limits.h>
 #include <algorithm>
 
@@ -188,7 +204,9 @@ __device__ __forceinline__ void rows_store(const RowsArgs &a, int row, int head,
 
 // AHEAD: steps that a stage's copies are issued before their use (RT > 1).  PAGE: pages of
 // 32 positions and more, whole tiles (32), of 16 where an instruction's rows are whole (16:
-// two a tile), of any (1: each lane looks up its own row's).
+// two a tile), of any (1: each lane looks up its own row's: with 1 in place of 32, us, 64 x 4096 of
+// 28/4 heads of 128 102 | 91, 8000 rows of 2048 448 | 415, a piece of 333 rows 33 | 25; in place of
+// 16, 1024 positions of 14/2 of 64 10.5 | 9.6).
 template <int D, int RT, int KW, int AHEAD, bool ONE, int PAGE>
 __global__ void __launch_bounds__(RT * KW * 64) __attribute__((amdgpu_waves_per_eu(2)))
 k_attn_rows(RowsArgs a, RowsParts pt) {
@@ -197,6 +215,8 @@ k_attn_rows(RowsArgs a, RowsParts pt) {
     constexpr int TI = TB / 1024;            // copy instructions per tile
     constexpr int TIW = (TI + RT - 1) / RT;  // of one wavefront
     constexpr int OROW = D + PF_OPAD;
+    // (K and V that one workgroup reads are kept out of the caches: us, 64 x 4096 of 28/4 heads
+    // 98 | 91, 2 x 65536 of 12/2 32 | 29; a prompt's are read by many)
     constexpr int AUX = ONE ? 2 : 0;
     // RT > 1: AHEAD + 1 stages (K tiles, then V tiles) used in turn, one barrier per step.
     // RT == 1: each wavefront stages its own tiles, K in sb and V in sb1, both refilled as
@@ -801,7 +821,10 @@ k_attn_rows(RowsArgs a, RowsParts pt) {
 
 // ---------------------------------------------------------------------------
 // The chunks' states of tiles that were cut: grid (tiles x KV groups, rows), 4 values of a
-// row per thread, its chunks taken G ways (G > 1: they meet in LDS, in their order)
+// row per thread, its chunks taken G ways (G > 1: they meet in LDS, in their order).
+// Latency bounds it: out = sum_k 2^(m_k - m) o_k / sum_k 2^(m_k - m) l_k, a row's parts from
+// the caches, four loads in flight; 3.0 us for 14 rows of 64 in 7 chunks, 4.6 us for
+// 24 rows of 128 in 64 chunks (8 ways; one way 12).
 // ---------------------------------------------------------------------------
 constexpr int RM_T = 256;
 template <int D, bool ONE, int G>
@@ -898,7 +921,8 @@ static RowsPlan rows_plan(const RowsArgs &a) {
     const long long pairs = (long long)a.max_new * per;
     p.one = pairs <= 64;
     // Wavefronts of a workgroup.  Rows of a sequence that fill one or two 32-row tiles: a
-    // workgroup for all of them, so that K and V are read once.  More (prompts): while the
+    // workgroup for all of them, so that K and V are read once (16 sequences of 1-8 rows of 7
+    // heads 32.0 us, a workgroup for each tile 35.3).  More (prompts): while the
     // 32-row tiles are few each is a workgroup's, its walk taken four ways; past that four
     // tiles share each staged K/V tile (us, 1x4 | 4x1: 28/4 heads of 128, 1000 rows 39 | 50,
     // 2048 (1792 tiles) 94 | 97, 3000 in a window of 1024 (2628) 127 | 107, 8000 of 2048
@@ -968,7 +992,7 @@ void launch_attn_rows_paged(const RowsArgs &a, void *workspace, hipStream_t st) 
     else if (p.rt == 1) { PAGES(DIM, 1, 4, 1, false); }       \
     else if (p.rt == 2) { PAGES(DIM, 2, 2, 1, true); }        \
     else { PAGES(DIM, 4, 1, 2, false); }
-    // (a row's chunks 8 ways where there are many)
+    // (a row's chunks 8 ways where there are many: 2 x 65536 positions in 64, 28.9 us against 36.7)
 #define MERGE(DIM, ONE, G)                                                                    \
     SI_LAUNCH((k_attn_rows_merge<DIM, ONE, G>),                                                 \
               dim3((unsigned)(p.tiles * a.kvheads),                                             \

@@ -16,6 +16,13 @@ namespace si {
 // ceil((have + add) / page) - taken more, pages that lie behind the window of position
 // have given back.  Three prefix sums over the sequences (rows, pages taken, pages given
 // back) then say where each writes.
+//
+// Latency bounds it: a step's numbers are 16 bytes a sequence and 16 a row (4000 sequences and as
+// many rows 1.7 MB, 0.3 us at a copy's rate), but a chain of dependent steps lies between them:
+// lengths, the sums over a wavefront and the workgroup, a row's search for its sequence, its
+// page's id, the stores.  One small workgroup takes 3.6 us, 4000 sequences of 5 rows and 40 pieces
+// of 2000 12 us over many and 2 for their state.  (Each sequence's rows written by its own thread
+// took 22 us for 200 sequences and 333 for the 4000.)
 // ---------------------------------------------------------------------------
 struct StepSeq {
     int have, add, taken, gone;  // as given, within their ranges
@@ -247,13 +254,19 @@ __global__ void __launch_bounds__(STATE_T) k_kv_step_state(KvStep a) {
                    min(max(a.free_in[1], 0), a.npages), code, a.status[2], a.status[3]);
 }
 
+// How many threads (us in a captured graph, 256 threads | 1024 | several workgroups; sequences x
+// rows each): 1 x 1 3.5 | 5.9 | 7.1, 64 x 4 4.8 | 7.2 | 7.7, 200 x 1 6.7 | 7.5 | 8.1, 200 x 8
+// 11.8 | 8.4 | 8.2 (its second launch is the host's too), 64 x 1 and 4000 of one 16.4 | 9.3 | 7.9,
+// 1024 x 1 36 | 11.0 | 8.9, 1000 x 8 80 | 18.6 | 9.0, 4000 x 2 421 | 61 | 12.5.  Of several
+// workgroups each has 512 rows or 128 sequences: with twice the rows 64 x 1 and 4000 take 8.5, with
+// four times the sequences 4000 x 1 15.7 instead of 12.5 (half of them: 12.3).
 void launch_kv_step(const KvStep &a, hipStream_t st) {
-    if (a.max_rows <= STEP_FEW && a.nseq <= STEP_FEW) {
+    if (a.max_rows <= 2 * STEP_FEW && a.nseq <= STEP_FEW) {
         SI_LAUNCH((k_kv_step<STEP_FEW, true>), dim3(1), dim3(STEP_FEW), 0, st, a);
-    } else if (a.max_rows <= 8 * STEP_T && a.nseq <= 4 * STEP_T) {
+    } else if (a.max_rows <= 2 * STEP_T && a.nseq <= STEP_T / 2) {
         SI_LAUNCH((k_kv_step<STEP_T, true>), dim3(1), dim3(STEP_T), 0, st, a);
     } else {
-        const int wgs = std::min(std::max(a.max_rows / STEP_T, a.nseq / 512), 128);
+        const int wgs = std::min(std::max(a.max_rows / 512, a.nseq / 128), 128);
         SI_LAUNCH((k_kv_step<STEP_T, false>), dim3(wgs, 2), dim3(STEP_T), 0, st, a);
         SI_LAUNCH(k_kv_step_state, dim3(a.nseq / STATE_T + 1), dim3(STATE_T), 0, st, a);
     }
@@ -263,7 +276,9 @@ void launch_kv_step(const KvStep &a, hipStream_t st) {
 // RoPE and the K/V append by slot (si_rope_kv_append_rows)
 //
 // The arithmetic and the bits of k_rope_kv: a' = a c - b s, b' = b c + a s, and the fp16
-// narrowing.  Memory bounds it; a thread takes four neighbouring pairs of a head (16-byte
+// narrowing.  Memory bounds it: 2060 rows of 28/4 heads of 128 move 73 MB in 14.1 us,
+// 5.2 TB/s (a large copy: 4.9); 40 rows of 14/2 heads of 64 take 3.7 us, the latency of a
+// row's place and then its values.  A thread takes four neighbouring pairs of a head (16-byte
 // loads and stores of q|k|v and q, 8-byte stores of the cache), or four values of V's two
 // halves.
 // ---------------------------------------------------------------------------
