@@ -50,28 +50,30 @@ METRIC = "decode layer µs + HBM GB/s; prefill tokens/s + int8 MFMA % (one GPU)"
 # traffic with "traffic_current": false.  Kernels not listed report traffic
 # null.  Summaries: profiles/cfgN_*.md.
 PMC_KIB = {
-    ("1", "k_matvec<8, 128, false>"): (330.9, 4.5, "7c19f3b3a4f1"),
-    ("2", "k_dec_attn<64, 8, false, false, 1, true>"): (2694.0, 35.5, "7c19f3b3a4f1"),
-    ("2", "k_dec_gateup<64, 512, false>"): (2534.4, 9.8, "7c19f3b3a4f1"),
-    ("2", "k_dec_wo<8, 512, false>"): (579.0, 3.5, "7c19f3b3a4f1"),
-    ("2", "k_matvec<8, 512, false>"): (1256.0, 3.5, "7c19f3b3a4f1"),
-    ("3", "k_gemm_f6<2, 2, 1, 2, true>"): (28104.0, 5320.0, "7c19f3b3a4f1"),
-    ("4", "k_gemm_f6<2, 2, 2, 2, true>"): (516401.8, 43150.8, "7c19f3b3a4f1"),
-    ("5", "k_dec_attn_rows<128, 4, false, false, false>"): (266839.0, 8192.0, "7c19f3b3a4f1"),
+    ("1", "k_matvec<8, 128, false>"): (330.9, 4.5, "fc6533fb34d6"),
+    ("2", "k_dec_attn<64, 8, false, false, 1, true>"): (2694.0, 35.5, "fc6533fb34d6"),
+    ("2", "k_dec_gateup<64, 512, false>"): (2534.4, 9.8, "fc6533fb34d6"),
+    ("2", "k_dec_wo<8, 512, false>"): (579.0, 3.5, "fc6533fb34d6"),
+    ("2", "k_matvec<8, 512, false>"): (1256.0, 3.5, "fc6533fb34d6"),
+    ("3", "k_gemm_f6<2, 2, 1, 2, true>"): (28104.0, 5320.0, "fc6533fb34d6"),
+    ("4", "k_gemm_f6<2, 2, 2, 2, true>"): (516860.2, 43136.8, "fc6533fb34d6"),
+    ("5", "k_dec_attn_rows<128, 4, false, false, false>"): (266839.0, 8192.0, "fc6533fb34d6"),
 }
 FETCH_SCALE, WRITE_SCALE = 2.000, 1.000
+# sources of kernels that no configuration runs
+NOT_RUN = ("si_kv4.hip", "si_rows.hip", "si_step.hip")
 _DIGEST = None
 
 
 def csrc_digest():
     """sha256 (first 12 hex digits) of the HIP sources (csrc/*.hip, *.hpp) but
-    si_kv4.hip, whose kernels no configuration runs."""
+    those whose kernels no configuration runs."""
     global _DIGEST
     if _DIGEST is None:
         h = hashlib.sha256()
         d = os.path.join(ROOT, "simple-inference_amd", "csrc")
         for f in sorted(os.listdir(d)):
-            if f.endswith((".hip", ".hpp")) and f != "si_kv4.hip":
+            if f.endswith((".hip", ".hpp")) and f not in NOT_RUN:
                 h.update(f.encode())
                 with open(os.path.join(d, f), "rb") as fh:
                     h.update(fh.read())
