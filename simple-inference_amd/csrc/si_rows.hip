@@ -933,8 +933,8 @@ static RowsPlan rows_plan(const RowsArgs &a) {
     p.kw = p.rt == 4 ? 1 : p.rt == 2 ? 2 : 4;
     const int rows = 32 * p.rt;
     // (of a batch of several sequences the tiles are about max_rows' and at most one more each)
-    const int about = p.one ? a.nseq
-                            : std::max(1, (int)(((long long)a.max_rows * per + rows - 1) / rows));
+    const int about =
+        std::max(1, p.one ? a.nseq : (int)(((long long)a.max_rows * per + rows - 1) / rows));
     p.tiles = p.one ? a.nseq
                     : (int)((long long)a.max_rows * per / rows) + std::min(a.nseq, a.max_rows);
     p.rows = (int)std::min<long long>(rows, pairs);

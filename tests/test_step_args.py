@@ -114,3 +114,10 @@ def test_attention_workspace_of_idle_sequences():
     need = si_amd.lib().si_attention_rows_workspace
     most = (8 + 40) * 4 * 7 * 32 * 130 * 4
     assert need(S, 65535, 40, 40, 8192, 4096, 4) == need(S, 40, 40, 40, 8192, 4096, 4) <= most
+
+
+def test_attention_workspace_of_nothing():
+    """No rows or no sequences need no room."""
+    need = si_amd.lib().si_attention_rows_workspace
+    for nseq, max_rows, max_new in ((0, 8, 4), (0, 8, 100), (2, 0, 4), (2, 0, 100), (0, 0, 1)):
+        assert need(S, nseq, max_rows, max_new, 65536, 65536, 4) == 0
