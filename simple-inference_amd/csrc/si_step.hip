@@ -58,6 +58,10 @@ __device__ __forceinline__ void ring_state(const KvStep &a, int begin, int count
     a.free_out[0] = code ? begin : (int)(to >= a.npages ? to - a.npages : to);
     a.free_out[1] = code ? count : (int)(count - more + back);
 }
+// whether that is written beside the state that this step starts from, not over it
+__host__ __device__ __forceinline__ bool apart(const KvStep &a) {
+    return a.held_out != a.held_in && a.free_out != a.free_in;
+}
 // ids that the sequence puts back into the ring, in the order of its list
 __device__ __forceinline__ int step_back(const KvStep &a, const StepSeq &s) {
     return s.ended ? min(a.kept, s.taken) + max(s.taken - a.kept - s.gone, 0) : s.now - s.gone;
@@ -76,6 +80,12 @@ struct StepSums {
         more += s.more;
         back += step_back(a, s);
         bad += s.bad;
+    }
+    __device__ __forceinline__ void add(const StepSums &x) {
+        rows += x.rows;
+        more += x.more;
+        back += x.back;
+        bad += x.bad;
     }
 };
 
@@ -132,33 +142,43 @@ __device__ __forceinline__ int ring_at(int npages, int begin, int k) {
 // Every workgroup adds up all sequences (they are few numbers, from the caches) and then
 // writes its share of the rows, the sequences' entries and the pages given back; so none
 // waits for another.  STATE: it also writes the state that the next step starts from,
-// which may lie where this step's did: one workgroup, after all have read it.  With
-// several a second launch does that.
+// which may lie where this step's did: one workgroup, a sequence a thread at most, after all
+// have read it.  Several do so if it lies elsewhere; else a second launch does.
 //
 // A page is taken by the row at its first position: what the list holds from `taken` on
 // has no other rows, so each page has one.
 template <int T, bool STATE>
 __global__ void __launch_bounds__(T) k_kv_step(KvStep a) {
-    // of each thread's sequences: where they start in the rows, the pages taken and those
-    // given back; the first one itself
-    __shared__ int rows_at[T], more_at[T], back_at[T];
-    __shared__ StepSeq first_of[T];
+    // where the parts that the sequences are cut into start in the rows, the pages taken
+    // and those given back (SUB parts a thread, so that few sequences lie between a part's
+    // start and a row's own); the sequences themselves
+    constexpr int SUB = STATE ? 1 : 4, PARTS = T * SUB;
+    __shared__ int rows_at[PARTS], more_at[PARTS], back_at[PARTS];
+    __shared__ StepSeq seq_of[STATE ? T : 1];
     // (of several workgroups half write rows, the others what else there is)
     const int tid = threadIdx.x, wg = blockIdx.x, wgs = gridDim.x;
     const bool do_rows = STATE || blockIdx.y == 0, do_rest = STATE || blockIdx.y == 1;
-    const int each = (a.nseq + T - 1) / T;
-    const int i0 = min(tid * each, a.nseq), i1 = min(i0 + each, a.nseq);
-    const int chunks = a.nseq ? (a.nseq + each - 1) / each : 0;
+    const int each = STATE ? 1 : (a.nseq + PARTS - 1) / PARTS;  // sequences of a part
+    const int parts = STATE ? a.nseq : a.nseq ? (a.nseq + each - 1) / each : 0;
     const int begin = min(max(a.free_in[0], 0), a.npages - 1);
     const int count = min(max(a.free_in[1], 0), a.npages);
-    StepSums at, total;
-    if (i0 < i1) {
-        const StepSeq s = step_seq(a, i0);
-        first_of[tid] = s;
-        at.add(a, s);
-    }
-#pragma unroll 4
-    for (int i = i0 + 1; i < i1; ++i) at.add(a, step_seq(a, i));
+    const auto sequence = [&](int i) {
+        if constexpr (STATE) return seq_of[i];
+        else return step_seq(a, i);
+    };
+    StepSums part[SUB], at, total;
+    for (int j = 0; j < each; ++j)
+#pragma unroll
+        for (int k = 0; k < SUB; ++k) {
+            const int i = (tid * SUB + k) * each + j;
+            if (i < a.nseq) {
+                const StepSeq s = step_seq(a, i);
+                if constexpr (STATE) seq_of[i] = s;
+                part[k].add(a, s);
+            }
+        }
+#pragma unroll
+    for (int k = 0; k < SUB; ++k) at.add(part[k]);
     step_scan<T>(at, total);
     // (ids that go back are none of the free ones: a state whose sum is more than the pool is
     // none that a step left, and they would be written over ids that are being taken)
@@ -166,22 +186,26 @@ __global__ void __launch_bounds__(T) k_kv_step(KvStep a) {
     const int code =
         (total.rows > a.max_rows ? 1 : 0) | (total.more > count ? 2 : 0) | (bad ? 4 : 0);
     // (a step that succeeds has fewer than 2^31 of each)
-    rows_at[tid] = (int)at.rows;
-    more_at[tid] = (int)at.more;
-    back_at[tid] = (int)at.back;
+#pragma unroll
+    for (int k = 0; k < SUB; ++k) {
+        rows_at[tid * SUB + k] = (int)at.rows;
+        more_at[tid * SUB + k] = (int)at.more;
+        back_at[tid * SUB + k] = (int)at.back;
+        at.add(part[k]);
+    }
     __syncthreads();
     const int nrows = code ? 0 : (int)total.rows, nback = code ? 0 : (int)total.back;
     for (int r = wg * T + tid; do_rows && r < a.max_rows; r += wgs * T) {
         int seq = -1, pos = -1;
         long long slot = -1;
         if (r < nrows) {
-            const int c = last_not_above(rows_at, chunks, r);
+            const int c = last_not_above(rows_at, parts, r);
             int row = rows_at[c], more = more_at[c], i = c * each;
-            StepSeq s = first_of[c];
-            while (r >= row + s.add) {  // within the chunk: its rows reach past r
+            StepSeq s = sequence(i);
+            while (r >= row + s.add) {  // within the part: its rows reach past r
                 row += s.add;
                 more += s.more;
-                s = step_seq(a, ++i);
+                s = sequence(++i);
             }
             seq = i;
             pos = s.have + r - row;
@@ -203,29 +227,29 @@ __global__ void __launch_bounds__(T) k_kv_step(KvStep a) {
     if (!do_rest) return;
     const int back0 = ring_at(a.npages, begin, count);
     for (int k = wg * T + tid; k < nback; k += wgs * T) {
-        const int c = last_not_above(back_at, chunks, k);
+        const int c = last_not_above(back_at, parts, k);
         int from = back_at[c], i = c * each;
-        StepSeq s = first_of[c];
+        StepSeq s = sequence(i);
         while (k >= from + step_back(a, s)) {
             from += step_back(a, s);
-            s = step_seq(a, ++i);
+            s = sequence(++i);
         }
         a.ring[ring_at(a.npages, back0, k)] =
             a.pages[(size_t)i * a.max_pages + step_back_page(a, s, k - from)];
     }
-    // the sequences' entries: a workgroup's threads that lie together
-    if (tid * wgs / T == wg && i0 < i1) {
-        int rows = (int)at.rows, more = (int)at.more;
-        StepSeq s = first_of[tid];
-        for (int i = i0;;) {
-            a.start[i] = code ? 0 : rows;
-            a.taken[i] = code ? 0 : more;
-            a.ctx[i] = code ? s.have : s.ended ? 0 : s.have + s.add;
+    for (int i = wg * T + tid; i < a.nseq; i += wgs * T) {
+        const int c = i / each;
+        int rows = rows_at[c], more = more_at[c];
+        for (int j = c * each; j < i; ++j) {
+            const StepSeq s = sequence(j);
             rows += s.add;
             more += s.more;
-            if (++i >= i1) break;
-            s = step_seq(a, i);
         }
+        const StepSeq s = sequence(i);
+        a.start[i] = code ? 0 : rows;
+        a.taken[i] = code ? 0 : more;
+        a.ctx[i] = code ? s.have : s.ended ? 0 : s.have + s.add;
+        if (!STATE && apart(a)) step_state(a, i, s, code);
     }
     if (wg == 0 && tid == 0) {
         a.start[a.nseq] = code ? 0 : (int)total.rows;
@@ -234,12 +258,11 @@ __global__ void __launch_bounds__(T) k_kv_step(KvStep a) {
         a.status[1] = (int)min(total.rows, (long long)INT_MAX);
         a.status[2] = (int)min(total.more, (long long)INT_MAX);
         a.status[3] = nback;
+        if (!STATE && apart(a)) ring_state(a, begin, count, code, total.more, nback);
     }
     if constexpr (STATE) {
         __syncthreads();
-        if (i0 < i1) step_state(a, i0, first_of[tid], code);
-#pragma unroll 4
-        for (int i = i0 + 1; i < i1; ++i) step_state(a, i, step_seq(a, i), code);
+        if (tid < a.nseq) step_state(a, tid, seq_of[tid], code);
         if (tid == 0) ring_state(a, begin, count, code, total.more, nback);
     }
 }
@@ -255,20 +278,21 @@ __global__ void __launch_bounds__(STATE_T) k_kv_step_state(KvStep a) {
 }
 
 // How many threads (us in a captured graph, 256 threads | 1024 | several workgroups; sequences x
-// rows each): 1 x 1 3.5 | 5.9 | 7.1, 64 x 4 4.8 | 7.2 | 7.7, 200 x 1 6.7 | 7.5 | 8.1, 200 x 8
-// 11.8 | 8.4 | 8.2 (its second launch is the host's too), 64 x 1 and 4000 of one 16.4 | 9.3 | 7.9,
-// 1024 x 1 36 | 11.0 | 8.9, 1000 x 8 80 | 18.6 | 9.0, 4000 x 2 421 | 61 | 12.5.  Of several
-// workgroups each has 512 rows or 128 sequences: with twice the rows 64 x 1 and 4000 take 8.5, with
-// four times the sequences 4000 x 1 15.7 instead of 12.5 (half of them: 12.3).
+// rows each): 1 x 1 3.3 | 5.6 | 5.9, 64 x 4 4.5 | 6.8 | 6.9, 200 x 1 6.4 | 7.1 | 7.1, 200 x 8
+// 11.4 | 8.0 | 7.2, 64 x 1 and 4000 of one 15.8 | 9.0 | 7.0, 1024 x 1 - | 10.8 | 7.8, 1000 x 8
+// - | 17.8 | 8.0, 4000 x 2 - | - | 9.6; several whose state lies where it did have a second
+// launch, 2 us and the host's.  Of several each has 512 rows or 128 sequences: with twice as
+// many 64 x 1 and 4000 take 7.8 and 1000 x 8 8.4, with half 7.0 and 8.0.
 void launch_kv_step(const KvStep &a, hipStream_t st) {
     if (a.max_rows <= 2 * STEP_FEW && a.nseq <= STEP_FEW) {
         SI_LAUNCH((k_kv_step<STEP_FEW, true>), dim3(1), dim3(STEP_FEW), 0, st, a);
-    } else if (a.max_rows <= 2 * STEP_T && a.nseq <= STEP_T / 2) {
+    } else if (a.max_rows <= 2 * STEP_T && a.nseq <= STEP_T / 2 && !apart(a)) {
         SI_LAUNCH((k_kv_step<STEP_T, true>), dim3(1), dim3(STEP_T), 0, st, a);
     } else {
         const int wgs = std::min(std::max(a.max_rows / 512, a.nseq / 128), 128);
         SI_LAUNCH((k_kv_step<STEP_T, false>), dim3(wgs, 2), dim3(STEP_T), 0, st, a);
-        SI_LAUNCH(k_kv_step_state, dim3(a.nseq / STATE_T + 1), dim3(STATE_T), 0, st, a);
+        if (!apart(a))
+            SI_LAUNCH(k_kv_step_state, dim3(a.nseq / STATE_T + 1), dim3(STATE_T), 0, st, a);
     }
 }
 
