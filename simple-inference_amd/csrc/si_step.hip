@@ -20,9 +20,9 @@ namespace si {
 // Latency bounds it: a step's numbers are 16 bytes a sequence and 16 a row (4000 sequences and as
 // many rows 1.7 MB, 0.3 us at a copy's rate), but a chain of dependent steps lies between them:
 // lengths, the sums over a wavefront and the workgroup, a row's search for its sequence, its
-// page's id, the stores.  One small workgroup takes 3.6 us, 4000 sequences of 5 rows and 40 pieces
-// of 2000 12 us over many and 2 for their state.  (Each sequence's rows written by its own thread
-// took 22 us for 200 sequences and 333 for the 4000.)
+// page's id, the stores.  One small workgroup takes 3.2 us, 4000 sequences of up to 5 rows and 40
+// pieces of 2000 10 us over many (12 where a row had up to four sequences to walk).  (Each
+// sequence's rows written by its own thread took 22 us for 200 sequences and 333 for the 4000.)
 // ---------------------------------------------------------------------------
 struct StepSeq {
     int have, add, taken, gone;  // as given, within their ranges
