@@ -95,3 +95,30 @@ def test_attention_graphs_share_a_workspace():
         graphs[i].replay()
         torch.cuda.synchronize()
         assert np.array_equal(host(b[i].out).reshape(want[i].shape), want[i]), k
+
+
+@pytest.mark.parametrize("nseq,max_rows", [(1500, 4000), (20, 1800), (20, 60)])
+def test_tables_replayed(nseq, max_rows):
+    """One captured step over many: the state is taken on in place, whichever form runs."""
+    torch = torch_cuda()
+    rng = np.random.default_rng(nseq)
+    page, window, sinks = 4, 9, 3
+    t = Tables(nseq, page, nseq * 9, 12, max_rows, window, sinks)
+    have, add = (torch.zeros(nseq, dtype=torch.int32, device="cuda") for _ in range(2))
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=side):
+        t.run(have, add)
+    h = np.zeros(nseq, np.int32)
+    for _ in range(6):
+        a = rng.integers(0, 4, nseq).astype(np.int32)
+        want = t.ref(h, a)
+        assert want["status"][0] == 0
+        have.copy_(dev(h))
+        add.copy_(dev(a))
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        t.check(want)
+        h = (np.maximum(h, 0) + np.where(h < 0, 0, a)).astype(np.int32)
+        h[rng.random(nseq) < 0.1] = -1
