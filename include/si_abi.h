@@ -456,7 +456,8 @@ int si_kv_copy_pages(void *const *pools, int npools, size_t page_bytes, int npag
  *              ceil(sinks / page_size) pages stay; those behind them of which no row
  *              from position have on sees anything (all positions <= have - window)
  *              are given back: their entries are stale from then on.  A later have
- *              may be lower (drafts that were not accepted), down to this one.  An
+ *              may be lower (drafts that were not accepted), down to this one: as long as
+ *              these pages lie behind its window too.  An
  *              ended sequence gives all of its pages back, and has (0, 0) again;
  *   free_ring  [npages], the free ids: free[1] of them from entry free[0] on, round
  *              the end.  Pages are taken from its front, sequence by sequence, and
@@ -464,9 +465,9 @@ int si_kv_copy_pages(void *const *pools, int npools, size_t page_bytes, int npag
  *   taken      [nseq + 1], pages taken before sequence i;
  *   status     [4]: {code, rows, pages taken, pages given back}.
  * Code 0 is success; otherwise the sum of 1 (more rows than max_rows), 2 (too few free
- * pages) and 4 (positions past max_pages pages, have past the taken ones, which
- * counts as a sequence without rows, or more pages in held and free than there are);
- * the step then has no rows and pages, held and
+ * pages) and 4 (positions past max_pages pages, have past the taken ones or so low that
+ * its window reaches given-back ones, each of which counts as a sequence without rows, or
+ * more pages in held and free than there are); the step then has no rows and pages, held and
  * free stay as they are.  held_out may be held_in, free_out free_in; nothing else
  * may overlap.  window >= 1 (INT_MAX: none is given back).  page_size: a power of two in 1..2^20. */
 int si_kv_step(int nseq, const int *have, const int *add, int max_rows, int window, int sinks,

@@ -38,12 +38,15 @@ __device__ __forceinline__ StepSeq step_seq(const KvStep &a, int i) {
     s.have = max(have, 0);
     s.taken = min(max(a.held_in[2 * i], 0), a.max_pages);
     s.gone = min(max(a.held_in[2 * i + 1], 0), max(s.taken - a.kept, 0));
-    s.bad = !s.ended && ((long long)s.have + add > a.max_pages * ps || s.have > s.taken * ps);
+    // (have - window + 1 positions lie behind every window from here on)
+    const int behind = (int)((max((long long)s.have - a.window + 1, 0ll)) >> a.shift);
+    // (rows from a have whose window reaches pages that were given back would see others' pages,
+    // or be written to them)
+    s.bad = !s.ended && ((long long)s.have + add > a.max_pages * ps || s.have > s.taken * ps ||
+                         (s.gone > 0 && behind < a.kept + s.gone));
     s.add = s.ended || s.bad ? 0 : add;
     const int need = (int)(((long long)s.have + s.add + ps - 1) >> a.shift);
     s.more = s.ended || s.bad ? 0 : max(need - s.taken, 0);
-    // (have - window + 1 positions lie behind every window from here on)
-    const int behind = (int)((max((long long)s.have - a.window + 1, 0ll)) >> a.shift);
     s.now = s.ended || s.bad ? s.gone : max(s.gone, min(behind, s.taken) - a.kept);
     return s;
 }

@@ -1,0 +1,54 @@
+"""The state that si_kv_step takes: what no step left is refused, and a refused step leaves
+everything as it was, in each of the kernel's forms (one small workgroup; one large; several with
+the new state over the old; several with it beside the old)."""
+import numpy as np
+import pytest
+
+from tests.gpu_helpers import dev
+from tests.test_gpu_step import Tables, host
+
+pytestmark = pytest.mark.gpu
+
+# sequences and max_rows that take each form, and whether the new state lies beside the old
+FORMS = [(3, 40, False), (300, 1200, False), (700, 3000, False), (700, 3000, True)]
+
+
+class Fleet:
+    """Tables whose first sequences are looked at; the others have no rows."""
+
+    def __init__(self, form, page=4, max_pages=8, window=4, sinks=0, npages=40):
+        self.nseq, max_rows, self.apart = form
+        self.t = Tables(self.nseq, page, npages, max_pages, max_rows, window, sinks, seed=2)
+
+    def all(self, first):
+        x = np.zeros(self.nseq, np.int32)
+        x[:len(first)] = first
+        return x
+
+    def step(self, have, add):
+        """The step's code, and whether lists, ring and state are as they were."""
+        t = self.t
+        before = [host(x).copy() for x in (t.pages, t.ring, t.free, t.held)]
+        free, held = (x.clone().fill_(-7) for x in (t.free, t.held)) if self.apart else (None, None)
+        t.run(dev(self.all(have)), dev(self.all(add)), free, held)
+        if self.apart:
+            t.free, t.held = free, held
+        after = [host(x) for x in (t.pages, t.ring, t.free, t.held)]
+        return int(host(t.status)[0]), all(np.array_equal(a, b) for a, b in zip(before, after))
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("sinks,lowest", [(0, 15), (3, 15), (6, 15)])
+def test_tables_positions_behind_those_given_back(form, sinks, lowest):
+    """A have whose rows would see, or be written to, pages that were given back: refused, down to
+    the lowest at which these still lie behind the window."""
+    f = Fleet(form, sinks=sinks)
+    assert f.step([0, 0, 0], [18, 4, 1]) == (0, False)
+    # of 18 positions 0 to 14 lie behind: three pages, but the sinks'
+    kept = -(-sinks // 4)
+    assert f.step([18, 4, 1], [0, 1, 0]) == (0, False)
+    assert host(f.t.held)[0].tolist() == [5, 3 - kept]
+    for have in (lowest - 1, 5, 1, 0):
+        assert f.step([have, 5, 1], [5, 1, 0]) == (4, True)
+        assert (host(f.t.slot) == -1).all() and (host(f.t.start) == 0).all()
+    assert f.step([lowest, 5, 1], [3, 1, 0])[0] == 0
