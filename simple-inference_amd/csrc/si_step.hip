@@ -251,7 +251,8 @@ __global__ void __launch_bounds__(T) k_kv_step(KvStep a) {
         const StepSeq s = sequence(i);
         a.start[i] = code ? 0 : rows;
         a.taken[i] = code ? 0 : more;
-        a.ctx[i] = code ? s.have : s.ended ? 0 : s.have + s.add;
+        // (of a refused step as given, so that a sequence that was to end still does in the next)
+        a.ctx[i] = code ? a.have[i] : s.ended ? 0 : s.have + s.add;
         if (!STATE && apart(a)) step_state(a, i, s, code);
     }
     if (wg == 0 && tid == 0) {

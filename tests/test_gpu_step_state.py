@@ -52,3 +52,19 @@ def test_tables_positions_behind_those_given_back(form, sinks, lowest):
         assert f.step([have, 5, 1], [5, 1, 0]) == (4, True)
         assert (host(f.t.slot) == -1).all() and (host(f.t.start) == 0).all()
     assert f.step([lowest, 5, 1], [3, 1, 0])[0] == 0
+
+
+@pytest.mark.parametrize("form", FORMS)
+def test_tables_refused_step_says_what_it_was_given(form):
+    """The contexts of a refused step are its have, of sequences that end too, so that the next
+    step, made from them, ends them."""
+    f = Fleet(form)
+    assert f.step([0, 0, 0], [18, 4, 2])[0] == 0
+    assert f.step([18, 4, 2], [1, 1, 1])[0] == 0
+    held = host(f.t.held).copy()
+    assert f.step([-1, 5, -3], [0, 28, 0]) == (4, True)
+    assert host(f.t.ctx)[:3].tolist() == [-1, 5, -3]
+    assert np.array_equal(host(f.t.held), held)
+    assert f.step(host(f.t.ctx)[:3], [0, 2, 0])[0] == 0
+    assert host(f.t.held)[:3].tolist() == [[0, 0], [2, 0], [0, 0]]
+    assert int(host(f.t.free)[1]) == 40 - 2
