@@ -467,7 +467,7 @@ int si_kv_copy_pages(void *const *pools, int npools, size_t page_bytes, int npag
  * Code 0 is success; otherwise the sum of 1 (more rows than max_rows), 2 (too few free
  * pages) and 4 (positions past max_pages pages, have past the taken ones or so low that
  * its window reaches given-back ones, each of which counts as a sequence without rows, or
- * more pages in held and free than there are); the step then has no rows, pages, held and
+ * more pages in the lists and the ring than npages); the step then has no rows, pages, held and
  * free stay as they are, and ctx is have, of sequences that end too.  held_out may be held_in, free_out free_in; nothing else
  * may overlap.  window >= 1 (INT_MAX: none is given back).  page_size: a power of two in 1..2^20. */
 int si_kv_step(int nseq, const int *have, const int *add, int max_rows, int window, int sinks,

@@ -77,18 +77,20 @@ __device__ __forceinline__ int step_back_page(const KvStep &a, const StepSeq &s,
 
 // what the sequences of a thread add up to, before (of) and in (the sums) the workgroup
 struct StepSums {
-    long long rows = 0, more = 0, back = 0, bad = 0;
+    // (held: pages in the lists before the step; a sequence that is refused counts as one of
+    // more pages than there can be)
+    long long rows = 0, more = 0, back = 0, held = 0;
     __device__ __forceinline__ void add(const KvStep &a, const StepSeq &s) {
         rows += s.add;
         more += s.more;
         back += step_back(a, s);
-        bad += s.bad;
+        held += s.bad ? 1ll << 40 : s.taken - s.gone;
     }
     __device__ __forceinline__ void add(const StepSums &x) {
         rows += x.rows;
         more += x.more;
         back += x.back;
-        bad += x.bad;
+        held += x.held;
     }
 };
 
@@ -103,14 +105,14 @@ __device__ __forceinline__ void step_scan(StepSums &v, StepSums &total) {
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
         const long long r = __shfl_up(x.rows, d, 64), m = __shfl_up(x.more, d, 64),
-                        k = __shfl_up(x.back, d, 64), e = __shfl_up(x.bad, d, 64);
-        if (lane >= d) x.rows += r, x.more += m, x.back += k, x.bad += e;
+                        k = __shfl_up(x.back, d, 64), h = __shfl_up(x.held, d, 64);
+        if (lane >= d) x.rows += r, x.more += m, x.back += k, x.held += h;
     }
     if (lane == 63) {
         part[0][wave] = x.rows;
         part[1][wave] = x.more;
         part[2][wave] = x.back;
-        part[3][wave] = x.bad;
+        part[3][wave] = x.held;
     }
     __syncthreads();
     x.rows -= v.rows, x.more -= v.more, x.back -= v.back;
@@ -118,7 +120,7 @@ __device__ __forceinline__ void step_scan(StepSums &v, StepSums &total) {
 #pragma unroll
     for (int w = 0; w < T / 64; ++w) {
         const long long r = part[0][w], m = part[1][w], k = part[2][w];
-        total.rows += r, total.more += m, total.back += k, total.bad += part[3][w];
+        total.rows += r, total.more += m, total.back += k, total.held += part[3][w];
         if (w < wave) x.rows += r, x.more += m, x.back += k;
     }
     v = x;
@@ -183,9 +185,10 @@ __global__ void __launch_bounds__(T) k_kv_step(KvStep a) {
 #pragma unroll
     for (int k = 0; k < SUB; ++k) at.add(part[k]);
     step_scan<T>(at, total);
-    // (ids that go back are none of the free ones: a state whose sum is more than the pool is
-    // none that a step left, and they would be written over ids that are being taken)
-    const bool bad = total.bad > 0 || count + total.back > a.npages;
+    // (a page is free or in one list: a state whose sum is more than the pool is none that a step
+    // left, a page of it would be handed out twice, and ids that go back written over ids that
+    // are being taken)
+    const bool bad = count + total.held > a.npages;
     const int code =
         (total.rows > a.max_rows ? 1 : 0) | (total.more > count ? 2 : 0) | (bad ? 4 : 0);
     // (a step that succeeds has fewer than 2^31 of each)

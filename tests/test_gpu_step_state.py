@@ -4,8 +4,8 @@ the new state over the old; several with it beside the old)."""
 import numpy as np
 import pytest
 
-from tests.gpu_helpers import dev
-from tests.test_gpu_step import Tables, host
+from tests.gpu_helpers import dev, torch_cuda
+from tests.test_gpu_step import Tables, filled, host
 
 pytestmark = pytest.mark.gpu
 
@@ -68,3 +68,30 @@ def test_tables_refused_step_says_what_it_was_given(form):
     assert f.step(host(f.t.ctx)[:3], [0, 2, 0])[0] == 0
     assert host(f.t.held)[:3].tolist() == [[0, 0], [2, 0], [0, 0]]
     assert int(host(f.t.free)[1]) == 40 - 2
+
+
+@pytest.mark.parametrize("form", FORMS)
+def test_tables_more_pages_than_the_pool(form):
+    """A ring and lists that together hold more ids than there are would hand out a page twice:
+    refused, also where nothing is given back."""
+    f = Fleet(form)
+    assert f.step([0, 0, 0], [7, 4, 1])[0] == 0  # four pages
+    begin = int(host(f.t.free)[0])
+    for count in (37, 40):
+        f.t.free.copy_(dev(np.array([begin, count], np.int32)))
+        for add in ([1, 0, 0], [0, 1, 0]):
+            assert f.step([7, 4, 1], add) == (4, True)
+    f.t.free.copy_(dev(np.array([begin, 36], np.int32)))
+    assert f.step([7, 4, 1], [0, 1, 0])[0] == 0
+
+
+def test_tables_whole_pool_held():
+    """Lists that hold every page of the pool, in place and full: no row more, but a step without
+    one, and one that ends a sequence."""
+    torch_cuda()
+    t, have = filled(npages=4)
+    for h, a, code in (([2, 2, 2, 2], [2, 2, 2, 2], 0), ([4, 4, 4, 4], [0, 0, 0, 1], 2),
+                       ([4, -1, 4, 4], [0, 0, 0, 0], 0), ([4, 0, 4, 4], [0, 0, 0, 1], 0)):
+        t.run(dev(np.array(h, np.int32)), dev(np.array(a, np.int32)))
+        assert host(t.status)[0] == code
+    assert host(t.free)[1] == 0
