@@ -457,8 +457,8 @@ int si_kv_copy_pages(void *const *pools, int npools, size_t page_bytes, int npag
  *              from position have on sees anything (all positions <= have - window)
  *              are given back: their entries are stale from then on.  A later have
  *              may be lower (drafts that were not accepted), down to this one: as long as
- *              these pages lie behind its window too.  An
- *              ended sequence gives all of its pages back, and has (0, 0) again;
+ *              these pages lie behind its window too.  An ended sequence gives all of its
+ *              pages back, and has (0, 0) again;
  *   free_ring  [npages], the free ids: free[1] of them from entry free[0] on, round
  *              the end.  Pages are taken from its front, sequence by sequence, and
  *              given back to its end in the same order (in use from the next step on);
@@ -466,10 +466,13 @@ int si_kv_copy_pages(void *const *pools, int npools, size_t page_bytes, int npag
  *   status     [4]: {code, rows, pages taken, pages given back}.
  * Code 0 is success; otherwise the sum of 1 (more rows than max_rows), 2 (too few free
  * pages) and 4 (positions past max_pages pages, have past the taken ones or so low that
- * its window reaches given-back ones, each of which counts as a sequence without rows, or
- * more pages in the lists and the ring than npages); the step then has no rows, pages, held and
- * free stay as they are, and ctx is have, of sequences that end too.  held_out may be held_in, free_out free_in; nothing else
- * may overlap.  window >= 1 (INT_MAX: none is given back).  page_size: a power of two in 1..2^20. */
+ * its window reaches given-back ones, or counts in held that no step left, each of which
+ * counts as a sequence without rows; more pages in the lists and the ring than npages; a
+ * ring of numbers outside 0..npages-1 and 0..npages); the step then has no rows, pages,
+ * held and free stay as they are (such a ring is empty, 0 and 0, from then on), and ctx
+ * is have, of sequences that end too.  held_out may be held_in, free_out free_in; nothing
+ * else may overlap.  window >= 1 (INT_MAX: none is given back).  page_size: a power of two
+ * in 1..2^20. */
 int si_kv_step(int nseq, const int *have, const int *add, int max_rows, int window, int sinks,
                int page_size, int npages, int max_pages, int *pages, int *free_ring,
                const int *free_in, int *free_out, const int *held_in, int *held_out, int *start,

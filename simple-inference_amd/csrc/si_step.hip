@@ -25,7 +25,7 @@ namespace si {
 // sequence's rows written by its own thread took 22 us for 200 sequences and 333 for the 4000.)
 // ---------------------------------------------------------------------------
 struct StepSeq {
-    int have, add, taken, gone;  // as given, within their ranges
+    int have, add, taken, gone;  // as given, within their ranges (outside: bad)
     int more, now;               // pages taken in this step; pages given back after it
     bool ended, bad;
 };
@@ -34,32 +34,47 @@ __device__ __forceinline__ StepSeq step_seq(const KvStep &a, int i) {
     StepSeq s;
     const long long ps = 1ll << a.shift;
     const int have = a.have[i], add = max(a.add[i], 0);
+    const int taken = a.held_in[2 * i], gone = a.held_in[2 * i + 1];
     s.ended = have < 0;
     s.have = max(have, 0);
-    s.taken = min(max(a.held_in[2 * i], 0), a.max_pages);
-    s.gone = min(max(a.held_in[2 * i + 1], 0), max(s.taken - a.kept, 0));
+    s.taken = min(max(taken, 0), a.max_pages);
+    s.gone = min(max(gone, 0), max(s.taken - a.kept, 0));
     // (have - window + 1 positions lie behind every window from here on)
     const int behind = (int)((max((long long)s.have - a.window + 1, 0ll)) >> a.shift);
-    // (rows from a have whose window reaches pages that were given back would see others' pages,
-    // or be written to them)
-    s.bad = !s.ended && ((long long)s.have + add > a.max_pages * ps || s.have > s.taken * ps ||
-                         (s.gone > 0 && behind < a.kept + s.gone));
+    // (counts that no step left; rows from a have whose window reaches pages that were given back
+    // would see others' pages, or be written to them)
+    s.bad = taken != s.taken || gone != s.gone ||
+            (!s.ended && ((long long)s.have + add > a.max_pages * ps || s.have > s.taken * ps ||
+                          (s.gone > 0 && behind < a.kept + s.gone)));
     s.add = s.ended || s.bad ? 0 : add;
     const int need = (int)(((long long)s.have + s.add + ps - 1) >> a.shift);
     s.more = s.ended || s.bad ? 0 : max(need - s.taken, 0);
     s.now = s.ended || s.bad ? s.gone : max(s.gone, min(behind, s.taken) - a.kept);
     return s;
 }
-// its state after the step, and the ring's
-__device__ __forceinline__ void step_state(const KvStep &a, int i, const StepSeq &s, int code) {
-    a.held_out[2 * i] = code ? s.taken : s.ended ? 0 : s.taken + s.more;
-    a.held_out[2 * i + 1] = code ? s.gone : s.ended ? 0 : s.now;
+// The ring's state as given, within its ranges.  One that is not is no step's: what its ids are
+// is not known, so that the step is refused and the ring empty from then on.
+struct StepRing {
+    int begin, count;
+    bool bad;
+};
+__device__ __forceinline__ StepRing step_ring(const KvStep &a) {
+    const int begin = a.free_in[0], count = a.free_in[1];
+    if (begin >= 0 && begin < a.npages && count >= 0 && count <= a.npages)
+        return {begin, count, false};
+    return {0, 0, true};
 }
-__device__ __forceinline__ void ring_state(const KvStep &a, int begin, int count, int code,
+// a sequence's state after the step, and the ring's
+__device__ __forceinline__ void step_state(const KvStep &a, int i, const StepSeq &s, int code) {
+    // (of a refused step as given, whatever it is)
+    a.held_out[2 * i] = code ? a.held_in[2 * i] : s.ended ? 0 : s.taken + s.more;
+    a.held_out[2 * i + 1] = code ? a.held_in[2 * i + 1] : s.ended ? 0 : s.now;
+}
+__device__ __forceinline__ void ring_state(const KvStep &a, const StepRing &ring, int code,
                                            long long more, long long back) {
-    const long long to = begin + more;  // (of a step that succeeds at most npages more)
-    a.free_out[0] = code ? begin : (int)(to >= a.npages ? to - a.npages : to);
-    a.free_out[1] = code ? count : (int)(count - more + back);
+    const long long to = ring.begin + more;  // (of a step that succeeds at most npages more)
+    a.free_out[0] = code ? ring.begin : (int)(to >= a.npages ? to - a.npages : to);
+    a.free_out[1] = code ? ring.count : (int)(ring.count - more + back);
 }
 // whether that is written beside the state that this step starts from, not over it
 __host__ __device__ __forceinline__ bool apart(const KvStep &a) {
@@ -165,8 +180,8 @@ __global__ void __launch_bounds__(T) k_kv_step(KvStep a) {
     const bool do_rows = STATE || blockIdx.y == 0, do_rest = STATE || blockIdx.y == 1;
     const int each = STATE ? 1 : (a.nseq + PARTS - 1) / PARTS;  // sequences of a part
     const int parts = STATE ? a.nseq : a.nseq ? (a.nseq + each - 1) / each : 0;
-    const int begin = min(max(a.free_in[0], 0), a.npages - 1);
-    const int count = min(max(a.free_in[1], 0), a.npages);
+    const StepRing ring = step_ring(a);
+    const int begin = ring.begin, count = ring.count;
     const auto sequence = [&](int i) {
         if constexpr (STATE) return seq_of[i];
         else return step_seq(a, i);
@@ -188,7 +203,7 @@ __global__ void __launch_bounds__(T) k_kv_step(KvStep a) {
     // (a page is free or in one list: a state whose sum is more than the pool is none that a step
     // left, a page of it would be handed out twice, and ids that go back written over ids that
     // are being taken)
-    const bool bad = count + total.held > a.npages;
+    const bool bad = ring.bad || count + total.held > a.npages;
     const int code =
         (total.rows > a.max_rows ? 1 : 0) | (total.more > count ? 2 : 0) | (bad ? 4 : 0);
     // (a step that succeeds has fewer than 2^31 of each)
@@ -265,12 +280,12 @@ __global__ void __launch_bounds__(T) k_kv_step(KvStep a) {
         a.status[1] = (int)min(total.rows, (long long)INT_MAX);
         a.status[2] = (int)min(total.more, (long long)INT_MAX);
         a.status[3] = nback;
-        if (!STATE && apart(a)) ring_state(a, begin, count, code, total.more, nback);
+        if (!STATE && apart(a)) ring_state(a, ring, code, total.more, nback);
     }
     if constexpr (STATE) {
         __syncthreads();
         if (tid < a.nseq) step_state(a, tid, seq_of[tid], code);
-        if (tid == 0) ring_state(a, begin, count, code, total.more, nback);
+        if (tid == 0) ring_state(a, ring, code, total.more, nback);
     }
 }
 
@@ -279,9 +294,7 @@ constexpr int STATE_T = 256;
 __global__ void __launch_bounds__(STATE_T) k_kv_step_state(KvStep a) {
     const int i = blockIdx.x * STATE_T + threadIdx.x, code = a.status[0];
     if (i < a.nseq) step_state(a, i, step_seq(a, i), code);
-    if (i == 0)
-        ring_state(a, min(max(a.free_in[0], 0), a.npages - 1),
-                   min(max(a.free_in[1], 0), a.npages), code, a.status[2], a.status[3]);
+    if (i == 0) ring_state(a, step_ring(a), code, a.status[2], a.status[3]);
 }
 
 // How many threads (us in a captured graph, 256 threads | 1024 | several workgroups; sequences x

@@ -85,6 +85,37 @@ def test_tables_more_pages_than_the_pool(form):
     assert f.step([7, 4, 1], [0, 1, 0])[0] == 0
 
 
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("held", [(9, 0), (-1, 0), (2, -1), (2, 3), (2 ** 31 - 1, 0), (0, 1),
+                                  (-2 ** 31, 2 ** 31 - 1)])
+@pytest.mark.parametrize("ends", [False, True])
+def test_tables_counts_that_no_step_left(form, held, ends):
+    """Pages taken or given back that cannot be: refused, and left as they are."""
+    f = Fleet(form)
+    assert f.step([0, 0, 0], [7, 4, 1])[0] == 0
+    h = host(f.t.held).copy()
+    h[1] = held
+    f.t.held.copy_(dev(h))
+    for _ in range(2):
+        assert f.step([7, -1 if ends else 0, 1], [0, 0, 0]) == (4, True)
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("free", [(40, 3), (-1, 3), (5, -1), (5, 41), (2 ** 31 - 1, 2 ** 31 - 1)])
+def test_tables_ring_that_no_step_left(form, free):
+    """A ring whose numbers cannot be: refused, and empty from then on, so that none of its ids
+    is handed out."""
+    f = Fleet(form)
+    assert f.step([0, 0, 0], [7, 4, 0])[0] == 0
+    kept = [host(x).copy() for x in (f.t.pages, f.t.ring, f.t.held)]
+    f.t.free.copy_(dev(np.array(free, np.int32)))
+    assert f.step([7, 4, 0], [1, 0, 0]) == (4, False)
+    assert host(f.t.free).tolist() == [0, 0]
+    for a, b in zip(kept, (f.t.pages, f.t.ring, f.t.held)):
+        assert np.array_equal(a, host(b))
+    assert f.step([7, 4, 0], [0, 0, 1])[0] == 2
+
+
 def test_tables_whole_pool_held():
     """Lists that hold every page of the pool, in place and full: no row more, but a step without
     one, and one that ends a sequence."""
