@@ -86,8 +86,9 @@ struct RowTile {
 __device__ __forceinline__ int seq_rows(const RowsArgs &a, int i, int &row0, int &p0) {
     const int s0 = max(a.start[i], 0), s1 = max(a.start[i + 1], 0);
     row0 = min(s0, a.max_rows);
-    // (rows are fewer than 2^24: what lies further before position 0 is all hidden)
-    p0 = max(min(a.ctx[i], a.max_ctx) - (s1 - s0), -(1 << 24));
+    // (a context below 0 is 0, of which the starts' difference may be taken in 32 bits; rows are
+    // fewer than 2^24: what lies further before position 0 is all hidden)
+    p0 = max(min(max(a.ctx[i], 0), a.max_ctx) - (s1 - s0), -(1 << 24));
     return min(max(min(s1, a.max_rows) - row0, 0), a.max_new);
 }
 

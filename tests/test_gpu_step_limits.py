@@ -122,3 +122,21 @@ def test_tables_replayed(nseq, max_rows):
         t.check(want)
         h = (np.maximum(h, 0) + np.where(h < 0, 0, a)).astype(np.int32)
         h[rng.random(nseq) < 0.1] = -1
+
+
+@pytest.mark.parametrize("ctx", [0, -1, -40, -2 ** 31 + 1, -2 ** 31])
+@pytest.mark.parametrize("new,max_new", [([3, 1], 3), ([7, 1], 7), ([60, 1], 60)])
+@pytest.mark.parametrize("last", [0, 2 ** 31 - 1])
+def test_attention_contexts_below_zero(ctx, new, max_new, last):
+    """Contexts that a sequence cannot have are 0: its rows lie before position 0 and are zeros,
+    also where the starts are as far apart as they can be; its neighbour's are as ever."""
+    b = Batch((14, 2, 64), [90, 90], new[::-1], 16, 50, 4, max_new=max_new)
+    want = b.run()
+    b.dc = dev(np.array([90, ctx], np.int32))
+    if last:
+        b.ds = dev(np.array([0, 1, last], np.int32))
+    out = dev(np.full((b.max_rows + 2, 14 * 64), 7.0, np.float32))
+    b.call(out)
+    got = host(out).reshape(-1, 14, 64)
+    assert np.array_equal(got[:1], want[:1])
+    assert (got[1:b.max_rows] == 0).all() and (got[b.max_rows:] == 7.0).all()
