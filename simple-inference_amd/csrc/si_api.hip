@@ -1428,7 +1428,6 @@ static int run_rows(si_layer *L, const float *x, int rows, uint16_t *kc, uint16_
         a.qs = L->attq.qs;
         a.d = L->attq.d;
         a.bsum = L->attq.s;
-        a.ws_most = L->attn_ws_bytes;
         launch_attn_rows_paged(a, L->attn_ws, st);
         if (tl_x && full && gemm_streams(rows, L->wo.n, L->wo.k)) {
             launch_q8_tile(L->attq.qs, L->attq.d, rows, QD, L->attq.tq, L->attq.td, st);
@@ -2099,6 +2098,9 @@ int si_layer_step(si_layer_t *L, const float *x, int nseq, int max_rows, int max
     r.pos = pos;
     r.slot = (const long long *)slot;
     r.args = rows_sizes(&L->s, nseq, max_rows, max_new, max_ctx, window, sinks);
+    r.args.ws_most = L->attn_ws_bytes;
+    SI_REQUIRE(attn_rows_fits(r.args), "%s: %d rows of %d heads are too many", what, max_rows,
+               L->s.qheads);
     r.args.start = start;
     r.args.ctx = ctx;
     return run_rows(L, x, max_rows, k_pool, v_pool, 0, 0, nullptr, 1, 0, max_ctx, out, flags,

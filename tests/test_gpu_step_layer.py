@@ -194,3 +194,32 @@ def test_step_refusals(oracle):
         with pytest.raises(si_amd.SiError):
             call(**bad)
     torch.cuda.synchronize()
+
+
+def test_step_too_many_rows(oracle):
+    """Rows and heads that one launch of the attention does not take are refused before anything
+    runs, as si_attention_rows has it; the largest step of the same heads that fits is not."""
+    torch = torch_cuda()
+    sd = dict(hidden=32, qheads=256, kvheads=256, hdim=32, ffn=0)
+    s, os_ = si_amd.make_shape(**sd), or_shape(**sd)
+    n, page, max_pages = 65535, 16, 2
+    L = si_amd.Layer(s, make_layer(oracle, os_, 5, ffn=False), n, 32)
+    t = Tables(n, page, 8, max_pages, n, 32, 0)
+    t.run(dev(np.zeros(n, np.int32)), dev(np.zeros(n, np.int32)))
+    k, v = (torch.full((8 * page * 256 * 32,), 7, dtype=torch.int16, device="cuda")
+            for _ in range(2))
+    x, out = (empty((n, 32), torch.float32) for _ in range(2))
+    out.fill_(7.0)
+
+    def call(max_new):
+        L.step(x, n, n, max_new, 32, 32, 0, t.start, t.ctx, t.pos, t.slot, k, v, 8, page, t.pages,
+               max_pages, out, si_amd.SI_LAYER_ATTN_ONLY)
+
+    with pytest.raises(si_amd.SiError, match="too many"):
+        call(65)
+    torch.cuda.synchronize()
+    assert (out == 7.0).all()
+    call(1)
+    torch.cuda.synchronize()
+    assert (k == 7).all() and (v == 7).all()
+    L.close()
