@@ -863,8 +863,10 @@ __global__ void __launch_bounds__(RM_T) k_attn_rows_merge(RowsArgs a, RowsParts 
             for (int i = 0; i < 4; ++i) y[i] *= old;
 #pragma unroll
             for (int u = 0; u < U; ++u) {
+                if (k0 + u * G >= n) continue;
+                // (of a chunk that the row sees nothing of all is 0; of one whose scores are NaN
+                // the reference is as low, and the sum NaN)
                 const float f = __builtin_amdgcn_exp2f(m[u] - ref);
-                if (m[u] == -INFINITY) continue;  // (a chunk that the row sees nothing of)
                 l = fmaf(s[u], f, l);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) y[i] = fmaf(v[u][i], f, y[i]);
