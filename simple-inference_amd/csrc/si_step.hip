@@ -38,18 +38,18 @@ __device__ __forceinline__ StepSeq step_seq(const KvStep &a, int i) {
     s.ended = have < 0;
     s.have = max(have, 0);
     s.taken = min(max(taken, 0), a.max_pages);
-    s.gone = min(max(gone, 0), max(s.taken - a.kept, 0));
-    // (have - window + 1 positions lie behind every window from here on)
+    // (have - window + 1 positions lie behind every window from here on; an ended sequence may
+    // have given back any of its pages)
     const int behind = (int)((max((long long)s.have - a.window + 1, 0ll)) >> a.shift);
+    s.now = max((s.ended ? s.taken : min(behind, s.taken)) - a.kept, 0);
     // (counts that no step left; rows from a have whose window reaches pages that were given back
     // would see others' pages, or be written to them)
-    s.bad = taken != s.taken || gone != s.gone ||
-            (!s.ended && ((long long)s.have + add > a.max_pages * ps || s.have > s.taken * ps ||
-                          (s.gone > 0 && behind < a.kept + s.gone)));
+    s.bad = taken != s.taken || (unsigned)gone > (unsigned)s.now ||
+            (!s.ended && ((long long)s.have + add > a.max_pages * ps || s.have > s.taken * ps));
+    s.gone = s.bad ? 0 : gone;
     s.add = s.ended || s.bad ? 0 : add;
     const int need = (int)(((long long)s.have + s.add + ps - 1) >> a.shift);
     s.more = s.ended || s.bad ? 0 : max(need - s.taken, 0);
-    s.now = s.ended || s.bad ? s.gone : max(s.gone, min(behind, s.taken) - a.kept);
     return s;
 }
 // The ring's state as given, within its ranges.  One that is not is no step's: what its ids are
