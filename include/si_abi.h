@@ -493,10 +493,12 @@ int si_rope_kv_append_rows(const si_shape_t *s, const float *qkv, int ldqkv, int
  * of sequence i at position p, ctx[i] - 1 for its last one, sees position t <= p of
  * the sequence where t > p - window or t < sinks (a sliding window, and a few first
  * positions that stay visible); what it does not see has no influence, infinities and
- * NaN included.  window >= 1 (INT_MAX: all of them), sinks >= 0.  Contexts below 0 are
- * 0 and above max_ctx max_ctx, starts outside 0..max_rows the nearer of these (a last sequence
- * may reach past max_rows); rows before position 0 are zeros; a sequence's rows past the
- * first max_new are left as they are.  q, pools, attn 16-byte aligned, qs 4-byte.
+ * NaN included.  Of what it sees a score of NaN or +inf makes the head's outputs NaN, one
+ * of -inf has no weight, and an infinity or NaN in V goes to that output alone.  window
+ * >= 1 (INT_MAX: all of them), sinks >= 0.  Contexts below 0 are 0 and above max_ctx
+ * max_ctx, starts outside 0..max_rows the nearer of these (a last sequence may reach past
+ * max_rows); rows before position 0 are zeros; a sequence's rows past the first max_new
+ * are left as they are.  q, pools, attn 16-byte aligned, qs 4-byte.
  * Of the shape qheads, kvheads and hdim are read; outputs as si_attention's.
  * workspace: si_attention_rows_workspace bytes, 256-byte aligned (calls that
  * overlap need one each). */

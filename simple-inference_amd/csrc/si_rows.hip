@@ -23,8 +23,16 @@
 //
 // Where a mask cuts a tile its hidden scores are replaced (not added to), and V's values
 // there are looked at: 0 x infinity would be NaN.  Only if one is not finite, the rows
-// that see it are found first (exact counts, by the matrix cores), get their infinity or
-// NaN, and the tile in LDS has zeros in such places from then on.
+// that see it are marked by NaN, and the tile in LDS has zeros in such places from then on.
+//
+// What a row sees of infinities and NaN it gets as the definition has it, wherever they lie: a score
+// of NaN or +inf makes its outputs NaN, one of -inf has no weight, and an infinity of V stays
+// one.  Two halves of q or of a weight would make NaN of them, or the lo half's sign; so a
+// workgroup whose outputs are not finite walks again (rows_walk, SURE), a tile at a time: a call
+// whose workgroups all do takes three to four times as long (64 x 4096 91 -> 284 us, a prompt of
+// 8000 404 -> 1700).  Where none does it costs an instruction an output and a barrier (us, without
+// | with: a piece of 333 rows 26.4 | 26.9, pieces among tokens 96.5 | 97.4, a prompt of 8000 404 |
+// 404, 64 x 4096 90.6 | 90.7).
 //
 // What bounds it (MI355X; a plain read reaches 6.2 TB/s, a large f16 product 1.18 PFLOP/s):
 //   single tokens, 64 sequences in windows of 4096, 28/4 heads of 128: memory, 539 MB in
@@ -203,65 +211,97 @@ __device__ __forceinline__ void rows_store(const RowsArgs &a, int row, int head,
     }
 }
 
-// AHEAD: steps that a stage's copies are issued before their use (RT > 1).  PAGE: pages of
-// 32 positions and more, whole tiles (32), of 16 where an instruction's rows are whole (16:
-// two a tile), of any (1: each lane looks up its own row's: with 1 in place of 32, us, 64 x 4096 of
-// 28/4 heads of 128 102 | 91, 8000 rows of 2048 448 | 415, a piece of 333 rows 33 | 25; in place of
-// 16, 1024 positions of 14/2 of 64 10.5 | 9.6).
-template <int D, int RT, int KW, int AHEAD, bool ONE, int PAGE>
-__global__ void __launch_bounds__(RT * KW * 64) __attribute__((amdgpu_waves_per_eu(2)))
-k_attn_rows(RowsArgs a, RowsParts pt) {
-    constexpr int NWV = RT * KW, NT = NWV * 64, KS = D / 16, DT = D / 32, CH = D / 8;
-    constexpr int TB = PF_T * D * 2;         // bytes of a K (or V) tile
-    constexpr int TI = TB / 1024;            // copy instructions per tile
-    constexpr int TIW = (TI + RT - 1) / RT;  // of one wavefront
-    constexpr int OROW = D + PF_OPAD;
-    // (K and V that one workgroup reads are kept out of the caches: us, 64 x 4096 of 28/4 heads
-    // 98 | 91, 2 x 65536 of 12/2 32 | 29; a prompt's are read by many)
-    constexpr int AUX = ONE ? 2 : 0;
+__device__ __forceinline__ bool finite_h(_Float16 x) {
+    return (__builtin_bit_cast(uint16_t, x) & 0x7c00u) != 0x7c00u;
+}
+// A state's factor, 2^-149 where it would be 0 in 32 bits, so that an infinity among the state's
+// outputs stays one (a finite output is moved by less than the 0 below 2^-126 moves it)
+__device__ __forceinline__ float some(float f) { return f < 0x1p-149f ? 0x1p-149f : f; }
+
+// AHEAD: steps that a stage's copies are issued before their use (RT > 1).
+template <int D, int RT, int KW, int AHEAD>
+struct RowsForm {
+    static constexpr int NWV = RT * KW, NT = NWV * 64, TB = PF_T * D * 2;  // bytes of a K (V) tile
+    static constexpr int OROW = D + PF_OPAD;
     // RT > 1: AHEAD + 1 stages (K tiles, then V tiles) used in turn, one barrier per step.
     // RT == 1: each wavefront stages its own tiles, K in sb and V in sb1, both refilled as
     // soon as they are in registers (no barrier).  KW > 1: at the end the wavefronts'
     // outputs, where there are two arrays half of them in each.
-    constexpr bool DB = RT > 1;
-    constexpr int STAGE = (DB ? 2 : 1) * KW * TB, NSTAGE = DB ? AHEAD + 1 : 1;
-    constexpr int MRG_W = DB ? NWV : (NWV + 1) / 2, MRG = KW > 1 ? MRG_W * PF_T * OROW * 4 : 0;
-    constexpr int SB = NSTAGE * STAGE > MRG ? NSTAGE * STAGE : MRG;
-    __shared__ __attribute__((aligned(16))) uint8_t sb[SB];
-    __shared__ __attribute__((aligned(16))) uint8_t sb1[DB ? 16 : SB];
-    __shared__ float mrg_m[KW > 1 ? NWV : 1][PF_T], mrg_l[KW > 1 ? NWV : 1][PF_T];
-    __shared__ int bad_step[2];  // whether a cut step's V holds infinities or NaN
+    static constexpr bool DB = RT > 1;
+    static constexpr int STAGE = (DB ? 2 : 1) * KW * TB, NSTAGE = DB ? AHEAD + 1 : 1;
+    static constexpr int MRG_W = DB ? NWV : (NWV + 1) / 2;
+    static constexpr int MRG = KW > 1 ? MRG_W * PF_T * OROW * 4 : 0;
+    static constexpr int SB = NSTAGE * STAGE > MRG ? NSTAGE * STAGE : MRG;
+};
 
-    const int tid = threadIdx.x, lane = tid & 63;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int kw = wave / RT, rt = wave % RT;
-    const int t = lane & 31, hh = lane >> 5;
-    // KV groups side by side: one group's tiles on the same XCDs where their count
-    // divides 8
-    const int g = blockIdx.x % a.kvheads;
-    const int tile_id = blockIdx.x / a.kvheads / pt.chunks;
-    const int chunk = blockIdx.x / a.kvheads % pt.chunks;
+// A workgroup's share of the call: a KV group's tile of rows, and a chunk of its tiles of K and V,
+// from v0 to v1
+struct RowsShare {
     RowTile rw;
-    if (!find_tile<ONE, NT>(a, 32 * RT, tile_id, rw)) return;
-    const int v0 = chunk * pt.chunk_tiles, v1 = min(rw.ntiles, v0 + pt.chunk_tiles);
-    if (chunk > 0 && v0 >= v1) return;
-    const bool whole = rw.ntiles <= pt.chunk_tiles;  // the results themselves, not a part
+    int g, tile, chunk, v0, v1;
+};
 
-    const int per = a.qheads / a.kvheads, kvd = a.kvheads * D;
+// A wavefront's rows, and lane t's own of them
+struct RowsWave {
+    int kw, rt, lane, t, hh;
+    bool any;                 // whether there are some
+    int first, last;          // positions of the first and the last
+    int row, head, pos;       // lane t's (the last one again past it)
+    template <int RT>
+    static __device__ __forceinline__ RowsWave of(const RowsArgs &a, const RowsShare &sh, int tid) {
+        RowsWave w;
+        const RowTile &rw = sh.rw;
+        const int per = a.qheads / a.kvheads, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+        w.lane = tid & 63;
+        w.kw = wave / RT, w.rt = wave % RT;
+        w.t = w.lane & 31, w.hh = w.lane >> 5;
+        const int p0 = rw.pair0 + min(32 * w.rt, rw.pairs - 1);
+        const int p1 = rw.pair0 + min(32 * w.rt + 31, rw.pairs - 1);
+        w.any = 32 * w.rt < rw.pairs;
+        w.first = rw.p0 + p0 / per, w.last = rw.p0 + p1 / per;
+        const int pair = min(rw.pair0 + 32 * w.rt + w.t, p1);
+        w.row = rw.row0 + pair / per, w.head = sh.g * per + pair % per;
+        w.pos = rw.p0 + pair / per;
+        return w;
+    }
+};
+
+// One wavefront's walk over its tiles: row t's reference c, this lane's share of the sum, and the
+// outputs (lane (t, hh): O[row t][32 dt + 8 (r / 4) + 4 hh + r % 4] in o[dt][r]).
+//
+// An infinity or NaN that a row sees, in K or V, makes its sums NaN, or infinite by the sign of a
+// lo half (q's and the weights' are of either sign, or 0).  A workgroup with such outputs walks
+// again, with SURE, a tile at a time: scores that are not finite from q's hi halves alone, whose signs are q's; V's
+// infinities and NaN, with zeros in their places, counted apart by what rows see them.
+// PAGE: pages of 32 positions and more, whole tiles (32), of 16 where an instruction's rows are
+// whole (16: two a tile), of any (1: each lane looks up its own row's: with 1 in place of 32, us,
+// 64 x 4096 of 28/4 heads of 128 102 | 91, 8000 rows of 2048 448 | 415, a piece of 333 rows 33 | 25;
+// in place of 16, 1024 positions of 14/2 of 64 10.5 | 9.6).
+template <int D, int RT, int KW, int AHEAD, bool ONE, int PAGE, bool SURE>
+__device__ __forceinline__ void rows_walk(const RowsArgs &a, const RowsShare &sh, int tid,
+                                          uint8_t *sb, uint8_t *sb1, int *bad_step, float &c,
+                                          float &lsum, f16v (&o)[D / 32]) {
+    using F = RowsForm<D, RT, KW, AHEAD>;
+    constexpr int KS = D / 16, DT = D / 32, CH = D / 8, TB = F::TB;
+    constexpr int TI = TB / 1024;            // copy instructions per tile
+    constexpr int TIW = (TI + RT - 1) / RT;  // of one wavefront
+    constexpr bool DB = F::DB;
+    constexpr int STAGE = F::STAGE, NSTAGE = F::NSTAGE;
+    // (K and V that one workgroup reads are kept out of the caches: us, 64 x 4096 of 28/4 heads
+    // 98 | 91, 2 x 65536 of 12/2 32 | 29; a prompt's are read by many)
+    constexpr int AUX = ONE ? 2 : 0;
+    const RowTile &rw = sh.rw;
+    const int g = sh.g, v0 = sh.v0, v1 = sh.v1, kvd = a.kvheads * D;
     const int steps = (v1 - v0 + KW - 1) / KW;
-    // this wavefront's rows: positions of the first, the last and lane t's own
-    const int wp0 = rw.pair0 + min(32 * rt, rw.pairs - 1);
-    const int wp1 = rw.pair0 + min(32 * rt + 31, rw.pairs - 1);
-    const bool rows_here = 32 * rt < rw.pairs;
-    const int wfirst = rw.p0 + wp0 / per, wlast = rw.p0 + wp1 / per;
-    const int mypair = min(rw.pair0 + 32 * rt + t, wp1);
-    const int myrow = rw.row0 + mypair / per, myhead = g * per + mypair % per;
-    const int prow = rw.p0 + mypair / per;
+    const RowsWave me = RowsWave::of<RT>(a, sh, tid);
+    const int lane = me.lane, kw = me.kw, rt = me.rt, t = me.t, hh = me.hh;
+    const int wfirst = me.first, wlast = me.last, prow = me.pos;
+    const bool rows_here = me.any;
 
     // lane (t, hh) has k-slice hh of row t of q: on its way while the pages are looked up
     float4 x0[KS], x1[KS];
     {
-        const float *qrow = a.q + ((size_t)myrow * a.qheads + myhead) * D + 8 * hh;
+        const float *qrow = a.q + ((size_t)me.row * a.qheads + me.head) * D + 8 * hh;
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
             x0[ks] = *(const float4 *)(qrow + 16 * ks);
@@ -349,7 +389,7 @@ k_attn_rows(RowsArgs a, RowsParts pt) {
     };
     // the first copies: K up to step AHEAD and V one step less (RT == 1: of step 0)
     Pages page = {}, page1 = {};
-    if (steps > 0) {
+    if (!SURE && steps > 0) {
         page = page_of(0);
         copy(a.k, sb, 0, page, true);
         if constexpr (DB) {
@@ -416,8 +456,8 @@ k_attn_rows(RowsArgs a, RowsParts pt) {
                  pf_v_slot<D>(s16 >> 2, 4 * dt + 2 * ((lane >> 4) & 1) + ((s16 & 3) >> 1)) * 16 +
                  (s16 & 1) * 8;
 
-    float c = -INFINITY, lsum = 0.0f;  // row t's reference; this lane's share of the sum
-    f16v o[DT];
+    c = -INFINITY;
+    lsum = 0.0f;
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) o[dt] = (f16v){};
 
@@ -478,7 +518,7 @@ k_attn_rows(RowsArgs a, RowsParts pt) {
             float to = c;
             if (d > RW_OVER) to = mx;
             else if (d < -RW_UNDER && mx > -INFINITY) to = c - fminf(-d, fmaxf(room, 0.0f));
-            const float alpha = to == c ? 1.0f : __builtin_amdgcn_exp2f(c - to);
+            const float alpha = to == c ? 1.0f : some(__builtin_amdgcn_exp2f(c - to));
             c = to;
             lsum *= alpha;
 #pragma unroll
@@ -576,10 +616,8 @@ k_attn_rows(RowsArgs a, RowsParts pt) {
             }
         return __ballot((bad & 0x80008000u) != 0) != 0;
     };
-    // the rows that see such values: how many infinities (1 each), negative ones (64) and
-    // NaN (both) each output meets, exactly, and the infinity or NaN that follows
-    typedef uint16_t u8v __attribute__((ext_vector_type(8)));
-    const auto meet_bad = [&](const uint8_t *vt, int v) {
+    // what rows see such values: NaN for the time being (the walk is taken again for them)
+    const auto mark_bad = [&](const uint8_t *vt, int v) {
         h8 seen[2];
         const Seen sn = seen_of(v);
 #pragma unroll
@@ -590,23 +628,13 @@ k_attn_rows(RowsArgs a, RowsParts pt) {
             f16v n = (f16v){};
 #pragma unroll
             for (int s2 = 0; s2 < 2; ++s2) {
-                const u8v x = __builtin_bit_cast(u8v, v_operand(vt, dt, s2));
-                h8 k;
+                h8 k = v_operand(vt, dt, s2);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const uint16_t b = x[e];
-                    const float f = (b & 0x3ffu) ? 65.0f : b >> 15 ? 64.0f : 1.0f;
-                    k[e] = (_Float16)((b & 0x7c00u) == 0x7c00u ? f : 0.0f);
-                }
+                for (int e = 0; e < 8; ++e) k[e] = (_Float16)(finite_h(k[e]) ? 0.0f : 1.0f);
                 n = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, seen[s2], n, 0, 0, 0);
             }
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                const int k = (int)n[e];
-                const float up = (k & 63) ? __builtin_inff() : 0.0f;
-                const float down = (k >> 6) ? -__builtin_inff() : 0.0f;
-                o[dt][e] += up + down;
-            }
+            for (int e = 0; e < 16; ++e) o[dt][e] = n[e] > 0.0f ? __builtin_nanf("") : o[dt][e];
         }
     };
     // this wavefront's share of a V tile with zeros in their places
@@ -624,7 +652,99 @@ k_attn_rows(RowsArgs a, RowsParts pt) {
                 *at = w;
             }
     };
-    if constexpr (DB) {
+    if constexpr (SURE) {
+        uint8_t *const vt = DB ? sb + KW * TB : sb1;
+        bool in_turn = false;
+#pragma unroll 1
+        for (int st = 0; st < steps; ++st) {
+            pf_wait<0>();  // the last tile is read
+            if constexpr (DB) pf_barrier();
+            const Pages now = page_of(st);
+            copy(a.k, sb, st, now, true);
+            copy(a.v, vt, st, now, false);
+            pf_wait<0>();
+            if constexpr (DB) pf_barrier();
+            const int v = nth(st);
+            if (!(v0 + st * KW + kw < v1 && rows_here && rw.touches(a, v, wfirst, wlast))) {
+                in_turn = false;
+                continue;  // (wavefront-uniform; the barriers are at the loop's head)
+            }
+            // The first walk's sums in its order, so that rows without such values keep their
+            // bits: there, after a step that computed weights, q's halves take turns.  (A load,
+            // its products, the next: registers are short.)
+            f16v s = (f16v){}, by_hi = (f16v){};
+            const auto product = [&](int ks, bool hi) {
+                const h8 x = *(const h8 *)(sb + ka[ks]);
+                s = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, hi ? qh[ks] : ql[ks], s, 0, 0, 0);
+                if (hi) by_hi = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, qh[ks], by_hi, 0, 0, 0);
+                __builtin_amdgcn_sched_barrier(0);
+            };
+            if (in_turn) {
+#pragma unroll
+                for (int i = 0; i < 2 * KS; ++i) product(i / 2, i % 2);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 2 * KS; ++i) product(i % KS, i >= KS);
+            }
+            in_turn = DB;
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+                s[r] = fabsf(s[r]) < __builtin_inff() ? s[r] : by_hi[r];
+            refer(s, v, true);
+            weights(s);
+            // positions of any weight, and visible ones of none (a score of -inf), a bit each
+            uint32_t live = 0, none = 0;
+            {
+                const Seen sn = seen_of(v);
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    if (sn.at(r) && s[r] != -INFINITY) live |= 1u << r;
+                    if (sn.at(r) && s[r] == -INFINITY) none |= 1u << r;
+                }
+            }
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) {
+                // infinities count 1, negative ones 64, NaN and products with 0 both (exactly: a
+                // tile has 32 positions)
+                f16v n = (f16v){};
+#pragma unroll
+                for (int s2 = 0; s2 < 2; ++s2) {
+                    const h8 y = v_operand(vt, dt, s2);
+                    h8 x, w;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) x[e] = finite_h(y[e]) ? y[e] : (_Float16)0.0f;
+                    o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, ph[s2], o[dt], 0, 0, 0);
+                    o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, pl[s2], o[dt], 0, 0, 0);
+                    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const uint16_t b = __builtin_bit_cast(uint16_t, (_Float16)y[e]);
+                        const float kind = (b & 0x3ffu) ? 65.0f : b >> 15 ? 64.0f : 1.0f;
+                        x[e] = (_Float16)(finite_h(y[e]) ? 0.0f : kind);
+                        w[e] = (_Float16)(float)((live >> (8 * s2 + e)) & 1u);
+                    }
+                    n = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, w, n, 0, 0, 0);
+                    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        x[e] = (_Float16)(finite_h(y[e]) ? 0.0f : 65.0f);
+                        w[e] = (_Float16)(float)((none >> (8 * s2 + e)) & 1u);
+                    }
+                    n = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, w, n, 0, 0, 0);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const int k = (int)n[e];
+                    const float up = (k & 63) ? __builtin_inff() : 0.0f;
+                    const float down = (k >> 6) ? -__builtin_inff() : 0.0f;
+                    o[dt][e] += up + down;
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+    } else if constexpr (DB) {
         // K runs a step ahead of V: a step's weights are computed among the next one's
         // scores.  After its barrier the next K and this V are in, and the buffers of the
         // last K and V free; the copies into them have AHEAD steps to arrive.
@@ -664,7 +784,7 @@ k_attn_rows(RowsArgs a, RowsParts pt) {
                 if (any_bad(vt) && lane == 0) bad_step[st & 1] = 1;
                 __syncthreads();
                 if (bad_step[st & 1]) {
-                    if (use) meet_bad(vt, v);
+                    if (use) mark_bad(vt, v);
                     __syncthreads();
                     drop_bad(vt);
                     __syncthreads();
@@ -688,7 +808,7 @@ k_attn_rows(RowsArgs a, RowsParts pt) {
             const bool more = v + KW < v1, cut = !rw.inside(a, v, wfirst, wlast);
             pf_wait<0>();  // K and V are in
             if (cut && any_bad(sb1)) {
-                meet_bad(sb1, v);
+                mark_bad(sb1, v);
                 pf_wait<0>();  // (its reads are done)
                 drop_bad(sb1);
                 pf_wait<0>();
@@ -723,6 +843,24 @@ k_attn_rows(RowsArgs a, RowsParts pt) {
                 }
         }
     }
+}
+
+// The outputs of a workgroup's walks (or its chunk's states): 0, or NaN where one of this thread's is
+// not finite.
+template <int D, int RT, int KW, int AHEAD>
+__device__ __forceinline__ float rows_put(const RowsArgs &a, const RowsParts &pt,
+                                          const RowsShare &sh, int tid, uint8_t *sb, uint8_t *sb1,
+                                          float (*mrg_m)[PF_T], float (*mrg_l)[PF_T], float c,
+                                          float lsum, const f16v (&o)[D / 32]) {
+    using F = RowsForm<D, RT, KW, AHEAD>;
+    constexpr int NT = F::NT, DT = D / 32, OROW = F::OROW, MRG_W = F::MRG_W;
+    const RowTile &rw = sh.rw;
+    const bool whole = rw.ntiles <= pt.chunk_tiles;  // the results themselves, not a part
+    const int g = sh.g, per = a.qheads / a.kvheads, tile_id = sh.tile, chunk = sh.chunk;
+    const RowsWave me = RowsWave::of<RT>(a, sh, tid);
+    const int rt = me.rt, t = me.t, hh = me.hh, wave = me.kw * RT + rt;
+    const int myrow = me.row, myhead = me.head, prow = me.pos;
+    float z = 0.0f;
     lsum += swap32_f(lsum);
 
     // lane (t, hh) holds O[row t][32 dt + 8 (r / 4) + 4 hh + r % 4] in o[dt][r]
@@ -743,6 +881,8 @@ k_attn_rows(RowsArgs a, RowsParts pt) {
             if (a.qs) quant_block_pair16(y, q, dbits, sum);  // every lane
             if (lr >= rw.pairs) continue;
 #pragma unroll
+            for (int r = 0; r < 16; ++r) z = fmaf(y[r], 0.0f, z);
+#pragma unroll
             for (int r4 = 0; r4 < 4; ++r4)
                 *(f4 *)(a.attn + off + 32 * dt + 8 * r4 + 4 * hh) =
                     (f4){y[4 * r4], y[4 * r4 + 1], y[4 * r4 + 2], y[4 * r4 + 3]};
@@ -755,7 +895,7 @@ k_attn_rows(RowsArgs a, RowsParts pt) {
                 if (a.bsum) a.bsum[off / SI_QK + dt] = (int16_t)sum;
             }
         }
-        return;
+        return z;
     }
     pf_wait<0>();  // no copy in flight (a wavefront without tiles never waited for its own)
     __syncthreads();  // every wavefront is done with the stages
@@ -794,7 +934,7 @@ k_attn_rows(RowsArgs a, RowsParts pt) {
         }
         const float inv = whole ? 1.0f / l : 1.0f;
 #pragma unroll
-        for (int k = 0; k < KW; ++k) mrg_m[k * RT + w0][tr] = f[k] * inv;
+        for (int k = 0; k < KW; ++k) mrg_m[k * RT + w0][tr] = some(f[k] * inv);
     }
     __syncthreads();
     // 4 consecutive elements of a row per thread: merge the KW states, quantize (8 lanes
@@ -813,10 +953,61 @@ k_attn_rows(RowsArgs a, RowsParts pt) {
         if (!whole) {
             *(f4 *)(pt.o + part_row(pt, a.kvheads, tile_id, g, chunk, lr) * D + dd) =
                 (f4){y[0], y[1], y[2], y[3]};
-            continue;
+        } else {
+            const int pair = rw.pair0 + lr;
+            rows_store<D>(a, rw.row0 + pair / per, g * per + pair % per, dd, rw.p0 + pair / per, y);
         }
-        const int pair = rw.pair0 + lr;
-        rows_store<D>(a, rw.row0 + pair / per, g * per + pair % per, dd, rw.p0 + pair / per, y);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) z = fmaf(y[i], 0.0f, z);
+    }
+    return z;
+}
+
+// The second walk and its outputs.
+template <int D, int RT, int KW, int AHEAD, bool ONE, int PAGE>
+__device__ __forceinline__ void rows_again(RowsArgs a, RowsParts pt, RowsShare sh, int tid,
+                                                     uint8_t *sb, uint8_t *sb1,
+                                                     float (*mrg_m)[PF_T], float (*mrg_l)[PF_T]) {
+    float c, lsum;
+    f16v o[D / 32];
+    rows_walk<D, RT, KW, AHEAD, ONE, PAGE, true>(a, sh, tid, sb, sb1, nullptr, c, lsum, o);
+    rows_put<D, RT, KW, AHEAD>(a, pt, sh, tid, sb, sb1, mrg_m, mrg_l, c, lsum, o);
+}
+
+template <int D, int RT, int KW, int AHEAD, bool ONE, int PAGE>
+__global__ void __launch_bounds__(RT * KW * 64) __attribute__((amdgpu_waves_per_eu(2)))
+k_attn_rows(RowsArgs a, RowsParts pt) {
+    using F = RowsForm<D, RT, KW, AHEAD>;
+    __shared__ __attribute__((aligned(16))) uint8_t sb[F::SB];
+    __shared__ __attribute__((aligned(16))) uint8_t sb1[F::DB ? 16 : F::SB];
+    __shared__ float mrg_m[KW > 1 ? F::NWV : 1][PF_T], mrg_l[KW > 1 ? F::NWV : 1][PF_T];
+    __shared__ int bad_step[3];  // whether a cut step's V holds infinities or NaN (of two steps in
+                                 // turn); whether outputs are not finite
+
+    const int tid = threadIdx.x;
+    if (tid == 0) bad_step[2] = 0;  // (a barrier of the walk or the outputs lies before its use)
+    // KV groups side by side: one group's tiles on the same XCDs where their count
+    // divides 8
+    RowsShare sh;
+    sh.g = blockIdx.x % a.kvheads;
+    sh.tile = blockIdx.x / a.kvheads / pt.chunks;
+    sh.chunk = blockIdx.x / a.kvheads % pt.chunks;
+    if (!find_tile<ONE, F::NT>(a, 32 * RT, sh.tile, sh.rw)) return;
+    sh.v0 = sh.chunk * pt.chunk_tiles, sh.v1 = min(sh.rw.ntiles, sh.v0 + pt.chunk_tiles);
+    if (sh.chunk > 0 && sh.v0 >= sh.v1) return;
+
+    float c, lsum;
+    f16v o[D / 32];
+    rows_walk<D, RT, KW, AHEAD, ONE, PAGE, false>(a, sh, tid, sb, sb1, bad_step, c, lsum, o);
+    const float z =
+        rows_put<D, RT, KW, AHEAD>(a, pt, sh, tid, sb, sb1, mrg_m, mrg_l, c, lsum, o);
+    if (__ballot(!(z == 0.0f)) && (tid & 63) == 0) bad_step[2] = 1;
+    __syncthreads();
+    if (bad_step[2]) {
+        // (a lane's numbers are made anew, not kept in registers through the first walk)
+        int again = tid;
+        asm volatile("" : "+v"(again));
+        rows_again<D, RT, KW, AHEAD, ONE, PAGE>(a, pt, sh, again, sb, sb1, mrg_m, mrg_l);
     }
 }
 
@@ -856,7 +1047,8 @@ __global__ void __launch_bounds__(RM_T) k_attn_rows_merge(RowsArgs a, RowsParts 
             float to = M;
 #pragma unroll
             for (int u = 0; u < U; ++u) to = fmaxf(to, m[u]);
-            const float ref = to == -INFINITY ? 0.0f : to, old = __builtin_amdgcn_exp2f(M - ref);
+            const float ref = to == -INFINITY ? 0.0f : to;
+            const float old = some(__builtin_amdgcn_exp2f(M - ref));
             M = to;
             l *= old;
 #pragma unroll
@@ -866,7 +1058,7 @@ __global__ void __launch_bounds__(RM_T) k_attn_rows_merge(RowsArgs a, RowsParts 
                 if (k0 + u * G >= n) continue;
                 // (of a chunk that the row sees nothing of all is 0; of one whose scores are NaN
                 // the reference is as low, and the sum NaN)
-                const float f = __builtin_amdgcn_exp2f(m[u] - ref);
+                const float f = some(__builtin_amdgcn_exp2f(m[u] - ref));
                 l = fmaf(s[u], f, l);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) y[i] = fmaf(v[u][i], f, y[i]);
@@ -892,7 +1084,7 @@ __global__ void __launch_bounds__(RM_T) k_attn_rows_merge(RowsArgs a, RowsParts 
         l = y[0] = y[1] = y[2] = y[3] = 0.0f;
 #pragma unroll
         for (int w = 0; w < G; ++w) {
-            const float f = __builtin_amdgcn_exp2f(all_m[w][grp % ROWS] - ref);
+            const float f = some(__builtin_amdgcn_exp2f(all_m[w][grp % ROWS] - ref));
             l = fmaf(all_l[w][grp % ROWS], f, l);
 #pragma unroll
             for (int i = 0; i < 4; ++i) y[i] = fmaf(all_y[w][at][i], f, y[i]);

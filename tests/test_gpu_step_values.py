@@ -62,6 +62,35 @@ HEADS = [(14, 2, 64), (28, 4, 128), (8, 8, 32), (24, 8, 96)]
 PLACES = [(300, 5, (1, 4, 705, 730, 800, 863, 960, 995)), (2 ** 31 - 1, 0, (0, 31, 500, 992, 998))]
 
 
+@pytest.mark.parametrize("heads", HEADS)
+@pytest.mark.parametrize("page", [8, 16, 64])
+@pytest.mark.parametrize("new", [1, 6, 40])
+@pytest.mark.parametrize("window,sinks,places", PLACES)
+def test_values_that_are_seen(heads, page, new, window, sinks, places):
+    """Infinities of either sign, both, and NaN in V, one value each: that value alone is not
+    finite, and has the sign that the definition gives."""
+    b = Batch(heads, [1000, 90], [new, 1], page, window, sinks, seed=new)
+    g, D = heads[1], heads[2]
+    for n, pos in enumerate(places):
+        put(b, 0, pos, n % g, (3 * n) % D, v=[INF, -INF, NAN, INF][n % 4])
+        put(b, 0, pos, (n + 1) % g, D - 1, v=[INF, -INF][n % 2])
+    put(b, 1, 50, 0, 1, v=-INF)
+    check(b, b.run())
+
+
+@pytest.mark.parametrize("heads", HEADS[:2])
+@pytest.mark.parametrize("new", [1, 6, 40])
+@pytest.mark.parametrize("window,sinks,places", PLACES)
+def test_keys_that_are_seen(heads, new, window, sinks, places):
+    """An infinite key: the heads that it meets with a negative q give it no weight, the others are
+    NaN; so is a head that meets a NaN."""
+    for n, pos in enumerate(places):
+        b = Batch(heads, [1000, 90], [new, 1], 16, window, sinks, seed=n)
+        put(b, 0, pos, 0, n, k=[INF, -INF][n % 2], v=[None, 2.0, INF][n % 3])
+        put(b, 1, 60, 0, 5, k=NAN)
+        check(b, b.run())
+
+
 # 21 and 161 K/V tiles, cut in chunks of 5: the last one holds one tile, and that one position
 @pytest.mark.parametrize("heads,ctx,new", [((14, 2, 64), 641, 1), ((14, 2, 64), 5121, 1),
                                            ((28, 4, 128), 641, 2), ((28, 4, 128), 5121, 2),
@@ -75,3 +104,20 @@ def test_last_position_of_many_chunks(heads, ctx, new, value):
     got = b.run()
     assert np.isnan(got[new - 1]).all()
     check(b, got)
+
+
+@pytest.mark.parametrize("value", [INF, -INF, NAN])
+def test_values_far_below_the_largest(value):
+    """A position whose weight is next to nothing in 32 bits gives its infinity all the same, in
+    its own tile, wavefront and chunk."""
+    heads = (12, 2, 128)
+    for new, at in ((1, 3), (1, 700), (1, 1500), (12, 700)):
+        b = Batch(heads, [3000], [new], 64, 2 ** 31 - 1, 0, seed=7)
+        # the last 100 positions' scores lie 200 and more above the others'
+        top = b.q.reshape(-1, 2, 6, 128).sum((0, 2))
+        top /= np.linalg.norm(top, axis=-1, keepdims=True)
+        b.q += 6 * top[None, :, None].repeat(6, 2).reshape(1, 12, 128)
+        for pos in range(2900, 3000):
+            put(b, 0, pos, slice(None), slice(None), k=(top * 500).astype(np.float16))
+        put(b, 0, at, 1, 9, v=value)
+        check(b, b.run())
