@@ -3,8 +3,10 @@ wherever the position lies in the walk and however the walk is cut."""
 import numpy as np
 import pytest
 
+import si_amd
 from tests import step_ref
-from tests.test_gpu_step import Batch
+from tests.gpu_helpers import torch_cuda
+from tests.test_gpu_step import P, Batch, host, st
 
 pytestmark = pytest.mark.gpu
 
@@ -121,3 +123,29 @@ def test_values_far_below_the_largest(value):
             put(b, 0, pos, slice(None), slice(None), k=(top * 500).astype(np.float16))
         put(b, 0, at, 1, 9, v=value)
         check(b, b.run())
+
+
+@pytest.mark.parametrize("heads", HEADS)
+@pytest.mark.parametrize("new", [1, 6, 40])
+def test_quantized_around_them(heads, new):
+    """The Q8_0 of blocks without such values, of the rows that have them and of their neighbours, as
+    si_quantize_q8_rows has it."""
+    torch = torch_cuda()
+    b = Batch(heads, [400, 90], [new, 1], 16, 300, 4, seed=new)
+    put(b, 0, 398 - new // 2, 0, 3, v=INF)
+    put(b, 0, 200, 1, heads[2] - 1, v=NAN)
+    b.upload()
+    n, qd = b.max_rows, heads[0] * heads[2]
+    out = torch.full((n, qd), 7.0, device="cuda")
+    bufs = [torch.full((n, qd), 7, dtype=torch.int8, device="cuda"),
+            *(torch.full((n, qd // 32), 7, dtype=torch.int16, device="cuda") for _ in range(2))]
+    b.call(out, bufs)
+    fine = torch.isfinite(out).view(n, -1, 32).all(2)
+    assert not fine.all() and fine.any(1).all()
+    clean = torch.where(torch.isfinite(out), out, 0.0).contiguous()
+    want = [torch.empty_like(x) for x in bufs]
+    si_amd.call("si_quantize_q8_rows", P(clean), n, qd, *(P(x) for x in want), st())
+    assert torch.equal(bufs[0].view(n, -1, 32)[fine], want[0].view(n, -1, 32)[fine])
+    for x, y in zip(bufs[1:], want[1:]):
+        assert torch.equal(x[fine], y[fine])
+    check(b, host(out).reshape(n, *heads[::2]))
