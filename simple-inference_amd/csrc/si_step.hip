@@ -25,50 +25,48 @@ namespace si {
 // sequence's rows written by its own thread took 22 us for 200 sequences and 333 for the 4000.)
 // ---------------------------------------------------------------------------
 struct StepSeq {
-    int have, add, taken, gone;  // as given, within their ranges (outside: bad)
+    int have, add, taken, gone;  // as given (add: 0 of a sequence without rows)
     int more, now;               // pages taken in this step; pages given back after it
-    bool ended, bad;
+    bool ended, bad;             // (bad: the step is refused, only what was given is of use)
 };
 
 __device__ __forceinline__ StepSeq step_seq(const KvStep &a, int i) {
     StepSeq s;
     const long long ps = 1ll << a.shift;
-    const int have = a.have[i], add = max(a.add[i], 0);
-    const int taken = a.held_in[2 * i], gone = a.held_in[2 * i + 1];
-    s.ended = have < 0;
-    s.have = max(have, 0);
-    s.taken = min(max(taken, 0), a.max_pages);
+    const int add = max(a.add[i], 0);
+    s.have = a.have[i];
+    s.taken = a.held_in[2 * i];
+    s.gone = a.held_in[2 * i + 1];
+    s.ended = s.have < 0;
+    const int taken = min(max(s.taken, 0), a.max_pages);
     // (have - window + 1 positions lie behind every window from here on; an ended sequence may
     // have given back any of its pages)
     const int behind = (int)((max((long long)s.have - a.window + 1, 0ll)) >> a.shift);
-    s.now = max((s.ended ? s.taken : min(behind, s.taken)) - a.kept, 0);
+    s.now = max((s.ended ? taken : min(behind, taken)) - a.kept, 0);
     // (counts that no step left; rows from a have whose window reaches pages that were given back
     // would see others' pages, or be written to them)
-    s.bad = taken != s.taken || (unsigned)gone > (unsigned)s.now ||
-            (!s.ended && ((long long)s.have + add > a.max_pages * ps || s.have > s.taken * ps));
-    s.gone = s.bad ? 0 : gone;
+    s.bad = taken != s.taken || (unsigned)s.gone > (unsigned)s.now ||
+            (!s.ended && ((long long)s.have + add > a.max_pages * ps || s.have > taken * ps));
     s.add = s.ended || s.bad ? 0 : add;
     const int need = (int)(((long long)s.have + s.add + ps - 1) >> a.shift);
-    s.more = s.ended || s.bad ? 0 : max(need - s.taken, 0);
+    s.more = s.ended || s.bad ? 0 : max(need - taken, 0);
     return s;
 }
-// The ring's state as given, within its ranges.  One that is not is no step's: what its ids are
-// is not known, so that the step is refused and the ring empty from then on.
+// The ring's state.  One outside its ranges is no step's: what its ids are is not known, so that
+// the step is refused and the ring empty from then on.
 struct StepRing {
     int begin, count;
     bool bad;
 };
 __device__ __forceinline__ StepRing step_ring(const KvStep &a) {
     const int begin = a.free_in[0], count = a.free_in[1];
-    if (begin >= 0 && begin < a.npages && count >= 0 && count <= a.npages)
-        return {begin, count, false};
-    return {0, 0, true};
+    const bool bad = begin < 0 || begin >= a.npages || count < 0 || count > a.npages;
+    return {bad ? 0 : begin, bad ? 0 : count, bad};
 }
-// a sequence's state after the step, and the ring's
+// a sequence's state after the step (of a refused one as given, whatever it is), and the ring's
 __device__ __forceinline__ void step_state(const KvStep &a, int i, const StepSeq &s, int code) {
-    // (of a refused step as given, whatever it is)
-    a.held_out[2 * i] = code ? a.held_in[2 * i] : s.ended ? 0 : s.taken + s.more;
-    a.held_out[2 * i + 1] = code ? a.held_in[2 * i + 1] : s.ended ? 0 : s.now;
+    a.held_out[2 * i] = code ? s.taken : s.ended ? 0 : s.taken + s.more;
+    a.held_out[2 * i + 1] = code ? s.gone : s.ended ? 0 : s.now;
 }
 __device__ __forceinline__ void ring_state(const KvStep &a, const StepRing &ring, int code,
                                            long long more, long long back) {
@@ -98,7 +96,7 @@ struct StepSums {
     __device__ __forceinline__ void add(const KvStep &a, const StepSeq &s) {
         rows += s.add;
         more += s.more;
-        back += step_back(a, s);
+        back += s.bad ? 0 : step_back(a, s);
         held += s.bad ? 1ll << 40 : s.taken - s.gone;
     }
     __device__ __forceinline__ void add(const StepSums &x) {
@@ -270,7 +268,7 @@ __global__ void __launch_bounds__(T) k_kv_step(KvStep a) {
         a.start[i] = code ? 0 : rows;
         a.taken[i] = code ? 0 : more;
         // (of a refused step as given, so that a sequence that was to end still does in the next)
-        a.ctx[i] = code ? a.have[i] : s.ended ? 0 : s.have + s.add;
+        a.ctx[i] = code ? s.have : s.ended ? 0 : s.have + s.add;
         if (!STATE && apart(a)) step_state(a, i, s, code);
     }
     if (wg == 0 && tid == 0) {
