@@ -50,14 +50,14 @@ METRIC = "decode layer µs + HBM GB/s; prefill tokens/s + int8 MFMA % (one GPU)"
 # traffic with "traffic_current": false.  Kernels not listed report traffic
 # null.  Summaries: profiles/cfgN_*.md.
 PMC_KIB = {
-    ("1", "k_matvec<8, 128, false>"): (330.9, 4.5, "fc6533fb34d6"),
-    ("2", "k_dec_attn<64, 8, false, false, 1, true>"): (2694.0, 35.5, "fc6533fb34d6"),
-    ("2", "k_dec_gateup<64, 512, false>"): (2534.4, 9.8, "fc6533fb34d6"),
-    ("2", "k_dec_wo<8, 512, false>"): (579.0, 3.5, "fc6533fb34d6"),
-    ("2", "k_matvec<8, 512, false>"): (1256.0, 3.5, "fc6533fb34d6"),
-    ("3", "k_gemm_f6<2, 2, 1, 2, true>"): (28104.0, 5320.0, "fc6533fb34d6"),
-    ("4", "k_gemm_f6<2, 2, 2, 2, true>"): (516860.2, 43136.8, "fc6533fb34d6"),
-    ("5", "k_dec_attn_rows<128, 4, false, false, false>"): (266839.0, 8192.0, "fc6533fb34d6"),
+    ("1", "k_matvec<8, 128, false>"): (330.9, 4.5, "bd7e698598d6"),
+    ("2", "k_dec_attn<64, 8, false, false, 1, true>"): (2694.0, 35.5, "bd7e698598d6"),
+    ("2", "k_dec_gateup<64, 512, false>"): (2534.4, 9.8, "bd7e698598d6"),
+    ("2", "k_dec_wo<8, 512, false>"): (579.0, 3.5, "bd7e698598d6"),
+    ("2", "k_matvec<8, 512, false>"): (1256.0, 3.5, "bd7e698598d6"),
+    ("3", "k_gemm_f6<2, 2, 1, 2, true>"): (28104.0, 5320.0, "bd7e698598d6"),
+    ("4", "k_gemm_f6<2, 2, 2, 2, true>"): (516916.1, 43136.2, "bd7e698598d6"),
+    ("5", "k_dec_attn_rows<128, 4, false, false, false>"): (266839.0, 8192.0, "bd7e698598d6"),
 }
 FETCH_SCALE, WRITE_SCALE = 2.000, 1.000
 # sources of kernels that no configuration runs

@@ -36,14 +36,14 @@
 //
 // What bounds it (MI355X; a plain read reaches 6.2 TB/s, a large f16 product 1.18 PFLOP/s):
 //   single tokens, 64 sequences in windows of 4096, 28/4 heads of 128: memory, 539 MB in
-//     88 us, 6.1 TB/s.
+//     88 to 90 us, 6.1 TB/s.
 //   few of them (2 x 65536 positions of 12/2 heads, 16 x 4096 of 28/4 with up to 8 rows): the
-//     chunks' start, 129 MB in 23 us and 92 MB in 29 us, and the merge's launch after them, 4.5.
-//   one short window (1024 of 14/2 heads of 64): latency, 6.2 us + 3.0 of the merge.
+//     chunks' start, 129 MB in 24 us and 92 MB in 29 us, and the merge's launch after them, 4.5.
+//   one short window (1024 of 14/2 heads of 64): latency, 6.3 us + 3.0 of the merge.
 //   prompts (8000 rows in a window of 2048, 28/4): 415 us, 205 GFLOP, twice that issued for the
 //     halves: 1.0 PFLOP/s at the 1.9 GHz that the clock keeps.  Matrix cores busy half of the
 //     cycles; without the lo halves 300 us (and errors of 2^-11), without exponentials 366.
-//   pieces of prompts (333 rows after 1500) and pieces among single tokens: 25 and 100 us, the
+//   pieces of prompts (333 rows after 1500) and pieces among single tokens: 26 and 97 to 107 us, the
 //     latency of the steps and of a workgroup's start (6 us: its sequence, pages, q).
 // Why these tiles: a lane holds one row's half of a tile's scores, so that a row's maximum and sum
 // take one exchange and its weights are the next product's operand as they are, without LDS.  One

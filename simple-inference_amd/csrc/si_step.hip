@@ -319,7 +319,7 @@ void launch_kv_step(const KvStep &a, hipStream_t st) {
 //
 // The arithmetic and the bits of k_rope_kv: a' = a c - b s, b' = b c + a s, and the fp16
 // narrowing.  Memory bounds it: 2060 rows of 28/4 heads of 128 move 73 MB in 14.1 us,
-// 5.2 TB/s (a large copy: 4.9); 40 rows of 14/2 heads of 64 take 3.7 us, the latency of a
+// 5.2 TB/s (large copies 4.9 to 5.9); 40 rows of 14/2 heads of 64 take 3.7 us, the latency of a
 // row's place and then its values.  A thread takes four neighbouring pairs of a head (16-byte
 // loads and stores of q|k|v and q, 8-byte stores of the cache), or four values of V's two
 // halves.
