@@ -149,3 +149,33 @@ def test_quantized_around_them(heads, new):
     for x, y in zip(bufs[1:], want[1:]):
         assert torch.equal(x[fine], y[fine])
     check(b, host(out).reshape(n, *heads[::2]))
+
+
+def test_values_between_replays():
+    """One captured call, whose pools hold such values in some replays: each is the eager call's."""
+    torch = torch_cuda()
+    heads = (28, 4, 128)
+    for new in ([1, 1], [6, 2], [50, 1]):
+        b = Batch(heads, [1500, 300], new, 16, 1000, 4, seed=new[0])
+        pools = []
+        for value in (None, INF, NAN, None, -INF):
+            if value is not None:
+                put(b, 0, 1490, 1, 7, v=value)
+                put(b, 1, 200, 2, 9, k=value)
+            want = b.run()
+            pools.append((b.dk.clone(), b.dv.clone(), want))
+            put(b, 0, 1490, 1, 7, v=0.5)
+            put(b, 1, 200, 2, 9, k=0.5)
+        out, side, graph = torch.full_like(b.out, 7.0), torch.cuda.Stream(), torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph, stream=side):
+            b.call(out, ws=b.ws)
+        for k in (0, 1, 0, 2, 3, 4, 1, 0):
+            dk, dv, want = pools[k]
+            b.dk.copy_(dk)
+            b.dv.copy_(dv)
+            out.fill_(7.0)
+            torch.cuda.synchronize()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert np.array_equal(host(out).reshape(want.shape), want, equal_nan=True), (new, k)
