@@ -271,8 +271,10 @@ struct RowsWave {
 //
 // An infinity or NaN that a row sees, in K or V, makes its sums NaN, or infinite by the sign of a
 // lo half (q's and the weights' are of either sign, or 0).  A workgroup with such outputs walks
-// again, with SURE, a tile at a time: scores that are not finite from q's hi halves alone, whose signs are q's; V's
-// infinities and NaN, with zeros in their places, counted apart by what rows see them.
+// again, with SURE, a tile at a time: scores that are not finite from q's hi halves alone, whose
+// signs are q's; V's infinities and NaN, with zeros in their places, counted apart by what rows
+// see them.
+//
 // PAGE: pages of 32 positions and more, whole tiles (32), of 16 where an instruction's rows are
 // whole (16: two a tile), of any (1: each lane looks up its own row's: with 1 in place of 32, us,
 // 64 x 4096 of 28/4 heads of 128 102 | 91, 8000 rows of 2048 448 | 415, a piece of 333 rows 33 | 25;
